@@ -311,6 +311,84 @@ int t2w_attention(const void* q, const void* k_pool, const void* v_pool, void* o
                   const int* tiles, int n_tiles, int heads, int chunk, float scale, int n_rows, int kv_max,
                   void* stream);
 
+/* ---------------------------------------------------------------- paged 8-bit key/value cache
+ * A cache of blocks of 32 tokens in OCP e4m3, each block with one power-of-two scale (E8M0: exponent + 127) per
+ * key/value head for its keys and one for its values; half the memory of the bf16 slot pools.  No counterpart in the
+ * reference, whose pools are 16-bit (engine/runtime/dit_fast.py:60-97).  Three calls serve a step: t2w_kv8_plan builds
+ * the tables from the requests' lengths on the GPU, t2w_kv8_append stores the new keys and values, t2w_kv8_attention
+ * reads the cache.  All lengths and tables are device data, so a graph captured once serves calls of other lengths.
+ *
+ * Row r of a call is one request: its cache is blocks table[r * ld_table + 0 ..], block j holding its tokens
+ * 32 j .. 32 j + 31; its new tokens are rows row_start[r] .. row_start[r + 1] - 1 of the packed token tensors and the
+ * last ones of its kv_total[r] cached tokens.  A row may have no new token.  At most 4096 rows; int tables. */
+
+enum { T2W_KV8_BLOCK = 32, T2W_KV8_BF16 = 0, T2W_KV8_FP16 = 1 };
+
+/* Value (token t of its block, channel d) is code * 2^(exponent - 127).  Key codes: byte (d / 16) * 512 + t * 16 + d % 16
+ * of the (block, head)'s 32 * head_dim; value codes: byte (t / 8) * 8 * head_dim + (d / 2) * 16 + (d % 2) * 8 + t % 8. */
+typedef struct {
+  void* k; void* v;               /* [n_blocks, kv_heads, 32 * head_dim] e4m3 codes, 16-byte aligned */
+  uint8_t* k_exp; uint8_t* v_exp; /* [n_blocks, kv_heads] */
+  int n_blocks, kv_heads, head_dim; /* head_dim 64 or 128 */
+} t2w_kv8_pages;
+
+/* Tables of a call in which row r, holding kv_len[r] tokens, gets new_len[r] more.  Blocks beyond its ceil(kv_len / 32)
+ * come from free_ids[*free_head ..] in row order, and only their entries of `table` are written.  Outputs: kv_total =
+ * kv_len + new_len; row_start (n_rows + 1, the exclusive sums of new_len); for each of the n_tok tokens the call has room
+ * for its row, its position in the row and its slot (block * 32 + place), -1 behind the last token; free_head_out =
+ * *free_head + the blocks taken (keep it as the next call's free_head).  No output may lie on an input.
+ * status: 0, or the sum of 1 (a negative length), 2 (more than n_tok tokens), 4 (a row longer than its table is wide) and
+ * 8 (too few free blocks); then nothing is taken or written to `table`, row_start is 0 (no new tokens: the other two
+ * calls do nothing) and kv_total = kv_len.  The ids in table and free_ids are not checked here but where they are used. */
+typedef struct {
+  const int* kv_len; const int* new_len; int n_rows;
+  int* table; int width, ld_table;
+  const int* free_ids; int n_free; const int* free_head;
+  int n_tok;
+  int* kv_total; int* row_start; int* tok_row; int* tok_pos; int* slots; int* free_head_out; int* status;
+} t2w_kv8_plan_args;
+int t2w_kv8_plan(const t2w_kv8_plan_args* a, void* stream);
+
+/* Quantizes the new tokens' keys and values into their rows' blocks.  A block's scale is the smallest power of two that
+ * keeps its largest magnitude within 448; a block in use whose scale a new token raises has its old codes requantized.  A
+ * token and head with a key or value that is not finite counts for no scale and is stored as NaN keys and zero values:
+ * queries that see it get NaN, others do not.  New blocks are zero behind their last token; other places and blocks stay as
+ * they are.  A block may belong to one row only (blocks shared by rows may be read, not appended to); block ids outside the
+ * pages are skipped.  max_new: 0, or the longest row's new tokens, which sizes the grid (longer rows are stored all the
+ * same). */
+typedef struct {
+  t2w_kv8_pages pages;
+  const void* k; const void* v;   /* [n_tok, kv_heads, head_dim], token rows ldk / ldv elements apart (multiples of 8) */
+  long long ldk, ldv;
+  int dtype, n_tok;               /* T2W_KV8_BF16 or T2W_KV8_FP16 */
+  const int* table; int width, ld_table;
+  const int* row_start; const int* kv_total; int n_rows, max_new;
+} t2w_kv8_append_args;
+int t2w_kv8_append(const t2w_kv8_append_args* a, void* stream);
+
+/* out = softmax(scale q K^T) V of every new token over its row's cache (its own and the other new tokens appended before),
+ * fp32 softmax and sums.  heads / kv_heads (1 to 16) query heads share a key head, in order.  chunk: 0 a query sees all
+ * of its row; c > 0 it sees the row's earlier tokens and those new ones whose chunk of c new tokens is not behind its own
+ * (1: causal).  A query that sees nothing gets zeros.  Rows of `out` behind the last token are left as they were.  A row
+ * longer than its table is wide, or one with block ids outside the pages that a query sees, gets NaN.
+ * max_new: 0, or a bound on every row's new tokens; max_kv: 0, or one on kv_total: they choose the kernel and how it
+ * splits the keys.  A row of more than max_new new tokens gets NaN; one of more than max_kv keys is still right. */
+typedef struct {
+  t2w_kv8_pages pages;
+  const void* q; void* out;       /* [n_tok, heads, head_dim], token rows ldq / ldo elements apart (multiples of 8) */
+  long long ldq, ldo;
+  int dtype, n_tok, heads;
+  const int* table; int width, ld_table;
+  const int* row_start; const int* kv_total; int n_rows, chunk;
+  float scale;
+  int max_new, max_kv;
+  void* workspace; size_t workspace_bytes; /* t2w_kv8_attention_workspace_bytes of the same arguments, 16-byte aligned;
+                                            * nothing in it needs clearing or outlives the call, and calls that may
+                                            * overlap need one each */
+} t2w_kv8_attention_args;
+size_t t2w_kv8_attention_workspace_bytes(const t2w_kv8_attention_args* a);
+int t2w_kv8_attention(const t2w_kv8_attention_args* a, void* stream);
+
 /* ---------------------------------------------------------------- HiFT vocoder (fp32) */
 
 typedef struct t2w_hift t2w_hift;

@@ -99,6 +99,27 @@ class FlowArgs(C.Structure):
                 ("mu_out", P), ("workspace", P), ("workspace_bytes", C.c_size_t)]
 
 
+class KV8Pages(C.Structure):
+    _fields_ = [(n, P) for n in ("k", "v", "k_exp", "v_exp")] + [(n, I) for n in ("n_blocks", "kv_heads", "head_dim")]
+
+
+class KV8PlanArgs(C.Structure):
+    _fields_ = [("kv_len", P), ("new_len", P), ("n_rows", I), ("table", P), ("width", I), ("ld_table", I), ("free_ids", P), ("n_free", I),
+                ("free_head", P), ("n_tok", I)] + \
+               [(n, P) for n in ("kv_total", "row_start", "tok_row", "tok_pos", "slots", "free_head_out", "status")]
+
+
+class KV8AppendArgs(C.Structure):
+    _fields_ = [("pages", KV8Pages), ("k", P), ("v", P), ("ldk", C.c_longlong), ("ldv", C.c_longlong), ("dtype", I), ("n_tok", I),
+                ("table", P), ("width", I), ("ld_table", I), ("row_start", P), ("kv_total", P), ("n_rows", I), ("max_new", I)]
+
+
+class KV8AttentionArgs(C.Structure):
+    _fields_ = [("pages", KV8Pages), ("q", P), ("out", P), ("ldq", C.c_longlong), ("ldo", C.c_longlong), ("dtype", I), ("n_tok", I),
+                ("heads", I), ("table", P), ("width", I), ("ld_table", I), ("row_start", P), ("kv_total", P), ("n_rows", I), ("chunk", I),
+                ("scale", F), ("max_new", I), ("max_kv", I), ("workspace", P), ("workspace_bytes", C.c_size_t)]
+
+
 _SIGS = {
     "t2w_abi_version": (I, []),
     "t2w_last_error": (C.c_char_p, []),
@@ -138,6 +159,10 @@ _SIGS = {
     "t2w_flow_workspace_bytes": (C.c_size_t, [P, I, I, I, I, I]),
     "t2w_flow_encode": (I, [P, C.POINTER(FlowArgs), P]),
     "t2w_flow_speaker": (I, [P, P, P, I, P]),
+    "t2w_kv8_plan": (I, [C.POINTER(KV8PlanArgs), P]),
+    "t2w_kv8_append": (I, [C.POINTER(KV8AppendArgs), P]),
+    "t2w_kv8_attention": (I, [C.POINTER(KV8AttentionArgs), P]),
+    "t2w_kv8_attention_workspace_bytes": (C.c_size_t, [C.POINTER(KV8AttentionArgs)]),
     "t2w_device_cus": (I, [C.POINTER(I)]),
     "t2w_stream_create_cu_mask": (I, [C.POINTER(C.c_uint32), I, C.POINTER(P)]),
     "t2w_stream_destroy": (I, [P]),

@@ -1,0 +1,386 @@
+// Paged 8-bit key/value cache: block tables and slot maps built on the GPU from request lengths, and the append that
+// quantizes new keys and values into the cache.  Block format: kv8_internal.h.
+#include "kv8_internal.h"
+
+namespace t2w {
+
+namespace {
+
+// ---------------------------------------------------------------- tables
+// Row r holds kv_len[r] tokens in ceil(kv_len[r] / 32) blocks and gets new_len[r] more.  With the exclusive sums S of the
+// new lengths and B of the blocks that each row needs beyond its own, token n of the call belongs to the row with
+// S[r] <= n < S[r + 1], stands at position p = kv_len[r] + n - S[r], and its block p / 32 is the row's own or the new
+// block free_ids[head + B[r] + p / 32 - own blocks].
+//
+// One launch and no wait between workgroups: every workgroup sums all rows by itself (16 rows a thread at most, a scan
+// within each wave and one over the four waves), keeps S, B and kv_len in LDS, and then writes the tables of its own
+// TOKENS tokens.  The token at a block's first place writes that block into the table, so each new entry has one writer
+// and none is read in the same call.
+constexpr int PLAN_TOKENS = 1024;  // tokens of a workgroup, four a thread
+
+__global__ void __launch_bounds__(256) kv8_plan_kernel(t2w_kv8_plan_args a) {
+  __shared__ int s_tok[KV8_MAX_ROWS + 1], s_blk[KV8_MAX_ROWS], s_kv[KV8_MAX_ROWS];
+  __shared__ int w_tok[4], w_blk[4], w_bad[4];
+  __shared__ long long w_tot[4][2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per = (a.n_rows + 255) / 256, r0 = tid * per;
+  const int head = a.free_head[0];
+  int tok = 0, blk = 0, bad = 0;
+  long long tok64 = 0, blk64 = 0;
+  for (int i = 0; i < per; ++i) {
+    const int r = r0 + i;
+    if (r >= a.n_rows) break;
+    const int kv = a.kv_len[r], nw = a.new_len[r];
+    bad |= (kv < 0 || nw < 0) ? 1 : 0;
+    const long long want = ((long long)kv + nw + KV8_BLOCK - 1) / KV8_BLOCK, have = ((long long)kv + KV8_BLOCK - 1) / KV8_BLOCK;
+    bad |= want > a.width ? 4 : 0;
+    s_kv[r] = kv;
+    s_tok[r] = tok;  // within the thread for now
+    s_blk[r] = blk;
+    tok += nw;
+    blk += (int)(want - have);
+    tok64 += nw;
+    blk64 += want - have;
+  }
+  // sums before this thread: within the wave, then over the waves.  The 32-bit sums may wrap only where the 64-bit
+  // totals say that the call fails.
+  int it = tok, ib = blk;
+  long long t64 = tok64, b64 = blk64;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int ut = __shfl_up(it, o, 64), ub = __shfl_up(ib, o, 64);
+    if (lane >= o) { it += ut; ib += ub; }
+    t64 += __shfl_xor(t64, o, 64);
+    b64 += __shfl_xor(b64, o, 64);
+    bad |= __shfl_xor(bad, o, 64);
+  }
+  if (lane == 63) { w_tok[wave] = it; w_blk[wave] = ib; }
+  if (lane == 0) { w_tot[wave][0] = t64; w_tot[wave][1] = b64; w_bad[wave] = bad; }
+  __syncthreads();
+  int bt = it - tok, bb = ib - blk;
+  for (int w = 0; w < wave; ++w) { bt += w_tok[w]; bb += w_blk[w]; }
+  const long long n_tok = w_tot[0][0] + w_tot[1][0] + w_tot[2][0] + w_tot[3][0];
+  const long long n_blk = w_tot[0][1] + w_tot[1][1] + w_tot[2][1] + w_tot[3][1];
+  int status = w_bad[0] | w_bad[1] | w_bad[2] | w_bad[3];
+  status |= n_tok > a.n_tok ? 2 : 0;
+  status |= (head < 0 || head + n_blk > a.n_free) ? 8 : 0;
+  const bool ok = status == 0;
+  for (int i = 0; i < per; ++i) {
+    const int r = r0 + i;
+    if (r >= a.n_rows) break;
+    const int st = s_tok[r] + bt;
+    s_tok[r] = st;
+    s_blk[r] += bb;
+    if (blockIdx.x == 0) {
+      const int kv = s_kv[r];
+      a.row_start[r] = ok ? st : 0;
+      a.kv_total[r] = ok ? kv + a.new_len[r] : kv;
+    }
+  }
+  if (tid == 0) {
+    s_tok[a.n_rows] = ok ? (int)n_tok : 0;
+    if (blockIdx.x == 0) {
+      a.row_start[a.n_rows] = ok ? (int)n_tok : 0;
+      a.free_head_out[0] = ok ? head + (int)n_blk : head;
+      a.status[0] = status;
+    }
+  }
+  __syncthreads();
+  const int n0 = blockIdx.x * PLAN_TOKENS + tid * 4;
+  if (n0 >= a.n_tok) return;
+  const int total = s_tok[a.n_rows];
+  int row[4], pos[4], slot[4];
+  int r = 0;
+  if (n0 < total) {  // the last row that starts at or before n0: rows without tokens start where the next one does
+    int lo = 0, hi = a.n_rows;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_tok[mid] <= n0) lo = mid; else hi = mid;
+    }
+    r = lo;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int n = n0 + j;
+    row[j] = pos[j] = slot[j] = -1;
+    if (n < total) {
+      while (s_tok[r + 1] <= n) ++r;  // n < total = s_tok[n_rows]: ends at the row that holds n
+      const int kv = s_kv[r], p = kv + n - s_tok[r], b = p / KV8_BLOCK, have = (kv + KV8_BLOCK - 1) / KV8_BLOCK;
+      int* entry = a.table + (size_t)r * a.ld_table + b;
+      const int id = b < have ? *entry : a.free_ids[head + s_blk[r] + b - have];
+      if (p % KV8_BLOCK == 0) *entry = id;
+      row[j] = r;
+      pos[j] = p;
+      slot[j] = (int)((unsigned)id * KV8_BLOCK + p % KV8_BLOCK);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (n0 + j < a.n_tok) {
+      a.tok_row[n0 + j] = row[j];
+      a.tok_pos[n0 + j] = pos[j];
+      a.slots[n0 + j] = slot[j];
+    }
+}
+
+// ---------------------------------------------------------------- append
+// A block's scale is 2^e with the smallest e that keeps its largest magnitude within e4m3's 448 (mx_exp), so a code is
+// e4m3(x / 2^e) and nothing clips.  A block that holds tokens already takes max(e_old, e_new); where that is larger than
+// e_old, its codes c become e4m3(c * 2^(e_old - e)), which is exact except where a code leaves e4m3's normal range: that
+// is why the scales are powers of two.  A token with a key or value that is not finite counts for no scale and is stored
+// as a key of NaN codes and a value of zeros: a query that sees it gets NaN, through its score, and no other query does
+// (a NaN among the values would reach every query of a tile through 0 * NaN).  A new block is zero behind its last token.
+//
+// Memory bound (2 bytes read and 1 written a value).  A workgroup takes one touched block of two heads, a wave the keys or
+// the values of one of them.  The keys' wave loads 16 channels of a key per lane (32 bytes) and stores them as 16; the
+// values' wave loads a channel pair of every key (rows of D values are read whole, 4 bytes a lane) and so holds eight keys
+// of two channels, the stored order, in its own registers: no LDS, no shuffles.
+template <bool BF>
+__device__ __forceinline__ float lo16(uint32_t w) { if constexpr (BF) return lo2f(w); else return lo2h(w); }
+template <bool BF>
+__device__ __forceinline__ float hi16(uint32_t w) { if constexpr (BF) return hi2f(w); else return hi2h(w); }
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+
+// codes of four bytes times f (a power of two <= 1), rounded to nearest even; NaN stays NaN
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float f) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  int o = __builtin_amdgcn_cvt_pk_fp8_f32(lo[0] * f, lo[1] * f, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(hi[0] * f, hi[1] * f, o, true);
+}
+
+__device__ __forceinline__ int wave_max_i(int v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// the largest magnitude of packed maxima (sign bits cleared), as the bits of one 16-bit value
+__device__ __forceinline__ int top16(uint32_t m) { return wave_max_i(max((int)(m & 0xffffu), (int)(m >> 16))); }
+
+template <bool BF, int D>
+__global__ void __launch_bounds__(256) kv8_append_kernel(t2w_kv8_append_args a, int per_row) {
+  constexpr int INF = BF ? 0x7f80 : 0x7c00;  // magnitudes from here on are not finite
+  __shared__ uint32_t s_bad[2][2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hw = wave >> 1;
+  const bool is_v = wave & 1;
+  const int head = blockIdx.y * 2 + hw;
+  const bool live = head < a.pages.kv_heads;
+  int row, at;
+  if (per_row > 0) {
+    row = blockIdx.x / per_row;
+    at = blockIdx.x - row * per_row;
+  } else {
+    row = kv8_find_row(a.row_start, a.n_rows, KV8_BLOCK, 2, blockIdx.x);
+    at = blockIdx.x - (a.row_start[row] / KV8_BLOCK + 2 * row);
+  }
+  const int start = a.row_start[row], n_new = a.row_start[row + 1] - start, total = a.kv_total[row];
+  if (start < 0 || n_new <= 0 || start > a.n_tok - n_new || total < n_new) return;  // nothing new, or a malformed table
+  const int old = total - n_new;
+  const int b_first = old / KV8_BLOCK, b_last = min((total - 1) / KV8_BLOCK, a.width - 1);
+  // a row's last workgroup goes on to its end: rows longer than the caller's bound are still stored whole
+  const bool on = per_row > 0 && at == per_row - 1;
+  for (int b = b_first + at; b <= b_last; ++b) {
+    const int id = a.table[(size_t)row * a.ld_table + b];
+    if ((unsigned)id < (unsigned)a.pages.n_blocks) {
+      const int first = max(old - b * KV8_BLOCK, 0), end = min(total - b * KV8_BLOCK, KV8_BLOCK);  // new tokens [first, end)
+      const int tok0 = start + b * KV8_BLOCK - old;  // token of place 0 (may lie before the row's first one)
+      const size_t page = ((size_t)id * a.pages.kv_heads + head) * (size_t)(KV8_BLOCK * D);
+      constexpr int NC = D / 16, KP = 64 / NC, NP = NC / 2;  // the keys' wave: NC lanes a key, KP keys a pass
+      constexpr int VK = D == 128 ? 32 : 16;                // the values' wave: keys of a lane
+      const int c = lane % NC, kl = lane / NC;
+      const int p = D == 128 ? lane : lane & 31, g0 = D == 128 ? 0 : 2 * (lane >> 5);
+      uint4 xk[NP][2];
+      uint32_t xv[VK];
+      uint32_t m = 0;
+      if (live) {
+        if (!is_v) {
+          const uint16_t* src = (const uint16_t*)a.k + head * D + c * 16;
+#pragma unroll
+          for (int n = 0; n < NP; ++n) {
+            const int t = n * KP + kl;
+            xk[n][0] = xk[n][1] = make_uint4(0, 0, 0, 0);
+            if (t >= first && t < end) {
+              const uint4* q = (const uint4*)(src + (long long)(tok0 + t) * a.ldk);
+              xk[n][0] = q[0];
+              xk[n][1] = q[1];
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NP; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t w[4] = {xk[n][h].x, xk[n][h].y, xk[n][h].z, xk[n][h].w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) m = max_u16x2(m, w[j] & 0x7fff7fffu);
+            }
+        } else {
+          const uint16_t* src = (const uint16_t*)a.v + head * D + 2 * p;
+#pragma unroll
+          for (int j = 0; j < VK; ++j) {
+            const int t = g0 * 8 + j;
+            xv[j] = 0;
+            if (t >= first && t < end) xv[j] = *(const uint32_t*)(src + (long long)(tok0 + t) * a.ldv);
+          }
+#pragma unroll
+          for (int j = 0; j < VK; ++j) m = max_u16x2(m, xv[j] & 0x7fff7fffu);
+        }
+      }
+      int top = top16(m);
+      uint32_t bad = 0;  // tokens of this head with a key (the keys' wave) or value (the values') that is not finite
+      auto off16 = [&](uint32_t w) { return (int)(w & 0x7fffu) >= INF || (int)((w >> 16) & 0x7fffu) >= INF; };
+      if (top >= INF) {
+        if (!is_v) {
+#pragma unroll
+          for (int n = 0; n < NP; ++n) {
+            bool f = false;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) f |= off16(xk[n][h].x) || off16(xk[n][h].y) || off16(xk[n][h].z) || off16(xk[n][h].w);
+            const uint64_t bits = __builtin_amdgcn_ballot_w64(f);
+#pragma unroll
+            for (int q = 0; q < KP; ++q) bad |= ((bits >> (q * NC)) & ((1u << NC) - 1u)) ? 1u << (n * KP + q) : 0u;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < VK; ++j) {
+            const uint64_t bits = __builtin_amdgcn_ballot_w64(off16(xv[j]));
+            if constexpr (D == 128) {
+              bad |= bits ? 1u << j : 0u;
+            } else {
+              bad |= (uint32_t)bits ? 1u << j : 0u;
+              bad |= (uint32_t)(bits >> 32) ? 1u << (16 + j) : 0u;
+            }
+          }
+        }
+      }
+      if (lane == 0) s_bad[hw][is_v] = bad;
+      __syncthreads();
+      bad = s_bad[hw][0] | s_bad[hw][1];
+      __syncthreads();  // before the next block's flags
+      if (bad) {        // the maximum again, without the tokens that are not finite
+        m = 0;
+        if (!is_v) {
+#pragma unroll
+          for (int n = 0; n < NP; ++n)
+            if (!((bad >> (n * KP + kl)) & 1u)) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t w[4] = {xk[n][h].x, xk[n][h].y, xk[n][h].z, xk[n][h].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) m = max_u16x2(m, w[j] & 0x7fff7fffu);
+              }
+            }
+        } else {
+#pragma unroll
+          for (int j = 0; j < VK; ++j) {
+            if ((bad >> (g0 * 8 + j)) & 1u) xv[j] = 0;  // stored as zeros
+            m = max_u16x2(m, xv[j] & 0x7fff7fffu);
+          }
+        }
+        top = top16(m);
+      }
+      if (live) {
+        uint8_t* exps = (is_v ? a.pages.v_exp : a.pages.k_exp) + (size_t)id * a.pages.kv_heads + head;
+        const bool fresh = first == 0;
+        int e = mx_exp(lo16<BF>((uint32_t)top)), shift = 0;
+        if (!fresh) {
+          const int was = (int)*exps - 127;
+          shift = max(e - was, 0);
+          e = max(e, was);
+        }
+        e = min(max(e, -126), 126);
+        const float f = shift < 126 ? __uint_as_float((uint32_t)(127 - shift) << 23) : 0.f;
+        if (lane == 0) *exps = (uint8_t)(e + 127);
+        if (!is_v) {
+          uint4* dst = (uint4*)((uint8_t*)a.pages.k + page) + c * 32;
+#pragma unroll
+          for (int n = 0; n < NP; ++n) {
+            const int t = n * KP + kl;
+            uint4 o = make_uint4(0, 0, 0, 0);
+            if (t >= first && t < end) {
+              uint32_t r[4];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint4 u = xk[n][h];
+                r[2 * h] = mx_pack4(lo16<BF>(u.x), hi16<BF>(u.x), lo16<BF>(u.y), hi16<BF>(u.y), e);
+                r[2 * h + 1] = mx_pack4(lo16<BF>(u.z), hi16<BF>(u.z), lo16<BF>(u.w), hi16<BF>(u.w), e);
+              }
+              o = make_uint4(r[0], r[1], r[2], r[3]);
+              if ((bad >> t) & 1u) o = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
+              dst[t] = o;
+            } else if (fresh) {
+              dst[t] = o;
+            } else if (shift > 0 && t < first) {
+              const uint4 u = dst[t];
+              dst[t] = make_uint4(rescale4(u.x, f), rescale4(u.y, f), rescale4(u.z, f), rescale4(u.w, f));
+            }
+          }
+        } else {
+          uint4* dst = (uint4*)((uint8_t*)a.pages.v + page) + p;
+#pragma unroll
+          for (int gg = 0; gg < VK / 8; ++gg) {
+            const int g = g0 + gg, t0 = g * 8;
+            const bool has_new = t0 < end && t0 + 8 > first, has_old = t0 < first;
+            if (!(fresh || has_new || (has_old && shift > 0))) continue;
+            uint32_t r[4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t* x = xv + gg * 8 + 4 * h;
+              r[h] = mx_pack4(lo16<BF>(x[0]), lo16<BF>(x[1]), lo16<BF>(x[2]), lo16<BF>(x[3]), e);
+              r[2 + h] = mx_pack4(hi16<BF>(x[0]), hi16<BF>(x[1]), hi16<BF>(x[2]), hi16<BF>(x[3]), e);
+            }
+            if (!fresh) {  // the group's other places keep what they hold; its old tokens at the new scale
+              const uint4 u = dst[g * (D / 2)];
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t s = shift > 0 ? rescale4(w[j], f) : w[j];
+                uint32_t o = 0;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                  const int t = t0 + 4 * (j & 1) + y;
+                  const uint32_t mask = 0xffu << (8 * y);
+                  o |= (t < first ? s : t < end ? r[j] : w[j]) & mask;
+                }
+                r[j] = o;
+              }
+            }
+            dst[g * (D / 2)] = make_uint4(r[0], r[1], r[2], r[3]);
+          }
+        }
+      }
+    }
+    if (!on) break;
+  }
+}
+
+}  // namespace
+
+hipError_t kv8_plan(const t2w_kv8_plan_args& a, hipStream_t st) {
+  const int wgs = a.n_tok > 0 ? (a.n_tok + PLAN_TOKENS - 1) / PLAN_TOKENS : 1;
+  hipLaunchKernelGGL(kv8_plan_kernel, dim3(wgs), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+hipError_t kv8_append(const t2w_kv8_append_args& a, hipStream_t st) {
+  if (a.n_tok <= 0 || a.n_rows <= 0) return hipSuccess;
+  // blocks that a row of up to max_new new tokens touches; more than the whole call's list would be: the list
+  const long list = a.n_tok / KV8_BLOCK + 2L * a.n_rows;
+  int per_row = a.max_new > 0 ? (int)(((long)a.max_new + KV8_BLOCK - 2) / KV8_BLOCK + 1) : 0;
+  if (per_row > 0 && (long)per_row * a.n_rows > list) per_row = 0;
+  const dim3 grid((unsigned)(per_row > 0 ? (long)per_row * a.n_rows : list), (unsigned)((a.pages.kv_heads + 1) / 2));
+#define T2W_KV8_APPEND(BF, D) hipLaunchKernelGGL((kv8_append_kernel<BF, D>), grid, dim3(256), 0, st, a, per_row)
+  if (a.dtype == T2W_KV8_BF16) {
+    if (a.pages.head_dim == 64) T2W_KV8_APPEND(true, 64); else T2W_KV8_APPEND(true, 128);
+  } else {
+    if (a.pages.head_dim == 64) T2W_KV8_APPEND(false, 64); else T2W_KV8_APPEND(false, 128);
+  }
+#undef T2W_KV8_APPEND
+  return hipGetLastError();
+}
+
+}  // namespace t2w

@@ -1,0 +1,605 @@
+"""The paged 8-bit key/value cache on the GPU against the float64 oracle: tables, append, attention, and a run of them.
+
+Codes, exponents and tables have to be equal: a scale is a power of two, so x / 2^e is exact and rounds the same way in
+every precision.  Attention's bound per output, with u = 2^-24 (an fp32 rounding), eps / 2 the type's: the scores' fp32
+dot products of D exact products are off by at most (D + 2) u times their absolute sums, the scaled score, its
+difference from the maximum and exp2 add a few u times the score, and a relative error of p_j by that much moves
+sum p v / sum p by at most twice that times sum p |v|; a probability rounded to 16 bits for the matrix unit is off by
+2^-11 at most, the sums by another (32 + D) u at any length that the tests have; the output's own rounding is eps / 2 of it.
+"""
+
+import random
+
+import numpy as np
+import pytest
+import torch
+
+import t2w_amd  # noqa: F401
+from oracle import kv8 as ok
+from t2w_amd import kv8
+
+pytestmark = pytest.mark.gpu
+BF, FP = torch.bfloat16, torch.float16
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def need(n):
+    return -(-n // 32)
+
+
+def host(pages):
+    """Code values (not scaled) and exponents as the oracle's arrays."""
+    unit = kv8.KV8Pages(pages.k, pages.v, torch.full_like(pages.k_exp, 127), torch.full_like(pages.v_exp, 127))
+    k, v = unit.values()
+    return (k.cpu().double().numpy(), v.cpu().double().numpy(), pages.k_exp.cpu().numpy().astype(int) - 127,
+            pages.v_exp.cpu().numpy().astype(int) - 127)
+
+
+def scaled(pages):
+    k, v = pages.values()
+    return k.cpu().double().numpy(), v.cpu().double().numpy()
+
+
+def random_pages(nb, g, d, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    p = kv8.KV8Pages.empty(nb, g, d)
+    for t in (p.k, p.v):
+        t.copy_(torch.randn(t.shape, generator=gen, device="cuda").mul(60).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8))
+    p.k_exp.copy_(torch.randint(119, 124, p.k_exp.shape, generator=gen, device="cuda"))
+    p.v_exp.copy_(torch.randint(116, 126, p.v_exp.shape, generator=gen, device="cuda"))
+    return p
+
+
+def random_table(totals, extra, seed, spare=2):
+    """A table of the rows' blocks in random order, the entries behind them invalid; the block count of the pages."""
+    n = sum(need(t) for t in totals) + spare
+    ids = list(range(n))
+    random.Random(seed).shuffle(ids)
+    width = max([need(t) for t in totals] + [1]) + extra
+    t = np.full((len(totals), width), -7, np.int32)
+    for r, x in enumerate(totals):
+        for b in range(need(x)):
+            t[r, b] = ids.pop()
+    return t, n
+
+
+def starts(new):
+    return [0] + np.cumsum(new).tolist()
+
+
+# --- tables -----------------------------------------------------------------------------------------------------------
+
+def run_plan(kv, new, width, n_free, head, n_tok, seed=0, pad=0):
+    g = np.random.default_rng(seed)
+    table = g.integers(0, 5000, (len(kv), width + pad)).astype(np.int32)
+    free = g.permutation(100000)[:n_free].astype(np.int32)
+    want = ok.plan(kv, new, table[:, :width], free, head, n_tok)
+    plan = kv8.KV8Plan(len(kv), n_tok)
+    dt = torch.from_numpy(table.copy()).cuda()
+    plan.build(ints(kv), ints(new), dt[:, :width], torch.from_numpy(free).cuda(), ints([head]))
+    got = [plan.kv_total, plan.row_start, plan.tok_row, plan.tok_pos, plan.slots, plan.free_head[0], plan.status[0], dt[:, :width]]
+    for name, a, b in zip(("kv_total", "row_start", "tok_row", "tok_pos", "slots", "free_head", "status", "table"), got, want):
+        assert np.array_equal(a.cpu().numpy(), np.asarray(b)), name
+    assert np.array_equal(dt[:, width:].cpu().numpy(), table[:, width:])
+    return plan, want
+
+
+@pytest.mark.parametrize("rows", [1, 2, 63, 64, 65, 255, 256, 257, 1000, 4096])
+@pytest.mark.parametrize("most", [1, 70])
+def test_plan_rows(dev, rows, most):
+    rng = random.Random(rows * 7 + most)
+    kv = [rng.choice((0, 1, 31, 32, 33, 64, rng.randrange(500))) for _ in range(rows)]
+    new = [rng.choice((0, 1, 31, 32, 33, rng.randrange(most + 1))) if most > 1 else rng.randrange(2) for _ in range(rows)]
+    blocks = sum(need(a + b) - need(a) for a, b in zip(kv, new))
+    run_plan(kv, new, 20, blocks + 9, 9, sum(new) + rng.randrange(3), seed=rows, pad=rows % 3)
+
+
+def test_plan_lengths(dev):
+    run_plan([0], [0], 1, 0, 0, 0)
+    run_plan([0], [0], 1, 0, 0, 5)
+    run_plan([5], [1], 1, 0, 0, 1)
+    run_plan([32], [1], 2, 1, 0, 1)
+    run_plan([0, 0, 40000, 7], [0, 70001, 3, 0], 4000, 3000, 1, 70100)
+    run_plan([31] * 40, [1] * 40, 1, 0, 0, 1024)  # nothing to take
+
+
+@pytest.mark.parametrize("kv,new,width,n_free,head,n_tok,status", [
+    ([3, -1], [1, 1], 4, 9, 0, 8, 1), ([3, 4], [1, -2], 4, 9, 0, 8, 1), ([0, 0], [5, 4], 4, 9, 0, 8, 2), ([100, 0], [29, 1], 4, 9, 0, 64, 4),
+    ([0, 0], [33, 1], 4, 5, 3, 64, 8), ([0], [1], 4, 5, 6, 64, 8), ([0], [1], 4, 5, -1, 64, 8), ([-1, 0], [40, 90], 2, 0, 0, 64, 15),
+    ([2 ** 31 - 1, 5], [2 ** 31 - 1, 2 ** 31 - 1], 4, 9, 0, 64, 14)], ids=str)
+def test_plan_that_cannot_be_served(dev, kv, new, width, n_free, head, n_tok, status):
+    """Nothing is taken, the table stays, no row has new tokens, and ``check`` says what is wrong."""
+    plan, want = run_plan(kv, new, width, n_free, head, n_tok)
+    assert want[6] == status
+    with pytest.raises(RuntimeError, match="kv8 plan"):
+        plan.check()
+
+
+# --- append -------------------------------------------------------------------------------------------------------------
+
+def check_append(pages, k, v, table, new, totals, max_new=0):
+    want = host(pages)
+    ok.append(*want, k.double().cpu().numpy(), v.double().cpu().numpy(), table, starts(new), totals)
+    kv8.append(pages, k, v, torch.from_numpy(table).cuda(), ints(starts(new)), ints(totals), max_new=max_new)
+    for name, a, b in zip(("k", "v", "k_exp", "v_exp"), host(pages), want):
+        assert np.array_equal(a, b, equal_nan=True), name
+
+
+def new_kv(n, g, d, dt, seed, spread=3):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    def one():
+        x = torch.randn(n, g, d, generator=gen, device="cuda")
+        return (x * torch.exp2(spread * torch.randn(n, 1, 1, generator=gen, device="cuda"))).to(dt)
+    return one(), one()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("g", [1, 2, 5])
+@pytest.mark.parametrize("bound", [0, 70, 3])
+def test_append_lengths(dev, d, dt, g, bound):
+    """Old and new lengths around the block's, rows without new tokens; with the longest row's length, none and one that
+    is too small."""
+    old = [0, 0, 1, 31, 32, 33, 40, 63, 64, 5, 17, 30]
+    new = [1, 70, 1, 1, 1, 31, 0, 2, 33, 27, 64, 3]
+    totals = [a + b for a, b in zip(old, new)]
+    table, nb = random_table(totals, 1, seed=g)
+    k, v = new_kv(sum(new), g, d, dt, seed=d + g)
+    check_append(random_pages(nb, g, d, g), k, v, table, new, totals, max_new=bound)
+
+
+@pytest.mark.parametrize("rows", [63, 64, 65, 300, 4096])
+def test_append_many_rows(dev, rows):
+    rng = random.Random(rows)
+    old = [rng.randrange(40) for _ in range(rows)]
+    new = [rng.choice((0, 1, 1, 2, 35)) if rows < 4096 else rng.randrange(2) for _ in range(rows)]
+    totals = [a + b for a, b in zip(old, new)]
+    table, nb = random_table(totals, 0, seed=1)
+    k, v = new_kv(sum(new), 1, 64, BF, seed=rows)
+    pages = random_pages(nb, 1, 64, 2)
+    for bound in (0, max(new)):
+        check_append(pages, k, v, table, new, totals, max_new=bound)  # the second time over what the first one stored
+
+
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_append_strided_and_extremes(dev, dt):
+    """Slices of a joint projection; zeros, subnormals, the type's largest values, negative zeros."""
+    n, g, d = 40, 3, 64
+    x = torch.randn(n, 11, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(dt)
+    k, v = x[:, 4:7], x[:, 8:11]
+    k[3], k[4], v[5], v[33:] = 0, torch.finfo(dt).max, torch.finfo(dt).smallest_normal / 4, 0
+    k[6], v[7] = -0.0, -torch.finfo(dt).max
+    old, new = [0, 7, 30], [33, 2, 5]
+    totals = [a + b for a, b in zip(old, new)]
+    table, nb = random_table(totals, 0, seed=3)
+    check_append(random_pages(nb, g, d, 5), k, v, table, new, totals)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("factor", [2.0 ** -12, 1.0, 2.0 ** 6, 2.0 ** 40])
+def test_append_rescales_the_block(dev, d, factor):
+    """Token by token into one block, each step ``factor`` larger or smaller: the old codes follow the scale."""
+    pages = random_pages(2, 2, d, 1)
+    table = np.array([[1]], np.int32)
+    for t in range(33 - 1):
+        k, v = new_kv(1, 2, d, BF, seed=t)
+        s = factor ** min(t, 3)
+        check_append(pages, (k * s).to(BF), (v * s).to(BF), table, [1], [t + 1], max_new=1)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_append_not_finite(dev, d, dt):
+    """Infinities and NaN in keys or values, one head of them, first and last channels and tokens, a whole block."""
+    old, new = [0, 9, 32], [40, 20, 3]
+    totals = [a + b for a, b in zip(old, new)]
+    table, nb = random_table(totals, 0, seed=2)
+    k, v = new_kv(sum(new), 3, d, dt, seed=1)
+    k[0, 0, 0] = float("inf")
+    v[31, 1, d - 1] = float("nan")
+    k[33, 2, 17], v[33, 2, 5] = float("nan"), float("-inf")
+    v[45, 0, 3] = float("-inf")
+    k[60:63, 1] = float("nan")
+    check_append(random_pages(nb, 3, d, 4), k, v, table, new, totals)
+
+
+def test_append_skips_foreign_blocks(dev):
+    """Ids outside the pages and rows past their table store nothing; the others are stored."""
+    old, new = [0, 3, 0], [40, 2, 33]
+    totals = [a + b for a, b in zip(old, new)]
+    table = np.array([[-1, 2], [5, 0], [1, 2 ** 31 - 1]], np.int32)
+    k, v = new_kv(sum(new), 2, 64, BF, seed=1)
+    check_append(random_pages(5, 2, 64, 1), k, v, table, new, totals)
+    check_append(random_pages(5, 2, 64, 1), k, v, table, new, totals, max_new=40)
+    wide = np.array([[3], [4], [1]], np.int32)  # 40 and 33 tokens in one block's width: their first 32
+    pages = random_pages(5, 2, 64, 1)
+    want = host(pages)
+    for r, t0 in ((0, 0), (2, 42)):
+        ok.append(*want, k[t0:t0 + 32].double().cpu().numpy(), v[t0:t0 + 32].double().cpu().numpy(), wide[r:r + 1], [0, 32], [32])
+    ok.append(*want, k[40:42].double().cpu().numpy(), v[40:42].double().cpu().numpy(), wide[1:2], [0, 2], [5])
+    kv8.append(pages, k, v, torch.from_numpy(wide).cuda(), ints(starts(new)), ints(totals))
+    for a, b in zip(host(pages), want):
+        assert np.array_equal(a, b)
+
+
+# --- attention ------------------------------------------------------------------------------------------------------------
+
+def attn_bound(o, mag, top, d, dt):
+    u = 2.0 ** -24
+    rel_p = 2 * ((d + 2) * u * top + 8 * u * (top * 1.4427 + 2) + 2.0 ** -11) + 2 * (32 + d) * u
+    return torch.finfo(dt).eps / 2 * np.abs(o) * 1.01 + rel_p[:, :, None] * mag * 1.01 + 1e-30
+
+
+def check_attention(q, pages, table, new, totals, chunk, scale=None, **kw):
+    d = pages.head_dim
+    scale = scale or d ** -0.5
+    k, v = scaled(pages)
+    o, mag, top = ok.attention(q.double().cpu().numpy(), k, v, table, starts(new), totals, scale, chunk)
+    out = kv8.attention(q, pages, torch.from_numpy(table).cuda(), ints(starts(new)), ints(totals), scale=scale, chunk=chunk, **kw)
+    torch.cuda.synchronize()
+    n = sum(new)
+    got = out[:n].double().cpu().numpy()
+    bound = attn_bound(o, mag, top, d, q.dtype)[:n]
+    assert np.isfinite(got).all()
+    worst = float((np.abs(got - o[:n]) / bound).max()) if n else 0.0
+    assert worst <= 1, worst
+    return out
+
+
+def queries(n, h, d, dt, seed):
+    return torch.randn(n, h, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)).to(dt)
+
+
+HEADS = [(1, 1), (4, 4), (16, 16), (6, 2), (8, 2), (7, 1), (14, 2), (32, 2)]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("h,g", HEADS)
+def test_attention_steps(dev, d, dt, h, g):
+    """One token a row, caches from that token alone to several hundred, rows without a token."""
+    totals = [1, 2, 31, 32, 33, 64, 65, 200, 417, 7]
+    new = [1, 1, 1, 1, 1, 1, 0, 1, 1, 0]
+    table, nb = random_table(totals, 1, seed=h)
+    pages = random_pages(nb, g, d, seed=d)
+    q = queries(sum(new), h, d, dt, seed=g)
+    for bounds in ({"max_new": 1, "max_kv": 417}, {"max_new": 1}, {}):
+        check_attention(q, pages, table, new, totals, 1, **bounds)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("h,g", [(2, 2), (6, 2), (7, 1), (16, 1)])
+@pytest.mark.parametrize("chunk", [0, 1, 3, 25])
+def test_attention_windows(dev, d, dt, h, g, chunk):
+    """Windows of several lengths behind caches of several lengths."""
+    old = [0, 10, 32, 100, 63, 5, 0, 250]
+    new = [1, 50, 33, 2, 64, 0, 70, 17]
+    totals = [a + b for a, b in zip(old, new)]
+    table, nb = random_table(totals, 0, seed=chunk)
+    pages = random_pages(nb, g, d, seed=d + chunk)
+    q = queries(sum(new), h, d, dt, seed=g)
+    for bounds in ({"max_new": 70, "max_kv": max(totals)}, {}):
+        check_attention(q, pages, table, new, totals, chunk, **bounds)
+
+
+@pytest.mark.parametrize("new", [2, 4, 5, 9, 16, 17, 31])
+@pytest.mark.parametrize("h,g", [(4, 4), (8, 2), (14, 2)])
+def test_attention_few_tokens(dev, new, h, g):
+    """A few tokens a row (drafts being checked): the packed rows of a tile around its sizes, long caches."""
+    totals = [new, 300, 1500, 40 + new]
+    table, nb = random_table(totals, 0, seed=new)
+    pages = random_pages(nb, g, 128, seed=new)
+    q = queries(4 * new, h, 128, BF, seed=g)
+    check_attention(q, pages, table, [new] * 4, totals, 1, max_new=new, max_kv=1500)
+
+
+@pytest.mark.parametrize("d,dt", [(64, BF), (128, FP)])
+@pytest.mark.parametrize("rows,new,old", [(1, 1, 5000), (2, 3, 3000), (1, 130, 900), (1, 200, 0), (3, 129, 64)])
+def test_attention_long(dev, d, dt, rows, new, old):
+    """Key lists that few workgroups have to themselves: split and joined."""
+    totals = [old + new - 37 * r for r in range(rows)]
+    table, nb = random_table(totals, 3, seed=new)
+    pages = random_pages(nb, 2, d, seed=1)
+    q = queries(rows * new, 4, d, dt, seed=2)
+    for chunk in (0, 1):
+        for bounds in ({"max_new": new, "max_kv": max(totals)}, {"max_new": new, "max_kv": 100}, {"max_new": new, "max_kv": 1 << 20}, {}):
+            check_attention(q, pages, table, [new] * rows, totals, chunk, **bounds)
+
+
+@pytest.mark.parametrize("rows", [65, 500, 4096])
+def test_attention_many_rows(dev, rows):
+    rng = random.Random(rows)
+    new = [rng.choice((0, 1, 2)) if rows < 4096 else int(r % 64 == 5) for r in range(rows)]
+    totals = [n + rng.randrange(60) for n in new]
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, 1, 64, seed=3)
+    q = queries(sum(new), 2, 64, BF, seed=4)
+    for bounds in ({"max_new": 2, "max_kv": 62}, {}):
+        check_attention(q, pages, table, new, totals, 1, **bounds)
+
+
+@pytest.mark.parametrize("new", [1, 40, 140])
+def test_attention_scores_of_any_size(dev, new):
+    """Large scores (one key takes all), and scores far below zero everywhere: no underflow to an empty row."""
+    totals = [new + 100, new]
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, 2, 64, seed=5)
+    q = queries(2 * new, 4, 64, BF, seed=6)
+    check_attention(q * 16, pages, table, [new] * 2, totals, 1)
+    pages.k.bitwise_and_(0x7F)  # keys of one sign, queries of the other
+    check_attention(-(q.abs() * 1024).to(BF), pages, table, [new] * 2, totals, 1)
+    pages.k_exp.add_(60)  # scores of 2^60 and more: the maximum alone counts
+    out = kv8.attention(-q.abs(), pages, torch.from_numpy(table).cuda(), ints([0, new, 2 * new]), ints(totals), scale=1.0, chunk=1)
+    assert torch.isfinite(out).all() and (out.abs().amax((1, 2)) > 0).all()
+
+
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_scales_of_any_size(dev, new, dt):
+    """Value scales that differ by 2^20 between blocks, growing and falling along the row."""
+    totals = [new + 200, new + 90]
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, 2, 64, seed=5)
+    for r in range(2):
+        for b in range(need(totals[r])):
+            pages.v_exp[table[r, b]] = 112 + (7 * b % 21 if r else 3 * b)
+    q = queries(2 * new, 2, 64, dt, seed=6)
+    check_attention(q, pages, table, [new] * 2, totals, 0)
+
+
+@pytest.mark.parametrize("new", [2, 40, 140])
+def test_attention_empty_rows(dev, new):
+    """Rows whose cache is shorter than their queries (kv_total < new): the first ones see nothing and get zeros."""
+    new_l, totals = [new, new, new], [new - 1, 0, new // 2]
+    table, nb = random_table(totals, 1, seed=1)
+    pages = random_pages(nb, 2, 64, seed=5)
+    q = queries(3 * new, 4, 64, BF, seed=6)
+    for chunk in (0, 1, 7):
+        for bounds in ({"max_new": new}, {}):
+            check_attention(q, pages, table, new_l, totals, chunk, **bounds)
+
+
+@pytest.mark.parametrize("new", [1, 40, 140])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_ignores_what_lies_behind(dev, new, d):
+    """NaN codes and E8M0 NaN scales behind the rows' last tokens and in blocks of nobody, ids behind the rows' tables."""
+    totals = [new + 100, new + 11, new]
+    table, nb = random_table(totals, 2, seed=1)
+    pages = random_pages(nb, 2, d, seed=5)
+    used = sorted(x for r, t in enumerate(totals) for x in table[r, :need(t)])
+    for b in set(range(nb)) - set(used):
+        pages.k[b], pages.v[b], pages.k_exp[b], pages.v_exp[b] = 255, 255, 255, 255
+    k, v = pages.k, pages.v
+    q = queries(3 * new, 4, d, BF, seed=6)
+    clean = check_attention(q, pages, table, [new] * 3, totals, 1).clone()
+    for r, t in enumerate(totals):
+        if t % 32:
+            b = int(table[r, t // 32])
+            k[b, :, :, t % 32:] = 0x7F
+            vv = v[b].permute(0, 1, 4, 2, 3).reshape(2, 32, d // 2, 2).clone()
+            vv[:, t % 32:] = 0xFF
+            v[b] = vv.reshape(2, 4, 8, d // 2, 2).permute(0, 1, 3, 4, 2)
+    for bounds in ({"max_new": new, "max_kv": max(totals)}, {"max_new": new}, {}):
+        out = kv8.attention(q, pages, torch.from_numpy(table).cuda(), ints(starts([new] * 3)), ints(totals), scale=d ** -0.5, chunk=1, **bounds)
+        assert torch.isfinite(out).all()
+    assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("new", [1, 40, 140])
+def test_attention_nan_tokens_reach_only_who_sees_them(dev, new):
+    """A NaN key (stored by the append for a token that is not finite) in causal windows: earlier queries are untouched."""
+    old = 70
+    totals = [old + new] * 2
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, 2, 64, seed=5)
+    q = queries(2 * new, 4, 64, BF, seed=6)
+    args = (torch.from_numpy(table).cuda(), ints(starts([new] * 2)), ints(totals))
+    clean = kv8.attention(q, pages, *args, scale=0.125, chunk=1)
+    at = old + new // 2
+    pages.k[int(table[0, at // 32]), 1, :, at % 32] = 0x7F
+    out = kv8.attention(q, pages, *args, scale=0.125, chunk=1)
+    hit = torch.zeros(2 * new, 4, dtype=torch.bool, device="cuda")
+    hit[new // 2:new, 2:] = True
+    assert out[hit].isnan().all() and torch.equal(out[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("new", [1, 40, 140])
+def test_attention_malformed_rows(dev, new):
+    """Block ids outside the pages and rows longer than their table: NaN for who sees them, the others as ever."""
+    totals = [new + 100] * 4
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, 2, 64, seed=5)
+    q = queries(4 * new, 2, 64, BF, seed=6)
+    start = ints(starts([new] * 4))
+    clean = kv8.attention(q, pages, torch.from_numpy(table).cuda(), start, ints(totals), scale=0.125, chunk=1)
+    table[1, 1] = nb
+    table[2, 0] = -1
+    out = kv8.attention(q, pages, torch.from_numpy(table).cuda(), start, ints(totals[:3] + [table.shape[1] * 32 + 1]), scale=0.125, chunk=1)
+    assert torch.equal(out[:new], clean[:new]) and out[new:].isnan().all()
+    if new > 1:  # a row of more new tokens than the bound says: NaN where the bound chose the kernel
+        out = kv8.attention(q[:new + 1], pages, torch.from_numpy(table[:2] * 0).cuda(), ints([0, new, new + 1]), ints(totals[:2]), scale=0.125, chunk=1,
+                            max_new=1)
+        assert (out[:new].isnan().all() or torch.isfinite(out[:new]).all()) and torch.isfinite(out[new]).all()
+
+
+@pytest.mark.parametrize("new", [1, 40, 140])
+def test_attention_strides_and_rows_behind(dev, new):
+    """q a slice of a joint projection, out a slice of a larger buffer; rows behind the last token stay; a caller's
+    workspace."""
+    totals = [new + 50, new]
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, 2, 64, seed=5)
+    qkv = torch.randn(2 * new + 3, 9, 64, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(BF)
+    buf = torch.full((2 * new + 3, 7, 64), 5.0, device="cuda", dtype=BF)
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    out = check_attention(qkv[:, 2:6], pages, table, [new] * 2, totals, 1, out=buf[:, 1:5], workspace=ws)
+    assert (out[2 * new:] == 5).all() and (buf[:, 0] == 5).all() and (buf[:, 5:] == 5).all()
+    again = kv8.attention(qkv[:, 2:6].contiguous(), pages, torch.from_numpy(table).cuda(), ints(starts([new] * 2)), ints(totals), scale=0.125, chunk=1)
+    assert torch.equal(again[:2 * new], out[:2 * new])
+
+
+def test_attention_same_bits_every_time(dev):
+    totals = [3000, 1700, 4000, 60]
+    for new in (1, 3, 60):
+        table, nb = random_table(totals, 0, seed=1)
+        pages = random_pages(nb, 2, 128, seed=5)
+        q = queries(4 * new, 8, 128, BF, seed=6)
+        args = (q, pages, torch.from_numpy(table).cuda(), ints(starts([new] * 4)), ints(totals))
+        first = kv8.attention(*args, scale=0.1, chunk=1, max_new=new, max_kv=4000)
+        for _ in range(5):
+            assert torch.equal(kv8.attention(*args, scale=0.1, chunk=1, max_new=new, max_kv=4000), first)
+
+
+def test_attention_on_other_streams(dev):
+    """Two calls at once on two streams, each with the workspace it takes for itself."""
+    totals = [5000, 4100]
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, 2, 128, seed=5)
+    args = (pages, torch.from_numpy(table).cuda(), ints([0, 1, 2]), ints(totals))
+    qs = [queries(2, 8, 128, BF, seed=s) for s in range(2)]
+    want = [kv8.attention(q, *args, scale=0.1, max_new=1, max_kv=5000) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    for _ in range(10):
+        got = []
+        for s, q in zip(streams, qs):
+            with torch.cuda.stream(s):
+                got.append(kv8.attention(q, *args, scale=0.1, max_new=1, max_kv=5000))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# --- a run of them ----------------------------------------------------------------------------------------------------------
+
+class Server:
+    """A tiny server's loop over the three calls, and the same with the oracle."""
+
+    def __init__(self, rows, h, g, d, dt, room, n_tok, seed=0):
+        self.h, self.g, self.d, self.dt, self.rows = h, g, d, dt, rows
+        self.nb = rows * room
+        self.pages = random_pages(self.nb, g, d, seed=9)
+        self.table = torch.full((rows, room), -1, dtype=torch.int32, device="cuda")
+        self.free = torch.randperm(self.nb, generator=torch.Generator().manual_seed(seed)).int().cuda()
+        self.kv, self.head = ints([0] * rows), ints([0])
+        self.plan = kv8.KV8Plan(rows, n_tok)
+        self.new = ints([0] * rows)
+        self.x = torch.zeros(n_tok, h + 2 * g, d, device="cuda", dtype=dt)
+        self.out = torch.zeros(n_tok, h, d, device="cuda", dtype=dt)
+
+    def step(self, max_new, max_kv):
+        """All on the GPU; the next step's lengths replace this one's at the end."""
+        p, h, g = self.plan, self.h, self.g
+        p.build(self.kv, self.new, self.table, self.free, self.head)
+        kv8.append(self.pages, self.x[:, h:h + g], self.x[:, h + g:], self.table, p.row_start, p.kv_total, max_new=max_new)
+        kv8.attention(self.x[:, :h], self.pages, self.table, p.row_start, p.kv_total, scale=self.d ** -0.5, chunk=1, max_new=max_new, max_kv=max_kv,
+                      out=self.out)
+        self.kv.copy_(p.kv_total)
+        self.head.copy_(p.free_head)
+
+    def check(self, state, new):
+        """The step's results against the oracle, which goes on from its own state."""
+        kc, vc, ke, ve, table, kv, head = state
+        total, start, _, _, slots, head, status, table = ok.plan(kv, new, table, self.free.cpu().numpy(), head, self.plan.n_tok)
+        assert status == 0 and int(self.plan.status) == 0
+        assert self.plan.slots.tolist() == slots and np.array_equal(self.table.cpu().numpy(), table) and int(self.head) == head
+        x = self.x.double().cpu().numpy()
+        h, g = self.h, self.g
+        ok.append(kc, vc, ke, ve, x[:, h:h + g], x[:, h + g:], table, start, total)
+        for a, b in zip(host(self.pages), (kc, vc, ke, ve)):
+            assert np.array_equal(a, b)
+        o, mag, top = ok.attention(x[:, :h], kc * np.exp2(ke)[..., None, None], vc * np.exp2(ve)[..., None, None], table, start, total, self.d ** -0.5, 1)
+        n = sum(new)
+        got = self.out.double().cpu().numpy()[:n]
+        assert (np.abs(got - o[:n]) <= attn_bound(o, mag, top, self.d, self.dt)[:n]).all()
+        return kc, vc, ke, ve, table, total, head
+
+    def state(self):
+        return (*(x.astype(float) for x in host(self.pages)), self.table.cpu().numpy(), [0] * self.rows, 0)
+
+
+@pytest.mark.parametrize("h,g,d,dt", [(4, 4, 64, BF), (8, 2, 128, FP)])
+def test_prompts_then_steps(dev, h, g, d, dt):
+    """Ragged prompts, then steps, some of rows that rest, then a second prompt chunk: every step against the oracle."""
+    s = Server(3, h, g, d, dt, room=8, n_tok=160)
+    state = s.state()
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for new in ([70, 33, 1], [1, 1, 1], [1, 0, 1], [0, 0, 0], [1, 1, 1], [2, 40, 31], [1, 1, 1]):
+        s.x.copy_(torch.randn(s.x.shape, generator=gen, device="cuda"))
+        s.new.copy_(ints(new))
+        s.step(max(new), 256)
+        torch.cuda.synchronize()
+        state = s.check(state, new)
+
+
+def test_graph_of_a_step(dev):
+    """One captured graph serves steps of other lengths; between the replays the program works on and waits.  Every replay
+    is checked against the oracle."""
+    s = Server(3, 8, 2, 64, BF, room=6, n_tok=96)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        s.step(0, 192)  # no new token: nothing changes
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s.step(0, 192)
+    state = s.state()
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    for new in ([40, 3, 0], [1, 1, 1], [1, 1, 64], [0, 1, 1], [33, 1, 30]):
+        s.x.copy_(torch.randn(s.x.shape, generator=gen, device="cuda"))
+        s.new.copy_(ints(new))
+        graph.replay()
+        torch.cuda.synchronize()
+        state = s.check(state, new)
+        torch.randn(1 << 20, device="cuda").sum().item()
+
+
+def test_two_graphs(dev):
+    """Two captured graphs of long steps, replayed in turn and checked every time: their workspaces are their own."""
+    totals = [5000, 4100]
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, 2, 128, seed=5)
+    args = (pages, torch.from_numpy(table).cuda(), ints([0, 1, 2]), ints(totals))
+    qs = [queries(2, 8, 128, BF, seed=s) for s in range(2)]
+    want = [kv8.attention(q, *args, scale=0.1, max_new=1, max_kv=5000) for q in qs]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for q in qs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(kv8.attention(q, *args, scale=0.1, max_new=1, max_kv=5000))
+        graphs.append(g)
+    for k in range(6):
+        outs[k % 2].zero_()
+        graphs[k % 2].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[k % 2], want[k % 2])
+
+
+def test_cache_error_against_16_bits(dev):
+    """What the 8 bits cost: attention over the cache against attention over the keys and values themselves.  A code is off
+    by at most 2^-4 of its value (and 2^-10 below e4m3's normal range, where the block's scale is at most 2^-8 of its
+    largest value doubled), so with E = 2^-4 a score is off by at most E scale sum |q k| =: ds, a probability by a factor in
+    exp(+-2 ds) and an output by E sum p |v| + (exp(2 ds) - 1) (1 + E) sum p |v|."""
+    n, h, g, d = 200, 8, 2, 64
+    s = Server(1, h, g, d, BF, room=8, n_tok=n)
+    s.x.copy_(torch.randn(s.x.shape, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda"))
+    s.new.copy_(ints([n]))
+    s.step(n, 256)
+    x = s.x.double().cpu()
+    k, v = x[:, h:h + g].repeat_interleave(h // g, 1), x[:, h + g:].repeat_interleave(h // g, 1)
+    p = torch.einsum("nhd,mhd->hnm", x[:, :h], k) * d ** -0.5
+    p = torch.softmax(p.masked_fill(torch.ones(n, n).triu(1).bool(), -torch.inf), -1)
+    ref = torch.einsum("hnm,mhd->nhd", p, v)
+    err = (s.out.double().cpu() - ref).abs()
+    low = 2.0 ** -10 * 2.0 ** -7  # a subnormal code's error, of the block's largest value
+    E = 2.0 ** -4
+    ak, av = k.abs() + low / E * k.abs().max(), v.abs() + low / E * v.abs().max()
+    ds = E * torch.einsum("nhd,mhd->hnm", x[:, :h].abs(), ak).amax(-1).T[..., None] * d ** -0.5
+    pv = torch.einsum("hnm,mhd->nhd", p, av)
+    bound = E * pv + (torch.exp(2 * ds) - 1) * (1 + E) * pv + 2.0 ** -8 * ref.abs() + 2.0 ** -9 * pv
+    assert (err <= bound).all()
