@@ -2,103 +2,521 @@
 // i sees, key and value codes times their blocks' scales.  Block format: kv8_internal.h.
 #include "kv8_internal.h"
 
+#include <type_traits>
+
 namespace t2w {
 
 namespace {
 
-// One wave per (token, head), 32 keys of a block at a time: lane (key, half) sums every other 16-channel chunk of its key
-// in fp32, the wave keeps the running maximum and sum, and each lane the output of one or two channels.
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+// Work of one launch.  A tile is `tt` tokens of a row, its packed rows (token, query head of the group), m = token * G +
+// head, sharing one key head; a part is a run of key blocks of a tile's row.
+struct KV8Split {
+  int G;        // query heads of a key head
+  int tt;       // tokens of a tile
+  int per_row;  // tile slots of a row, 0: tiles listed over all rows (kv8_find_row)
+  int n_tiles;  // tile slots of the call
+  int bps;      // key blocks of a part, more where a row would have over `parts` of them
+  int parts;    // most parts of a tile; 1: the kernel writes the outputs itself
+};
+
+// Workspace of split calls, parts joined by kv8_join_kernel: the parts' outputs, fp32 [tile slot][kv head][part][m][D],
+// then (maximum, sum) [tile slot][kv head][part][m][2].
+__host__ __device__ __forceinline__ size_t part_rows(const KV8Split& s, int kv_heads) {
+  return (size_t)s.n_tiles * kv_heads * s.parts * (s.tt * s.G);
+}
+
+struct Tile {
+  int row, start, i0, rows;  // its row, the row's first token, the tile's first token in it, packed rows
+  int cached, n_new, total;  // total = cached + n_new keys; cached < 0 where the row has fewer keys than queries
+  int end;                   // keys [0, end) are visible to some query of the tile
+  bool bad;                  // the row is longer than its table, or than max_new tokens: NaN outputs
+};
+
+// The tile of a slot, by the whole wave; false: nothing there.
+__device__ __forceinline__ bool find_tile(const t2w_kv8_attention_args& a, const KV8Split& s, int slot, Tile& t) {
+  int at;
+  if (s.per_row > 0) {
+    t.row = slot / s.per_row;
+    at = slot - t.row * s.per_row;
+  } else {
+    t.row = kv8_find_row(a.row_start, a.n_rows, s.tt, 1, slot);
+    at = slot - (a.row_start[t.row] / s.tt + t.row);
+  }
+  t.start = a.row_start[t.row];
+  t.n_new = a.row_start[t.row + 1] - t.start;
+  t.total = a.kv_total[t.row];
+  t.i0 = at * s.tt;
+  if (t.start < 0 || t.n_new <= 0 || t.start > a.n_tok - t.n_new || at < 0 || t.i0 >= t.n_new) return false;
+  t.bad = t.total < 0 || t.total > a.width * KV8_BLOCK || (s.per_row > 0 && t.n_new > s.per_row * s.tt);
+  const int n = min(s.tt, t.n_new - t.i0);
+  t.rows = n * s.G;
+  t.cached = t.total - t.n_new;
+  const int last = t.i0 + n - 1;
+  const int seen = a.chunk > 0 ? (int)min((long long)t.n_new, ((long long)(last / a.chunk) + 1) * a.chunk) : t.n_new;
+  t.end = max(t.cached + seen, 0);
+  return true;
+}
+
+// keys that query i (a token of the tile's row) sees
+__device__ __forceinline__ int seen_by(const t2w_kv8_attention_args& a, const Tile& t, int i) {
+  const int seen = a.chunk > 0 ? (int)min((long long)t.n_new, ((long long)(i / a.chunk) + 1) * a.chunk) : t.n_new;
+  return max(t.cached + seen, 0);
+}
+
+// parts of a tile and the blocks of one
+__device__ __forceinline__ int tile_parts(const KV8Split& s, int end, int& per) {
+  const int nb = (end + KV8_BLOCK - 1) / KV8_BLOCK;
+  per = max(s.bps, (nb + s.parts - 1) / s.parts);
+  return max(1, (nb + per - 1) / per);
+}
+
+// NaN to the tile's outputs, by `threads` threads; to the whole row's where it has more tokens than the bound
 template <bool BF, int D>
-__global__ void __launch_bounds__(256) kv8_attn_token_kernel(t2w_kv8_attention_args a) {
-  __shared__ float s_q[4][D];
+__device__ void nan_tile(const t2w_kv8_attention_args& a, const KV8Split& s, const Tile& t, int kv_head, int thread, int threads) {
+  const int n = s.per_row > 0 && t.n_new > s.per_row * s.tt ? t.n_new : t.rows / s.G;
+  for (int i = 0; i < n; ++i)
+    for (int x = thread; x < s.G * D; x += threads)
+      ((uint16_t*)a.out)[(long long)(t.start + t.i0 + i) * a.ldo + kv_head * s.G * D + x] = BF ? 0x7fc0 : 0x7e00;
+}
+
+__device__ __forceinline__ f16x8 as_f16x8(uint4 v) { return __builtin_bit_cast(f16x8, v); }
+
+__device__ __forceinline__ bf16x8 codes_bf16(uint32_t lo, uint32_t hi) {
+  const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true);
+  const auto c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true);
+  return as_bf16x8(make_uint4(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)));
+}
+// codes times a power of two
+__device__ __forceinline__ f16x8 codes_f16(uint32_t lo, uint32_t hi, float s) {
+  const auto a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, s, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, s, true);
+  const auto c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, s, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, s, true);
+  return as_f16x8(make_uint4(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)));
+}
+
+// K . Q^T of 8 key codes a lane and the query operand in the queries' own type: e4m3 codes are exact in both
+template <bool BF>
+__device__ __forceinline__ f32x4 mfma_qk(uint32_t lo, uint32_t hi, uint4 q, f32x4 c) {
+  if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_bf16(lo, hi), as_bf16x8(q), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16(lo, hi, 1.f), as_f16x8(q), c, 0, 0, 0);
+}
+template <bool BF>
+__device__ __forceinline__ f32x16 mfma_qk(uint32_t lo, uint32_t hi, uint4 q, f32x16 c) {
+  if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(codes_bf16(lo, hi), as_bf16x8(q), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_f16(lo, hi, 1.f), as_f16x8(q), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma_pv(f16x8 v, f16x8 p, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma_pv(f16x8 v, f16x8 p, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p, c, 0, 0, 0); }
+
+// maximum over the lanes that hold the same query: lanes l, l ^ 32 (32-query tiles) and l ^ 16 (16-query tiles).  Through
+// the LDS crossbar: it runs only when the reference moves, and hipcc drops the maximum of a v_permlane32_swap's two results.
+template <int MR>
+__device__ __forceinline__ float query_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 32, 64));
+  if constexpr (MR == 16) v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return v;
+}
+
+__device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float((uint32_t)min(max(biased, 0), 254) << 23); }
+
+// Softmax state of a wave's queries (lane column = query), shared by both kernels.  Scores are in units of log2, s = q . k
+// times c = scale log2(e) 2^(key exponent).
+//  * m is a reference that the running maximum may pass by 8 before it is moved (by the whole wave, then the true maximum so
+//    far): probabilities are 2^(s - m + 7) <= 2^15 in fp16, so most blocks need no exchange between lanes and no rescaling of
+//    the outputs, and a probability keeps fp16's 11 bits down to 2^-21 of the largest and 2^-32 of it absolutely.  fp16 and
+//    not bf16: bf16's 8 bits would cost as much again as the output's own rounding.
+//  * value codes enter as fp16, exact, times 2^(their exponent - E + 7), E the largest value exponent so far: 22 powers of two
+//    below the largest block's scale stay exact.
+//  * sums of probabilities come from the matrix unit too (a row of ones): the same rounded probabilities as the outputs'.
+struct Soft {
+  float m = -__builtin_inff();  // reference
+  float nb = 7.f;               // 7 - m, 7 where m is -inf
+  bool big = false;             // |m| so large that s - m in one fma would not be exact enough: scale the scores first
+};
+
+template <typename Acc>
+__device__ __forceinline__ void scale_acc(Acc& o, float f) {
+#pragma unroll
+  for (int r = 0; r < (int)(sizeof(Acc) / 4); ++r) o[r] *= f;
+}
+
+// Direct form, for tiles of few packed rows (steps, draft checks, windows of up to 64 packed rows): every wave loads its key
+// and value fragments from the pages into registers and converts them there; no LDS and no barrier before the end.  RW waves
+// of MR packed rows each, times 4 / RW waves that take every (4 / RW)-th block; their states are merged through LDS.
+//
+// Bound by memory: 2 D codes a token and key head are read once and meet at least MR query columns of the matrix unit, whose
+// unused columns cost nothing that matters.  MR = 16 (16x16x32 MFMA) has half the softmax work of MR = 32 (32x32x16) where
+// rows allow it.
+//
+// With S^T = K . Q^T the score MFMA leaves a lane scores of its own query only; the rows of K are fed in an order that makes
+// them the 8 (MR = 16) or 2 x 8 keys whose value bytes the same lane loads as the P . V operand:
+//   MR 16: lane (i = l % 16, g = l / 16); key operand kg row i = key 8 (i / 4) + 4 kg + i % 4, its scores: keys 8 g + 4 kg + r
+//   MR 32: lane (i = l % 32, h = l / 32); row i = key with bits 2 and 3 of i swapped, scores r: keys 16 (r / 8) + 8 h + r % 8
+// Channels are paired the same way on both sides: lane group x loads the 16-channel chunk n x' + x of keys and queries.
+template <bool BF, int D, int MR, int RW>
+__global__ void __launch_bounds__(256, MR == 16 ? (D == 64 ? 4 : 3) : 2) kv8_attn_direct_kernel(t2w_kv8_attention_args a, KV8Split sp) {
+  constexpr int KW = 4 / RW;                       // waves that share the keys of the same packed rows
+  constexpr int LG = 64 / MR;                      // lane groups: 4 or 2
+  constexpr int NQ = D / (8 * LG), NL = D / 32;    // query operands; 16-byte loads of a block's keys, and of its values
+  constexpr int KG = MR == 16 ? 2 : 1;             // score MFMA tiles of a block
+  constexpr int NT = D / (2 * MR);                 // output tile pairs (channel pairs 2 p, 2 p + 1, p = MR t + i)
+  typedef typename std::conditional<MR == 16, f32x4, f32x16>::type Acc;
+  constexpr int AR = MR == 16 ? 4 : 16;            // values of an Acc
+  __shared__ float s_acc[(KW > 1 ? KW / 2 : 1) * RW][NT * 2 * AR + 2][64];
+  __shared__ int s_e[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rw = wave % RW, kw = wave / RW;
+  const int slot = blockIdx.x / a.pages.kv_heads, kv_head = blockIdx.x - slot * a.pages.kv_heads, part = blockIdx.y;
+  Tile t;
+  if (!find_tile(a, sp, slot, t)) return;
+  if (t.bad) {
+    if (part == 0) nan_tile<BF, D>(a, sp, t, kv_head, threadIdx.x, 256);
+    return;
+  }
+  int per;
+  const int parts = tile_parts(sp, t.end, per);
+  if (part >= parts) return;
+  const int b0 = part * per, b1 = min(b0 + per, (t.end + KV8_BLOCK - 1) / KV8_BLOCK);
+  const int i = lane % MR, g = lane / MR;
+  const int m0 = rw * MR;
+  const bool idle = m0 >= t.rows;  // a wave without rows still meets the barriers
+  const int mrow = m0 + i;
+  const int tok = min(mrow, t.rows - 1) / sp.G, hq = min(mrow, t.rows - 1) - tok * sp.G;
+  const int lim = seen_by(a, t, t.i0 + tok);
+  const int lim_lo = seen_by(a, t, t.i0 + min(m0, t.rows - 1) / sp.G);  // the wave's first query sees least
+
+  uint4 q[NQ];
+  {
+    const uint16_t* src = (const uint16_t*)a.q + (long long)(t.start + t.i0 + tok) * a.ldq + (kv_head * sp.G + hq) * D;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) q[n] = *(const uint4*)(src + (LG * (n >> 1) + g) * 16 + (n & 1) * 8);
+  }
+  Acc o[NT][2], l;
+  for (int r = 0; r < AR; ++r) l[r] = 0.f;
+#pragma unroll
+  for (int x = 0; x < NT; ++x)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < AR; ++r) o[x][j][r] = 0.f;
+  Soft st;
+  int E = 0;  // biased value exponent that o is in units of
+  const float c0 = a.scale * 1.4426950408889634f;
+
+  // byte offsets of the lane's loads within a block's keys and values
+  int koff[NL], voff[NL];
+#pragma unroll
+  for (int n = 0; n < NL; ++n) {
+    if constexpr (MR == 16) {
+      const int kg = n % 2, j = n / 2;
+      koff[n] = (4 * j + g) * 512 + (8 * (i >> 2) + 4 * kg + (i & 3)) * 16;
+      voff[n] = g * 8 * D + (16 * n + i) * 16;
+    } else {
+      koff[n] = (2 * n + g) * 512 + ((i & 0x13) | ((i & 4) << 1) | ((i & 8) >> 1)) * 16;
+      const int kk = n % 2, x = n / 2;
+      voff[n] = (2 * kk + g) * 8 * D + (32 * x + i) * 16;
+    }
+  }
+  const size_t stride = (size_t)a.pages.kv_heads * (KV8_BLOCK * D);
+  const uint8_t* kbase = (const uint8_t*)a.pages.k + (size_t)kv_head * (KV8_BLOCK * D);
+  const uint8_t* vbase = (const uint8_t*)a.pages.v + (size_t)kv_head * (KV8_BLOCK * D);
+  const int* table = a.table + (size_t)t.row * a.ld_table;
+
+  struct Buf { uint4 k[NL], v[NL]; };
+  auto load = [&](Buf& f, int id) {
+    const uint8_t* kp = kbase + (size_t)id * stride;
+    const uint8_t* vp = vbase + (size_t)id * stride;
+#pragma unroll
+    for (int n = 0; n < NL; ++n) f.k[n] = *(const uint4*)(kp + koff[n]);
+#pragma unroll
+    for (int n = 0; n < NL; ++n) f.v[n] = *(const uint4*)(vp + voff[n]);
+  };
+  auto step = [&](Buf& f, int b, int ke, int ve) {
+    Acc sc[KG];
+#pragma unroll
+    for (int x = 0; x < KG; ++x)
+#pragma unroll
+      for (int r = 0; r < AR; ++r) sc[x][r] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int x = MR == 16 ? n % 2 : 0, j = MR == 16 ? n / 2 : n;
+      sc[x] = mfma_qk<BF>(f.k[n].x, f.k[n].y, q[2 * j], sc[x]);
+      sc[x] = mfma_qk<BF>(f.k[n].z, f.k[n].w, q[2 * j + 1], sc[x]);
+    }
+    float c = c0 * pow2_bits(ke);
+    const int key0 = b * KV8_BLOCK;
+    if (ke > 254) {  // a block id outside the pages, or an E8M0 NaN
+      c = c0;
+#pragma unroll
+      for (int x = 0; x < KG; ++x)
+#pragma unroll
+        for (int r = 0; r < AR; ++r) sc[x][r] = __builtin_nanf("");
+    }
+    if (key0 + KV8_BLOCK > lim_lo) {  // some query of the wave does not see all of the block
+#pragma unroll
+      for (int x = 0; x < KG; ++x)
+#pragma unroll
+        for (int r = 0; r < AR; ++r) {
+          const int key = MR == 16 ? 8 * g + 4 * x + r : 16 * (r >> 3) + 8 * g + (r & 7);
+          sc[x][r] = key0 + key < lim ? sc[x][r] : -__builtin_inff();
+        }
+    }
+    if (key0 + KV8_BLOCK > t.total) {  // the row's last block: values behind its last token count as zeros, whatever they are
+#pragma unroll
+      for (int n = 0; n < NL; ++n) {
+        const int gr = MR == 16 ? g : 2 * (n % 2) + g, left = t.total - key0 - 8 * gr;
+        const uint64_t keep = left >= 8 ? ~0ull : left <= 0 ? 0ull : (1ull << (8 * left)) - 1ull;
+        f.v[n].x &= (uint32_t)keep; f.v[n].y &= (uint32_t)(keep >> 32);
+        f.v[n].z &= (uint32_t)keep; f.v[n].w &= (uint32_t)(keep >> 32);
+      }
+    }
+    float mx = sc[0][0];
+#pragma unroll
+    for (int x = 0; x < KG; ++x)
+#pragma unroll
+      for (int r = 0; r < AR; ++r) mx = fmaxf(mx, sc[x][r]);
+    mx *= c;
+    if (__builtin_amdgcn_ballot_w64(mx > st.m + 8.f)) {
+      const float mn = fmaxf(st.m, query_max<MR>(mx));
+      const float alpha = st.m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(st.m - mn);
+      st.m = mn;
+      st.nb = mn == -__builtin_inff() ? 7.f : 7.f - mn;
+      st.big = st.big || __builtin_amdgcn_ballot_w64(fabsf(mn) > 4194304.f && mn != -__builtin_inff()) != 0;
+      scale_acc(l, alpha);
+#pragma unroll
+      for (int x = 0; x < NT; ++x) { scale_acc(o[x][0], alpha); scale_acc(o[x][1], alpha); }
+    }
+    if (st.big) {
+#pragma unroll
+      for (int x = 0; x < KG; ++x)
+#pragma unroll
+        for (int r = 0; r < AR; ++r) sc[x][r] *= c;
+      c = 1.f;
+    }
+    if (ve > E) {
+      const float f2 = E == 0 ? 0.f : pow2_bits(E - ve + 127);
+#pragma unroll
+      for (int x = 0; x < NT; ++x) { scale_acc(o[x][0], f2); scale_acc(o[x][1], f2); }
+      E = ve;
+    }
+    const float vs = pow2_bits(ve - E + 127 + 7);
+    constexpr int NP = MR == 16 ? 1 : 2;  // P operands of a block
+    f16x8 p[NP], one;
+#pragma unroll
+    for (int x = 0; x < NP; ++x)
+#pragma unroll
+      for (int y = 0; y < 8; y += 2) {
+        float e[2];
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const float s = MR == 16 ? sc[(y + z) / 4 % KG][(y + z) % 4] : sc[0][8 * x + y + z];
+          e[z] = __builtin_amdgcn_exp2f(fmaf(s, c, st.nb));
+        }
+        const f16x2_t h = __builtin_convertvector((f32x2_t{e[0], e[1]}), f16x2_t);
+        p[x][y] = h[0];
+        p[x][y + 1] = h[1];
+      }
+#pragma unroll
+    for (int y = 0; y < 8; ++y) one[y] = (_Float16)1.0f;
+#pragma unroll
+    for (int x = 0; x < NP; ++x) l = mfma_pv(one, p[x], l);
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int x = MR == 16 ? n : n / 2, kk = MR == 16 ? 0 : n % 2;
+      o[x][0] = mfma_pv(codes_f16(f.v[n].x, f.v[n].y, vs), p[kk], o[x][0]);
+      o[x][1] = mfma_pv(codes_f16(f.v[n].z, f.v[n].w, vs), p[kk], o[x][1]);
+    }
+  };
+
+  if (!idle) {
+    // the wave's blocks b0 + kw, + KW, ...: ids and exponents of the next 64 of them one a lane, the fragments of one
+    // block in flight while another is worked on
+    for (int base = b0 + kw; base < b1; base += 64 * KW) {
+      const int mine = base + lane * KW;
+      int id = mine < b1 ? table[mine] : 0, ke = 255, ve = 0;
+      if ((unsigned)id < (unsigned)a.pages.n_blocks) {
+        ke = a.pages.k_exp[(size_t)id * a.pages.kv_heads + kv_head];
+        ve = a.pages.v_exp[(size_t)id * a.pages.kv_heads + kv_head];
+      } else {
+        id = 0;
+      }
+      const int n = min(64, (b1 - base + KW - 1) / KW);
+      Buf f0, f1;
+      load(f0, __builtin_amdgcn_readlane(id, 0));
+      for (int x = 0; x < n; x += 2) {
+        if (x + 1 < n) load(f1, __builtin_amdgcn_readlane(id, x + 1));
+        step(f0, base + x * KW, __builtin_amdgcn_readlane(ke, x), __builtin_amdgcn_readlane(ve, x));
+        if (x + 1 < n) {
+          if (x + 2 < n) load(f0, __builtin_amdgcn_readlane(id, x + 2));
+          step(f1, base + (x + 1) * KW, __builtin_amdgcn_readlane(ke, x + 1), __builtin_amdgcn_readlane(ve, x + 1));
+        }
+      }
+    }
+  }
+  // merge the key waves pairwise: the upper half leaves its state, the lower half folds it in
+#pragma unroll
+  for (int w = KW / 2; w >= 1; w /= 2) {
+    if (kw >= w && kw < 2 * w) {
+      float (*dst)[64] = s_acc[(kw - w) * RW + rw];
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int r = 0; r < AR; ++r) dst[(x * 2 + j) * AR + r][lane] = o[x][j][r];
+      dst[NT * 2 * AR][lane] = st.m;
+      dst[NT * 2 * AR + 1][lane] = l[0];
+      if (lane == 0) s_e[wave] = E;
+    }
+    __syncthreads();
+    if (kw < w) {
+      const float (*src)[64] = s_acc[kw * RW + rw];
+      const float m2 = src[NT * 2 * AR][lane], l2 = src[NT * 2 * AR + 1][lane];
+      const int e2 = s_e[wave + w * RW], en = max(E, e2);
+      const float mn = fmaxf(st.m, m2);
+      const float f1 = st.m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(st.m - mn);
+      const float f2 = m2 == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m2 - mn);
+      // a state whose reference never moved holds zeros, or NaN from scores that were none
+      const float k1 = l[0] != l[0] ? __builtin_nanf("") : f1, k2 = l2 != l2 ? __builtin_nanf("") : f2;
+      const float g1 = E == en ? k1 : k1 * (E == 0 ? 0.f : pow2_bits(E - en + 127)), g2 = e2 == en ? k2 : k2 * (e2 == 0 ? 0.f : pow2_bits(e2 - en + 127));
+      l[0] = l[0] * k1 + l2 * k2;
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int r = 0; r < AR; ++r) o[x][j][r] = o[x][j][r] * g1 + src[(x * 2 + j) * AR + r][lane] * g2;
+      st.m = mn;
+      E = en;
+    }
+    if (w > 1) __syncthreads();
+  }
+  if (kw != 0 || mrow >= t.rows) return;
+  const float unit = pow2_bits(E) * 0.0078125f;  // 2^(E - 127 - 7); E = 0: no value block at all, o is zero
+  const float inv = l[0] == 0.f ? 0.f : 1.f / l[0];
+  if (parts == 1) {
+    uint16_t* out = (uint16_t*)a.out + (long long)(t.start + t.i0 + tok) * a.ldo + (kv_head * sp.G + hq) * D;
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int r = 0; r < AR; r += 4) {
+        // values r .. r + 3 of both tiles: 8 consecutive channels
+        const int d = MR == 16 ? 32 * x + 8 * g : 64 * x + 4 * r + 8 * g;
+        uint32_t w[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) w[y] = BF ? pack2(o[x][0][r + y] * inv * unit, o[x][1][r + y] * inv * unit) : pack2h(o[x][0][r + y] * inv * unit, o[x][1][r + y] * inv * unit);
+        *(uint4*)(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+  } else {
+    const size_t pr = ((size_t)slot * a.pages.kv_heads + kv_head) * sp.parts + part, rows = sp.tt * sp.G;
+    float* po = (float*)a.workspace + (pr * rows + mrow) * D;
+    float* ml = (float*)a.workspace + part_rows(sp, a.pages.kv_heads) * D + (pr * rows + mrow) * 2;
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int r = 0; r < AR; r += 4) {
+        const int d = MR == 16 ? 32 * x + 8 * g : 64 * x + 4 * r + 8 * g;
+#pragma unroll
+        for (int y = 0; y < 4; y += 2)
+          *(float4*)(po + d + 2 * y) = make_float4(o[x][0][r + y] * inv * unit, o[x][1][r + y] * inv * unit, o[x][0][r + y + 1] * inv * unit, o[x][1][r + y + 1] * inv * unit);
+      }
+    if (g == 0) *(float2*)ml = make_float2(st.m, l[0]);
+  }
+}
+
+// Joins the parts of split tiles: a wave per packed row, lane d its channels.
+template <bool BF, int D>
+__global__ void __launch_bounds__(256) kv8_join_kernel(t2w_kv8_attention_args a, KV8Split sp) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n = blockIdx.x, head = blockIdx.y * 4 + wave;
-  if (head >= a.heads) return;
-  const int kv_head = head / (a.heads / a.pages.kv_heads);
-  int lo = 0, hi = a.n_rows;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.row_start[mid] <= n) lo = mid; else hi = mid;
-  }
-  const int row = lo, start = a.row_start[row], n_new = a.row_start[row + 1] - start, total = a.kv_total[row];
-  const int i = n - start;
-  if (i < 0 || i >= n_new) return;  // behind the last row
-  const int seen_new = a.chunk > 0 ? (int)min((long long)n_new, ((long long)i / a.chunk + 1) * a.chunk) : n_new;
-  const int seen = min(max(total - n_new + seen_new, 0), total);
-  const bool bad_row = total < 0 || total > a.width * KV8_BLOCK;
-  const uint16_t* q = (const uint16_t*)a.q + (long long)n * a.ldq + head * D;
-  for (int d = lane; d < D; d += 64) s_q[wave][d] = BF ? bf2f(q[d]) : h2f(q[d]);
-  __builtin_amdgcn_wave_barrier();
+  const int slot = blockIdx.x / a.pages.kv_heads, kv_head = blockIdx.x - slot * a.pages.kv_heads, m = blockIdx.y * 4 + wave;
+  Tile t;
+  if (!find_tile(a, sp, slot, t) || t.bad) return;
+  int per;
+  const int parts = tile_parts(sp, t.end, per);
+  if (parts == 1 || m >= t.rows) return;
+  const size_t rows = sp.tt * sp.G, pr = ((size_t)slot * a.pages.kv_heads + kv_head) * sp.parts;
+  const float* po = (const float*)a.workspace + (pr * rows + m) * D;
+  const float* ml = (const float*)a.workspace + part_rows(sp, a.pages.kv_heads) * D + (pr * rows + m) * 2;
+  float top = -__builtin_inff();
+  for (int p = lane; p < parts; p += 64) top = fmaxf(top, ml[p * rows * 2]);
+#pragma unroll
+  for (int w = 32; w >= 1; w >>= 1) top = fmaxf(top, __shfl_xor(top, w, 64));
   constexpr int NV = D / 64;
-  float o[NV] = {}, m = -__builtin_inff(), l = 0.f;
-  const float c = a.scale * 1.4426950408889634f;
-  const int key = lane & 31, half = lane >> 5;
-  for (int b = 0; !bad_row && b * KV8_BLOCK < seen; ++b) {
-    int id = a.table[(size_t)row * a.ld_table + b];
-    const bool bad = (unsigned)id >= (unsigned)a.pages.n_blocks;
-    if (bad) id = 0;
-    const size_t pg = (size_t)id * a.pages.kv_heads + kv_head;
-    const uint8_t* kp = (const uint8_t*)a.pages.k + pg * (KV8_BLOCK * D);
-    const uint8_t* vp = (const uint8_t*)a.pages.v + pg * (KV8_BLOCK * D);
-    const float ks = ldexpf(1.f, (int)a.pages.k_exp[pg] - 127), vs = ldexpf(1.f, (int)a.pages.v_exp[pg] - 127);
-    float s = 0.f;
-    for (int ch = half; ch < D / 16; ch += 2) {
-      const uint4 u = *(const uint4*)(kp + ch * 512 + key * 16);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const auto x = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j], false);
-        const auto y = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j], true);
-        const float* qq = s_q[wave] + ch * 16 + j * 4;
-        s += x[0] * qq[0] + x[1] * qq[1] + y[0] * qq[2] + y[1] * qq[3];
-      }
+  float acc[NV] = {}, sum = 0.f;
+  for (int p0 = 0; p0 < parts; p0 += 64) {
+    float f = 0.f;
+    if (p0 + lane < parts) {
+      const float2 x = *(const float2*)(ml + (size_t)(p0 + lane) * rows * 2);
+      f = x.y != x.y ? __builtin_nanf("") : x.x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(x.x - top) * x.y;
     }
-    s += xor32(s);
-    s = b * KV8_BLOCK + key < seen ? (bad ? __builtin_nanf("") : s * ks * c) : -__builtin_inff();
-    float mx = s;
+    sum += wave_sum(f);
+    const int n = min(64, parts - p0);
+#pragma unroll 4
+    for (int p = 0; p < n; ++p) {
+      const float fp = __shfl(f, p, 64);
+      const float* src = po + (size_t)(p0 + p) * rows * D + lane * NV;
 #pragma unroll
-    for (int w = 16; w >= 1; w >>= 1) mx = fmaxf(mx, __shfl_xor(mx, w, 64));
-    const float mn = fmaxf(m, mx), mr = mn == -__builtin_inff() ? 0.f : mn;
-    const float alpha = __builtin_amdgcn_exp2f(m - mr), p = __builtin_amdgcn_exp2f(s - mr);
-    float ps = half ? 0.f : p;
-    l = l * alpha + wave_sum(ps);
-    m = mn;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) o[v] *= alpha;
-    const int left = seen - b * KV8_BLOCK;
-    for (int t = 0; t < KV8_BLOCK && t < left; ++t) {
-      const float pt = __shfl(p, t, 64) * vs;
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        const int d = lane + 64 * v;
-        const int code = vp[(t >> 3) * (8 * D) + (d >> 1) * 16 + (d & 1) * 8 + (t & 7)];
-        o[v] += pt * __builtin_amdgcn_cvt_pk_f32_fp8(code, false)[0];
-      }
+      for (int v = 0; v < NV; ++v) acc[v] += fp * src[v];
     }
   }
-  uint16_t* out = (uint16_t*)a.out + (long long)n * a.ldo + head * D;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int tok = m / sp.G;
+  uint16_t* out = (uint16_t*)a.out + (long long)(t.start + t.i0 + tok) * a.ldo + (kv_head * sp.G + m - tok * sp.G) * D + lane * NV;
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const float x = bad_row ? __builtin_nanf("") : l == 0.f ? 0.f : o[v] / l;
-    out[lane + 64 * v] = BF ? f2bf(x) : f2h(x);
-  }
+  for (int v = 0; v < NV; ++v) out[v] = BF ? f2bf(acc[v] * inv) : f2h(acc[v] * inv);
+}
+
+// Which form, tile and split a call takes: from its sizes and bounds alone, so that the workspace's size is known too.
+struct Choice {
+  int mr, rw;
+  KV8Split s;
+};
+
+Choice choose(const t2w_kv8_attention_args& a) {
+  Choice c;
+  c.s.G = a.heads / a.pages.kv_heads;
+  const long packed = a.max_new > 0 ? (long)min(a.max_new, a.n_tok) * c.s.G : 1 << 30;
+  c.mr = packed <= 16 ? 16 : 32;
+  c.rw = packed <= 32 ? 1 : 2;
+  c.s.tt = c.mr * c.rw / c.s.G;
+  c.s.per_row = a.max_new > 0 && a.max_new <= c.s.tt ? 1 : 0;
+  c.s.n_tiles = c.s.per_row ? a.n_rows : a.n_tok / c.s.tt + a.n_rows;
+  const long max_kv = a.max_kv > 0 ? min((long)a.max_kv, (long)a.width * KV8_BLOCK) : (long)a.width * KV8_BLOCK;
+  const long nb = (max_kv + KV8_BLOCK - 1) / KV8_BLOCK, groups = (long)c.s.n_tiles * a.pages.kv_heads;
+  long parts = (2048 + groups - 1) / groups;
+  long bps = (nb + parts - 1) / parts;
+  if (bps < 16) bps = 16;
+  parts = (nb + bps - 1) / bps;
+  c.s.bps = (int)bps;
+  c.s.parts = (int)(parts < 1 ? 1 : parts > 256 ? 256 : parts);
+  return c;
 }
 
 }  // namespace
 
-size_t kv8_attention_workspace(const t2w_kv8_attention_args&) { return 0; }
+size_t kv8_attention_workspace(const t2w_kv8_attention_args& a) {
+  const Choice c = choose(a);
+  return c.s.parts > 1 ? part_rows(c.s, a.pages.kv_heads) * (a.pages.head_dim + 2) * sizeof(float) : 0;
+}
+
+template <bool BF, int D>
+static hipError_t launch(const t2w_kv8_attention_args& a, const Choice& c, hipStream_t st) {
+  const dim3 grid((unsigned)(c.s.n_tiles * a.pages.kv_heads), c.s.parts);
+  if (c.mr == 16) hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 16, 1>), grid, dim3(256), 0, st, a, c.s);
+  else if (c.rw == 1) hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 1>), grid, dim3(256), 0, st, a, c.s);
+  else hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 2>), grid, dim3(256), 0, st, a, c.s);
+  if (c.s.parts > 1)
+    hipLaunchKernelGGL((kv8_join_kernel<BF, D>), dim3((unsigned)(c.s.n_tiles * a.pages.kv_heads), (c.s.tt * c.s.G + 3) / 4), dim3(256), 0, st, a, c.s);
+  return hipGetLastError();
+}
 
 hipError_t kv8_attention(const t2w_kv8_attention_args& a, hipStream_t st) {
   if (a.n_tok <= 0 || a.n_rows <= 0) return hipSuccess;
-  const dim3 grid((unsigned)a.n_tok, (unsigned)((a.heads + 3) / 4));
-#define T2W_KV8_ATTN(BF, D) hipLaunchKernelGGL((kv8_attn_token_kernel<BF, D>), grid, dim3(256), 0, st, a)
-  if (a.dtype == T2W_KV8_BF16) {
-    if (a.pages.head_dim == 64) T2W_KV8_ATTN(true, 64); else T2W_KV8_ATTN(true, 128);
-  } else {
-    if (a.pages.head_dim == 64) T2W_KV8_ATTN(false, 64); else T2W_KV8_ATTN(false, 128);
-  }
-#undef T2W_KV8_ATTN
-  return hipGetLastError();
+  const Choice c = choose(a);
+  if ((long)c.s.n_tiles * a.pages.kv_heads > 0x7fffffffL) return hipErrorInvalidValue;
+  if (a.dtype == T2W_KV8_BF16) return a.pages.head_dim == 64 ? launch<true, 64>(a, c, st) : launch<true, 128>(a, c, st);
+  return a.pages.head_dim == 64 ? launch<false, 64>(a, c, st) : launch<false, 128>(a, c, st);
 }
 
 }  // namespace t2w
