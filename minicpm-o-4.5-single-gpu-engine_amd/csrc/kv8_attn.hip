@@ -156,7 +156,7 @@ __device__ __forceinline__ void scale_acc(Acc& o, float f) {
 //   MR 32: lane (i = l % 32, h = l / 32); row i = key with bits 2 and 3 of i swapped, scores r: keys 16 (r / 8) + 8 h + r % 8
 // Channels are paired the same way on both sides: lane group x loads the 16-channel chunk n x' + x of keys and queries.
 template <bool BF, int D, int MR, int RW>
-__global__ void __launch_bounds__(256, MR == 16 ? (D == 64 ? 4 : 3) : 2) kv8_attn_direct_kernel(t2w_kv8_attention_args a, KV8Split sp) {
+__global__ void __launch_bounds__(256, MR == 16 ? (D == 64 ? 5 : 4) : (D == 64 ? 3 : 2)) kv8_attn_direct_kernel(t2w_kv8_attention_args a, KV8Split sp) {
   constexpr int KW = 4 / RW;                       // waves that share the keys of the same packed rows
   constexpr int LG = 64 / MR;                      // lane groups: 4 or 2
   constexpr int NQ = D / (8 * LG), NL = D / 32;    // query operands; 16-byte loads of a block's keys, and of its values
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(256, MR == 16 ? (D == 64 ? 4 : 3) : 2) kv8_att
   constexpr int AR = MR == 16 ? 4 : 16;            // values of an Acc
   __shared__ float s_acc[(KW > 1 ? KW / 2 : 1) * RW][NT * 2 * AR + 2][64];
   __shared__ int s_e[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rw = wave % RW, kw = wave / RW;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wave % RW, kw = wave / RW;
   const int slot = blockIdx.x / a.pages.kv_heads, kv_head = blockIdx.x - slot * a.pages.kv_heads, part = blockIdx.y;
   Tile t;
   if (!find_tile(a, sp, slot, t)) return;
@@ -204,35 +204,27 @@ __global__ void __launch_bounds__(256, MR == 16 ? (D == 64 ? 4 : 3) : 2) kv8_att
   int E = 0;  // biased value exponent that o is in units of
   const float c0 = a.scale * 1.4426950408889634f;
 
-  // byte offsets of the lane's loads within a block's keys and values
-  int koff[NL], voff[NL];
-#pragma unroll
-  for (int n = 0; n < NL; ++n) {
-    if constexpr (MR == 16) {
-      const int kg = n % 2, j = n / 2;
-      koff[n] = (4 * j + g) * 512 + (8 * (i >> 2) + 4 * kg + (i & 3)) * 16;
-      voff[n] = g * 8 * D + (16 * n + i) * 16;
-    } else {
-      koff[n] = (2 * n + g) * 512 + ((i & 0x13) | ((i & 4) << 1) | ((i & 8) >> 1)) * 16;
-      const int kk = n % 2, x = n / 2;
-      voff[n] = (2 * kk + g) * 8 * D + (32 * x + i) * 16;
-    }
-  }
+  // the lane's place in a block's keys and values; its loads lie at constant distances from there (load offsets)
+  const uint32_t koff = MR == 16 ? g * 512 + (8 * (i >> 2) + (i & 3)) * 16 : g * 512 + ((i & 0x13) | ((i & 4) << 1) | ((i & 8) >> 1)) * 16;
+  const uint32_t voff = g * 8 * D + i * 16;
   const size_t stride = (size_t)a.pages.kv_heads * (KV8_BLOCK * D);
   const uint8_t* kbase = (const uint8_t*)a.pages.k + (size_t)kv_head * (KV8_BLOCK * D);
   const uint8_t* vbase = (const uint8_t*)a.pages.v + (size_t)kv_head * (KV8_BLOCK * D);
   const int* table = a.table + (size_t)t.row * a.ld_table;
 
-  struct Buf { uint4 k[NL], v[NL]; };
-  auto load = [&](Buf& f, int id) {
+  // one block's codes; the next block's keys are loaded as soon as the scores have used these, its values after P . V
+  uint4 kf[NL], vf[NL];
+  auto load_k = [&](int id) {
     const uint8_t* kp = kbase + (size_t)id * stride;
+#pragma unroll
+    for (int n = 0; n < NL; ++n) kf[n] = *(const uint4*)(kp + koff + (MR == 16 ? (n / 2) * 2048 + (n % 2) * 64 : n * 1024));
+  };
+  auto load_v = [&](int id) {
     const uint8_t* vp = vbase + (size_t)id * stride;
 #pragma unroll
-    for (int n = 0; n < NL; ++n) f.k[n] = *(const uint4*)(kp + koff[n]);
-#pragma unroll
-    for (int n = 0; n < NL; ++n) f.v[n] = *(const uint4*)(vp + voff[n]);
+    for (int n = 0; n < NL; ++n) vf[n] = *(const uint4*)(vp + voff + (MR == 16 ? n * 256 : (n % 2) * 16 * D + (n / 2) * 512));
   };
-  auto step = [&](Buf& f, int b, int ke, int ve) {
+  auto step = [&](int b, int ke, int ve, int next) {  // next: the block id to load, -1: none
     Acc sc[KG];
 #pragma unroll
     for (int x = 0; x < KG; ++x)
@@ -241,25 +233,21 @@ __global__ void __launch_bounds__(256, MR == 16 ? (D == 64 ? 4 : 3) : 2) kv8_att
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
       const int x = MR == 16 ? n % 2 : 0, j = MR == 16 ? n / 2 : n;
-      sc[x] = mfma_qk<BF>(f.k[n].x, f.k[n].y, q[2 * j], sc[x]);
-      sc[x] = mfma_qk<BF>(f.k[n].z, f.k[n].w, q[2 * j + 1], sc[x]);
+      sc[x] = mfma_qk<BF>(kf[n].x, kf[n].y, q[2 * j], sc[x]);
+      sc[x] = mfma_qk<BF>(kf[n].z, kf[n].w, q[2 * j + 1], sc[x]);
     }
+    if (next >= 0) load_k(next);
     float c = c0 * pow2_bits(ke);
     const int key0 = b * KV8_BLOCK;
-    if (ke > 254) {  // a block id outside the pages, or an E8M0 NaN
-      c = c0;
-#pragma unroll
-      for (int x = 0; x < KG; ++x)
-#pragma unroll
-        for (int r = 0; r < AR; ++r) sc[x][r] = __builtin_nanf("");
-    }
-    if (key0 + KV8_BLOCK > lim_lo) {  // some query of the wave does not see all of the block
+    const bool off = ke > 254;  // a block id outside the pages, or an E8M0 NaN
+    if (off) c = c0;
+    if (off || key0 + KV8_BLOCK > lim_lo) {  // or some query of the wave does not see all of the block
 #pragma unroll
       for (int x = 0; x < KG; ++x)
 #pragma unroll
         for (int r = 0; r < AR; ++r) {
           const int key = MR == 16 ? 8 * g + 4 * x + r : 16 * (r >> 3) + 8 * g + (r & 7);
-          sc[x][r] = key0 + key < lim ? sc[x][r] : -__builtin_inff();
+          sc[x][r] = key0 + key < lim ? (off ? __builtin_nanf("") : sc[x][r]) : -__builtin_inff();
         }
     }
     if (key0 + KV8_BLOCK > t.total) {  // the row's last block: values behind its last token count as zeros, whatever they are
@@ -267,8 +255,8 @@ __global__ void __launch_bounds__(256, MR == 16 ? (D == 64 ? 4 : 3) : 2) kv8_att
       for (int n = 0; n < NL; ++n) {
         const int gr = MR == 16 ? g : 2 * (n % 2) + g, left = t.total - key0 - 8 * gr;
         const uint64_t keep = left >= 8 ? ~0ull : left <= 0 ? 0ull : (1ull << (8 * left)) - 1ull;
-        f.v[n].x &= (uint32_t)keep; f.v[n].y &= (uint32_t)(keep >> 32);
-        f.v[n].z &= (uint32_t)keep; f.v[n].w &= (uint32_t)(keep >> 32);
+        vf[n].x &= (uint32_t)keep; vf[n].y &= (uint32_t)(keep >> 32);
+        vf[n].z &= (uint32_t)keep; vf[n].w &= (uint32_t)(keep >> 32);
       }
     }
     float mx = sc[0][0];
@@ -324,14 +312,14 @@ __global__ void __launch_bounds__(256, MR == 16 ? (D == 64 ? 4 : 3) : 2) kv8_att
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
       const int x = MR == 16 ? n : n / 2, kk = MR == 16 ? 0 : n % 2;
-      o[x][0] = mfma_pv(codes_f16(f.v[n].x, f.v[n].y, vs), p[kk], o[x][0]);
-      o[x][1] = mfma_pv(codes_f16(f.v[n].z, f.v[n].w, vs), p[kk], o[x][1]);
+      o[x][0] = mfma_pv(codes_f16(vf[n].x, vf[n].y, vs), p[kk], o[x][0]);
+      o[x][1] = mfma_pv(codes_f16(vf[n].z, vf[n].w, vs), p[kk], o[x][1]);
     }
+    if (next >= 0) load_v(next);
   };
 
   if (!idle) {
-    // the wave's blocks b0 + kw, + KW, ...: ids and exponents of the next 64 of them one a lane, the fragments of one
-    // block in flight while another is worked on
+    // the wave's blocks b0 + kw, + KW, ...: ids and exponents of the next 64 of them one a lane
     for (int base = b0 + kw; base < b1; base += 64 * KW) {
       const int mine = base + lane * KW;
       int id = mine < b1 ? table[mine] : 0, ke = 255, ve = 0;
@@ -342,16 +330,10 @@ __global__ void __launch_bounds__(256, MR == 16 ? (D == 64 ? 4 : 3) : 2) kv8_att
         id = 0;
       }
       const int n = min(64, (b1 - base + KW - 1) / KW);
-      Buf f0, f1;
-      load(f0, __builtin_amdgcn_readlane(id, 0));
-      for (int x = 0; x < n; x += 2) {
-        if (x + 1 < n) load(f1, __builtin_amdgcn_readlane(id, x + 1));
-        step(f0, base + x * KW, __builtin_amdgcn_readlane(ke, x), __builtin_amdgcn_readlane(ve, x));
-        if (x + 1 < n) {
-          if (x + 2 < n) load(f0, __builtin_amdgcn_readlane(id, x + 2));
-          step(f1, base + (x + 1) * KW, __builtin_amdgcn_readlane(ke, x + 1), __builtin_amdgcn_readlane(ve, x + 1));
-        }
-      }
+      load_k(__builtin_amdgcn_readlane(id, 0));
+      load_v(__builtin_amdgcn_readlane(id, 0));
+      for (int x = 0; x < n; ++x)
+        step(base + x * KW, __builtin_amdgcn_readlane(ke, x), __builtin_amdgcn_readlane(ve, x), x + 1 < n ? __builtin_amdgcn_readlane(id, x + 1) : -1);
     }
   }
   // merge the key waves pairwise: the upper half leaves its state, the lower half folds it in
@@ -425,40 +407,56 @@ __global__ void __launch_bounds__(256, MR == 16 ? (D == 64 ? 4 : 3) : 2) kv8_att
   }
 }
 
-// Joins the parts of split tiles: a wave per packed row, lane d its channels.
-template <bool BF, int D>
+// Joins the parts of split tiles, WR waves to a packed row (4 where a row has many parts): each wave sums its share of them,
+// a lane D / 64 channels.
+template <bool BF, int D, int WR>
 __global__ void __launch_bounds__(256) kv8_join_kernel(t2w_kv8_attention_args a, KV8Split sp) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int slot = blockIdx.x / a.pages.kv_heads, kv_head = blockIdx.x - slot * a.pages.kv_heads, m = blockIdx.y * 4 + wave;
+  constexpr int NV = D / 64;
+  __shared__ float s_acc[WR > 1 ? 4 : 1][NV][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave % WR;
+  const int slot = blockIdx.x / a.pages.kv_heads, kv_head = blockIdx.x - slot * a.pages.kv_heads, m = blockIdx.y * (4 / WR) + wave / WR;
   Tile t;
   if (!find_tile(a, sp, slot, t) || t.bad) return;
   int per;
   const int parts = tile_parts(sp, t.end, per);
-  if (parts == 1 || m >= t.rows) return;
+  if (parts == 1 || m >= t.rows) return;  // with WR == 4 the whole workgroup
   const size_t rows = sp.tt * sp.G, pr = ((size_t)slot * a.pages.kv_heads + kv_head) * sp.parts;
-  const float* po = (const float*)a.workspace + (pr * rows + m) * D;
+  const float* po = (const float*)a.workspace + (pr * rows + m) * D + lane * NV;
   const float* ml = (const float*)a.workspace + part_rows(sp, a.pages.kv_heads) * D + (pr * rows + m) * 2;
+  // every lane its parts' (maximum, sum): up to 256 parts
+  float2 x[4];
   float top = -__builtin_inff();
-  for (int p = lane; p < parts; p += 64) top = fmaxf(top, ml[p * rows * 2]);
 #pragma unroll
-  for (int w = 32; w >= 1; w >>= 1) top = fmaxf(top, __shfl_xor(top, w, 64));
-  constexpr int NV = D / 64;
-  float acc[NV] = {}, sum = 0.f;
-  for (int p0 = 0; p0 < parts; p0 += 64) {
-    float f = 0.f;
-    if (p0 + lane < parts) {
-      const float2 x = *(const float2*)(ml + (size_t)(p0 + lane) * rows * 2);
-      f = x.y != x.y ? __builtin_nanf("") : x.x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(x.x - top) * x.y;
-    }
-    sum += wave_sum(f);
-    const int n = min(64, parts - p0);
-#pragma unroll 4
-    for (int p = 0; p < n; ++p) {
-      const float fp = __shfl(f, p, 64);
-      const float* src = po + (size_t)(p0 + p) * rows * D + lane * NV;
+  for (int n = 0; n < 4; ++n) {
+    const int p = n * 64 + lane;
+    x[n] = p < parts ? *(const float2*)(ml + (size_t)p * rows * 2) : make_float2(-__builtin_inff(), 0.f);
+    top = fmaxf(top, x[n].x);
+  }
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+  float sum = 0.f, acc[NV] = {};
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    if (n * 64 >= parts) break;
+    const float f = x[n].y != x[n].y ? __builtin_nanf("") : x[n].x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(x[n].x - top) * x[n].y;
+    sum += f;
+    const int cnt = min(64, parts - n * 64);
+#pragma unroll 8
+    for (int p = w; p < cnt; p += WR) {
+      const float fp = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), p));
+      const float* src = po + (size_t)(n * 64 + p) * rows * D;
 #pragma unroll
       for (int v = 0; v < NV; ++v) acc[v] += fp * src[v];
     }
+  }
+  sum = wave_sum(sum);
+  if constexpr (WR > 1) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) s_acc[w][v][lane] = acc[v];
+    __syncthreads();
+    if (w != 0) return;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) acc[v] = (s_acc[0][v][lane] + s_acc[1][v][lane]) + (s_acc[2][v][lane] + s_acc[3][v][lane]);
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int tok = m / sp.G;
@@ -484,10 +482,13 @@ Choice choose(const t2w_kv8_attention_args& a) {
   c.s.n_tiles = c.s.per_row ? a.n_rows : a.n_tok / c.s.tt + a.n_rows;
   const long max_kv = a.max_kv > 0 ? min((long)a.max_kv, (long)a.width * KV8_BLOCK) : (long)a.width * KV8_BLOCK;
   const long nb = (max_kv + KV8_BLOCK - 1) / KV8_BLOCK, groups = (long)c.s.n_tiles * a.pages.kv_heads;
-  long parts = (2048 + groups - 1) / groups;
-  long bps = (nb + parts - 1) / parts;
-  if (bps < 16) bps = 16;
-  parts = (nb + bps - 1) / bps;
+  long bps = nb;
+  if (nb > 48) {
+    const long parts = (512 + groups - 1) / groups;
+    bps = (nb + parts - 1) / parts;
+    if (bps < 16) bps = 16;
+  }
+  const long parts = (nb + bps - 1) / bps;
   c.s.bps = (int)bps;
   c.s.parts = (int)(parts < 1 ? 1 : parts > 256 ? 256 : parts);
   return c;
@@ -506,8 +507,9 @@ static hipError_t launch(const t2w_kv8_attention_args& a, const Choice& c, hipSt
   if (c.mr == 16) hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 16, 1>), grid, dim3(256), 0, st, a, c.s);
   else if (c.rw == 1) hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 1>), grid, dim3(256), 0, st, a, c.s);
   else hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 2>), grid, dim3(256), 0, st, a, c.s);
-  if (c.s.parts > 1)
-    hipLaunchKernelGGL((kv8_join_kernel<BF, D>), dim3((unsigned)(c.s.n_tiles * a.pages.kv_heads), (c.s.tt * c.s.G + 3) / 4), dim3(256), 0, st, a, c.s);
+  const unsigned groups = (unsigned)(c.s.n_tiles * a.pages.kv_heads), rows = (unsigned)(c.s.tt * c.s.G);
+  if (c.s.parts > 8) hipLaunchKernelGGL((kv8_join_kernel<BF, D, 4>), dim3(groups, rows), dim3(256), 0, st, a, c.s);
+  else if (c.s.parts > 1) hipLaunchKernelGGL((kv8_join_kernel<BF, D, 1>), dim3(groups, (rows + 3) / 4), dim3(256), 0, st, a, c.s);
   return hipGetLastError();
 }
 
