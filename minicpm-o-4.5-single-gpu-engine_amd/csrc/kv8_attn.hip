@@ -2,6 +2,7 @@
 // i sees, key and value codes times their blocks' scales.  Block format: kv8_internal.h.
 #include "kv8_internal.h"
 
+#include <stdlib.h>
 #include <type_traits>
 
 namespace t2w {
@@ -121,8 +122,8 @@ __device__ __forceinline__ float query_max(float v) {
 
 __device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float((uint32_t)min(max(biased, 0), 254) << 23); }
 
-// Softmax state of a wave's queries (lane column = query), shared by both kernels.  Scores are in units of log2, s = q . k
-// times c = scale log2(e) 2^(key exponent).
+// Softmax and output state of a wave's MR packed rows (lane column = query), shared by both kernels.  Scores are in units of
+// log2, s = q . k times c = scale log2(e) 2^(key exponent).
 //  * m is a reference that the running maximum may pass by 8 before it is moved (by the whole wave, then the true maximum so
 //    far): probabilities are 2^(s - m + 7) <= 2^15 in fp16, so most blocks need no exchange between lanes and no rescaling of
 //    the outputs, and a probability keeps fp16's 11 bits down to 2^-21 of the largest and 2^-32 of it absolutely.  fp16 and
@@ -130,21 +131,183 @@ __device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float(
 //  * value codes enter as fp16, exact, times 2^(their exponent - E + 7), E the largest value exponent so far: 22 powers of two
 //    below the largest block's scale stay exact.
 //  * sums of probabilities come from the matrix unit too (a row of ones): the same rounded probabilities as the outputs'.
-struct Soft {
+template <int MR, int D>
+struct State {
+  static constexpr int AR = MR == 16 ? 4 : 16;     // values of an accumulator
+  static constexpr int KG = MR == 16 ? 2 : 1;      // score tiles of a block
+  static constexpr int NP = MR == 16 ? 1 : 2;      // probability operands of a block
+  static constexpr int NT = D / (2 * MR);          // output tile pairs: channels 2 p and 2 p + 1, p = MR t + i
+  typedef typename std::conditional<MR == 16, f32x4, f32x16>::type Acc;
+  Acc o[NT][2], l;
   float m = -__builtin_inff();  // reference
   float nb = 7.f;               // 7 - m, 7 where m is -inf
   bool big = false;             // |m| so large that s - m in one fma would not be exact enough: scale the scores first
-};
+  int E = 0;                    // biased value exponent that o is in units of; 0: none yet
 
-template <typename Acc>
-__device__ __forceinline__ void scale_acc(Acc& o, float f) {
+  __device__ __forceinline__ State() {
 #pragma unroll
-  for (int r = 0; r < (int)(sizeof(Acc) / 4); ++r) o[r] *= f;
-}
+    for (int r = 0; r < AR; ++r) l[r] = 0.f;
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < AR; ++r) o[x][j][r] = 0.f;
+  }
+  __device__ __forceinline__ void scale_o(float f) {
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < AR; ++r) o[x][j][r] *= f;
+  }
+  // o in units of exponent e from here on
+  __device__ __forceinline__ void raise(int e) {
+    if (e > E) {
+      scale_o(E == 0 ? 0.f : pow2_bits(E - e + 127));
+      E = e;
+    }
+  }
+  // key of score r of tile x within its block
+  static __device__ __forceinline__ int key_of(int x, int r, int g) { return MR == 16 ? 8 * g + 4 * x + r : 16 * (r >> 3) + 8 * g + (r & 7); }
+
+  // Probabilities of NB blocks' scores in units 1 / c[y], invisible ones -inf; moves the reference where needed.
+  template <int NB>
+  __device__ __forceinline__ void probabilities(Acc (&sc)[NB][KG], float (&c)[NB], f16x8 (&p)[NB][NP]) {
+    float mx = -__builtin_inff();
+#pragma unroll
+    for (int y = 0; y < NB; ++y) {
+      float v = sc[y][0][0];
+#pragma unroll
+      for (int x = 0; x < KG; ++x)
+#pragma unroll
+        for (int r = 0; r < AR; ++r) v = fmaxf(v, sc[y][x][r]);
+      mx = fmaxf(mx, v * c[y]);
+    }
+    if (__builtin_amdgcn_ballot_w64(mx > m + 8.f)) {
+      const float mn = fmaxf(m, query_max<MR>(mx));
+      const float alpha = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      nb = mn == -__builtin_inff() ? 7.f : 7.f - mn;
+      big = big || __builtin_amdgcn_ballot_w64(fabsf(mn) > 4194304.f && mn != -__builtin_inff()) != 0;
+#pragma unroll
+      for (int r = 0; r < AR; ++r) l[r] *= alpha;
+      scale_o(alpha);
+    }
+    if (big) {
+#pragma unroll
+      for (int y = 0; y < NB; ++y) {
+#pragma unroll
+        for (int x = 0; x < KG; ++x)
+#pragma unroll
+          for (int r = 0; r < AR; ++r) sc[y][x][r] *= c[y];
+        c[y] = 1.f;
+      }
+    }
+#pragma unroll
+    for (int y = 0; y < NB; ++y)
+#pragma unroll
+      for (int x = 0; x < NP; ++x)
+#pragma unroll
+        for (int z = 0; z < 8; z += 2) {
+          float e[2];
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const float s = MR == 16 ? sc[y][(z + w) / 4 % KG][(z + w) % 4] : sc[y][0][8 * x + z + w];
+            e[w] = __builtin_amdgcn_exp2f(fmaf(s, c[y], nb));
+          }
+          const f16x2_t h = __builtin_convertvector((f32x2_t{e[0], e[1]}), f16x2_t);
+          p[y][x][z] = h[0];
+          p[y][x][z + 1] = h[1];
+        }
+    f16x8 one;
+#pragma unroll
+    for (int z = 0; z < 8; ++z) one[z] = (_Float16)1.0f;
+#pragma unroll
+    for (int y = 0; y < NB; ++y)
+#pragma unroll
+      for (int x = 0; x < NP; ++x) l = mfma_pv(one, p[y][x], l);
+  }
+
+  // the other state of the same rows, left in LDS by another wave (`put`), folded into this one
+  static constexpr int WORDS = NT * 2 * AR + 2;
+  __device__ __forceinline__ void put(float (*dst)[64], int lane) const {
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < AR; ++r) dst[(x * 2 + j) * AR + r][lane] = o[x][j][r];
+    dst[WORDS - 2][lane] = m;
+    dst[WORDS - 1][lane] = l[0];
+  }
+  __device__ __forceinline__ void fold(const float (*src)[64], int e2, int lane) {
+    const float m2 = src[WORDS - 2][lane], l2 = src[WORDS - 1][lane];
+    const int en = max(E, e2);
+    const float mn = fmaxf(m, m2);
+    const float f1 = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+    const float f2 = m2 == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m2 - mn);
+    // a state whose reference never moved holds zeros, or NaN from scores that were none
+    const float k1 = l[0] != l[0] ? __builtin_nanf("") : f1, k2 = l2 != l2 ? __builtin_nanf("") : f2;
+    const float g1 = E == en ? k1 : k1 * (E == 0 ? 0.f : pow2_bits(E - en + 127)), g2 = e2 == en ? k2 : k2 * (e2 == 0 ? 0.f : pow2_bits(e2 - en + 127));
+    l[0] = l[0] * k1 + l2 * k2;
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < AR; ++r) o[x][j][r] = o[x][j][r] * g1 + src[(x * 2 + j) * AR + r][lane] * g2;
+    m = mn;
+    E = en;
+  }
+
+  // Row mrow of the tile (lane group g): to the outputs, or to the call's workspace where the tile has several parts
+  template <bool BF>
+  __device__ __forceinline__ void store(const t2w_kv8_attention_args& a, const KV8Split& sp, const Tile& t, int slot, int kv_head, int part, int parts,
+                                        int mrow, int g) const {
+    const float unit = pow2_bits(E) * 0.0078125f;  // 2^(E - 127 - 7); E = 0: no value block at all, o is zero
+    const float inv = l[0] == 0.f ? 0.f : 1.f / l[0];
+    // values r .. r + 3 of both tiles of a pair are 8 consecutive channels, from d on
+    if (parts == 1) {
+      const int tok = mrow / sp.G, hq = mrow - tok * sp.G;
+      uint16_t* out = (uint16_t*)a.out + (long long)(t.start + t.i0 + tok) * a.ldo + (kv_head * sp.G + hq) * D;
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int r = 0; r < AR; r += 4) {
+          const int d = MR == 16 ? 32 * x + 8 * g : 64 * x + 4 * r + 8 * g;
+          uint32_t w[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const float u = o[x][0][r + y] * inv * unit, v = o[x][1][r + y] * inv * unit;
+            w[y] = BF ? pack2(u, v) : pack2h(u, v);
+          }
+          *(uint4*)(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    } else {
+      const size_t pr = ((size_t)slot * a.pages.kv_heads + kv_head) * sp.parts + part, rows = sp.tt * sp.G;
+      float* po = (float*)a.workspace + (pr * rows + mrow) * D;
+      float* ml = (float*)a.workspace + part_rows(sp, a.pages.kv_heads) * D + (pr * rows + mrow) * 2;
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int r = 0; r < AR; r += 4) {
+          const int d = MR == 16 ? 32 * x + 8 * g : 64 * x + 4 * r + 8 * g;
+#pragma unroll
+          for (int y = 0; y < 4; y += 2)
+            *(float4*)(po + d + 2 * y) = make_float4(o[x][0][r + y] * inv * unit, o[x][1][r + y] * inv * unit, o[x][0][r + y + 1] * inv * unit,
+                                                     o[x][1][r + y + 1] * inv * unit);
+        }
+      if (g == 0) *(float2*)ml = make_float2(m, l[0]);
+    }
+  }
+};
 
 // Direct form, for tiles of few packed rows (steps, draft checks, windows of up to 64 packed rows): every wave loads its key
 // and value fragments from the pages into registers and converts them there; no LDS and no barrier before the end.  RW waves
-// of MR packed rows each, times 4 / RW waves that take every (4 / RW)-th block; their states are merged through LDS.
+// of MR packed rows each, times 4 / RW waves that take every (4 / RW)-th run of NB blocks; their states are merged through
+// LDS.
 //
 // Bound by memory: 2 D codes a token and key head are read once and meet at least MR query columns of the matrix unit, whose
 // unused columns cost nothing that matters.  MR = 16 (16x16x32 MFMA) has half the softmax work of MR = 32 (32x32x16) where
@@ -153,18 +316,16 @@ __device__ __forceinline__ void scale_acc(Acc& o, float f) {
 // With S^T = K . Q^T the score MFMA leaves a lane scores of its own query only; the rows of K are fed in an order that makes
 // them the 8 (MR = 16) or 2 x 8 keys whose value bytes the same lane loads as the P . V operand:
 //   MR 16: lane (i = l % 16, g = l / 16); key operand kg row i = key 8 (i / 4) + 4 kg + i % 4, its scores: keys 8 g + 4 kg + r
-//   MR 32: lane (i = l % 32, h = l / 32); row i = key with bits 2 and 3 of i swapped, scores r: keys 16 (r / 8) + 8 h + r % 8
+//   MR 32: lane (i = l % 32, g = l / 32); row i = key with bits 2 and 3 of i swapped, scores r: keys 16 (r / 8) + 8 g + r % 8
 // Channels are paired the same way on both sides: lane group x loads the 16-channel chunk n x' + x of keys and queries.
-template <bool BF, int D, int MR, int RW>
-__global__ void __launch_bounds__(256, MR == 16 ? (D == 64 ? 5 : 4) : (D == 64 ? 3 : 2)) kv8_attn_direct_kernel(t2w_kv8_attention_args a, KV8Split sp) {
+template <bool BF, int D, int MR, int RW, int NB, int OCC>
+__global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_attention_args a, KV8Split sp) {
+  typedef State<MR, D> St;
   constexpr int KW = 4 / RW;                       // waves that share the keys of the same packed rows
   constexpr int LG = 64 / MR;                      // lane groups: 4 or 2
   constexpr int NQ = D / (8 * LG), NL = D / 32;    // query operands; 16-byte loads of a block's keys, and of its values
-  constexpr int KG = MR == 16 ? 2 : 1;             // score MFMA tiles of a block
-  constexpr int NT = D / (2 * MR);                 // output tile pairs (channel pairs 2 p, 2 p + 1, p = MR t + i)
-  typedef typename std::conditional<MR == 16, f32x4, f32x16>::type Acc;
-  constexpr int AR = MR == 16 ? 4 : 16;            // values of an Acc
-  __shared__ float s_acc[(KW > 1 ? KW / 2 : 1) * RW][NT * 2 * AR + 2][64];
+  constexpr int KG = St::KG, AR = St::AR, NP = St::NP;
+  __shared__ float s_acc[KW / 2 * RW][St::WORDS][64];
   __shared__ int s_e[4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wave % RW, kw = wave / RW;
   const int slot = blockIdx.x / a.pages.kv_heads, kv_head = blockIdx.x - slot * a.pages.kv_heads, part = blockIdx.y;
@@ -183,8 +344,9 @@ __global__ void __launch_bounds__(256, MR == 16 ? (D == 64 ? 5 : 4) : (D == 64 ?
   const bool idle = m0 >= t.rows;  // a wave without rows still meets the barriers
   const int mrow = m0 + i;
   const int tok = min(mrow, t.rows - 1) / sp.G, hq = min(mrow, t.rows - 1) - tok * sp.G;
-  const int lim = seen_by(a, t, t.i0 + tok);
-  const int lim_lo = seen_by(a, t, t.i0 + min(m0, t.rows - 1) / sp.G);  // the wave's first query sees least
+  const int lim = min(seen_by(a, t, t.i0 + tok), b1 * KV8_BLOCK);  // NB > 1: a last run may reach beyond the part
+  const int lim_lo = min(seen_by(a, t, t.i0 + min(m0, t.rows - 1) / sp.G), b1 * KV8_BLOCK);  // the wave's first query sees least
+  const int v_end = min(t.total, b1 * KV8_BLOCK);
 
   uint4 q[NQ];
   {
@@ -192,16 +354,7 @@ __global__ void __launch_bounds__(256, MR == 16 ? (D == 64 ? 5 : 4) : (D == 64 ?
 #pragma unroll
     for (int n = 0; n < NQ; ++n) q[n] = *(const uint4*)(src + (LG * (n >> 1) + g) * 16 + (n & 1) * 8);
   }
-  Acc o[NT][2], l;
-  for (int r = 0; r < AR; ++r) l[r] = 0.f;
-#pragma unroll
-  for (int x = 0; x < NT; ++x)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < AR; ++r) o[x][j][r] = 0.f;
-  Soft st;
-  int E = 0;  // biased value exponent that o is in units of
+  St st;
   const float c0 = a.scale * 1.4426950408889634f;
 
   // the lane's place in a block's keys and values; its loads lie at constant distances from there (load offsets)
@@ -212,199 +365,274 @@ __global__ void __launch_bounds__(256, MR == 16 ? (D == 64 ? 5 : 4) : (D == 64 ?
   const uint8_t* vbase = (const uint8_t*)a.pages.v + (size_t)kv_head * (KV8_BLOCK * D);
   const int* table = a.table + (size_t)t.row * a.ld_table;
 
-  // one block's codes; the next block's keys are loaded as soon as the scores have used these, its values after P . V
-  uint4 kf[NL], vf[NL];
-  auto load_k = [&](int id) {
-    const uint8_t* kp = kbase + (size_t)id * stride;
+  // one run's codes; the next run's keys are loaded as soon as the scores have used these, its values after P . V
+  uint4 kf[NB][NL], vf[NB][NL];
+  auto load_k = [&](int ids, int x) {
 #pragma unroll
-    for (int n = 0; n < NL; ++n) kf[n] = *(const uint4*)(kp + koff + (MR == 16 ? (n / 2) * 2048 + (n % 2) * 64 : n * 1024));
+    for (int y = 0; y < NB; ++y) {
+      const uint8_t* kp = kbase + (size_t)__builtin_amdgcn_readlane(ids, x * NB + y) * stride;
+#pragma unroll
+      for (int n = 0; n < NL; ++n) kf[y][n] = *(const uint4*)(kp + koff + (MR == 16 ? (n / 2) * 2048 + (n % 2) * 64 : n * 1024));
+    }
   };
-  auto load_v = [&](int id) {
-    const uint8_t* vp = vbase + (size_t)id * stride;
+  auto load_v = [&](int ids, int x) {
 #pragma unroll
-    for (int n = 0; n < NL; ++n) vf[n] = *(const uint4*)(vp + voff + (MR == 16 ? n * 256 : (n % 2) * 16 * D + (n / 2) * 512));
-  };
-  auto step = [&](int b, int ke, int ve, int next) {  // next: the block id to load, -1: none
-    Acc sc[KG];
+    for (int y = 0; y < NB; ++y) {
+      const uint8_t* vp = vbase + (size_t)__builtin_amdgcn_readlane(ids, x * NB + y) * stride;
 #pragma unroll
-    for (int x = 0; x < KG; ++x)
-#pragma unroll
-      for (int r = 0; r < AR; ++r) sc[x][r] = 0.f;
-#pragma unroll
-    for (int n = 0; n < NL; ++n) {
-      const int x = MR == 16 ? n % 2 : 0, j = MR == 16 ? n / 2 : n;
-      sc[x] = mfma_qk<BF>(kf[n].x, kf[n].y, q[2 * j], sc[x]);
-      sc[x] = mfma_qk<BF>(kf[n].z, kf[n].w, q[2 * j + 1], sc[x]);
+      for (int n = 0; n < NL; ++n) vf[y][n] = *(const uint4*)(vp + voff + (MR == 16 ? n * 256 : (n % 2) * 16 * D + (n / 2) * 512));
     }
-    if (next >= 0) load_k(next);
-    float c = c0 * pow2_bits(ke);
-    const int key0 = b * KV8_BLOCK;
-    const bool off = ke > 254;  // a block id outside the pages, or an E8M0 NaN
-    if (off) c = c0;
-    if (off || key0 + KV8_BLOCK > lim_lo) {  // or some query of the wave does not see all of the block
-#pragma unroll
-      for (int x = 0; x < KG; ++x)
-#pragma unroll
-        for (int r = 0; r < AR; ++r) {
-          const int key = MR == 16 ? 8 * g + 4 * x + r : 16 * (r >> 3) + 8 * g + (r & 7);
-          sc[x][r] = key0 + key < lim ? (off ? __builtin_nanf("") : sc[x][r]) : -__builtin_inff();
-        }
-    }
-    if (key0 + KV8_BLOCK > t.total) {  // the row's last block: values behind its last token count as zeros, whatever they are
-#pragma unroll
-      for (int n = 0; n < NL; ++n) {
-        const int gr = MR == 16 ? g : 2 * (n % 2) + g, left = t.total - key0 - 8 * gr;
-        const uint64_t keep = left >= 8 ? ~0ull : left <= 0 ? 0ull : (1ull << (8 * left)) - 1ull;
-        vf[n].x &= (uint32_t)keep; vf[n].y &= (uint32_t)(keep >> 32);
-        vf[n].z &= (uint32_t)keep; vf[n].w &= (uint32_t)(keep >> 32);
-      }
-    }
-    float mx = sc[0][0];
-#pragma unroll
-    for (int x = 0; x < KG; ++x)
-#pragma unroll
-      for (int r = 0; r < AR; ++r) mx = fmaxf(mx, sc[x][r]);
-    mx *= c;
-    if (__builtin_amdgcn_ballot_w64(mx > st.m + 8.f)) {
-      const float mn = fmaxf(st.m, query_max<MR>(mx));
-      const float alpha = st.m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(st.m - mn);
-      st.m = mn;
-      st.nb = mn == -__builtin_inff() ? 7.f : 7.f - mn;
-      st.big = st.big || __builtin_amdgcn_ballot_w64(fabsf(mn) > 4194304.f && mn != -__builtin_inff()) != 0;
-      scale_acc(l, alpha);
-#pragma unroll
-      for (int x = 0; x < NT; ++x) { scale_acc(o[x][0], alpha); scale_acc(o[x][1], alpha); }
-    }
-    if (st.big) {
-#pragma unroll
-      for (int x = 0; x < KG; ++x)
-#pragma unroll
-        for (int r = 0; r < AR; ++r) sc[x][r] *= c;
-      c = 1.f;
-    }
-    if (ve > E) {
-      const float f2 = E == 0 ? 0.f : pow2_bits(E - ve + 127);
-#pragma unroll
-      for (int x = 0; x < NT; ++x) { scale_acc(o[x][0], f2); scale_acc(o[x][1], f2); }
-      E = ve;
-    }
-    const float vs = pow2_bits(ve - E + 127 + 7);
-    constexpr int NP = MR == 16 ? 1 : 2;  // P operands of a block
-    f16x8 p[NP], one;
-#pragma unroll
-    for (int x = 0; x < NP; ++x)
-#pragma unroll
-      for (int y = 0; y < 8; y += 2) {
-        float e[2];
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const float s = MR == 16 ? sc[(y + z) / 4 % KG][(y + z) % 4] : sc[0][8 * x + y + z];
-          e[z] = __builtin_amdgcn_exp2f(fmaf(s, c, st.nb));
-        }
-        const f16x2_t h = __builtin_convertvector((f32x2_t{e[0], e[1]}), f16x2_t);
-        p[x][y] = h[0];
-        p[x][y + 1] = h[1];
-      }
-#pragma unroll
-    for (int y = 0; y < 8; ++y) one[y] = (_Float16)1.0f;
-#pragma unroll
-    for (int x = 0; x < NP; ++x) l = mfma_pv(one, p[x], l);
-#pragma unroll
-    for (int n = 0; n < NL; ++n) {
-      const int x = MR == 16 ? n : n / 2, kk = MR == 16 ? 0 : n % 2;
-      o[x][0] = mfma_pv(codes_f16(vf[n].x, vf[n].y, vs), p[kk], o[x][0]);
-      o[x][1] = mfma_pv(codes_f16(vf[n].z, vf[n].w, vs), p[kk], o[x][1]);
-    }
-    if (next >= 0) load_v(next);
   };
 
   if (!idle) {
-    // the wave's blocks b0 + kw, + KW, ...: ids and exponents of the next 64 of them one a lane
-    for (int base = b0 + kw; base < b1; base += 64 * KW) {
-      const int mine = base + lane * KW;
-      int id = mine < b1 ? table[mine] : 0, ke = 255, ve = 0;
-      if ((unsigned)id < (unsigned)a.pages.n_blocks) {
-        ke = a.pages.k_exp[(size_t)id * a.pages.kv_heads + kv_head];
-        ve = a.pages.v_exp[(size_t)id * a.pages.kv_heads + kv_head];
-      } else {
-        id = 0;
+    // the wave's runs: first blocks b0 + NB kw, + NB KW, ...; ids and exponents of the next 64 blocks one a lane
+    for (int base = b0 + NB * kw; base < b1; base += 64 * KW) {
+      const int mine = base + (lane / NB) * (NB * KW) + lane % NB;
+      int id = mine < b1 ? table[mine] : 0, ke = 127, ve = 0;  // a run's blocks beyond the part: nobody sees them
+      if (mine < b1) {
+        if ((unsigned)id < (unsigned)a.pages.n_blocks) {
+          ke = a.pages.k_exp[(size_t)id * a.pages.kv_heads + kv_head];
+          ve = a.pages.v_exp[(size_t)id * a.pages.kv_heads + kv_head];
+        } else {
+          id = 0;
+          ke = 255;
+        }
       }
-      const int n = min(64, (b1 - base + KW - 1) / KW);
-      load_k(__builtin_amdgcn_readlane(id, 0));
-      load_v(__builtin_amdgcn_readlane(id, 0));
-      for (int x = 0; x < n; ++x)
-        step(base + x * KW, __builtin_amdgcn_readlane(ke, x), __builtin_amdgcn_readlane(ve, x), x + 1 < n ? __builtin_amdgcn_readlane(id, x + 1) : -1);
+      const int n = min(64 / NB, (b1 - base + NB * KW - 1) / (NB * KW));
+      load_k(id, 0);
+      load_v(id, 0);
+      for (int x = 0; x < n; ++x) {
+        typename St::Acc sc[NB][KG];
+        float c[NB];
+#pragma unroll
+        for (int y = 0; y < NB; ++y) {
+#pragma unroll
+          for (int z = 0; z < KG; ++z)
+#pragma unroll
+            for (int r = 0; r < AR; ++r) sc[y][z][r] = 0.f;
+#pragma unroll
+          for (int w = 0; w < NL; ++w) {
+            const int z = MR == 16 ? w % 2 : 0, j = MR == 16 ? w / 2 : w;
+            sc[y][z] = mfma_qk<BF>(kf[y][w].x, kf[y][w].y, q[2 * j], sc[y][z]);
+            sc[y][z] = mfma_qk<BF>(kf[y][w].z, kf[y][w].w, q[2 * j + 1], sc[y][z]);
+          }
+        }
+        if (x + 1 < n) load_k(id, x + 1);
+        int ve_top = 0;
+#pragma unroll
+        for (int y = 0; y < NB; ++y) {
+          const int kx = __builtin_amdgcn_readlane(ke, x * NB + y), key0 = (base + x * NB * KW + y) * KV8_BLOCK;
+          const bool off = kx > 254;  // a block id outside the pages, or an E8M0 NaN
+          c[y] = off ? c0 : c0 * pow2_bits(kx);
+          if (off || key0 + KV8_BLOCK > lim_lo) {  // or some query of the wave does not see all of the block
+#pragma unroll
+            for (int z = 0; z < KG; ++z)
+#pragma unroll
+              for (int r = 0; r < AR; ++r)
+                sc[y][z][r] = key0 + St::key_of(z, r, g) < lim ? (off ? __builtin_nanf("") : sc[y][z][r]) : -__builtin_inff();
+          }
+          if (off || key0 + KV8_BLOCK > v_end) {  // values behind the last token count as zeros, whatever they are
+#pragma unroll
+            for (int w = 0; w < NL; ++w) {
+              const int left = off ? 0 : v_end - key0 - 8 * (MR == 16 ? g : 2 * (w % 2) + g);
+              const uint64_t keep = left >= 8 ? ~0ull : left <= 0 ? 0ull : (1ull << (8 * left)) - 1ull;
+              vf[y][w].x &= (uint32_t)keep; vf[y][w].y &= (uint32_t)(keep >> 32);
+              vf[y][w].z &= (uint32_t)keep; vf[y][w].w &= (uint32_t)(keep >> 32);
+            }
+          }
+          ve_top = max(ve_top, __builtin_amdgcn_readlane(ve, x * NB + y));
+        }
+        f16x8 p[NB][NP];
+        st.template probabilities<NB>(sc, c, p);
+        st.raise(ve_top);
+#pragma unroll
+        for (int y = 0; y < NB; ++y) {
+          const float vs = pow2_bits(__builtin_amdgcn_readlane(ve, x * NB + y) - st.E + 127 + 7);
+#pragma unroll
+          for (int w = 0; w < NL; ++w) {
+            const int z = MR == 16 ? w : w / 2, kk = MR == 16 ? 0 : w % 2;
+            st.o[z][0] = mfma_pv(codes_f16(vf[y][w].x, vf[y][w].y, vs), p[y][kk], st.o[z][0]);
+            st.o[z][1] = mfma_pv(codes_f16(vf[y][w].z, vf[y][w].w, vs), p[y][kk], st.o[z][1]);
+          }
+        }
+        if (x + 1 < n) load_v(id, x + 1);
+      }
     }
   }
   // merge the key waves pairwise: the upper half leaves its state, the lower half folds it in
 #pragma unroll
   for (int w = KW / 2; w >= 1; w /= 2) {
     if (kw >= w && kw < 2 * w) {
-      float (*dst)[64] = s_acc[(kw - w) * RW + rw];
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int r = 0; r < AR; ++r) dst[(x * 2 + j) * AR + r][lane] = o[x][j][r];
-      dst[NT * 2 * AR][lane] = st.m;
-      dst[NT * 2 * AR + 1][lane] = l[0];
-      if (lane == 0) s_e[wave] = E;
+      st.put(s_acc[(kw - w) * RW + rw], lane);
+      if (lane == 0) s_e[wave] = st.E;
     }
     __syncthreads();
-    if (kw < w) {
-      const float (*src)[64] = s_acc[kw * RW + rw];
-      const float m2 = src[NT * 2 * AR][lane], l2 = src[NT * 2 * AR + 1][lane];
-      const int e2 = s_e[wave + w * RW], en = max(E, e2);
-      const float mn = fmaxf(st.m, m2);
-      const float f1 = st.m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(st.m - mn);
-      const float f2 = m2 == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m2 - mn);
-      // a state whose reference never moved holds zeros, or NaN from scores that were none
-      const float k1 = l[0] != l[0] ? __builtin_nanf("") : f1, k2 = l2 != l2 ? __builtin_nanf("") : f2;
-      const float g1 = E == en ? k1 : k1 * (E == 0 ? 0.f : pow2_bits(E - en + 127)), g2 = e2 == en ? k2 : k2 * (e2 == 0 ? 0.f : pow2_bits(e2 - en + 127));
-      l[0] = l[0] * k1 + l2 * k2;
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int r = 0; r < AR; ++r) o[x][j][r] = o[x][j][r] * g1 + src[(x * 2 + j) * AR + r][lane] * g2;
-      st.m = mn;
-      E = en;
-    }
+    if (kw < w) st.fold(s_acc[kw * RW + rw], s_e[wave + w * RW], lane);
     if (w > 1) __syncthreads();
   }
-  if (kw != 0 || mrow >= t.rows) return;
-  const float unit = pow2_bits(E) * 0.0078125f;  // 2^(E - 127 - 7); E = 0: no value block at all, o is zero
-  const float inv = l[0] == 0.f ? 0.f : 1.f / l[0];
-  if (parts == 1) {
-    uint16_t* out = (uint16_t*)a.out + (long long)(t.start + t.i0 + tok) * a.ldo + (kv_head * sp.G + hq) * D;
-#pragma unroll
-    for (int x = 0; x < NT; ++x)
-#pragma unroll
-      for (int r = 0; r < AR; r += 4) {
-        // values r .. r + 3 of both tiles: 8 consecutive channels
-        const int d = MR == 16 ? 32 * x + 8 * g : 64 * x + 4 * r + 8 * g;
-        uint32_t w[4];
-#pragma unroll
-        for (int y = 0; y < 4; ++y) w[y] = BF ? pack2(o[x][0][r + y] * inv * unit, o[x][1][r + y] * inv * unit) : pack2h(o[x][0][r + y] * inv * unit, o[x][1][r + y] * inv * unit);
-        *(uint4*)(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-  } else {
-    const size_t pr = ((size_t)slot * a.pages.kv_heads + kv_head) * sp.parts + part, rows = sp.tt * sp.G;
-    float* po = (float*)a.workspace + (pr * rows + mrow) * D;
-    float* ml = (float*)a.workspace + part_rows(sp, a.pages.kv_heads) * D + (pr * rows + mrow) * 2;
-#pragma unroll
-    for (int x = 0; x < NT; ++x)
-#pragma unroll
-      for (int r = 0; r < AR; r += 4) {
-        const int d = MR == 16 ? 32 * x + 8 * g : 64 * x + 4 * r + 8 * g;
-#pragma unroll
-        for (int y = 0; y < 4; y += 2)
-          *(float4*)(po + d + 2 * y) = make_float4(o[x][0][r + y] * inv * unit, o[x][1][r + y] * inv * unit, o[x][0][r + y + 1] * inv * unit, o[x][1][r + y + 1] * inv * unit);
-      }
-    if (g == 0) *(float2*)ml = make_float2(st.m, l[0]);
+  if (kw == 0 && mrow < t.rows) st.template store<BF>(a, sp, t, slot, kv_head, part, parts, mrow, g);
+}
+
+// Tile form, for tiles of many packed rows (prompts): RW waves of 32 packed rows each share the keys, two blocks a step.  The
+// workgroup loads a step's codes (one step ahead, in registers), converts them once, and leaves them in LDS as the MFMA
+// operands (double buffered, one barrier a step); every wave then reads whole fragments, 16 consecutive bytes a lane.
+template <bool BF, int D, int RW>
+__global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_attention_args a, KV8Split sp) {
+  typedef State<32, D> St;
+  constexpr int T = 64 * RW, NC = 4 * D / T;  // threads; 16-byte code chunks of a step's keys, and of its values, a thread
+  constexpr int CB = 2 * D;                   // chunks of a block
+  __shared__ uint4 s_k[2][2][2 * CB], s_v[2][2][2 * CB];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // the last tiles first: a causal prompt's longest
+  const int slot = sp.n_tiles - 1 - blockIdx.x / a.pages.kv_heads, kv_head = blockIdx.x % a.pages.kv_heads, part = blockIdx.y;
+  Tile t;
+  if (!find_tile(a, sp, slot, t)) return;
+  if (t.bad) {
+    if (part == 0) nan_tile<BF, D>(a, sp, t, kv_head, tid, T);
+    return;
   }
+  int per;
+  const int parts = tile_parts(sp, t.end, per);
+  if (part >= parts) return;
+  const int b0 = part * per, b1 = min(b0 + per, (t.end + KV8_BLOCK - 1) / KV8_BLOCK), steps = (b1 - b0 + 1) / 2;
+  const int i = lane & 31, g = lane >> 5;
+  const int m0 = wave * 32, mrow = m0 + i, last = min(m0 + 31, t.rows - 1);
+  const int tok = min(mrow, t.rows - 1) / sp.G, hq = min(mrow, t.rows - 1) - tok * sp.G;
+  const int lim = min(seen_by(a, t, t.i0 + tok), b1 * KV8_BLOCK);
+  const int lim_lo = min(seen_by(a, t, t.i0 + min(m0, t.rows - 1) / sp.G), b1 * KV8_BLOCK);
+  const int lim_hi = m0 >= t.rows ? 0 : min(seen_by(a, t, t.i0 + last / sp.G), b1 * KV8_BLOCK);  // the wave's rows see no key from there on
+  const int v_end = min(t.total, b1 * KV8_BLOCK);
+
+  uint4 q[D / 16];
+  {
+    const uint16_t* src = (const uint16_t*)a.q + (long long)(t.start + t.i0 + tok) * a.ldq + (kv_head * sp.G + hq) * D;
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) q[n] = *(const uint4*)(src + (2 * (n >> 1) + g) * 16 + (n & 1) * 8);
+  }
+  St st;
+  const float c0 = a.scale * 1.4426950408889634f;
+  const size_t stride = (size_t)a.pages.kv_heads * (KV8_BLOCK * D);
+  const uint8_t* kbase = (const uint8_t*)a.pages.k + (size_t)kv_head * (KV8_BLOCK * D);
+  const uint8_t* vbase = (const uint8_t*)a.pages.v + (size_t)kv_head * (KV8_BLOCK * D);
+  const int* table = a.table + (size_t)t.row * a.ld_table;
+
+  // ids and exponents of 64 blocks (32 steps) one a lane, the next 64's on the way
+  auto ids_of = [&](int chunk) {
+    const int b = b0 + chunk * 64 + lane;
+    return b < b1 ? table[b] : 0;
+  };
+  auto exps_of = [&](int chunk, int& id, int& ke, int& ve) {
+    ke = 127;
+    ve = 0;
+    if (b0 + chunk * 64 + lane >= b1) return;  // a last step's second block beyond the part: nobody sees it
+    if ((unsigned)id < (unsigned)a.pages.n_blocks) {
+      ke = a.pages.k_exp[(size_t)id * a.pages.kv_heads + kv_head];
+      ve = a.pages.v_exp[(size_t)id * a.pages.kv_heads + kv_head];
+    } else {
+      id = 0;
+      ke = 255;
+    }
+  };
+  int id = ids_of(0), ke, ve;
+  exps_of(0, id, ke, ve);
+  int id2 = ids_of(1), ke2 = 127, ve2 = 0;
+
+  uint4 rk[NC], rv[NC];
+  int nke[2], nve[2];  // exponents of the step in registers
+  int nE = 0;          // value unit of the step that was converted last
+  auto load = [&](int s) {
+    const int x = 2 * (s & 31);
+    if (s > 0 && x == 0) { id = id2; ke = ke2; ve = ve2; id2 = ids_of(s / 32 + 1); }
+    if (x == 32) exps_of(s / 32 + 1, id2, ke2, ve2);
+    nke[0] = __builtin_amdgcn_readlane(ke, x); nke[1] = __builtin_amdgcn_readlane(ke, x + 1);
+    nve[0] = __builtin_amdgcn_readlane(ve, x); nve[1] = __builtin_amdgcn_readlane(ve, x + 1);
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const int y = __builtin_amdgcn_readfirstlane((tid + T * n) / CB), r = (tid + T * n) % CB;
+      const size_t page = (size_t)__builtin_amdgcn_readlane(id, x + y) * stride;
+      rk[n] = *(const uint4*)(kbase + page + (uint32_t)(r * 16));
+      rv[n] = *(const uint4*)(vbase + page + (uint32_t)(r * 16));
+    }
+  };
+  auto convert = [&](int s, int buf) {
+    nE = max(nE, max(nve[0], nve[1]));
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const int y = __builtin_amdgcn_readfirstlane((tid + T * n) / CB), r = (tid + T * n) % CB;
+      const int ex = y ? nke[1] : nke[0], key0 = (b0 + 2 * s + y) * KV8_BLOCK;
+      const float vs = pow2_bits((y ? nve[1] : nve[0]) - nE + 127 + 7);
+      uint4 v = rv[n];
+      if (ex > 254 || key0 + KV8_BLOCK > v_end) {  // values behind the last token count as zeros, whatever they are
+        const int left = ex > 254 ? 0 : v_end - key0 - 8 * (r / (D / 2));
+        const uint64_t keep = left >= 8 ? ~0ull : left <= 0 ? 0ull : (1ull << (8 * left)) - 1ull;
+        v.x &= (uint32_t)keep; v.y &= (uint32_t)(keep >> 32);
+        v.z &= (uint32_t)keep; v.w &= (uint32_t)(keep >> 32);
+      }
+      // keys: chunk c of 16 channels, key k -> two operands of 8 channels, at the key's operand row
+      const int c = r >> 5, k = r & 31, row = (k & 0x13) | ((k & 4) << 1) | ((k & 8) >> 1);
+      uint4* kd = &s_k[buf][y][c * 64 + row];
+      if constexpr (BF) {
+        kd[0] = __builtin_bit_cast(uint4, codes_bf16(rk[n].x, rk[n].y));
+        kd[32] = __builtin_bit_cast(uint4, codes_bf16(rk[n].z, rk[n].w));
+      } else {
+        kd[0] = __builtin_bit_cast(uint4, codes_f16(rk[n].x, rk[n].y, 1.f));
+        kd[32] = __builtin_bit_cast(uint4, codes_f16(rk[n].z, rk[n].w, 1.f));
+      }
+      // values: group of 8 keys, channel pair -> an operand of 8 keys for each channel
+      uint4* vd = &s_v[buf][y][r / (D / 2) * D + r % (D / 2)];
+      vd[0] = __builtin_bit_cast(uint4, codes_f16(v.x, v.y, vs));
+      vd[D / 2] = __builtin_bit_cast(uint4, codes_f16(v.z, v.w, vs));
+    }
+  };
+
+  load(0);
+  convert(0, 0);
+  __syncthreads();
+  for (int s = 0; s < steps; ++s) {
+    const int buf = s & 1, E = nE, kx[2] = {nke[0], nke[1]};
+    if (s + 1 < steps) load(s + 1);
+    const int key0 = (b0 + 2 * s) * KV8_BLOCK;
+    if (key0 < lim_hi) {
+      typename St::Acc sc[2][1];
+      float c[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[y][0][r] = 0.f;
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+          const uint4 kf = s_k[buf][y][(2 * (n >> 1) + g) * 64 + (n & 1) * 32 + i];
+          if constexpr (BF) sc[y][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(kf), as_bf16x8(q[n]), sc[y][0], 0, 0, 0);
+          else sc[y][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_f16x8(kf), as_f16x8(q[n]), sc[y][0], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const bool off = kx[y] > 254;
+        c[y] = off ? c0 : c0 * pow2_bits(kx[y]);
+        if (off || key0 + (y + 1) * KV8_BLOCK > lim_lo) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            sc[y][0][r] = key0 + y * KV8_BLOCK + St::key_of(0, r, g) < lim ? (off ? __builtin_nanf("") : sc[y][0][r]) : -__builtin_inff();
+        }
+      }
+      f16x8 p[2][2];
+      st.template probabilities<2>(sc, c, p);
+      st.raise(E);
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int x = 0; x < St::NT; ++x)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              st.o[x][j] = mfma_pv(as_f16x8(s_v[buf][y][(2 * kk + g) * D + j * (D / 2) + 32 * x + i]), p[y][kk], st.o[x][j]);
+    }
+    if (s + 1 < steps) convert(s + 1, buf ^ 1);
+    __syncthreads();
+  }
+  if (mrow < t.rows) st.template store<BF>(a, sp, t, slot, kv_head, part, parts, mrow, g);
 }
 
 // Joins the parts of split tiles, WR waves to a packed row (4 where a row has many parts): each wave sums its share of them,
@@ -467,7 +695,8 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(t2w_kv8_attention_args a,
 
 // Which form, tile and split a call takes: from its sizes and bounds alone, so that the workspace's size is known too.
 struct Choice {
-  int mr, rw;
+  int mr, rw;   // packed rows of a wave, waves that share the keys' loads
+  bool tile;    // the tile form
   KV8Split s;
 };
 
@@ -475,8 +704,10 @@ Choice choose(const t2w_kv8_attention_args& a) {
   Choice c;
   c.s.G = a.heads / a.pages.kv_heads;
   const long packed = a.max_new > 0 ? (long)min(a.max_new, a.n_tok) * c.s.G : 1 << 30;
+  static const int V = getenv("T2W_V") ? atoi(getenv("T2W_V")) : 0;
   c.mr = packed <= 16 ? 16 : 32;
-  c.rw = packed <= 32 ? 1 : 2;
+  c.rw = packed <= 32 ? 1 : packed <= 64 || V == 1 ? 2 : 4;
+  c.tile = c.rw == 4 || (V == 2 && c.rw == 2);
   c.s.tt = c.mr * c.rw / c.s.G;
   c.s.per_row = a.max_new > 0 && a.max_new <= c.s.tt ? 1 : 0;
   c.s.n_tiles = c.s.per_row ? a.n_rows : a.n_tok / c.s.tt + a.n_rows;
@@ -504,9 +735,11 @@ size_t kv8_attention_workspace(const t2w_kv8_attention_args& a) {
 template <bool BF, int D>
 static hipError_t launch(const t2w_kv8_attention_args& a, const Choice& c, hipStream_t st) {
   const dim3 grid((unsigned)(c.s.n_tiles * a.pages.kv_heads), c.s.parts);
-  if (c.mr == 16) hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 16, 1>), grid, dim3(256), 0, st, a, c.s);
-  else if (c.rw == 1) hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 1>), grid, dim3(256), 0, st, a, c.s);
-  else hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 2>), grid, dim3(256), 0, st, a, c.s);
+  if (c.tile && c.rw == 2) hipLaunchKernelGGL((kv8_attn_tile_kernel<BF, D, 2>), grid, dim3(128), 0, st, a, c.s);
+  else if (c.tile) hipLaunchKernelGGL((kv8_attn_tile_kernel<BF, D, 4>), grid, dim3(256), 0, st, a, c.s);
+  else if (c.mr == 16) hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 16, 1, 1, D == 64 ? 5 : 4>), grid, dim3(256), 0, st, a, c.s);
+  else if (c.rw == 1) hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 1, 1, D == 64 ? 3 : 2>), grid, dim3(256), 0, st, a, c.s);
+  else hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 2, 1, D == 64 ? 3 : 2>), grid, dim3(256), 0, st, a, c.s);
   const unsigned groups = (unsigned)(c.s.n_tiles * a.pages.kv_heads), rows = (unsigned)(c.s.tt * c.s.G);
   if (c.s.parts > 8) hipLaunchKernelGGL((kv8_join_kernel<BF, D, 4>), dim3(groups, rows), dim3(256), 0, st, a, c.s);
   else if (c.s.parts > 1) hipLaunchKernelGGL((kv8_join_kernel<BF, D, 1>), dim3(groups, (rows + 3) / 4), dim3(256), 0, st, a, c.s);
