@@ -172,19 +172,14 @@ struct State {
   // key of score r of tile x within its block
   static __device__ __forceinline__ int key_of(int x, int r, int g) { return MR == 16 ? 8 * g + 4 * x + r : 16 * (r >> 3) + 8 * g + (r & 7); }
 
-  // Probabilities of NB blocks' scores in units 1 / c[y], invisible ones -inf; moves the reference where needed.
-  template <int NB>
-  __device__ __forceinline__ void probabilities(Acc (&sc)[NB][KG], float (&c)[NB], f16x8 (&p)[NB][NP]) {
-    float mx = -__builtin_inff();
+  // Moves the reference where a block's scores, in units 1 / c and -inf where invisible, pass it; scales them where `big`.
+  __device__ __forceinline__ void move(Acc (&sc)[KG], float& c) {
+    float mx = sc[0][0];
 #pragma unroll
-    for (int y = 0; y < NB; ++y) {
-      float v = sc[y][0][0];
+    for (int x = 0; x < KG; ++x)
 #pragma unroll
-      for (int x = 0; x < KG; ++x)
-#pragma unroll
-        for (int r = 0; r < AR; ++r) v = fmaxf(v, sc[y][x][r]);
-      mx = fmaxf(mx, v * c[y]);
-    }
+      for (int r = 0; r < AR; ++r) mx = fmaxf(mx, sc[x][r]);
+    mx *= c;
     if (__builtin_amdgcn_ballot_w64(mx > m + 8.f)) {
       const float mn = fmaxf(m, query_max<MR>(mx));
       const float alpha = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
@@ -197,37 +192,34 @@ struct State {
     }
     if (big) {
 #pragma unroll
-      for (int y = 0; y < NB; ++y) {
+      for (int x = 0; x < KG; ++x)
 #pragma unroll
-        for (int x = 0; x < KG; ++x)
-#pragma unroll
-          for (int r = 0; r < AR; ++r) sc[y][x][r] *= c[y];
-        c[y] = 1.f;
-      }
+        for (int r = 0; r < AR; ++r) sc[x][r] *= c;
+      c = 1.f;
     }
+  }
+  // a block's probabilities, the operands of P . V
+  __device__ __forceinline__ void exps(const Acc (&sc)[KG], float c, f16x8 (&p)[NP]) const {
 #pragma unroll
-    for (int y = 0; y < NB; ++y)
+    for (int x = 0; x < NP; ++x)
 #pragma unroll
-      for (int x = 0; x < NP; ++x)
+      for (int z = 0; z < 8; z += 2) {
+        float e[2];
 #pragma unroll
-        for (int z = 0; z < 8; z += 2) {
-          float e[2];
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const float s = MR == 16 ? sc[y][(z + w) / 4 % KG][(z + w) % 4] : sc[y][0][8 * x + z + w];
-            e[w] = __builtin_amdgcn_exp2f(fmaf(s, c[y], nb));
-          }
-          const f16x2_t h = __builtin_convertvector((f32x2_t{e[0], e[1]}), f16x2_t);
-          p[y][x][z] = h[0];
-          p[y][x][z + 1] = h[1];
+        for (int w = 0; w < 2; ++w) {
+          const float s = MR == 16 ? sc[(z + w) / 4 % KG][(z + w) % 4] : sc[0][8 * x + z + w];
+          e[w] = __builtin_amdgcn_exp2f(fmaf(s, c, nb));
         }
+        const f16x2_t h = __builtin_convertvector((f32x2_t{e[0], e[1]}), f16x2_t);
+        p[x][z] = h[0];
+        p[x][z + 1] = h[1];
+      }
+  }
+  __device__ __forceinline__ void sum(f16x8 p) {
     f16x8 one;
 #pragma unroll
     for (int z = 0; z < 8; ++z) one[z] = (_Float16)1.0f;
-#pragma unroll
-    for (int y = 0; y < NB; ++y)
-#pragma unroll
-      for (int x = 0; x < NP; ++x) l = mfma_pv(one, p[y][x], l);
+    l = mfma_pv(one, p, l);
   }
 
   // the other state of the same rows, left in LDS by another wave (`put`), folded into this one
@@ -306,8 +298,7 @@ struct State {
 
 // Direct form, for tiles of few packed rows (steps, draft checks, windows of up to 64 packed rows): every wave loads its key
 // and value fragments from the pages into registers and converts them there; no LDS and no barrier before the end.  RW waves
-// of MR packed rows each, times 4 / RW waves that take every (4 / RW)-th run of NB blocks; their states are merged through
-// LDS.
+// of MR packed rows each, times 4 / RW waves that take every (4 / RW)-th block; their states are merged through LDS.
 //
 // Bound by memory: 2 D codes a token and key head are read once and meet at least MR query columns of the matrix unit, whose
 // unused columns cost nothing that matters.  MR = 16 (16x16x32 MFMA) has half the softmax work of MR = 32 (32x32x16) where
@@ -318,7 +309,7 @@ struct State {
 //   MR 16: lane (i = l % 16, g = l / 16); key operand kg row i = key 8 (i / 4) + 4 kg + i % 4, its scores: keys 8 g + 4 kg + r
 //   MR 32: lane (i = l % 32, g = l / 32); row i = key with bits 2 and 3 of i swapped, scores r: keys 16 (r / 8) + 8 g + r % 8
 // Channels are paired the same way on both sides: lane group x loads the 16-channel chunk n x' + x of keys and queries.
-template <bool BF, int D, int MR, int RW, int NB, int OCC>
+template <bool BF, int D, int MR, int RW, int OCC>
 __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_attention_args a, KV8Split sp) {
   typedef State<MR, D> St;
   constexpr int KW = 4 / RW;                       // waves that share the keys of the same packed rows
@@ -344,9 +335,8 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
   const bool idle = m0 >= t.rows;  // a wave without rows still meets the barriers
   const int mrow = m0 + i;
   const int tok = min(mrow, t.rows - 1) / sp.G, hq = min(mrow, t.rows - 1) - tok * sp.G;
-  const int lim = min(seen_by(a, t, t.i0 + tok), b1 * KV8_BLOCK);  // NB > 1: a last run may reach beyond the part
-  const int lim_lo = min(seen_by(a, t, t.i0 + min(m0, t.rows - 1) / sp.G), b1 * KV8_BLOCK);  // the wave's first query sees least
-  const int v_end = min(t.total, b1 * KV8_BLOCK);
+  const int lim = seen_by(a, t, t.i0 + tok);
+  const int lim_lo = seen_by(a, t, t.i0 + min(m0, t.rows - 1) / sp.G);  // the wave's first query sees least
 
   uint4 q[NQ];
   {
@@ -365,97 +355,79 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
   const uint8_t* vbase = (const uint8_t*)a.pages.v + (size_t)kv_head * (KV8_BLOCK * D);
   const int* table = a.table + (size_t)t.row * a.ld_table;
 
-  // one run's codes; the next run's keys are loaded as soon as the scores have used these, its values after P . V
-  uint4 kf[NB][NL], vf[NB][NL];
-  auto load_k = [&](int ids, int x) {
+  // one block's codes; the next block's keys are loaded as soon as the scores have used these, its values after P . V
+  uint4 kf[NL], vf[NL];
+  auto load_k = [&](int id) {
+    const uint8_t* kp = kbase + (size_t)id * stride;
 #pragma unroll
-    for (int y = 0; y < NB; ++y) {
-      const uint8_t* kp = kbase + (size_t)__builtin_amdgcn_readlane(ids, x * NB + y) * stride;
-#pragma unroll
-      for (int n = 0; n < NL; ++n) kf[y][n] = *(const uint4*)(kp + koff + (MR == 16 ? (n / 2) * 2048 + (n % 2) * 64 : n * 1024));
-    }
+    for (int n = 0; n < NL; ++n) kf[n] = *(const uint4*)(kp + koff + (MR == 16 ? (n / 2) * 2048 + (n % 2) * 64 : n * 1024));
   };
-  auto load_v = [&](int ids, int x) {
+  auto load_v = [&](int id) {
+    const uint8_t* vp = vbase + (size_t)id * stride;
 #pragma unroll
-    for (int y = 0; y < NB; ++y) {
-      const uint8_t* vp = vbase + (size_t)__builtin_amdgcn_readlane(ids, x * NB + y) * stride;
-#pragma unroll
-      for (int n = 0; n < NL; ++n) vf[y][n] = *(const uint4*)(vp + voff + (MR == 16 ? n * 256 : (n % 2) * 16 * D + (n / 2) * 512));
-    }
+    for (int n = 0; n < NL; ++n) vf[n] = *(const uint4*)(vp + voff + (MR == 16 ? n * 256 : (n % 2) * 16 * D + (n / 2) * 512));
   };
 
   if (!idle) {
-    // the wave's runs: first blocks b0 + NB kw, + NB KW, ...; ids and exponents of the next 64 blocks one a lane
-    for (int base = b0 + NB * kw; base < b1; base += 64 * KW) {
-      const int mine = base + (lane / NB) * (NB * KW) + lane % NB;
-      int id = mine < b1 ? table[mine] : 0, ke = 127, ve = 0;  // a run's blocks beyond the part: nobody sees them
-      if (mine < b1) {
-        if ((unsigned)id < (unsigned)a.pages.n_blocks) {
-          ke = a.pages.k_exp[(size_t)id * a.pages.kv_heads + kv_head];
-          ve = a.pages.v_exp[(size_t)id * a.pages.kv_heads + kv_head];
-        } else {
-          id = 0;
-          ke = 255;
-        }
+    // the wave's blocks b0 + kw, + KW, ...: ids and exponents of the next 64 of them one a lane
+    for (int base = b0 + kw; base < b1; base += 64 * KW) {
+      const int mine = base + lane * KW;
+      int id = mine < b1 ? table[mine] : 0, ke = 255, ve = 0;
+      if ((unsigned)id < (unsigned)a.pages.n_blocks) {
+        ke = a.pages.k_exp[(size_t)id * a.pages.kv_heads + kv_head];
+        ve = a.pages.v_exp[(size_t)id * a.pages.kv_heads + kv_head];
+      } else {
+        id = 0;
       }
-      const int n = min(64 / NB, (b1 - base + NB * KW - 1) / (NB * KW));
-      load_k(id, 0);
-      load_v(id, 0);
+      const int n = min(64, (b1 - base + KW - 1) / KW);
+      load_k(__builtin_amdgcn_readlane(id, 0));
+      load_v(__builtin_amdgcn_readlane(id, 0));
       for (int x = 0; x < n; ++x) {
-        typename St::Acc sc[NB][KG];
-        float c[NB];
+        const int kx = __builtin_amdgcn_readlane(ke, x), vx = __builtin_amdgcn_readlane(ve, x);
+        const int next = x + 1 < n ? __builtin_amdgcn_readlane(id, x + 1) : -1, key0 = (base + x * KW) * KV8_BLOCK;
+        typename St::Acc sc[KG];
 #pragma unroll
-        for (int y = 0; y < NB; ++y) {
+        for (int z = 0; z < KG; ++z)
+#pragma unroll
+          for (int r = 0; r < AR; ++r) sc[z][r] = 0.f;
+#pragma unroll
+        for (int w = 0; w < NL; ++w) {
+          const int z = MR == 16 ? w % 2 : 0, j = MR == 16 ? w / 2 : w;
+          sc[z] = mfma_qk<BF>(kf[w].x, kf[w].y, q[2 * j], sc[z]);
+          sc[z] = mfma_qk<BF>(kf[w].z, kf[w].w, q[2 * j + 1], sc[z]);
+        }
+        if (next >= 0) load_k(next);
+        const bool off = kx > 254;  // a block id outside the pages, or an E8M0 NaN
+        float c = off ? c0 : c0 * pow2_bits(kx);
+        if (off || key0 + KV8_BLOCK > lim_lo) {  // or some query of the wave does not see all of the block
 #pragma unroll
           for (int z = 0; z < KG; ++z)
 #pragma unroll
-            for (int r = 0; r < AR; ++r) sc[y][z][r] = 0.f;
+            for (int r = 0; r < AR; ++r) sc[z][r] = key0 + St::key_of(z, r, g) < lim ? (off ? __builtin_nanf("") : sc[z][r]) : -__builtin_inff();
+        }
+        if (off || key0 + KV8_BLOCK > t.total) {  // values behind the last token count as zeros, whatever they are
 #pragma unroll
           for (int w = 0; w < NL; ++w) {
-            const int z = MR == 16 ? w % 2 : 0, j = MR == 16 ? w / 2 : w;
-            sc[y][z] = mfma_qk<BF>(kf[y][w].x, kf[y][w].y, q[2 * j], sc[y][z]);
-            sc[y][z] = mfma_qk<BF>(kf[y][w].z, kf[y][w].w, q[2 * j + 1], sc[y][z]);
+            const int left = off ? 0 : t.total - key0 - 8 * (MR == 16 ? g : 2 * (w % 2) + g);
+            const uint64_t keep = left >= 8 ? ~0ull : left <= 0 ? 0ull : (1ull << (8 * left)) - 1ull;
+            vf[w].x &= (uint32_t)keep; vf[w].y &= (uint32_t)(keep >> 32);
+            vf[w].z &= (uint32_t)keep; vf[w].w &= (uint32_t)(keep >> 32);
           }
         }
-        if (x + 1 < n) load_k(id, x + 1);
-        int ve_top = 0;
+        st.move(sc, c);
+        st.raise(vx);
+        f16x8 p[NP];
+        st.exps(sc, c, p);
 #pragma unroll
-        for (int y = 0; y < NB; ++y) {
-          const int kx = __builtin_amdgcn_readlane(ke, x * NB + y), key0 = (base + x * NB * KW + y) * KV8_BLOCK;
-          const bool off = kx > 254;  // a block id outside the pages, or an E8M0 NaN
-          c[y] = off ? c0 : c0 * pow2_bits(kx);
-          if (off || key0 + KV8_BLOCK > lim_lo) {  // or some query of the wave does not see all of the block
+        for (int w = 0; w < NP; ++w) st.sum(p[w]);
+        const float vs = pow2_bits(vx - st.E + 127 + 7);
 #pragma unroll
-            for (int z = 0; z < KG; ++z)
-#pragma unroll
-              for (int r = 0; r < AR; ++r)
-                sc[y][z][r] = key0 + St::key_of(z, r, g) < lim ? (off ? __builtin_nanf("") : sc[y][z][r]) : -__builtin_inff();
-          }
-          if (off || key0 + KV8_BLOCK > v_end) {  // values behind the last token count as zeros, whatever they are
-#pragma unroll
-            for (int w = 0; w < NL; ++w) {
-              const int left = off ? 0 : v_end - key0 - 8 * (MR == 16 ? g : 2 * (w % 2) + g);
-              const uint64_t keep = left >= 8 ? ~0ull : left <= 0 ? 0ull : (1ull << (8 * left)) - 1ull;
-              vf[y][w].x &= (uint32_t)keep; vf[y][w].y &= (uint32_t)(keep >> 32);
-              vf[y][w].z &= (uint32_t)keep; vf[y][w].w &= (uint32_t)(keep >> 32);
-            }
-          }
-          ve_top = max(ve_top, __builtin_amdgcn_readlane(ve, x * NB + y));
+        for (int w = 0; w < NL; ++w) {
+          const int z = MR == 16 ? w : w / 2, kk = MR == 16 ? 0 : w % 2;
+          st.o[z][0] = mfma_pv(codes_f16(vf[w].x, vf[w].y, vs), p[kk], st.o[z][0]);
+          st.o[z][1] = mfma_pv(codes_f16(vf[w].z, vf[w].w, vs), p[kk], st.o[z][1]);
         }
-        f16x8 p[NB][NP];
-        st.template probabilities<NB>(sc, c, p);
-        st.raise(ve_top);
-#pragma unroll
-        for (int y = 0; y < NB; ++y) {
-          const float vs = pow2_bits(__builtin_amdgcn_readlane(ve, x * NB + y) - st.E + 127 + 7);
-#pragma unroll
-          for (int w = 0; w < NL; ++w) {
-            const int z = MR == 16 ? w : w / 2, kk = MR == 16 ? 0 : w % 2;
-            st.o[z][0] = mfma_pv(codes_f16(vf[y][w].x, vf[y][w].y, vs), p[y][kk], st.o[z][0]);
-            st.o[z][1] = mfma_pv(codes_f16(vf[y][w].z, vf[y][w].w, vs), p[y][kk], st.o[z][1]);
-          }
-        }
-        if (x + 1 < n) load_v(id, x + 1);
+        if (next >= 0) load_v(next);
       }
     }
   }
@@ -481,7 +453,8 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
   typedef State<32, D> St;
   constexpr int T = 64 * RW, NC = 4 * D / T;  // threads; 16-byte code chunks of a step's keys, and of its values, a thread
   constexpr int CB = 2 * D;                   // chunks of a block
-  __shared__ uint4 s_k[2][2][2 * CB], s_v[2][2][2 * CB];
+  extern __shared__ uint4 s_kv[];
+  uint4 (*s_k)[2][2 * CB] = (uint4 (*)[2][2 * CB])s_kv, (*s_v)[2][2 * CB] = s_k + 3;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // the last tiles first: a causal prompt's longest
   const int slot = sp.n_tiles - 1 - blockIdx.x / a.pages.kv_heads, kv_head = blockIdx.x % a.pages.kv_heads, part = blockIdx.y;
@@ -585,52 +558,88 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
     }
   };
 
+  uint4 kf[D / 16], vf[2][St::NT][2];
+  auto read_k = [&](int buf, int y) {
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) kf[n] = s_k[buf][y][(2 * (n >> 1) + g) * 64 + (n & 1) * 32 + i];
+  };
+  auto scores = [&](typename St::Acc& sc) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sc[r] = 0.f;
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) {
+      if constexpr (BF) sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(kf[n]), as_bf16x8(q[n]), sc, 0, 0, 0);
+      else sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_f16x8(kf[n]), as_f16x8(q[n]), sc, 0, 0, 0);
+    }
+  };
+  // one block: its scores are in `sc`; the next block's go into `sn` while its probabilities are made
+  auto block = [&](int buf, int y, int key0, int kx, int E, typename St::Acc (&sc)[1], int nbuf, int ny, typename St::Acc (&sn)[1]) {
+    read_k(nbuf, ny);
+    const bool off = kx > 254;
+    float c = off ? c0 : c0 * pow2_bits(kx);
+    if (off || key0 + KV8_BLOCK > lim_lo) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[0][r] = key0 + St::key_of(0, r, g) < lim ? (off ? __builtin_nanf("") : sc[0][r]) : -__builtin_inff();
+    }
+    st.move(sc, c);
+    st.raise(E);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int x = 0; x < St::NT; ++x)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) vf[kk][x][j] = s_v[buf][y][(2 * kk + g) * D + j * (D / 2) + 32 * x + i];
+    // the order is pinned: each score MFMA with its share of the exponentials, so that matrix and vector unit work at once
+    constexpr int NQ = D / 16, NE = 16 / NQ;
+    f16x8 p[2];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sn[0][r] = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      if constexpr (BF) sn[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(kf[n]), as_bf16x8(q[n]), sn[0], 0, 0, 0);
+      else sn[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_f16x8(kf[n]), as_f16x8(q[n]), sn[0], 0, 0, 0);
+#pragma unroll
+      for (int z = NE * n; z < NE * (n + 1); z += 2) {
+        const f16x2_t h = __builtin_convertvector((f32x2_t{__builtin_amdgcn_exp2f(fmaf(sc[0][z], c, st.nb)), __builtin_amdgcn_exp2f(fmaf(sc[0][z + 1], c, st.nb))}), f16x2_t);
+        p[z >> 3][z & 7] = h[0];
+        p[z >> 3][(z & 7) + 1] = h[1];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      st.sum(p[kk]);
+#pragma unroll
+      for (int x = 0; x < St::NT; ++x)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) st.o[x][j] = mfma_pv(as_f16x8(vf[kk][x][j]), p[kk], st.o[x][j]);
+    }
+  };
+
   load(0);
   convert(0, 0);
+  int kx0 = nke[0], kx1 = nke[1], E = nE;
+  if (steps > 1) load(1);
   __syncthreads();
+  typename St::Acc s0[1], s1[1];
+  read_k(0, 0);
+  scores(s0[0]);
+  int cur = 0;
   for (int s = 0; s < steps; ++s) {
-    const int buf = s & 1, E = nE, kx[2] = {nke[0], nke[1]};
-    if (s + 1 < steps) load(s + 1);
-    const int key0 = (b0 + 2 * s) * KV8_BLOCK;
-    if (key0 < lim_hi) {
-      typename St::Acc sc[2][1];
-      float c[2];
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sc[y][0][r] = 0.f;
-#pragma unroll
-        for (int n = 0; n < D / 16; ++n) {
-          const uint4 kf = s_k[buf][y][(2 * (n >> 1) + g) * 64 + (n & 1) * 32 + i];
-          if constexpr (BF) sc[y][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(kf), as_bf16x8(q[n]), sc[y][0], 0, 0, 0);
-          else sc[y][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_f16x8(kf), as_f16x8(q[n]), sc[y][0], 0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const bool off = kx[y] > 254;
-        c[y] = off ? c0 : c0 * pow2_bits(kx[y]);
-        if (off || key0 + (y + 1) * KV8_BLOCK > lim_lo) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            sc[y][0][r] = key0 + y * KV8_BLOCK + St::key_of(0, r, g) < lim ? (off ? __builtin_nanf("") : sc[y][0][r]) : -__builtin_inff();
-        }
-      }
-      f16x8 p[2][2];
-      st.template probabilities<2>(sc, c, p);
-      st.raise(E);
-#pragma unroll
-      for (int y = 0; y < 2; ++y)
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-          for (int x = 0; x < St::NT; ++x)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              st.o[x][j] = mfma_pv(as_f16x8(s_v[buf][y][(2 * kk + g) * D + j * (D / 2) + 32 * x + i]), p[y][kk], st.o[x][j]);
+    const int nxt = cur == 2 ? 0 : cur + 1, key0 = (b0 + 2 * s) * KV8_BLOCK;
+    const bool on = key0 < lim_hi;
+    if (on) block(cur, 0, key0, kx0, E, s0, cur, 1, s1);
+    int nkx0 = 127, nkx1 = 127;
+    if (s + 1 < steps) {
+      nkx0 = nke[0]; nkx1 = nke[1];
+      convert(s + 1, nxt);
+      if (s + 2 < steps) load(s + 2);
     }
-    if (s + 1 < steps) convert(s + 1, buf ^ 1);
     __syncthreads();
+    if (on) block(cur, 1, key0 + KV8_BLOCK, kx1, E, s1, nxt, 0, s0);
+    kx0 = nkx0; kx1 = nkx1; E = nE;
+    cur = nxt;
   }
   if (mrow < t.rows) st.template store<BF>(a, sp, t, slot, kv_head, part, parts, mrow, g);
 }
@@ -706,16 +715,17 @@ Choice choose(const t2w_kv8_attention_args& a) {
   const long packed = a.max_new > 0 ? (long)min(a.max_new, a.n_tok) * c.s.G : 1 << 30;
   static const int V = getenv("T2W_V") ? atoi(getenv("T2W_V")) : 0;
   c.mr = packed <= 16 ? 16 : 32;
-  c.rw = packed <= 32 ? 1 : packed <= 64 || V == 1 ? 2 : 4;
-  c.tile = c.rw == 4 || (V == 2 && c.rw == 2);
+  c.rw = packed <= 32 ? 1 : packed <= 64 || V == 1 ? 2 : a.pages.head_dim == 128 ? 8 : 4;
+  c.tile = c.rw >= 4;
   c.s.tt = c.mr * c.rw / c.s.G;
   c.s.per_row = a.max_new > 0 && a.max_new <= c.s.tt ? 1 : 0;
   c.s.n_tiles = c.s.per_row ? a.n_rows : a.n_tok / c.s.tt + a.n_rows;
   const long max_kv = a.max_kv > 0 ? min((long)a.max_kv, (long)a.width * KV8_BLOCK) : (long)a.width * KV8_BLOCK;
   const long nb = (max_kv + KV8_BLOCK - 1) / KV8_BLOCK, groups = (long)c.s.n_tiles * a.pages.kv_heads;
+  const long want = c.tile ? 256 : 512;
   long bps = nb;
   if (nb > 48) {
-    const long parts = (512 + groups - 1) / groups;
+    const long parts = (want + groups - 1) / groups;
     bps = (nb + parts - 1) / parts;
     if (bps < 16) bps = 16;
   }
@@ -735,11 +745,18 @@ size_t kv8_attention_workspace(const t2w_kv8_attention_args& a) {
 template <bool BF, int D>
 static hipError_t launch(const t2w_kv8_attention_args& a, const Choice& c, hipStream_t st) {
   const dim3 grid((unsigned)(c.s.n_tiles * a.pages.kv_heads), c.s.parts);
-  if (c.tile && c.rw == 2) hipLaunchKernelGGL((kv8_attn_tile_kernel<BF, D, 2>), grid, dim3(128), 0, st, a, c.s);
-  else if (c.tile) hipLaunchKernelGGL((kv8_attn_tile_kernel<BF, D, 4>), grid, dim3(256), 0, st, a, c.s);
-  else if (c.mr == 16) hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 16, 1, 1, D == 64 ? 5 : 4>), grid, dim3(256), 0, st, a, c.s);
-  else if (c.rw == 1) hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 1, 1, D == 64 ? 3 : 2>), grid, dim3(256), 0, st, a, c.s);
-  else hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 2, 1, D == 64 ? 3 : 2>), grid, dim3(256), 0, st, a, c.s);
+  if (c.tile) {
+    constexpr int RW = D == 128 ? 8 : 4, LDS = 3 * 2 * 2 * KV8_BLOCK * D * 2;  // three steps of two blocks, keys and values in 16 bits
+    static const hipError_t attr = hipFuncSetAttribute((const void*)kv8_attn_tile_kernel<BF, D, RW>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (attr != hipSuccess) return attr;
+    hipLaunchKernelGGL((kv8_attn_tile_kernel<BF, D, RW>), grid, dim3(64 * RW), LDS, st, a, c.s);
+  } else if (c.mr == 16) {
+    hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 16, 1, D == 64 ? 5 : 4>), grid, dim3(256), 0, st, a, c.s);
+  } else if (c.rw == 1) {
+    hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 1, D == 64 ? 3 : 2>), grid, dim3(256), 0, st, a, c.s);
+  } else {
+    hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 2, D == 64 ? 3 : 2>), grid, dim3(256), 0, st, a, c.s);
+  }
   const unsigned groups = (unsigned)(c.s.n_tiles * a.pages.kv_heads), rows = (unsigned)(c.s.tt * c.s.G);
   if (c.s.parts > 8) hipLaunchKernelGGL((kv8_join_kernel<BF, D, 4>), dim3(groups, rows), dim3(256), 0, st, a, c.s);
   else if (c.s.parts > 1) hipLaunchKernelGGL((kv8_join_kernel<BF, D, 1>), dim3(groups, (rows + 3) / 4), dim3(256), 0, st, a, c.s);
