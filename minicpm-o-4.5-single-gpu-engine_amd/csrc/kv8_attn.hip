@@ -130,7 +130,7 @@ __device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float(
 //    not bf16: bf16's 8 bits would cost as much again as the output's own rounding.
 //  * value codes enter as fp16, exact, times 2^(their exponent - E + 7), E the largest value exponent so far: 22 powers of two
 //    below the largest block's scale stay exact.
-//  * sums of probabilities come from the matrix unit too (a row of ones): the same rounded probabilities as the outputs'.
+//  * sums of probabilities are of the same rounded fp16 values as the outputs' (fp32 dot products, a lane its own keys').
 template <int MR, int D>
 struct State {
   static constexpr int AR = MR == 16 ? 4 : 16;     // values of an accumulator
@@ -138,15 +138,14 @@ struct State {
   static constexpr int NP = MR == 16 ? 1 : 2;      // probability operands of a block
   static constexpr int NT = D / (2 * MR);          // output tile pairs: channels 2 p and 2 p + 1, p = MR t + i
   typedef typename std::conditional<MR == 16, f32x4, f32x16>::type Acc;
-  Acc o[NT][2], l;
+  Acc o[NT][2];
+  float l = 0.f;                // sum of the lane's probabilities; of the query's when the lane groups are added
   float m = -__builtin_inff();  // reference
   float nb = 7.f;               // 7 - m, 7 where m is -inf
   bool big = false;             // |m| so large that s - m in one fma would not be exact enough: scale the scores first
   int E = 0;                    // biased value exponent that o is in units of; 0: none yet
 
   __device__ __forceinline__ State() {
-#pragma unroll
-    for (int r = 0; r < AR; ++r) l[r] = 0.f;
 #pragma unroll
     for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -172,13 +171,17 @@ struct State {
   // key of score r of tile x within its block
   static __device__ __forceinline__ int key_of(int x, int r, int g) { return MR == 16 ? 8 * g + 4 * x + r : 16 * (r >> 3) + 8 * g + (r & 7); }
 
-  // Moves the reference where a block's scores, in units 1 / c and -inf where invisible, pass it; scales them where `big`.
-  __device__ __forceinline__ void move(Acc (&sc)[KG], float& c) {
+  static __device__ __forceinline__ float top(const Acc (&sc)[KG]) {
     float mx = sc[0][0];
 #pragma unroll
     for (int x = 0; x < KG; ++x)
 #pragma unroll
       for (int r = 0; r < AR; ++r) mx = fmaxf(mx, sc[x][r]);
+    return mx;
+  }
+  // Moves the reference where a block's scores, in units 1 / c and -inf where invisible, of maximum mx, pass it; scales them
+  // where `big`.
+  __device__ __forceinline__ void move(Acc (&sc)[KG], float& c, float mx) {
     mx *= c;
     if (__builtin_amdgcn_ballot_w64(mx > m + 8.f)) {
       const float mn = fmaxf(m, query_max<MR>(mx));
@@ -186,8 +189,7 @@ struct State {
       m = mn;
       nb = mn == -__builtin_inff() ? 7.f : 7.f - mn;
       big = big || __builtin_amdgcn_ballot_w64(fabsf(mn) > 4194304.f && mn != -__builtin_inff()) != 0;
-#pragma unroll
-      for (int r = 0; r < AR; ++r) l[r] *= alpha;
+      l *= alpha;
       scale_o(alpha);
     }
     if (big) {
@@ -216,10 +218,9 @@ struct State {
       }
   }
   __device__ __forceinline__ void sum(f16x8 p) {
-    f16x8 one;
+    const f16x2_t one = {(_Float16)1.0f, (_Float16)1.0f};
 #pragma unroll
-    for (int z = 0; z < 8; ++z) one[z] = (_Float16)1.0f;
-    l = mfma_pv(one, p, l);
+    for (int z = 0; z < 8; z += 2) l = __builtin_amdgcn_fdot2(f16x2_t{p[z], p[z + 1]}, one, l, false);
   }
 
   // the other state of the same rows, left in LDS by another wave (`put`), folded into this one
@@ -232,7 +233,7 @@ struct State {
 #pragma unroll
         for (int r = 0; r < AR; ++r) dst[(x * 2 + j) * AR + r][lane] = o[x][j][r];
     dst[WORDS - 2][lane] = m;
-    dst[WORDS - 1][lane] = l[0];
+    dst[WORDS - 1][lane] = l;
   }
   __device__ __forceinline__ void fold(const float (*src)[64], int e2, int lane) {
     const float m2 = src[WORDS - 2][lane], l2 = src[WORDS - 1][lane];
@@ -240,10 +241,8 @@ struct State {
     const float mn = fmaxf(m, m2);
     const float f1 = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
     const float f2 = m2 == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m2 - mn);
-    // a state whose reference never moved holds zeros, or NaN from scores that were none
-    const float k1 = l[0] != l[0] ? __builtin_nanf("") : f1, k2 = l2 != l2 ? __builtin_nanf("") : f2;
-    const float g1 = E == en ? k1 : k1 * (E == 0 ? 0.f : pow2_bits(E - en + 127)), g2 = e2 == en ? k2 : k2 * (e2 == 0 ? 0.f : pow2_bits(e2 - en + 127));
-    l[0] = l[0] * k1 + l2 * k2;
+    const float g1 = E == en ? f1 : f1 * (E == 0 ? 0.f : pow2_bits(E - en + 127)), g2 = e2 == en ? f2 : f2 * (e2 == 0 ? 0.f : pow2_bits(e2 - en + 127));
+    l = l * f1 + l2 * f2;
 #pragma unroll
     for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -259,7 +258,9 @@ struct State {
   __device__ __forceinline__ void store(const t2w_kv8_attention_args& a, const KV8Split& sp, const Tile& t, int slot, int kv_head, int part, int parts,
                                         int mrow, int g) const {
     const float unit = pow2_bits(E) * 0.0078125f;  // 2^(E - 127 - 7); E = 0: no value block at all, o is zero
-    const float inv = l[0] == 0.f ? 0.f : 1.f / l[0];
+    float sum = l + __shfl_xor(l, 32, 64);
+    if constexpr (MR == 16) sum += __shfl_xor(sum, 16, 64);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     // values r .. r + 3 of both tiles of a pair are 8 consecutive channels, from d on
     if (parts == 1) {
       const int tok = mrow / sp.G, hq = mrow - tok * sp.G;
@@ -291,7 +292,7 @@ struct State {
             *(float4*)(po + d + 2 * y) = make_float4(o[x][0][r + y] * inv * unit, o[x][1][r + y] * inv * unit, o[x][0][r + y + 1] * inv * unit,
                                                      o[x][1][r + y + 1] * inv * unit);
         }
-      if (g == 0) *(float2*)ml = make_float2(m, l[0]);
+      if (g == 0) *(float2*)ml = make_float2(m, sum);
     }
   }
 };
@@ -414,7 +415,7 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
             vf[w].z &= (uint32_t)keep; vf[w].w &= (uint32_t)(keep >> 32);
           }
         }
-        st.move(sc, c);
+        st.move(sc, c, St::top(sc));
         st.raise(vx);
         f16x8 p[NP];
         st.exps(sc, c, p);
@@ -527,37 +528,35 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
       rv[n] = *(const uint4*)(vbase + page + (uint32_t)(r * 16));
     }
   };
-  auto convert = [&](int s, int buf) {
+  // the step in registers to LDS, in four pieces a chunk; `unit` comes first
+  auto unit = [&](int s) {
     nE = max(nE, max(nve[0], nve[1]));
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      const int y = __builtin_amdgcn_readfirstlane((tid + T * n) / CB), r = (tid + T * n) % CB;
-      const int ex = y ? nke[1] : nke[0], key0 = (b0 + 2 * s + y) * KV8_BLOCK;
-      const float vs = pow2_bits((y ? nve[1] : nve[0]) - nE + 127 + 7);
-      uint4 v = rv[n];
-      if (ex > 254 || key0 + KV8_BLOCK > v_end) {  // values behind the last token count as zeros, whatever they are
-        const int left = ex > 254 ? 0 : v_end - key0 - 8 * (r / (D / 2));
+      const int y = __builtin_amdgcn_readfirstlane((tid + T * n) / CB), r = (tid + T * n) % CB, key0 = (b0 + 2 * s + y) * KV8_BLOCK;
+      if (nke[y] > 254 || key0 + KV8_BLOCK > v_end) {  // values behind the last token count as zeros, whatever they are
+        const int left = nke[y] > 254 ? 0 : v_end - key0 - 8 * (r / (D / 2));
         const uint64_t keep = left >= 8 ? ~0ull : left <= 0 ? 0ull : (1ull << (8 * left)) - 1ull;
-        v.x &= (uint32_t)keep; v.y &= (uint32_t)(keep >> 32);
-        v.z &= (uint32_t)keep; v.w &= (uint32_t)(keep >> 32);
+        rv[n].x &= (uint32_t)keep; rv[n].y &= (uint32_t)(keep >> 32);
+        rv[n].z &= (uint32_t)keep; rv[n].w &= (uint32_t)(keep >> 32);
       }
-      // keys: chunk c of 16 channels, key k -> two operands of 8 channels, at the key's operand row
-      const int c = r >> 5, k = r & 31, row = (k & 0x13) | ((k & 4) << 1) | ((k & 8) >> 1);
-      uint4* kd = &s_k[buf][y][c * 64 + row];
-      if constexpr (BF) {
-        kd[0] = __builtin_bit_cast(uint4, codes_bf16(rk[n].x, rk[n].y));
-        kd[32] = __builtin_bit_cast(uint4, codes_bf16(rk[n].z, rk[n].w));
-      } else {
-        kd[0] = __builtin_bit_cast(uint4, codes_f16(rk[n].x, rk[n].y, 1.f));
-        kd[32] = __builtin_bit_cast(uint4, codes_f16(rk[n].z, rk[n].w, 1.f));
-      }
-      // values: group of 8 keys, channel pair -> an operand of 8 keys for each channel
-      uint4* vd = &s_v[buf][y][r / (D / 2) * D + r % (D / 2)];
-      vd[0] = __builtin_bit_cast(uint4, codes_f16(v.x, v.y, vs));
-      vd[D / 2] = __builtin_bit_cast(uint4, codes_f16(v.z, v.w, vs));
     }
   };
-
+  auto convert = [&](int piece, int buf) {
+    const int n = piece >> 2;
+    const int y = __builtin_amdgcn_readfirstlane((tid + T * n) / CB), r = (tid + T * n) % CB;
+    if ((piece & 3) < 2) {  // keys: chunk c of 16 channels, key k -> two operands of 8 channels, at the key's operand row
+      const int c = r >> 5, k = r & 31, row = (k & 0x13) | ((k & 4) << 1) | ((k & 8) >> 1);
+      const uint32_t lo = (piece & 1) ? rk[n].z : rk[n].x, hi = (piece & 1) ? rk[n].w : rk[n].y;
+      uint4* kd = &s_k[buf][y][c * 64 + (piece & 1) * 32 + row];
+      if constexpr (BF) *kd = __builtin_bit_cast(uint4, codes_bf16(lo, hi));
+      else *kd = __builtin_bit_cast(uint4, codes_f16(lo, hi, 1.f));
+    } else {  // values: group of 8 keys, channel pair -> an operand of 8 keys for each channel
+      const float vs = pow2_bits((y ? nve[1] : nve[0]) - nE + 127 + 7);
+      const uint32_t lo = (piece & 1) ? rv[n].z : rv[n].x, hi = (piece & 1) ? rv[n].w : rv[n].y;
+      s_v[buf][y][r / (D / 2) * D + (piece & 1) * (D / 2) + r % (D / 2)] = __builtin_bit_cast(uint4, codes_f16(lo, hi, vs));
+    }
+  };
   uint4 kf[D / 16], vf[2][St::NT][2];
   auto read_k = [&](int buf, int y) {
 #pragma unroll
@@ -572,16 +571,20 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
       else sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_f16x8(kf[n]), as_f16x8(q[n]), sc, 0, 0, 0);
     }
   };
-  // one block: its scores are in `sc`; the next block's go into `sn` while its probabilities are made
-  auto block = [&](int buf, int y, int key0, int kx, int E, typename St::Acc (&sc)[1], int nbuf, int ny, typename St::Acc (&sn)[1]) {
+  // One block: its scores are in `sc`, their maximum in mx; the next block's go into `sn` while its probabilities are made,
+  // and into mx while P . V runs, where the next step's codes are converted too (cbuf >= 0).  The order within a phase is
+  // pinned, a few vector instructions behind each MFMA, so that both units work at once.
+  float mx;
+  auto block = [&](int buf, int y, int key0, int kx, int E, typename St::Acc (&sc)[1], int nbuf, int ny, typename St::Acc (&sn)[1], auto conv, int cbuf) {
     read_k(nbuf, ny);
     const bool off = kx > 254;
     float c = off ? c0 : c0 * pow2_bits(kx);
     if (off || key0 + KV8_BLOCK > lim_lo) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) sc[0][r] = key0 + St::key_of(0, r, g) < lim ? (off ? __builtin_nanf("") : sc[0][r]) : -__builtin_inff();
+      mx = St::top(sc);
     }
-    st.move(sc, c);
+    st.move(sc, c, mx);
     st.raise(E);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk)
@@ -589,7 +592,6 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
       for (int x = 0; x < St::NT; ++x)
 #pragma unroll
         for (int j = 0; j < 2; ++j) vf[kk][x][j] = s_v[buf][y][(2 * kk + g) * D + j * (D / 2) + 32 * x + i];
-    // the order is pinned: each score MFMA with its share of the exponentials, so that matrix and vector unit work at once
     constexpr int NQ = D / 16, NE = 16 / NQ;
     f16x8 p[2];
 #pragma unroll
@@ -607,37 +609,53 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    constexpr int NV = 2 * St::NT, NM = 2 * NV;  // P . V products of half a block, of all of it
+    constexpr int CP = decltype(conv)::value ? 4 * NC : 0;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      st.sum(p[kk]);
+    for (int n = 0; n < NM; ++n) {
+      const int kk = n / NV, w = n % NV;
+      st.o[w >> 1][w & 1] = mfma_pv(as_f16x8(vf[kk][w >> 1][w & 1]), p[kk], st.o[w >> 1][w & 1]);
+      if (w == 0) st.sum(p[kk]);
 #pragma unroll
-      for (int x = 0; x < St::NT; ++x)
+      for (int z = CP * n / NM; z < CP * (n + 1) / NM; ++z) convert(z, cbuf);
+      if (n == NM - 4) mx = fmaxf(fmaxf(sn[0][0], sn[0][1]), fmaxf(sn[0][2], sn[0][3]));
+      if (n > NM - 4) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) st.o[x][j] = mfma_pv(as_f16x8(vf[kk][x][j]), p[kk], st.o[x][j]);
+        for (int z = 4 * (n - NM + 4); z < 4 * (n - NM + 5); ++z) mx = fmaxf(mx, sn[0][z]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
   load(0);
-  convert(0, 0);
+  unit(0);
+#pragma unroll
+  for (int z = 0; z < 4 * NC; ++z) convert(z, 0);
   int kx0 = nke[0], kx1 = nke[1], E = nE;
   if (steps > 1) load(1);
   __syncthreads();
   typename St::Acc s0[1], s1[1];
   read_k(0, 0);
   scores(s0[0]);
+  mx = St::top(s0);
   int cur = 0;
   for (int s = 0; s < steps; ++s) {
     const int nxt = cur == 2 ? 0 : cur + 1, key0 = (b0 + 2 * s) * KV8_BLOCK;
-    const bool on = key0 < lim_hi;
-    if (on) block(cur, 0, key0, kx0, E, s0, cur, 1, s1);
+    const bool on = key0 < lim_hi, more = s + 1 < steps;
     int nkx0 = 127, nkx1 = 127;
-    if (s + 1 < steps) {
+    if (more) {
+      unit(s + 1);
       nkx0 = nke[0]; nkx1 = nke[1];
-      convert(s + 1, nxt);
-      if (s + 2 < steps) load(s + 2);
     }
+    if (on) {
+      block(cur, 0, key0, kx0, E, s0, cur, 1, s1, std::true_type(), nxt);  // after the last step: into a buffer that nobody reads
+    } else {
+#pragma unroll
+      for (int z = 0; z < 4 * NC; ++z) convert(z, nxt);
+    }
+    if (s + 2 < steps) load(s + 2);
     __syncthreads();
-    if (on) block(cur, 1, key0 + KV8_BLOCK, kx1, E, s1, nxt, 0, s0);
+    if (on) block(cur, 1, key0 + KV8_BLOCK, kx1, E, s1, nxt, 0, s0, std::false_type(), 0);
     kx0 = nkx0; kx1 = nkx1; E = nE;
     cur = nxt;
   }
@@ -722,7 +740,7 @@ Choice choose(const t2w_kv8_attention_args& a) {
   c.s.n_tiles = c.s.per_row ? a.n_rows : a.n_tok / c.s.tt + a.n_rows;
   const long max_kv = a.max_kv > 0 ? min((long)a.max_kv, (long)a.width * KV8_BLOCK) : (long)a.width * KV8_BLOCK;
   const long nb = (max_kv + KV8_BLOCK - 1) / KV8_BLOCK, groups = (long)c.s.n_tiles * a.pages.kv_heads;
-  const long want = c.tile ? 256 : 512;
+  const long want = c.tile && a.pages.head_dim == 128 ? 256 : 512;
   long bps = nb;
   if (nb > 48) {
     const long parts = (want + groups - 1) / groups;
