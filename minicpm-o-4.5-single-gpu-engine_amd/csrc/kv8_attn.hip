@@ -769,11 +769,11 @@ static hipError_t launch(const t2w_kv8_attention_args& a, const Choice& c, hipSt
     if (attr != hipSuccess) return attr;
     hipLaunchKernelGGL((kv8_attn_tile_kernel<BF, D, RW>), grid, dim3(64 * RW), LDS, st, a, c.s);
   } else if (c.mr == 16) {
-    hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 16, 1, D == 64 ? 5 : 4>), grid, dim3(256), 0, st, a, c.s);
+    hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 16, 1, D == 64 ? 6 : 4>), grid, dim3(256), 0, st, a, c.s);
   } else if (c.rw == 1) {
-    hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 1, D == 64 ? 3 : 2>), grid, dim3(256), 0, st, a, c.s);
+    hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 1, D == 64 ? 4 : 2>), grid, dim3(256), 0, st, a, c.s);
   } else {
-    hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 2, D == 64 ? 3 : 2>), grid, dim3(256), 0, st, a, c.s);
+    hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 2, D == 64 ? 4 : 2>), grid, dim3(256), 0, st, a, c.s);
   }
   const unsigned groups = (unsigned)(c.s.n_tiles * a.pages.kv_heads), rows = (unsigned)(c.s.tt * c.s.G);
   if (c.s.parts > 8) hipLaunchKernelGGL((kv8_join_kernel<BF, D, 4>), dim3(groups, rows), dim3(256), 0, st, a, c.s);

@@ -25,6 +25,8 @@ from . import _lib
 
 BLOCK = 32       # tokens of a block
 MAX_ROWS = 4096  # rows of a call
+# torch's current stream of a device as the raw handle, without the 2 us of making a Stream object for each call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 
 
@@ -98,10 +100,10 @@ def _call(fn, args, dev, what: str) -> None:
     if dev.type != "cuda":
         raise ValueError(f"kv8 {what}: the tensors must be on the GPU")
     if dev.index == torch.cuda.current_device():
-        _lib.check(fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream), what)
+        _lib.check(fn(C.byref(args), _raw_stream(dev.index)), what)
     else:
         with torch.cuda.device(dev):
-            _lib.check(fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream), what)
+            _lib.check(fn(C.byref(args), _raw_stream(dev.index)), what)
 
 
 PLAN_ERRORS = {1: "a length is negative", 2: "more tokens than the plan has room for", 4: "a row outgrows its block table", 8: "too few free blocks"}
