@@ -316,7 +316,9 @@ def run(s):
     if own:
         import t2w_amd  # noqa: F401
         from t2w_amd import kv8
-        pages = kv8.KV8Pages(s["k"], s["v"], s["k_exp"], s["v_exp"])
+        pages = s.get("pages")
+        if pages is None:  # a user's program makes the handle once, with the cache
+            pages = s["pages"] = kv8.KV8Pages(s["k"], s["v"], s["k_exp"], s["v_exp"])
         if s["op"] == "append":
             kv8.append(pages, s["k_new"], s["v_new"], s["table"], s["row_start"], s["kv_total"], max_new=s["max_new"])
             return {"k": s["k"].view(torch.float8_e4m3fn), "v": s["v"].view(torch.float8_e4m3fn), "k_exp": s["k_exp"], "v_exp": s["v_exp"]}
