@@ -175,10 +175,12 @@ def attention(q: torch.Tensor, pages: KV8Pages, table: torch.Tensor, row_start: 
     dev, d, rows = pages.device, pages.head_dim, kv_total.shape[0]
     ldq = _tokens("q", q, None, d, dev)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    ldo = _tokens("out", out, q.shape[0], d, dev)
-    if out.dtype != q.dtype or out.shape[1] != q.shape[1]:
-        raise ValueError("kv8 attention: out must have q's type and heads")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        ldo = q.shape[1] * d
+    else:
+        ldo = _tokens("out", out, q.shape[0], d, dev)
+        if out.dtype != q.dtype or out.shape[1] != q.shape[1]:
+            raise ValueError("kv8 attention: out must have q's type and heads")
     L = _lib.lib()
     a = _lib.KV8AttentionArgs(pages.struct, q.data_ptr(), out.data_ptr(), ldq, ldo, _DTYPES[q.dtype], q.shape[0], q.shape[1],
                               *_table(table, rows, dev), _ints("row_start", row_start, rows + 1, dev),
