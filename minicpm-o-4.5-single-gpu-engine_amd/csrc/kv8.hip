@@ -18,17 +18,6 @@ namespace {
 // writer and none is read in the same call.  Bound by latency: a launch, the lengths' load, an id's load, the stores.
 constexpr int PLAN_TOKENS = 1024;  // tokens of a workgroup
 
-// sum over lanes 0 .. l of the wave, in lane l: shifts within the 16-lane rows, then each row's last lane to those behind it
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-  return v;
-}
-
 // T threads of PER rows and PLAN_TOKENS / T tokens.  VEC: the lengths and the token tables are 16-byte aligned.
 template <int T, int PER, bool VEC>
 __global__ void __launch_bounds__(T) kv8_plan_kernel(t2w_kv8_plan_args a) {

@@ -2,7 +2,6 @@
 // i sees, key and value codes times their blocks' scales.  Block format: kv8_internal.h.
 #include "kv8_internal.h"
 
-#include <stdlib.h>
 #include <type_traits>
 
 namespace t2w {
@@ -38,17 +37,35 @@ struct Tile {
 
 // The tile of a slot, by the whole wave; false: nothing there.
 __device__ __forceinline__ bool find_tile(const t2w_kv8_attention_args& a, const KV8Split& s, int slot, Tile& t) {
-  int at;
+  int at, next;
   if (s.per_row > 0) {
     t.row = slot / s.per_row;
     at = slot - t.row * s.per_row;
+    t.start = a.row_start[t.row];
+    next = a.row_start[t.row + 1];
+    t.total = a.kv_total[t.row];
+  } else if (a.n_rows <= 64) {  // all rows at once, one a lane, and their tiles counted: the slots without one come last
+    const int lane = threadIdx.x & 63, r = min(lane, a.n_rows - 1);
+    const int start = a.row_start[r], stop = a.row_start[r + 1], total = a.kv_total[r];
+    const int tiles = lane < a.n_rows && stop > start ? (stop - start - 1) / s.tt + 1 : 0, before = wave_scan(tiles) - tiles;
+    t.row = max((int)__popcll(__builtin_amdgcn_ballot_w64(lane < a.n_rows && before <= slot)) - 1, 0);
+    t.start = __builtin_amdgcn_readlane(start, t.row);
+    next = __builtin_amdgcn_readlane(stop, t.row);
+    t.total = __builtin_amdgcn_readlane(total, t.row);
+    at = slot - __builtin_amdgcn_readlane(before, t.row);
   } else {
     t.row = kv8_find_row(a.row_start, a.n_rows, s.tt, 1, slot);
-    at = slot - (a.row_start[t.row] / s.tt + t.row);
+    t.start = a.row_start[t.row];
+    next = a.row_start[t.row + 1];
+    t.total = a.kv_total[t.row];
+    at = slot - (t.start / s.tt + t.row);
   }
-  t.start = a.row_start[t.row];
-  t.n_new = a.row_start[t.row + 1] - t.start;
-  t.total = a.kv_total[t.row];
+  // the same in every lane, which the compiler does not see on every way here
+  t.row = __builtin_amdgcn_readfirstlane(t.row);
+  t.start = __builtin_amdgcn_readfirstlane(t.start);
+  t.n_new = __builtin_amdgcn_readfirstlane(next) - t.start;
+  t.total = __builtin_amdgcn_readfirstlane(t.total);
+  at = __builtin_amdgcn_readfirstlane(at);
   t.i0 = at * s.tt;
   if (t.start < 0 || t.n_new <= 0 || t.start > a.n_tok - t.n_new || at < 0 || t.i0 >= t.n_new) return false;
   t.bad = t.total < 0 || t.total > a.width * KV8_BLOCK || (s.per_row > 0 && t.n_new > s.per_row * s.tt);
@@ -321,6 +338,10 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
   __shared__ int s_e[4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wave % RW, kw = wave / RW;
   const int slot = blockIdx.x / a.pages.kv_heads, kv_head = blockIdx.x - slot * a.pages.kv_heads, part = blockIdx.y;
+  // the first ids are under way with the row's lengths where its number is known and parts have their planned size
+  const int ahead = part * sp.bps + kw;
+  int id_ahead = 0;
+  if (sp.per_row > 0 && ahead + lane * KW < a.width) id_ahead = a.table[(size_t)(slot / sp.per_row) * a.ld_table + ahead + lane * KW];
   Tile t;
   if (!find_tile(a, sp, slot, t)) return;
   if (t.bad) {
@@ -373,7 +394,7 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
     // the wave's blocks b0 + kw, + KW, ...: ids and exponents of the next 64 of them one a lane
     for (int base = b0 + kw; base < b1; base += 64 * KW) {
       const int mine = base + lane * KW;
-      int id = mine < b1 ? table[mine] : 0, ke = 255, ve = 0;
+      int id = mine >= b1 ? 0 : sp.per_row > 0 && base == ahead ? id_ahead : table[mine], ke = 255, ve = 0;
       if ((unsigned)id < (unsigned)a.pages.n_blocks) {
         ke = a.pages.k_exp[(size_t)id * a.pages.kv_heads + kv_head];
         ve = a.pages.v_exp[(size_t)id * a.pages.kv_heads + kv_head];
@@ -452,8 +473,8 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
 template <bool BF, int D, int RW>
 __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_attention_args a, KV8Split sp) {
   typedef State<32, D> St;
-  constexpr int T = 64 * RW, NC = 4 * D / T;  // threads; 16-byte code chunks of a step's keys, and of its values, a thread
-  constexpr int CB = 2 * D;                   // chunks of a block
+  constexpr int CB = 2 * D, T = 64 * RW;      // 16-byte code chunks of a block's keys, and of its values; threads
+  constexpr int NC = 2 * CB / T;              // chunks of a step (two blocks) a thread
   extern __shared__ uint4 s_kv[];
   uint4 (*s_k)[2][2 * CB] = (uint4 (*)[2][2 * CB])s_kv, (*s_v)[2][2 * CB] = s_k + 3;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -722,34 +743,48 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(t2w_kv8_attention_args a,
 
 // Which form, tile and split a call takes: from its sizes and bounds alone, so that the workspace's size is known too.
 struct Choice {
-  int mr, rw;   // packed rows of a wave, waves that share the keys' loads
-  bool tile;    // the tile form
+  int mr, rw;  // packed rows of a wave, waves that share the keys' loads
+  bool tile;   // the tile form
   KV8Split s;
 };
 
 Choice choose(const t2w_kv8_attention_args& a) {
   Choice c;
-  c.s.G = a.heads / a.pages.kv_heads;
-  const long packed = a.max_new > 0 ? (long)min(a.max_new, a.n_tok) * c.s.G : 1 << 30;
-  static const int V = getenv("T2W_V") ? atoi(getenv("T2W_V")) : 0;
+  const int G = c.s.G = a.heads / a.pages.kv_heads;
+  const long max_new = a.max_new > 0 ? min(a.max_new, a.n_tok) : a.n_tok, packed = max_new * G;
+  const long max_kv = a.max_kv > 0 ? min((long)a.max_kv, (long)a.width * KV8_BLOCK) : (long)a.width * KV8_BLOCK;
+  const long nb = (max_kv + KV8_BLOCK - 1) / KV8_BLOCK;
+  // The direct form on as few packed rows as hold the longest row, up to 64.  With heads of 128 the tile form takes calls
+  // whose 256-row tiles (and parts) fill the chip, one workgroup a CU, and are mostly full: 32 heads over 8 (us, direct /
+  // tile): one row of 8,000 tokens 625 / 550, 2,048 behind 32,000 1,250 / 1,095, four of 500 30.7 / 27.8; a row of 1,000
+  // tokens alone (128 workgroups) 24.7 / 37.8, 32 of 70 behind 2,000 (tiles 55% full) 130 / 161.  With heads of 64 the
+  // direct form was the faster one everywhere (128-row tiles: 1,000 tokens 14.8 / 24.6, 8,000 202 / 214).
   c.mr = packed <= 16 ? 16 : 32;
-  c.rw = packed <= 32 ? 1 : packed <= 64 || V == 1 ? 2 : a.pages.head_dim == 128 ? 8 : 4;
-  c.tile = c.rw >= 4;
-  c.s.tt = c.mr * c.rw / c.s.G;
+  c.rw = packed <= 32 ? 1 : 2;
+  c.tile = false;
+  const long tt = 256 / G, rows = a.max_new > 0 ? (a.n_tok + max_new - 1) / max_new : 1;  // rows, were all of them longest
+  const long tiles = rows * ((max_new + tt - 1) / tt), groups = tiles * a.pages.kv_heads;
+  const long fit = groups >= 256 ? 1 : min(256 / max(groups, 1L), max(nb / 64, 1L));
+  if (a.pages.head_dim == 128 && packed > 64 && groups * fit >= 224 && a.n_tok * 10L >= tiles * tt * 7) {
+    c.tile = true;
+    c.rw = 8;
+  }
+  c.s.tt = c.mr * c.rw / G;
   c.s.per_row = a.max_new > 0 && a.max_new <= c.s.tt ? 1 : 0;
   c.s.n_tiles = c.s.per_row ? a.n_rows : a.n_tok / c.s.tt + a.n_rows;
-  const long max_kv = a.max_kv > 0 ? min((long)a.max_kv, (long)a.width * KV8_BLOCK) : (long)a.width * KV8_BLOCK;
-  const long nb = (max_kv + KV8_BLOCK - 1) / KV8_BLOCK, groups = (long)c.s.n_tiles * a.pages.kv_heads;
-  const long want = c.tile && a.pages.head_dim == 128 ? 256 : 512;
-  long bps = nb;
-  if (nb > 48) {
-    const long parts = (want + groups - 1) / groups;
-    bps = (nb + parts - 1) / parts;
-    if (bps < 16) bps = 16;
+  // Parts: the tile form's, so that one round of workgroups fills the chip.  The direct form's lists of up to 48 blocks stay
+  // whole (a second launch costs more: one row of 1,500 keys 9.6 us whole, 10.5 split); longer ones are cut where
+  // workgroups are few, to 512 in all and 16 blocks or more a part (two rows of 131,072 keys: 103 us with 512 workgroups,
+  // 111 with 1,024, 120 with 2,048; 64 rows of up to 8,192: 139, 152, 150).
+  long parts = 1;
+  if (c.tile) {
+    parts = fit;
+  } else if (nb > 48) {
+    const long g = (long)c.s.n_tiles * a.pages.kv_heads;
+    parts = min((512 + g - 1) / g, (nb + 15) / 16);
   }
-  const long parts = (nb + bps - 1) / bps;
-  c.s.bps = (int)bps;
-  c.s.parts = (int)(parts < 1 ? 1 : parts > 256 ? 256 : parts);
+  c.s.bps = (int)((nb + parts - 1) / parts);
+  c.s.parts = (int)min((nb + c.s.bps - 1) / c.s.bps, 256L);
   return c;
 }
 
@@ -764,10 +799,13 @@ template <bool BF, int D>
 static hipError_t launch(const t2w_kv8_attention_args& a, const Choice& c, hipStream_t st) {
   const dim3 grid((unsigned)(c.s.n_tiles * a.pages.kv_heads), c.s.parts);
   if (c.tile) {
-    constexpr int RW = D == 128 ? 8 : 4, LDS = 3 * 2 * 2 * KV8_BLOCK * D * 2;  // three steps of two blocks, keys and values in 16 bits
-    static const hipError_t attr = hipFuncSetAttribute((const void*)kv8_attn_tile_kernel<BF, D, RW>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-    if (attr != hipSuccess) return attr;
-    hipLaunchKernelGGL((kv8_attn_tile_kernel<BF, D, RW>), grid, dim3(64 * RW), LDS, st, a, c.s);
+    if constexpr (D == 128) {
+      constexpr int LDS = 3 * 2 * 2 * KV8_BLOCK * D * 2;  // three steps of two blocks, keys and values in 16 bits
+      static const hipError_t attr =  // once per process (thread-safe initialisation): the LDS above 64 KB
+          hipFuncSetAttribute((const void*)kv8_attn_tile_kernel<BF, D, 8>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+      if (attr != hipSuccess) return attr;
+      hipLaunchKernelGGL((kv8_attn_tile_kernel<BF, D, 8>), grid, dim3(512), LDS, st, a, c.s);
+    }
   } else if (c.mr == 16) {
     hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 16, 1, D == 64 ? 6 : 4>), grid, dim3(256), 0, st, a, c.s);
   } else if (c.rw == 1) {

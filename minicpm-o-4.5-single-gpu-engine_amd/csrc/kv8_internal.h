@@ -17,6 +17,17 @@ namespace t2w {
 constexpr int KV8_BLOCK = 32;
 constexpr int KV8_MAX_ROWS = 4096;  // rows of a call: the tables kernel holds three integers of each in LDS
 
+// sum over lanes 0 .. l of the wave, in lane l: shifts within the 16-lane rows, then each row's last lane to those behind it
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
 // Row that owns entry t of a list in which row r starts at row_start[r] / div + mult * r (the starts ascend with r): the
 // last row whose start is at most t, 0 if there is none.  All 64 lanes of a wave call it together; two dependent loads at
 // most (n_rows <= 4096), one up to 64 rows.
