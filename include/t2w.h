@@ -371,8 +371,8 @@ int t2w_kv8_append(const t2w_kv8_append_args* a, void* stream);
  * of its row; c > 0 it sees the row's earlier tokens and those new ones whose chunk of c new tokens is not behind its own
  * (1: causal).  A query that sees nothing gets zeros.  Rows of `out` behind the last token are left as they were.  A row
  * longer than its table is wide, or one with block ids outside the pages that a query sees, gets NaN.
- * max_new: 0, or a bound on every row's new tokens; max_kv: 0, or one on kv_total: they choose the kernel and how it
- * splits the keys.  A row of more than max_new new tokens gets NaN; one of more than max_kv keys is still right. */
+ * At most 2^24 new tokens.  max_new: 0, or a bound on every row's new tokens; max_kv: 0, or one on kv_total: they choose
+ * the kernel and how it splits the keys.  A row of more than max_new new tokens gets NaN; one of more than max_kv keys is still right. */
 typedef struct {
   t2w_kv8_pages pages;
   const void* q; void* out;       /* [n_tok, heads, head_dim], token rows ldq / ldo elements apart (multiples of 8) */

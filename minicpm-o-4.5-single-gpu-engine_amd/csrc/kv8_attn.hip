@@ -44,21 +44,34 @@ __device__ __forceinline__ bool find_tile(const t2w_kv8_attention_args& a, const
     t.start = a.row_start[t.row];
     next = a.row_start[t.row + 1];
     t.total = a.kv_total[t.row];
-  } else if (a.n_rows <= 64) {  // all rows at once, one a lane, and their tiles counted: the slots without one come last
+  } else if (a.n_rows <= 64) {
+    // All rows at once, one a lane.  Slots go by the tile's place in its row, the last ones first: the tiles of a causal
+    // prompt that see most start first.  With N(x) the tiles at place x or later, slot s is at the largest x with N(x) > s.
     const int lane = threadIdx.x & 63, r = min(lane, a.n_rows - 1);
     const int start = a.row_start[r], stop = a.row_start[r + 1], total = a.kv_total[r];
-    const int tiles = lane < a.n_rows && stop > start ? (stop - start - 1) / s.tt + 1 : 0, before = wave_scan(tiles) - tiles;
-    t.row = max((int)__popcll(__builtin_amdgcn_ballot_w64(lane < a.n_rows && before <= slot)) - 1, 0);
+    const int tiles = lane < a.n_rows && stop > start ? min((stop - start - 1) / s.tt + 1, 1 << 24) : 0;
+    auto from = [&](int x) { return __builtin_amdgcn_readlane(wave_scan(max(tiles - x, 0)), 63); };
+    if (from(0) <= slot) return false;
+    int lo = 0, hi = s.n_tiles + 1;  // no row has more tiles than the call has slots
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (from(mid) > slot) lo = mid; else hi = mid;
+    }
+    const uint64_t have = __builtin_amdgcn_ballot_w64(tiles > lo);
+    const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(have >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)have, 0));
+    const int nth = slot - from(lo + 1);  // of the rows with a tile there
+    t.row = min((int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(tiles > lo && rank == nth) | (1ull << 63)), a.n_rows - 1);
     t.start = __builtin_amdgcn_readlane(start, t.row);
     next = __builtin_amdgcn_readlane(stop, t.row);
     t.total = __builtin_amdgcn_readlane(total, t.row);
-    at = slot - __builtin_amdgcn_readlane(before, t.row);
-  } else {
-    t.row = kv8_find_row(a.row_start, a.n_rows, s.tt, 1, slot);
+    at = lo;
+  } else {  // the last rows' last tiles first
+    const int back = s.n_tiles - 1 - slot;
+    t.row = kv8_find_row(a.row_start, a.n_rows, s.tt, 1, back);
     t.start = a.row_start[t.row];
     next = a.row_start[t.row + 1];
     t.total = a.kv_total[t.row];
-    at = slot - (t.start / s.tt + t.row);
+    at = back - (t.start / s.tt + t.row);
   }
   // the same in every lane, which the compiler does not see on every way here
   t.row = __builtin_amdgcn_readfirstlane(t.row);
@@ -478,8 +491,7 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
   extern __shared__ uint4 s_kv[];
   uint4 (*s_k)[2][2 * CB] = (uint4 (*)[2][2 * CB])s_kv, (*s_v)[2][2 * CB] = s_k + 3;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // the last tiles first: a causal prompt's longest
-  const int slot = sp.n_tiles - 1 - blockIdx.x / a.pages.kv_heads, kv_head = blockIdx.x % a.pages.kv_heads, part = blockIdx.y;
+  const int slot = blockIdx.x / a.pages.kv_heads, kv_head = blockIdx.x - slot * a.pages.kv_heads, part = blockIdx.y;
   Tile t;
   if (!find_tile(a, sp, slot, t)) return;
   if (t.bad) {

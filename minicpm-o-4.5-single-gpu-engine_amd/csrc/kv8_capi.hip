@@ -81,6 +81,7 @@ static const char* check_attention(const t2w_kv8_attention_args* a) {
   if (a->dtype != T2W_KV8_BF16 && a->dtype != T2W_KV8_FP16) return "kv8 attention: dtype must be bf16 or fp16";
   if (a->heads < 1 || a->heads % a->pages.kv_heads || a->heads / a->pages.kv_heads > 16) return "kv8 attention: heads must be 1 to 16 times kv_heads";
   if (a->n_tok < 0 || a->chunk < 0 || a->max_new < 0 || a->max_kv < 0) return "kv8 attention: negative n_tok, chunk, max_new or max_kv";
+  if (a->n_tok > (1 << 24)) return "kv8 attention: at most 2^24 new tokens";
   if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return "kv8 attention: scale must be positive and finite";
   return nullptr;
 }

@@ -67,7 +67,7 @@ def test_append_refuses(kw, text):
     refused(_lib.lib().t2w_kv8_append, set_all(a, kw), text)
 
 
-@pytest.mark.parametrize("kw,text", PAGES_BAD + [({"out": None}, "null operand"), ({"heads": 12}, "heads"), ({"heads": 136}, "heads"), ({"heads": 0}, "heads"),
+@pytest.mark.parametrize("kw,text", PAGES_BAD + [({"out": None}, "null operand"), ({"heads": 12}, "heads"), ({"heads": 136}, "heads"), ({"heads": 0}, "heads"), ({"n_tok": (1 << 24) + 1}, "2^24"),
                                                  ({"chunk": -1}, "negative"), ({"max_kv": -5}, "negative"), ({"scale": 0.0}, "scale"),
                                                  ({"scale": float("nan")}, "scale"), ({"scale": float("inf")}, "scale"), ({"ldq": 4088}, "overlap"),
                                                  ({"ldo": 4100}, "strides"), ({"q": (1 << 20) + 2}, "aligned")], ids=str)
