@@ -154,8 +154,7 @@ __device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float(
 
 // Softmax and output state of a wave's MR packed rows (lane column = query), shared by both kernels.  Scores are in units of
 // log2, s = q . k times c = scale log2(e) 2^(key exponent).
-//  * m is a reference that the running maximum may pass by 8 before it is moved (by the whole wave, then the true maximum so
-//    far): probabilities are 2^(s - m + 7) <= 2^15 in fp16, so most blocks need no exchange between lanes and no rescaling of
+//  * m is a reference that the running maximum may pass by 8 before it is moved (then to the true maximum so far): probabilities are 2^(s - m + 7) <= 2^15 in fp16, so most blocks need no exchange between lanes and no rescaling of
 //    the outputs, and a probability keeps fp16's 11 bits down to 2^-21 of the largest and 2^-32 of it absolutely.  fp16 and
 //    not bf16: bf16's 8 bits would cost as much again as the output's own rounding.
 //  * value codes enter as fp16, exact, times 2^(their exponent - E + 7), E the largest value exponent so far: 22 powers of two
@@ -214,7 +213,7 @@ struct State {
   __device__ __forceinline__ void move(Acc (&sc)[KG], float& c, float mx) {
     mx *= c;
     if (__builtin_amdgcn_ballot_w64(mx > m + 8.f)) {
-      const float mn = fmaxf(m, query_max<MR>(mx));
+      const float seen = query_max<MR>(mx), mn = seen > m + 8.f ? seen : m;  // each query by its own scores alone
       const float alpha = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       nb = mn == -__builtin_inff() ? 7.f : 7.f - mn;

@@ -97,19 +97,20 @@ def attention(q, keys, vals, table, row_start, kv_total, scale, chunk):
     G = keys.shape[1]
     out, mag, top = np.zeros((N, H, D)), np.zeros((N, H, D)), np.zeros((N, H))
     for r in range(len(kv_total)):
-        new, total = row_start[r + 1] - row_start[r], kv_total[r]
+        a, b, total = row_start[r], row_start[r + 1], kv_total[r]
+        i = np.arange(b - a)
+        see = total - (b - a) + (b - a if chunk == 0 else np.minimum(b - a, (i // chunk + 1) * chunk)) + 0 * i
+        if b == a or see.max() <= 0:
+            continue
         ids = table[r, :-(-total // BLOCK)]
-        for i in range(new):
-            see = total - new + (new if chunk == 0 else min(new, (i // chunk + 1) * chunk))
-            if see <= 0:
-                continue
-            n = row_start[r] + i
-            for h in range(H):
-                g = h // (H // G)
-                kk, vv = keys[ids, g].reshape(-1, D)[:see], vals[ids, g].reshape(-1, D)[:see]
-                s = kk @ q[n, h] * scale
-                p = np.exp(s - s.max())
-                p /= p.sum()
-                out[n, h], mag[n, h] = p @ vv, p @ np.abs(vv)
-                top[n, h] = scale * (np.abs(kk) @ np.abs(q[n, h])).max()
+        hide = np.arange(total)[None] >= see[:, None]
+        for h in range(H):
+            g = h // (H // G)
+            kk, vv = keys[ids, g].reshape(-1, D)[:total], vals[ids, g].reshape(-1, D)[:total]
+            s = np.where(hide, -np.inf, q[a:b, h] @ kk.T * scale)
+            m = s.max(1, keepdims=True)
+            p = np.exp(s - np.where(np.isfinite(m), m, 0.0))
+            p /= np.maximum(p.sum(1, keepdims=True), 1e-300)
+            out[a:b, h], mag[a:b, h] = p @ vv, p @ np.abs(vv)
+            top[a:b, h] = scale * np.where(hide, 0.0, np.abs(q[a:b, h]) @ np.abs(kk).T).max(1)
     return out, mag, top

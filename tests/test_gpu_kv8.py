@@ -5,7 +5,8 @@ every precision.  Attention's bound per output, with u = 2^-24 (an fp32 rounding
 dot products of D exact products are off by at most (D + 2) u times their absolute sums, the scaled score, its
 difference from the maximum and exp2 add a few u times the score, and a relative error of p_j by that much moves
 sum p v / sum p by at most twice that times sum p |v|; a probability rounded to 16 bits for the matrix unit is off by
-2^-11 at most, the sums by another (32 + D) u at any length that the tests have; the output's own rounding is eps / 2 of it.
+2^-11 at most, the sums by another (32 + D) u at any length that the tests have; the output's own rounding is eps / 2 of it,
+or half the type's smallest step (fp16: 2^-25) where it lies below the normal range, whose steps do not shrink any more.
 """
 
 import random
@@ -230,7 +231,8 @@ def test_append_skips_foreign_blocks(dev):
 def attn_bound(o, mag, top, d, dt):
     u = 2.0 ** -24
     rel_p = 2 * ((d + 2) * u * top + 8 * u * (top * 1.4427 + 2) + 2.0 ** -11) + 2 * (32 + d) * u
-    return torch.finfo(dt).eps / 2 * np.abs(o) * 1.01 + rel_p[:, :, None] * mag * 1.01 + 1e-30
+    f = torch.finfo(dt)
+    return f.eps / 2 * np.maximum(np.abs(o), f.smallest_normal) * 1.01 + rel_p[:, :, None] * mag * 1.01
 
 
 def check_attention(q, pages, table, new, totals, chunk, scale=None, **kw):
@@ -310,6 +312,45 @@ def test_attention_long(dev, d, dt, rows, new, old):
             check_attention(q, pages, table, [new] * rows, totals, chunk, **bounds)
 
 
+# calls that the tile form takes: heads of 128, 256-row tiles mostly full, 224 workgroups or more
+TILE = [(1, 32, 7, 200), (2, 32, 7, 101), (4, 16, 7, 97), (7, 16, 7, 70), (16, 14, 8, 31), (3, 29, 8, 170)]  # group, kv_heads, rows, new
+
+
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("G,g,rows,new", TILE)
+@pytest.mark.parametrize("chunk", [0, 1, 7])
+def test_attention_prompts(dev, dt, G, g, rows, new, chunk):
+    """Many packed rows: whole prompts and prompts behind cached tokens of several lengths, some ragged."""
+    new_l = [max(1, new - (5 * r if r % 3 == 1 else 0)) for r in range(rows)]
+    totals = [n + (0, 1, 40, 95, 300)[r % 5] for r, n in enumerate(new_l)]
+    table, nb = random_table(totals, 1, seed=G)
+    pages = random_pages(nb, g, 128, seed=new)
+    q = queries(sum(new_l), G * g, 128, dt, seed=g)
+    check_attention(q, pages, table, new_l, totals, chunk, max_new=new, max_kv=max(totals))
+
+
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_attention_prompt_in_parts(dev, dt):
+    """A chunk of a prompt over a long cache: key lists cut so that the tiles fill the chip, block ids beyond the first 64
+    of a part."""
+    table, nb = random_table([17000], 1, seed=3)
+    pages = random_pages(nb, 32, 128, seed=3)
+    for chunk in (0, 1):
+        check_attention(queries(256, 32, 128, dt, seed=4), pages, table, [256], [17000], chunk, max_new=256, max_kv=17000)
+
+
+def test_attention_rows_of_many_tiles(dev):
+    """More than 64 rows, of one to three tiles and none."""
+    new = [(0, 1, 130, 64, 200, 65, 3)[r % 7] for r in range(80)]
+    totals = [n + 9 * (r % 11) for r, n in enumerate(new)]
+    table, nb = random_table(totals, 0, seed=1)
+    for d, h in ((64, 1), (128, 4)):
+        pages = random_pages(nb, h, d, seed=3)
+        q = queries(sum(new), h, d, BF, seed=4)
+        for bounds in ({"max_new": 200, "max_kv": 300}, {}):
+            check_attention(q, pages, table, new, totals, 1, **bounds)
+
+
 @pytest.mark.parametrize("rows", [65, 500, 4096])
 def test_attention_many_rows(dev, rows):
     rng = random.Random(rows)
@@ -363,65 +404,75 @@ def test_attention_empty_rows(dev, new):
             check_attention(q, pages, table, new_l, totals, chunk, **bounds)
 
 
-@pytest.mark.parametrize("new", [1, 40, 140])
-@pytest.mark.parametrize("d", [64, 128])
-def test_attention_ignores_what_lies_behind(dev, new, d):
+FORMS = [(1, 4, 2, 64, 3), (40, 4, 2, 64, 3), (140, 4, 2, 64, 3), (1, 4, 2, 128, 3), (20, 4, 2, 128, 4), (40, 2, 2, 128, 3), (101, 64, 32, 128, 7)]
+
+
+@pytest.mark.parametrize("new,h,g,d,rows", FORMS)
+def test_attention_ignores_what_lies_behind(dev, new, h, g, d, rows):
     """NaN codes and E8M0 NaN scales behind the rows' last tokens and in blocks of nobody, ids behind the rows' tables."""
-    totals = [new + 100, new + 11, new]
+    totals = [new + (100, 11, 0)[r % 3] for r in range(rows)]
     table, nb = random_table(totals, 2, seed=1)
-    pages = random_pages(nb, 2, d, seed=5)
+    pages = random_pages(nb, g, d, seed=5)
     used = sorted(x for r, t in enumerate(totals) for x in table[r, :need(t)])
     for b in set(range(nb)) - set(used):
         pages.k[b], pages.v[b], pages.k_exp[b], pages.v_exp[b] = 255, 255, 255, 255
     k, v = pages.k, pages.v
-    q = queries(3 * new, 4, d, BF, seed=6)
-    clean = check_attention(q, pages, table, [new] * 3, totals, 1).clone()
+    q = queries(rows * new, h, d, BF, seed=6)
+    clean = check_attention(q, pages, table, [new] * rows, totals, 1, max_new=new, max_kv=max(totals)).clone()
     for r, t in enumerate(totals):
         if t % 32:
             b = int(table[r, t // 32])
             k[b, :, :, t % 32:] = 0x7F
-            vv = v[b].permute(0, 1, 4, 2, 3).reshape(2, 32, d // 2, 2).clone()
+            vv = v[b].permute(0, 1, 4, 2, 3).reshape(g, 32, d // 2, 2).clone()
             vv[:, t % 32:] = 0xFF
-            v[b] = vv.reshape(2, 4, 8, d // 2, 2).permute(0, 1, 3, 4, 2)
-    for bounds in ({"max_new": new, "max_kv": max(totals)}, {"max_new": new}, {}):
-        out = kv8.attention(q, pages, torch.from_numpy(table).cuda(), ints(starts([new] * 3)), ints(totals), scale=d ** -0.5, chunk=1, **bounds)
+            v[b] = vv.reshape(g, 4, 8, d // 2, 2).permute(0, 1, 3, 4, 2)
+    for bounds in ({}, {"max_new": new}, {"max_new": new, "max_kv": max(totals)}):
+        out = kv8.attention(q, pages, torch.from_numpy(table).cuda(), ints(starts([new] * rows)), ints(totals), scale=d ** -0.5, chunk=1, **bounds)
         assert torch.isfinite(out).all()
     assert torch.equal(out, clean)
 
 
-@pytest.mark.parametrize("new", [1, 40, 140])
-def test_attention_nan_tokens_reach_only_who_sees_them(dev, new):
+@pytest.mark.parametrize("new,h,g,d,rows", FORMS)
+def test_attention_nan_tokens_reach_only_who_sees_them(dev, new, h, g, d, rows):
     """A NaN key (stored by the append for a token that is not finite) in causal windows: earlier queries are untouched."""
     old = 70
-    totals = [old + new] * 2
+    totals = [old + new] * rows
     table, nb = random_table(totals, 0, seed=1)
-    pages = random_pages(nb, 2, 64, seed=5)
-    q = queries(2 * new, 4, 64, BF, seed=6)
-    args = (torch.from_numpy(table).cuda(), ints(starts([new] * 2)), ints(totals))
-    clean = kv8.attention(q, pages, *args, scale=0.125, chunk=1)
+    pages = random_pages(nb, g, d, seed=5)
+    q = queries(rows * new, h, d, BF, seed=6)
+    args = (torch.from_numpy(table).cuda(), ints(starts([new] * rows)), ints(totals))
+    clean = kv8.attention(q, pages, *args, scale=0.125, chunk=1, max_new=new)
     at = old + new // 2
     pages.k[int(table[0, at // 32]), 1, :, at % 32] = 0x7F
-    out = kv8.attention(q, pages, *args, scale=0.125, chunk=1)
-    hit = torch.zeros(2 * new, 4, dtype=torch.bool, device="cuda")
-    hit[new // 2:new, 2:] = True
+    out = kv8.attention(q, pages, *args, scale=0.125, chunk=1, max_new=new)
+    hit = torch.zeros(rows * new, h, dtype=torch.bool, device="cuda")
+    hit[new // 2:new, h // g:2 * (h // g)] = True
     assert out[hit].isnan().all() and torch.equal(out[~hit], clean[~hit])
 
 
-@pytest.mark.parametrize("new", [1, 40, 140])
-def test_attention_malformed_rows(dev, new):
-    """Block ids outside the pages and rows longer than their table: NaN for who sees them, the others as ever."""
-    totals = [new + 100] * 4
+@pytest.mark.parametrize("new,h,g,d,rows", FORMS)
+def test_attention_malformed_rows(dev, new, h, g, d, rows):
+    """Block ids outside the pages and rows longer than their table: NaN for who sees them, the others as ever.  Block 0 of
+    the pages holds NaN codes, as memory that nothing was appended to may."""
+    rows = max(rows, 4)
+    totals = [new + 100] * rows
     table, nb = random_table(totals, 0, seed=1)
-    pages = random_pages(nb, 2, 64, seed=5)
-    q = queries(4 * new, 2, 64, BF, seed=6)
-    start = ints(starts([new] * 4))
-    clean = kv8.attention(q, pages, torch.from_numpy(table).cuda(), start, ints(totals), scale=0.125, chunk=1)
+    table = np.where(table == 0, nb - 1, table) if 0 in table else table  # block 0 belongs to nobody
+    pages = random_pages(nb, g, d, seed=5)
+    pages.k[0], pages.v[0] = 0x7F, 0xFF
+    q = queries(rows * new, h, d, BF, seed=6)
+    start = ints(starts([new] * rows))
+    clean = kv8.attention(q, pages, torch.from_numpy(table).cuda(), start, ints(totals), scale=0.125, chunk=1, max_new=new)
+    assert torch.isfinite(clean).all()
     table[1, 1] = nb
     table[2, 0] = -1
-    out = kv8.attention(q, pages, torch.from_numpy(table).cuda(), start, ints(totals[:3] + [table.shape[1] * 32 + 1]), scale=0.125, chunk=1)
-    assert torch.equal(out[:new], clean[:new]) and out[new:].isnan().all()
+    table[0, (totals[0] - 1) // 32] = 1 << 30  # the last new tokens' block: the tokens before it do not see it
+    out = kv8.attention(q, pages, torch.from_numpy(table).cuda(), start, ints(totals[:3] + [table.shape[1] * 32 + 1] + totals[4:]), scale=0.125, chunk=1,
+                        max_new=new)
+    first = max(0, (totals[0] - 1) // 32 * 32 - 100)  # row 0's first token that does
+    assert torch.equal(out[:first], clean[:first]) and out[first:4 * new].isnan().all() and torch.equal(out[4 * new:], clean[4 * new:])
     if new > 1:  # a row of more new tokens than the bound says: NaN where the bound chose the kernel
-        out = kv8.attention(q[:new + 1], pages, torch.from_numpy(table[:2] * 0).cuda(), ints([0, new, new + 1]), ints(totals[:2]), scale=0.125, chunk=1,
+        out = kv8.attention(q[:new + 1], pages, torch.from_numpy(table[:2] * 0 + 1).cuda(), ints([0, new, new + 1]), ints(totals[:2]), scale=0.125, chunk=1,
                             max_new=1)
         assert (out[:new].isnan().all() or torch.isfinite(out[:new]).all()) and torch.isfinite(out[new]).all()
 
