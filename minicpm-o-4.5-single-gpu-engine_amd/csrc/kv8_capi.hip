@@ -55,6 +55,11 @@ int t2w_kv8_plan(const t2w_kv8_plan_args* a, void* stream) {
   for (const auto& x : in)
     for (const auto& y : out)
       if (x.p && y.p && x.n && y.n && meet(x.p, x.n, y.p, y.n)) return kerr("kv8 plan: an output lies on an input");
+  const size_t span = a->n_rows > 0 ? ((size_t)(a->n_rows - 1) * a->ld_table + a->width) * 4 : 0;
+  for (const auto& x : in)
+    if (span && x.n && meet(x.p, x.n, a->table, span)) return kerr("kv8 plan: the table lies on an input");
+  for (const auto& y : out)
+    if (span && y.n && meet(y.p, y.n, a->table, span)) return kerr("kv8 plan: an output lies on the table");
   const hipError_t e = kv8_plan(*a, (hipStream_t)stream);
   return e == hipSuccess ? 0 : kerr("kv8 plan", e);
 }

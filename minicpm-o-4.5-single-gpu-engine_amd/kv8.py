@@ -25,8 +25,11 @@ from . import _lib
 
 BLOCK = 32       # tokens of a block
 MAX_ROWS = 4096  # rows of a call
-# torch's current stream of a device as the raw handle, without the 2 us of making a Stream object for each call
+# A step's calls take 4 to 8 us on the GPU: the host's part is kept as short.  torch's current stream of a device as the raw
+# handle, without the 2 us of making a Stream object for each call; the current device likewise.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_I32 = torch.int32
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 
 
@@ -73,33 +76,39 @@ class KV8Pages:
 
 def _ints(what: str, t: torch.Tensor, n: int, dev) -> int:
     """Device pointer of a contiguous int32 vector of ``n`` entries."""
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != dev or not t.is_contiguous():
+    if t.dtype is not _I32 or t.dim() != 1 or t.numel() != n or t.device != dev or not t.is_contiguous():
         raise ValueError(f"kv8: {what} must be a contiguous int32 vector of {n} on {dev}")
     return t.data_ptr()
 
 
 def _table(t: torch.Tensor, rows: int, dev) -> tuple[int, int, int]:
-    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1 or t.stride(1) != 1 or t.device != dev:
-        raise ValueError(f"kv8: the table must be int32 [{rows}, width] with whole rows on {dev}")
-    return t.data_ptr(), t.shape[1], t.stride(0) if rows > 1 else t.shape[1]
+    if t.dtype is not _I32 or t.dim() != 2 or t.device != dev:
+        raise ValueError(f"kv8: the table must be int32 [{rows}, width] on {dev}")
+    n, width = t.shape
+    ld, one = t.stride()
+    if n != rows or width < 1 or (one != 1 and width > 1):
+        raise ValueError(f"kv8: the table must have {rows} rows, each contiguous")
+    return t.data_ptr(), width, ld if rows > 1 else width
 
 
 def _tokens(what: str, t: torch.Tensor, n, d: int, dev) -> int:
     """Elements between the token rows of [n_tok, heads, head_dim] (a token's heads lie side by side)."""
-    if t.dim() != 3 or t.shape[2] != d or t.stride(2) != 1 or (t.stride(1) != d and t.shape[1] > 1) or t.device != dev:
-        raise ValueError(f"kv8: {what} must be [n_tok, heads, {d}] on {dev}, a token's heads side by side")
-    if t.dtype not in _DTYPES:
-        raise ValueError(f"kv8: {what} must be bfloat16 or float16")
-    if n is not None and t.shape[0] != n:
+    if t.dim() != 3 or t.device != dev or t.dtype not in _DTYPES:
+        raise ValueError(f"kv8: {what} must be bfloat16 or float16 [n_tok, heads, {d}] on {dev}")
+    rows, heads, width = t.shape
+    ld, head, one = t.stride()
+    if width != d or one != 1 or (head != d and heads > 1):
+        raise ValueError(f"kv8: {what} must be [n_tok, heads, {d}], a token's heads side by side")
+    if n is not None and rows != n:
         raise ValueError(f"kv8: {what} must have {n} tokens")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * d
+    return ld if rows > 1 else heads * d
 
 
 def _call(fn, args, dev, what: str) -> None:
     """One library call on torch's current stream of ``dev``."""
     if dev.type != "cuda":
         raise ValueError(f"kv8 {what}: the tensors must be on the GPU")
-    if dev.index == torch.cuda.current_device():
+    if dev.index == _current_device():
         _lib.check(fn(C.byref(args), _raw_stream(dev.index)), what)
     else:
         with torch.cuda.device(dev):

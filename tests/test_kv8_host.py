@@ -42,7 +42,8 @@ def set_all(a, kw):
 PLAN_BAD = [({"n_rows": -1}, "n_rows"), ({"n_rows": 4097}, "n_rows"), ({"width": 0}, "width"), ({"ld_table": 3}, "width"), ({"n_tok": -1}, "negative"),
             ({"n_free": -1}, "negative"), ({"kv_len": None}, "null"), ({"table": None}, "null"), ({"status": None}, "null"), ({"slots": None}, "null"),
             ({"free_head_out": 3 << 20}, "output lies on an input"), ({"kv_total": 1 << 20}, "output lies on an input"),
-            ({"row_start": (2 << 20) + 12}, "output lies on an input"), ({"slots": (5 << 20) + 60}, "output lies on an input")]
+            ({"row_start": (2 << 20) + 12}, "output lies on an input"), ({"slots": (5 << 20) + 60}, "output lies on an input"), ({"table": (1 << 20) - 60}, "table lies on an input"),
+            ({"status": (4 << 20) + 60}, "output lies on the table")]
 
 
 @pytest.mark.parametrize("kw,text", PLAN_BAD, ids=str)
