@@ -372,7 +372,7 @@ int t2w_kv8_append(const t2w_kv8_append_args* a, void* stream);
  * (1: causal).  A query that sees nothing gets zeros.  Rows of `out` behind the last token are left as they were.  A row
  * longer than its table is wide, or one with block ids outside the pages that a query sees, gets NaN.
  * At most 2^24 new tokens.  max_new: 0, or a bound on every row's new tokens; max_kv: 0, or one on kv_total: they choose
- * the kernel and how it splits the keys.  A row of more than max_new new tokens gets NaN; one of more than max_kv keys is still right. */
+ * the kernel and how it splits the keys.  A row of more than max_new new tokens may get NaN; one of more than max_kv keys is still right. */
 typedef struct {
   t2w_kv8_pages pages;
   const void* q; void* out;       /* [n_tok, heads, head_dim], token rows ldq / ldo elements apart (multiples of 8) */

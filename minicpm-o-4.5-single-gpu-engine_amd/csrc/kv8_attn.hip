@@ -2,6 +2,7 @@
 // i sees, key and value codes times their blocks' scales.  Block format: kv8_internal.h.
 #include "kv8_internal.h"
 
+#include <atomic>
 #include <type_traits>
 
 namespace t2w {
@@ -16,7 +17,7 @@ typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 struct KV8Split {
   int G;        // query heads of a key head
   int tt;       // tokens of a tile
-  int per_row;  // tile slots of a row, 0: tiles listed over all rows (kv8_find_row)
+  int per_row;  // tile slots of a row, 0: tiles listed over all rows (find_tile)
   int n_tiles;  // tile slots of the call
   int bps;      // key blocks of a part, more where a row would have over `parts` of them
   int parts;    // most parts of a tile; 1: the kernel writes the outputs itself
@@ -154,9 +155,10 @@ __device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float(
 
 // Softmax and output state of a wave's MR packed rows (lane column = query), shared by both kernels.  Scores are in units of
 // log2, s = q . k times c = scale log2(e) 2^(key exponent).
-//  * m is a reference that the running maximum may pass by 8 before it is moved (then to the true maximum so far): probabilities are 2^(s - m + 7) <= 2^15 in fp16, so most blocks need no exchange between lanes and no rescaling of
-//    the outputs, and a probability keeps fp16's 11 bits down to 2^-21 of the largest and 2^-32 of it absolutely.  fp16 and
-//    not bf16: bf16's 8 bits would cost as much again as the output's own rounding.
+//  * m is a reference that the running maximum may pass by 8 before it is moved (then to the true maximum so far):
+//    probabilities are 2^(s - m + 7) <= 2^15 in fp16, so most blocks need no exchange between lanes and no rescaling of the
+//    outputs, and a probability keeps fp16's 11 bits down to 2^-21 of the largest and 2^-32 of it absolutely.  fp16 and not
+//    bf16: bf16's 8 bits would cost as much again as the output's own rounding.
 //  * value codes enter as fp16, exact, times 2^(their exponent - E + 7), E the largest value exponent so far: 22 powers of two
 //    below the largest block's scale stay exact.
 //  * sums of probabilities are of the same rounded fp16 values as the outputs' (fp32 dot products, a lane its own keys').
@@ -331,8 +333,11 @@ struct State {
 // of MR packed rows each, times 4 / RW waves that take every (4 / RW)-th block; their states are merged through LDS.
 //
 // Bound by memory: 2 D codes a token and key head are read once and meet at least MR query columns of the matrix unit, whose
-// unused columns cost nothing that matters.  MR = 16 (16x16x32 MFMA) has half the softmax work of MR = 32 (32x32x16) where
-// rows allow it.
+// unused columns cost nothing that matters (64 rows of up to 8,192 keys, 32 heads over 8 of 128: 735 MB in 137 us, 5.35 TB/s
+// where a copy reaches 5.14 and reads alone 5.87).  One register set a block: the next block's keys load as soon as the
+// scores have used these, its values after P . V; two sets spilled and took 221 us.  MR = 16 (16x16x32 MFMA) has half the
+// softmax work of MR = 32 (32x32x16) where rows allow it.  Heads of 64 run four workgroups a CU, so that 1,024 workgroups of
+// windows are all resident (64 rows of 50 tokens over 370 keys: 16.5 us; three a CU 19.7).
 //
 // With S^T = K . Q^T the score MFMA leaves a lane scores of its own query only; the rows of K are fed in an order that makes
 // them the 8 (MR = 16) or 2 x 8 keys whose value bytes the same lane loads as the P . V operand:
@@ -481,7 +486,15 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
 
 // Tile form, for tiles of many packed rows (prompts): RW waves of 32 packed rows each share the keys, two blocks a step.  The
 // workgroup loads a step's codes (one step ahead, in registers), converts them once, and leaves them in LDS as the MFMA
-// operands (double buffered, one barrier a step); every wave then reads whole fragments, 16 consecutive bytes a lane.
+// operands; every wave then reads whole fragments, 16 consecutive bytes a lane.  Three LDS steps: one is read, the next one
+// written, and with one barrier in the middle of a step no wave writes what another may still read of the step before.
+//
+// A 32x32x16 MFMA keeps the matrix unit for 32 cycles and the vector issue port for 16: four vector instructions behind each
+// are free.  So a block's exponentials run between the next block's score MFMAs, and the conversion and the next maximum
+// between the value MFMAs.  2,048 tokens over 32,000 (32 heads over 8 of 128, fp16, causal): 1,070 us, 1.03 PFLOP/s against
+// 1.17 of a large library product on the same card; 45% of the cycles on the matrix unit, 43% issuing vector instructions,
+// the LDS reads (16 KB a wave and block) about half.  Without the interleaving 1,190 us; sums on the matrix unit 1,115; four
+// waves and two workgroups a CU 1,174 against 1,096 in the same run.
 template <bool BF, int D, int RW>
 __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_attention_args a, KV8Split sp) {
   typedef State<32, D> St;
@@ -812,9 +825,16 @@ static hipError_t launch(const t2w_kv8_attention_args& a, const Choice& c, hipSt
   if (c.tile) {
     if constexpr (D == 128) {
       constexpr int LDS = 3 * 2 * 2 * KV8_BLOCK * D * 2;  // three steps of two blocks, keys and values in 16 bits
-      static const hipError_t attr =  // once per process (thread-safe initialisation): the LDS above 64 KB
-          hipFuncSetAttribute((const void*)kv8_attn_tile_kernel<BF, D, 8>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-      if (attr != hipSuccess) return attr;
+      static std::atomic<uint64_t> done{0};  // devices whose LDS limit of this kernel is raised above 64 KB
+      int dev = 0;
+      hipError_t e = hipGetDevice(&dev);
+      if (e != hipSuccess) return e;
+      const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+      if (!(done.load(std::memory_order_acquire) & bit)) {
+        e = hipFuncSetAttribute((const void*)kv8_attn_tile_kernel<BF, D, 8>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) return e;
+        done.fetch_or(bit, std::memory_order_release);
+      }
       hipLaunchKernelGGL((kv8_attn_tile_kernel<BF, D, 8>), grid, dim3(512), LDS, st, a, c.s);
     }
   } else if (c.mr == 16) {

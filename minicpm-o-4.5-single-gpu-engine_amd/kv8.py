@@ -104,6 +104,11 @@ def _tokens(what: str, t: torch.Tensor, n, d: int, dev) -> int:
     return ld if rows > 1 else heads * d
 
 
+def _small(what: str, n: int) -> None:
+    if n > 0x7FFFFFFF:  # the struct's ints would wrap
+        raise ValueError(f"kv8: {what} beyond 2^31 - 1")
+
+
 def _call(fn, args, dev, what: str) -> None:
     """One library call on torch's current stream of ``dev``."""
     if dev.type != "cuda":
@@ -167,6 +172,7 @@ def append(pages: KV8Pages, k: torch.Tensor, v: torch.Tensor, table: torch.Tenso
     a joint projection), into their rows' blocks.  ``max_new``: the longest row's new tokens if known (sizes the grid)."""
     dev, d, rows = pages.device, pages.head_dim, kv_total.shape[0]
     ldk, ldv = _tokens("k", k, None, d, dev), _tokens("v", v, k.shape[0], d, dev)
+    _small("max_new", max_new)
     if k.dtype != v.dtype or k.shape[1] != pages.kv_heads or v.shape[1] != pages.kv_heads:
         raise ValueError(f"kv8 append: k and v of one type with {pages.kv_heads} heads")
     a = _lib.KV8AppendArgs(pages.struct, k.data_ptr(), v.data_ptr(), ldk, ldv, _DTYPES[k.dtype], k.shape[0], *_table(table, rows, dev),
@@ -180,9 +186,10 @@ def attention(q: torch.Tensor, pages: KV8Pages, table: torch.Tensor, row_start: 
     """softmax(scale q K^T) V of every new token ``q`` [n_tok, heads, head_dim] over its row's cache; ``heads`` is 1 to 16 times
     the pages' heads.  ``chunk``: 0 a token sees all of its row, c > 0 the row's earlier tokens and the new ones of its own and
     earlier chunks of c (1: causal).  ``max_new`` / ``max_kv``: bounds on the rows' new and total tokens, 0 unknown (a row
-    of more than ``max_new`` gets NaN).  Rows of ``out`` behind the last token are left as they were."""
+    of more than ``max_new`` may get NaN).  Rows of ``out`` behind the last token are left as they were."""
     dev, d, rows = pages.device, pages.head_dim, kv_total.shape[0]
     ldq = _tokens("q", q, None, d, dev)
+    _small("chunk, max_new or max_kv", max(chunk, max_new, max_kv))
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         ldo = q.shape[1] * d

@@ -145,6 +145,11 @@ def test_append_and_attention_refuse():
     for out in (torch.zeros_like(q, dtype=torch.float16), q[:3].clone(), q[:, :4].clone()):
         with pytest.raises(ValueError):
             kv8.attention(q, p, *rows, scale=0.1, out=out)
+    for kw in ({"max_new": 1 << 32}, {"max_kv": 1 << 31}, {"chunk": (1 << 32) + 1}):
+        with pytest.raises(ValueError, match="2\\^31"):
+            kv8.attention(q, p, *rows, scale=0.1, **kw)
+    with pytest.raises(ValueError, match="2\\^31"):
+        kv8.append(p, x, x, *rows, max_new=1 << 32)
     with pytest.raises(ValueError, match="GPU"):
         kv8.attention(q, p, *rows, scale=0.1)
 
