@@ -314,7 +314,7 @@ int t2w_attention(const void* q, const void* k_pool, const void* v_pool, void* o
 /* ---------------------------------------------------------------- paged 8-bit key/value cache
  * A cache of blocks of 32 tokens in OCP e4m3, each block with one power-of-two scale (E8M0: exponent + 127) per
  * key/value head for its keys and one for its values; half the memory of the bf16 slot pools.  No counterpart in the
- * reference, whose pools are 16-bit (engine/runtime/dit_fast.py:60-97).  Three calls serve a step: t2w_kv8_plan builds
+ * reference, whose pools are 16-bit (engine/runtime/dit_fast.py:59-64).  Three calls serve a step: t2w_kv8_plan builds
  * the tables from the requests' lengths on the GPU, t2w_kv8_append stores the new keys and values, t2w_kv8_attention
  * reads the cache.  All lengths and tables are device data, so a graph captured once serves calls of other lengths.
  *

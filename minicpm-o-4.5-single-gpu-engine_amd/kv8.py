@@ -1,6 +1,6 @@
 """Paged 8-bit key/value cache on the MI355X kernels: e4m3 blocks of 32 tokens with a power-of-two scale per block and
 head, half the memory of the bf16 slot pools (host side of ``t2w_kv8_*``, ``include/t2w.h``; no counterpart in the reference,
-whose pools are 16-bit, ``engine/runtime/dit_fast.py:60-97``).
+whose pools are 16-bit, ``engine/runtime/dit_fast.py:59-64``).
 
 A step over many requests is three calls on the caller's stream, none of which waits for the GPU or needs the lengths on the
 host, so that one captured graph serves steps of any lengths::
@@ -12,7 +12,8 @@ host, so that one captured graph serves steps of any lengths::
     out = attention(q, pages, table, plan.row_start, plan.kv_total, scale=head_dim ** -0.5, chunk=1)
 
 The next step's ``kv_len`` and ``free_head`` are ``plan.kv_total`` and ``plan.free_head``; a plan's outputs must not be its own
-inputs, so a loop alternates two plans or copies them.  Lengths, tables and ids are int32 tensors on the GPU.
+inputs, so a loop alternates two plans or copies them.  Lengths, tables and ids are int32 tensors on the GPU.  No gradients
+flow through these calls.
 """
 
 from __future__ import annotations

@@ -1,6 +1,6 @@
 """The paged 8-bit key/value cache in plain float64: tables from request lengths, the quantizing append, attention.
 
-No counterpart in the reference (its key/value pools are 16-bit, ``engine/runtime/dit_fast.py:60-97``): this restates the
+No counterpart in the reference (its key/value pools are 16-bit, ``engine/runtime/dit_fast.py:59-64``): this restates the
 operators' own definition (``include/t2w.h``, t2w_kv8_*), with loops over rows, blocks and heads.
 """
 

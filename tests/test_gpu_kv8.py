@@ -493,6 +493,34 @@ def test_attention_strides_and_rows_behind(dev, new):
     assert torch.equal(again[:2 * new], out[:2 * new])
 
 
+def test_pages_beyond_32_bit_offsets(dev):
+    """Blocks whose bytes lie beyond 4 GiB in the pages: the same codes and outputs as at the pages' start."""
+    g, d, nb = 8, 128, 140000  # 32 KB a block: 4.6 GB of keys, as much of values
+    dev_ = torch.device("cuda", torch.cuda.current_device())
+    e = lambda *s: torch.empty(s, dtype=torch.uint8, device=dev_)  # noqa: E731
+    big = kv8.KV8Pages(e(nb, g, d // 16, 32, 16), e(nb, g, 4, d // 2, 2, 8), e(nb, g), e(nb, g))
+    assert big.k.numel() > 1 << 32
+    for old, new, h in ((0, 70, 16), (70, 1, 16), (71, 1, 128), (72, 40, 8)):
+        n = need(old + new)
+        low = kv8.KV8Pages(*(t[:n] for t in (big.k, big.v, big.k_exp, big.v_exp)))
+        k, v = new_kv(new, g, d, BF, seed=new)
+        q = queries(new, h, d, BF, seed=old)
+        outs = []
+        for pages, first in ((low, 0), (big, nb - n - 1)):
+            table = torch.arange(first, first + n, dtype=torch.int32, device="cuda")[None]
+            if first:  # what the low blocks held before this step lies in the high ones too
+                for t in (big.k, big.v, big.k_exp, big.v_exp):
+                    t[first:first + n].copy_(before[t.data_ptr()])
+            else:
+                before = {t.data_ptr(): t[:n].clone() for t in (big.k, big.v, big.k_exp, big.v_exp)}
+            args = (table, ints([0, new]), ints([old + new]))
+            kv8.append(pages, k, v, *args, max_new=new)
+            outs.append(kv8.attention(q, pages, *args, scale=0.1, chunk=1, max_new=new, max_kv=old + new))
+        assert torch.isfinite(outs[0]).all() and torch.equal(*outs)
+        for t in (big.k, big.v, big.k_exp, big.v_exp):
+            assert torch.equal(t[:n], t[nb - n - 1:nb - 1])
+
+
 def test_attention_same_bits_every_time(dev):
     totals = [3000, 1700, 4000, 60]
     for new in (1, 3, 60):
