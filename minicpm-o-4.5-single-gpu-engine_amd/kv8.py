@@ -187,7 +187,7 @@ def attention(q: torch.Tensor, pages: KV8Pages, table: torch.Tensor, row_start: 
     """softmax(scale q K^T) V of every new token ``q`` [n_tok, heads, head_dim] over its row's cache; ``heads`` is 1 to 16 times
     the pages' heads.  ``chunk``: 0 a token sees all of its row, c > 0 the row's earlier tokens and the new ones of its own and
     earlier chunks of c (1: causal).  ``max_new`` / ``max_kv``: bounds on the rows' new and total tokens, 0 unknown (a row
-    of more than ``max_new`` may get NaN).  Rows of ``out`` behind the last token are left as they were."""
+    of more than ``max_new`` may get NaN).  ``out`` may be ``q``; its rows behind the last token are left as they were."""
     dev, d, rows = pages.device, pages.head_dim, kv_total.shape[0]
     ldq = _tokens("q", q, None, d, dev)
     _small("chunk, max_new or max_kv", max(chunk, max_new, max_kv))

@@ -521,6 +521,20 @@ def test_pages_beyond_32_bit_offsets(dev):
             assert torch.equal(t[:n], t[nb - n - 1:nb - 1])
 
 
+@pytest.mark.parametrize("h,g,d,new,old", [(16, 16, 64, 1, 700), (32, 8, 128, 1, 4000), (16, 16, 64, 50, 320), (32, 8, 128, 500, 77)])
+def test_attention_in_place(dev, h, g, d, new, old):
+    """The outputs over the queries' own memory: the bits of the call with an output of its own (each kernel form, split or not)."""
+    totals = [old + new, new, old + new + 31, old + new - 7]
+    table, nb = random_table(totals, 0, seed=new)
+    pages = random_pages(nb, g, d, 5)
+    q = queries(4 * new, h, d, BF, seed=6)
+    args = (pages, torch.from_numpy(table).cuda(), ints(starts([new] * 4)), ints(totals))
+    kw = dict(scale=d ** -0.5, chunk=1, max_new=new, max_kv=max(totals))
+    want = kv8.attention(q, *args, **kw)
+    assert kv8.attention(q, *args, out=q, **kw) is q
+    assert torch.equal(q, want)
+
+
 def test_attention_same_bits_every_time(dev):
     totals = [3000, 1700, 4000, 60]
     for new in (1, 3, 60):
