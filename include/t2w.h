@@ -320,7 +320,8 @@ int t2w_attention(const void* q, const void* k_pool, const void* v_pool, void* o
  *
  * Row r of a call is one request: its cache is blocks table[r * ld_table + 0 ..], block j holding its tokens
  * 32 j .. 32 j + 31; its new tokens are rows row_start[r] .. row_start[r + 1] - 1 of the packed token tensors and the
- * last ones of its kv_total[r] cached tokens.  A row may have no new token.  At most 4096 rows; int tables. */
+ * last ones of its kv_total[r] cached tokens.  A row may have no new token, and the first row may start behind token 0 (some
+ * rows of a larger call, by slices of its tables).  At most 4096 rows; int tables. */
 
 enum { T2W_KV8_BLOCK = 32, T2W_KV8_BF16 = 0, T2W_KV8_FP16 = 1 };
 

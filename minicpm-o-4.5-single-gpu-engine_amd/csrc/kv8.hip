@@ -225,6 +225,7 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(t2w_kv8_append_args a, 
   } else {
     row = kv8_find_row(a.row_start, a.n_rows, KV8_BLOCK, 2, item);
     at = item - (a.row_start[row] / KV8_BLOCK + 2 * row);
+    if (at < 0) return;  // in front of the first row, whose tokens need not be the call's first ones
   }
   const int start = a.row_start[row], n_new = a.row_start[row + 1] - start, total = a.kv_total[row];
   if (start < 0 || n_new <= 0 || start > a.n_tok - n_new || total < n_new) return;  // nothing new, or a malformed table

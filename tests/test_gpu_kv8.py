@@ -225,6 +225,28 @@ def test_append_skips_foreign_blocks(dev):
     for a, b in zip(host(pages), want):
         assert np.array_equal(a, b)
 
+@pytest.mark.parametrize("first", [1, 3, 70])
+def test_append_rows_of_a_larger_call(dev, first):
+    """The last rows of a call by slices of its tables: starts beyond the first token, nothing done before the first row.  The
+    table's entries before the slice are blocks of a scale byte 0, which any second look at them would raise."""
+    rows = 75
+    new = [(1, 40, 0, 33)[r % 4] for r in range(rows)]
+    old = [(0, 5, 32, 31)[r % 4] for r in range(rows)]
+    totals = [a + b for a, b in zip(old, new)]
+    table, nb = random_table(totals, 0, seed=first, spare=3)
+    spare = sorted(set(range(nb)) - set(table[r, b] for r, t in enumerate(totals) for b in range(need(t))))
+    for r in range(first):
+        table[r, :] = spare[r % len(spare)]
+    pages = random_pages(nb, 2, 64, seed=1)
+    pages.k_exp[spare], pages.v_exp[spare] = 0, 0
+    k, v = new_kv(sum(new), 2, 64, BF, seed=2)
+    want = host(pages)
+    ok.append(*want, k.double().cpu().numpy(), v.double().cpu().numpy(), table[first:], starts(new)[first:], totals[first:])
+    dt = torch.from_numpy(table).cuda()
+    kv8.append(pages, k, v, dt[first:], ints(starts(new))[first:], ints(totals)[first:])
+    for name, a, b in zip(("k", "v", "k_exp", "v_exp"), host(pages), want):
+        assert np.array_equal(a, b), name
+
 
 # --- attention ------------------------------------------------------------------------------------------------------------
 
