@@ -21,24 +21,26 @@ struct KV8Split {
   int n_tiles;  // tile slots of the call
   int bps;      // key blocks of a part, more where a row would have over `parts` of them
   int parts;    // most parts of a tile; 1: the kernel writes the outputs itself
+  int cap;      // tile form: (tile, key head, part)s that the workspace holds, whatever the number of tiles; 0: all of `parts`
 };
 
 // Workspace of split calls, parts joined by kv8_join_kernel: the parts' outputs, fp32 [tile slot][kv head][part][m][D],
 // then (maximum, sum) [tile slot][kv head][part][m][2].
 __host__ __device__ __forceinline__ size_t part_rows(const KV8Split& s, int kv_heads) {
-  return (size_t)s.n_tiles * kv_heads * s.parts * (s.tt * s.G);
+  return (s.cap > 0 ? (size_t)s.cap : (size_t)s.n_tiles * kv_heads * s.parts) * (s.tt * s.G);
 }
 
 struct Tile {
   int row, start, i0, rows;  // its row, the row's first token, the tile's first token in it, packed rows
   int cached, n_new, total;  // total = cached + n_new keys; cached < 0 where the row has fewer keys than queries
   int end;                   // keys [0, end) are visible to some query of the tile
+  int slot, parts;           // its slot, and its most parts
   bool bad;                  // the row is longer than its table, or than max_new tokens: NaN outputs
 };
 
 // The tile of a slot, by the whole wave; false: nothing there.
 __device__ __forceinline__ bool find_tile(const t2w_kv8_attention_args& a, const KV8Split& s, int slot, Tile& t) {
-  int at, next;
+  int at, next, live = 1;  // live: the call's tiles, where s.cap asks for them
   if (s.per_row > 0) {
     t.row = slot / s.per_row;
     at = slot - t.row * s.per_row;
@@ -52,7 +54,8 @@ __device__ __forceinline__ bool find_tile(const t2w_kv8_attention_args& a, const
     const int start = a.row_start[r], stop = a.row_start[r + 1], total = a.kv_total[r];
     const int tiles = lane < a.n_rows && stop > start ? min((stop - start - 1) / s.tt + 1, 1 << 24) : 0;
     auto from = [&](int x) { return __builtin_amdgcn_readlane(wave_scan(max(tiles - x, 0)), 63); };
-    if (from(0) <= slot) return false;
+    live = from(0);
+    if (live <= slot) return false;
     int lo = 0, hi = s.n_tiles + 1;  // no row has more tiles than the call has slots
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -66,6 +69,28 @@ __device__ __forceinline__ bool find_tile(const t2w_kv8_attention_args& a, const
     next = __builtin_amdgcn_readlane(stop, t.row);
     t.total = __builtin_amdgcn_readlane(total, t.row);
     at = lo;
+  } else if (s.cap > 0) {
+    // More rows, the tiles counted, the last rows' last ones first: each lane sums a run of rows, then the rows of the run
+    // that holds the tile go one to a lane.
+    const int lane = threadIdx.x & 63, step = (a.n_rows + 63) / 64;
+    auto tiles_of = [&](int r) {
+      if (r >= a.n_rows) return 0;
+      const int start = a.row_start[r], stop = a.row_start[r + 1];
+      return stop > start ? min((stop - start - 1) / s.tt + 1, 1 << 18) : 0;  // 2^24 tokens, tiles of 16 or more: 2^20 + 4,096 in all
+    };
+    int mine = 0;
+    for (int i = 0; i < step; ++i) mine += tiles_of(lane * step + i);
+    const int upto = wave_scan(mine);
+    live = __builtin_amdgcn_readlane(upto, 63);
+    if (live <= slot) return false;
+    const int back = live - 1 - slot, run = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > back) | (1ull << 63));
+    const int n = lane < step ? tiles_of(run * step + lane) : 0, to = wave_scan(n) + __builtin_amdgcn_readlane(upto - mine, run);
+    const int nth = __builtin_ctzll(__builtin_amdgcn_ballot_w64(to > back) | (1ull << 63));
+    t.row = min(run * step + nth, a.n_rows - 1);
+    at = back - __builtin_amdgcn_readlane(to - n, nth);
+    t.start = a.row_start[t.row];
+    next = a.row_start[t.row + 1];
+    t.total = a.kv_total[t.row];
   } else {  // the last rows' last tiles first
     const int back = s.n_tiles - 1 - slot;
     t.row = kv8_find_row(a.row_start, a.n_rows, s.tt, 1, back);
@@ -89,6 +114,8 @@ __device__ __forceinline__ bool find_tile(const t2w_kv8_attention_args& a, const
   const int last = t.i0 + n - 1;
   const int seen = a.chunk > 0 ? (int)min((long long)t.n_new, ((long long)(last / a.chunk) + 1) * a.chunk) : t.n_new;
   t.end = max(t.cached + seen, 0);
+  t.slot = slot;
+  t.parts = s.cap > 0 ? min(s.parts, max(1, s.cap / a.pages.kv_heads / live)) : s.parts;  // slot < live: all partials lie within s.cap
   return true;
 }
 
@@ -99,9 +126,9 @@ __device__ __forceinline__ int seen_by(const t2w_kv8_attention_args& a, const Ti
 }
 
 // parts of a tile and the blocks of one
-__device__ __forceinline__ int tile_parts(const KV8Split& s, int end, int& per) {
-  const int nb = (end + KV8_BLOCK - 1) / KV8_BLOCK;
-  per = max(s.bps, (nb + s.parts - 1) / s.parts);
+__device__ __forceinline__ int tile_parts(const KV8Split& s, const Tile& t, int& per) {
+  const int nb = (t.end + KV8_BLOCK - 1) / KV8_BLOCK;
+  per = max(s.bps, (nb + t.parts - 1) / t.parts);
   return max(1, (nb + per - 1) / per);
 }
 
@@ -286,7 +313,7 @@ struct State {
 
   // Row mrow of the tile (lane group g): to the outputs, or to the call's workspace where the tile has several parts
   template <bool BF>
-  __device__ __forceinline__ void store(const t2w_kv8_attention_args& a, const KV8Split& sp, const Tile& t, int slot, int kv_head, int part, int parts,
+  __device__ __forceinline__ void store(const t2w_kv8_attention_args& a, const KV8Split& sp, const Tile& t, int kv_head, int part, int parts,
                                         int mrow, int g) const {
     const float unit = pow2_bits(E) * 0.0078125f;  // 2^(E - 127 - 7); E = 0: no value block at all, o is zero
     float sum = l + __shfl_xor(l, 32, 64);
@@ -310,7 +337,7 @@ struct State {
           *(uint4*)(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     } else {
-      const size_t pr = ((size_t)slot * a.pages.kv_heads + kv_head) * sp.parts + part, rows = sp.tt * sp.G;
+      const size_t pr = ((size_t)t.slot * a.pages.kv_heads + kv_head) * t.parts + part, rows = sp.tt * sp.G;
       float* po = (float*)a.workspace + (pr * rows + mrow) * D;
       float* ml = (float*)a.workspace + part_rows(sp, a.pages.kv_heads) * D + (pr * rows + mrow) * 2;
 #pragma unroll
@@ -366,7 +393,7 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
     return;
   }
   int per;
-  const int parts = tile_parts(sp, t.end, per);
+  const int parts = tile_parts(sp, t, per);
   if (part >= parts) return;
   const int b0 = part * per, b1 = min(b0 + per, (t.end + KV8_BLOCK - 1) / KV8_BLOCK);
   const int i = lane % MR, g = lane / MR;
@@ -481,7 +508,7 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
     if (kw < w) st.fold(s_acc[kw * RW + rw], s_e[wave + w * RW], lane);
     if (w > 1) __syncthreads();
   }
-  if (kw == 0 && mrow < t.rows) st.template store<BF>(a, sp, t, slot, kv_head, part, parts, mrow, g);
+  if (kw == 0 && mrow < t.rows) st.template store<BF>(a, sp, t, kv_head, part, parts, mrow, g);
 }
 
 // Tile form, for tiles of many packed rows (prompts): RW waves of 32 packed rows each share the keys, two blocks a step.  The
@@ -511,7 +538,7 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
     return;
   }
   int per;
-  const int parts = tile_parts(sp, t.end, per);
+  const int parts = tile_parts(sp, t, per);
   if (part >= parts) return;
   const int b0 = part * per, b1 = min(b0 + per, (t.end + KV8_BLOCK - 1) / KV8_BLOCK), steps = (b1 - b0 + 1) / 2;
   const int i = lane & 31, g = lane >> 5;
@@ -704,7 +731,7 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
     kx0 = nkx0; kx1 = nkx1; E = nE;
     cur = nxt;
   }
-  if (mrow < t.rows) st.template store<BF>(a, sp, t, slot, kv_head, part, parts, mrow, g);
+  if (mrow < t.rows) st.template store<BF>(a, sp, t, kv_head, part, parts, mrow, g);
 }
 
 // Joins the parts of split tiles, WR waves to a packed row (4 where a row has many parts): each wave sums its share of them,
@@ -718,9 +745,9 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(t2w_kv8_attention_args a,
   Tile t;
   if (!find_tile(a, sp, slot, t) || t.bad) return;
   int per;
-  const int parts = tile_parts(sp, t.end, per);
+  const int parts = tile_parts(sp, t, per);
   if (parts == 1 || m >= t.rows) return;  // with WR == 4 the whole workgroup
-  const size_t rows = sp.tt * sp.G, pr = ((size_t)slot * a.pages.kv_heads + kv_head) * sp.parts;
+  const size_t rows = sp.tt * sp.G, pr = ((size_t)slot * a.pages.kv_heads + kv_head) * t.parts;
   const float* po = (const float*)a.workspace + (pr * rows + m) * D + lane * NV;
   const float* ml = (const float*)a.workspace + part_rows(sp, a.pages.kv_heads) * D + (pr * rows + m) * 2;
   // every lane its parts' (maximum, sum): up to 256 parts
@@ -786,16 +813,21 @@ Choice choose(const t2w_kv8_attention_args& a) {
   c.mr = packed <= 16 ? 16 : 32;
   c.rw = packed <= 32 ? 1 : 2;
   c.tile = false;
-  const long tt = 256 / G, rows = a.max_new > 0 ? (a.n_tok + max_new - 1) / max_new : 1;  // rows, were all of them longest
-  const long tiles = rows * ((max_new + tt - 1) / tt), groups = tiles * a.pages.kv_heads;
+  // Tiles: as many rows as there can be of the longest; without a bound every row may end in a part of one.
+  const long tt = 256 / G, rows = a.max_new > 0 ? (a.n_tok + max_new - 1) / max_new : 1, slots = a.n_tok / tt + min(a.n_rows, a.n_tok);
+  const long tiles = a.max_new > 0 || a.n_rows == 1 ? rows * ((max_new + tt - 1) / tt) : slots, groups = tiles * a.pages.kv_heads;
   const long fit = groups >= 256 ? 1 : min(256 / max(groups, 1L), max(nb / 64, 1L));
   if (a.pages.head_dim == 128 && packed > 64 && groups * fit >= 224 && a.n_tok * 10L >= tiles * tt * 7) {
     c.tile = true;
     c.rw = 8;
   }
   c.s.tt = c.mr * c.rw / G;
-  c.s.per_row = a.max_new > 0 && a.max_new <= c.s.tt ? 1 : 0;
-  c.s.n_tiles = c.s.per_row ? a.n_rows : a.n_tok / c.s.tt + a.n_rows;
+  // How many tiles there are only the GPU knows (rows may rest): the tile form's workspace is that of one round of workgroups,
+  // and the kernel counts the tiles and takes fewer parts where there are more of them (parts for every slot took 2.2 GB for 64
+  // rows of a token without bounds, tables 2,048 wide, and 35 GB for 4,096 rows of which one has 256 tokens).
+  c.s.cap = c.tile && fit > 1 ? 256 : 0;
+  c.s.per_row = a.max_new > 0 && a.max_new <= c.s.tt && c.s.cap == 0 ? 1 : 0;
+  c.s.n_tiles = c.s.cap > 0 ? (int)slots : c.s.per_row ? a.n_rows : a.n_tok / c.s.tt + a.n_rows;
   // Parts: the tile form's, so that one round of workgroups fills the chip.  The direct form's lists of up to 48 blocks stay
   // whole (a second launch costs more: one row of 1,500 keys 9.6 us whole, 10.5 split); longer ones are cut where
   // workgroups are few, to 512 in all and 16 blocks or more a part (two rows of 131,072 keys: 103 us with 512 workgroups,
@@ -844,7 +876,9 @@ static hipError_t launch(const t2w_kv8_attention_args& a, const Choice& c, hipSt
   } else {
     hipLaunchKernelGGL((kv8_attn_direct_kernel<BF, D, 32, 2, D == 64 ? 4 : 2>), grid, dim3(256), 0, st, a, c.s);
   }
-  const unsigned groups = (unsigned)(c.s.n_tiles * a.pages.kv_heads), rows = (unsigned)(c.s.tt * c.s.G);
+  // counted tiles have parts only where they are few (and cap / 2 is at least the key heads where there are parts at all)
+  const int joined = c.s.cap > 0 ? min(c.s.n_tiles, c.s.cap / 2 / a.pages.kv_heads) : c.s.n_tiles;
+  const unsigned groups = (unsigned)(joined * a.pages.kv_heads), rows = (unsigned)(c.s.tt * c.s.G);
   if (c.s.parts > 8) hipLaunchKernelGGL((kv8_join_kernel<BF, D, 4>), dim3(groups, rows), dim3(256), 0, st, a, c.s);
   else if (c.s.parts > 1) hipLaunchKernelGGL((kv8_join_kernel<BF, D, 1>), dim3(groups, (rows + 3) / 4), dim3(256), 0, st, a, c.s);
   return hipGetLastError();

@@ -587,6 +587,23 @@ def test_attention_on_other_streams(dev):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
+@pytest.mark.parametrize("rows,n_tok,at,width,old", [(64, 64, None, 2048, 700), (200, 200, None, 512, 90), (64, 256, 5, 600, 16500), (70, 256, 69, 600, 16500),
+                                                     (4096, 256, 1234, 600, 16500), (130, 400, 64, 600, 16500)])
+@pytest.mark.parametrize("bounds", [False, True])
+def test_attention_idle_rows_and_wide_tables(dev, rows, n_tok, at, width, old, bounds):
+    """Many rows of one token and a wide table; one prompt chunk among rows that rest or have a token (32 heads over 8 of 128)."""
+    new = [1] * rows if at is None else [0] * rows
+    if at is not None:
+        new[at] = min(n_tok, 256)
+        for r in range(n_tok - new[at]):
+            new[(at + 1 + r) % rows if r < rows - 1 else at] += 1
+    totals = [n + (old if n > 1 else 5 * (r % 50)) if n else 0 for r, n in enumerate(new)]
+    table, nb = random_table(totals, 0, seed=rows)
+    table = np.concatenate([table, np.full((rows, width - table.shape[1]), -1, np.int32)], 1)
+    pages = random_pages(nb, 8, 128, seed=1)
+    q = queries(sum(new), 32, 128, BF, seed=2)
+    check_attention(q, pages, table, new, totals, 1, **({"max_new": max(new), "max_kv": max(totals)} if bounds else {}))
+
 
 # --- a run of them ----------------------------------------------------------------------------------------------------------
 

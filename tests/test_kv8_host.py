@@ -185,3 +185,37 @@ def test_oracle_rounding():
         e = ok.exponent(a)
         assert a <= 448.0 * 2.0 ** e and (e == -126 or a > 448.0 * 2.0 ** (e - 1))
     assert ok.exponent(0.0) == ok.exponent(1e-40) == -126
+
+def attn_args(n_tok, n_rows, width, heads=32, kv_heads=8, dim=128, max_new=0, max_kv=0):
+    return _lib.KV8AttentionArgs(c_pages(kv_heads=kv_heads, head_dim=dim), 1 << 20, 1 << 20, heads * dim, heads * dim, 0, n_tok, heads, 1 << 20, width,
+                                 width, 1 << 20, 1 << 20, n_rows, 1, 0.1, max_new, max_kv, None, 0)
+
+
+def workspace(*a, **kw):
+    return _lib.lib().t2w_kv8_attention_workspace_bytes(C.byref(attn_args(*a, **kw)))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 128), (32, 32, 128), (128, 8, 128), (1, 1, 128), (16, 16, 64), (64, 4, 64)])
+def test_attention_workspace_is_bounded(heads, kv_heads, dim):
+    """What a call asks for does not grow with idle rows, wide tables or missing bounds: at most 1,024 (tile, key head, part)
+    of 64 packed rows, or 256 of 256."""
+    most = 0
+    for n_tok in (1, 4, 64, 256, 1000, 2048, 5000):
+        for n_rows in (1, 2, 7, 64, 65, 256, 4096):
+            for width in (1, 40, 512, 2048, 1 << 20):
+                for max_new in (0, 1, 40, n_tok):
+                    for max_kv in (0, 3000, 32000):
+                        most = max(most, workspace(n_tok, n_rows, width, heads, kv_heads, dim, max_new, max_kv))
+    assert most <= 65536 * (dim + 2) * 4
+
+
+def test_steps_without_bounds_take_no_prompt_tiles():
+    """64 and 256 rows of one token, no bounds, wide tables: tiles of few packed rows, whose parts need little memory."""
+    assert workspace(64, 64, 2048) <= 16 << 20 and workspace(256, 256, 512) == 0
+    assert workspace(64, 64, 2048, max_new=1) == 0
+
+
+@pytest.mark.parametrize("rows", [1, 64, 70, 4096])
+def test_a_chunk_among_resting_rows_is_split(rows):
+    """256 tokens of one row over a long cache: the tile form in parts, its 256 parts of 256 packed rows, however many rows rest."""
+    assert workspace(256, rows, 600, max_new=256, max_kv=16756) == 65536 * (128 + 2) * 4
