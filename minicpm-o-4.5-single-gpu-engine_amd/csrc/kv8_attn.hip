@@ -3,6 +3,7 @@
 #include "kv8_internal.h"
 
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 namespace t2w {
@@ -22,6 +23,8 @@ struct KV8Split {
   int bps;      // key blocks of a part, more where a row would have over `parts` of them
   int parts;    // most parts of a tile; 1: the kernel writes the outputs itself
   int cap;      // tile form: (tile, key head, part)s that the workspace holds, whatever the number of tiles; 0: all of `parts`
+  float cm;     // scale log2(e) = cm 2^ce, cm in [0.72, 1.45): the product itself may leave fp32's range, or its normal one
+  int ce;
 };
 
 // Workspace of split calls, parts joined by kv8_join_kernel: the parts' outputs, fp32 [tile slot][kv head][part][m][D],
@@ -181,7 +184,7 @@ __device__ __forceinline__ float query_max(float v) {
 __device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float((uint32_t)min(max(biased, 0), 254) << 23); }
 
 // Softmax and output state of a wave's MR packed rows (lane column = query), shared by both kernels.  Scores are in units of
-// log2, s = q . k times c = scale log2(e) 2^(key exponent).
+// log2, s = q . k times c = scale log2(e) 2^(key exponent), a normal number or applied to the scores themselves (scale_scores).
 //  * m is a reference that the running maximum may pass by 8 before it is moved (then to the true maximum so far):
 //    probabilities are 2^(s - m + 7) <= 2^15 in fp16, so most blocks need no exchange between lanes and no rescaling of the
 //    outputs, and a probability keeps fp16's 11 bits down to 2^-21 of the largest and 2^-32 of it absolutely.  fp16 and not
@@ -236,6 +239,15 @@ struct State {
 #pragma unroll
       for (int r = 0; r < AR; ++r) mx = fmaxf(mx, sc[x][r]);
     return mx;
+  }
+  // Whether a block's factor c = cm 2^e is a normal number; where it is not, its scores are scaled themselves, in fp32's whole
+  // range (a factor of 0 would make NaN of an invisible score's -inf).
+  static __device__ __forceinline__ bool normal(int e) { return e >= -125 && e <= 126; }
+  static __device__ __forceinline__ void scale_scores(Acc (&sc)[KG], float cm, int e) {
+#pragma unroll
+    for (int x = 0; x < KG; ++x)
+#pragma unroll
+      for (int r = 0; r < AR; ++r) sc[x][r] = __builtin_amdgcn_ldexpf(sc[x][r] * cm, e);
   }
   // Moves the reference where a block's scores, in units 1 / c and -inf where invisible, of maximum mx, pass it; scales them
   // where `big`.
@@ -411,7 +423,6 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
     for (int n = 0; n < NQ; ++n) q[n] = *(const uint4*)(src + (LG * (n >> 1) + g) * 16 + (n & 1) * 8);
   }
   St st;
-  const float c0 = a.scale * 1.4426950408889634f;
 
   // the lane's place in a block's keys and values; its loads lie at constant distances from there (load offsets)
   const uint32_t koff = MR == 16 ? g * 512 + (8 * (i >> 2) + (i & 3)) * 16 : g * 512 + ((i & 0x13) | ((i & 4) << 1) | ((i & 8) >> 1)) * 16;
@@ -464,8 +475,13 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
         }
         if (next >= 0) load_k(next);
         const bool off = kx > 254;  // a block id outside the pages, or an E8M0 NaN
-        float c = off ? c0 : c0 * pow2_bits(kx);
-        if (off || key0 + KV8_BLOCK > lim_lo) {  // or some query of the wave does not see all of the block
+        const int ex = sp.ce + (off ? 0 : kx - 127);
+        float c = __builtin_amdgcn_ldexpf(sp.cm, ex);
+        if (off || !St::normal(ex) || key0 + KV8_BLOCK > lim_lo) {  // or some query of the wave does not see all of the block
+          if (!St::normal(ex)) {
+            St::scale_scores(sc, sp.cm, ex);
+            c = 1.f;
+          }
 #pragma unroll
           for (int z = 0; z < KG; ++z)
 #pragma unroll
@@ -556,7 +572,6 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
     for (int n = 0; n < D / 16; ++n) q[n] = *(const uint4*)(src + (2 * (n >> 1) + g) * 16 + (n & 1) * 8);
   }
   St st;
-  const float c0 = a.scale * 1.4426950408889634f;
   const size_t stride = (size_t)a.pages.kv_heads * (KV8_BLOCK * D);
   const uint8_t* kbase = (const uint8_t*)a.pages.k + (size_t)kv_head * (KV8_BLOCK * D);
   const uint8_t* vbase = (const uint8_t*)a.pages.v + (size_t)kv_head * (KV8_BLOCK * D);
@@ -650,8 +665,13 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
   auto block = [&](int buf, int y, int key0, int kx, int E, typename St::Acc (&sc)[1], int nbuf, int ny, typename St::Acc (&sn)[1], auto conv, int cbuf) {
     read_k(nbuf, ny);
     const bool off = kx > 254;
-    float c = off ? c0 : c0 * pow2_bits(kx);
-    if (off || key0 + KV8_BLOCK > lim_lo) {
+    const int ex = sp.ce + (off ? 0 : kx - 127);
+    float c = __builtin_amdgcn_ldexpf(sp.cm, ex);
+    if (off || !St::normal(ex) || key0 + KV8_BLOCK > lim_lo) {
+      if (!St::normal(ex)) {
+        St::scale_scores(sc, sp.cm, ex);
+        c = 1.f;
+      }
 #pragma unroll
       for (int r = 0; r < 16; ++r) sc[0][r] = key0 + St::key_of(0, r, g) < lim ? (off ? __builtin_nanf("") : sc[0][r]) : -__builtin_inff();
       mx = St::top(sc);
@@ -826,6 +846,7 @@ Choice choose(const t2w_kv8_attention_args& a) {
   // and the kernel counts the tiles and takes fewer parts where there are more of them (parts for every slot took 2.2 GB for 64
   // rows of a token without bounds, tables 2,048 wide, and 35 GB for 4,096 rows of which one has 256 tokens).
   c.s.cap = c.tile && fit > 1 ? 256 : 0;
+  c.s.cm = std::frexp(a.scale, &c.s.ce) * 1.4426950408889634f;
   c.s.per_row = a.max_new > 0 && a.max_new <= c.s.tt && c.s.cap == 0 ? 1 : 0;
   c.s.n_tiles = c.s.cap > 0 ? (int)slots : c.s.per_row ? a.n_rows : a.n_tok / c.s.tt + a.n_rows;
   // Parts: the tile form's, so that one round of workgroups fills the chip.  The direct form's lists of up to 48 blocks stay

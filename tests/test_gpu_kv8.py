@@ -604,6 +604,41 @@ def test_attention_idle_rows_and_wide_tables(dev, rows, n_tok, at, width, old, b
     q = queries(sum(new), 32, 128, BF, seed=2)
     check_attention(q, pages, table, new, totals, 1, **({"max_new": max(new), "max_kv": max(totals)} if bounds else {}))
 
+# every kernel form: (new, old, heads, kv_heads, dim, rows); 16 packed rows, 32, 2 x 32, key lists in parts, the tile form, its parts
+ALL_FORMS = [(1, 100, 4, 2, 64, 3), (12, 100, 4, 2, 128, 3), (40, 100, 4, 2, 64, 3), (1, 2500, 4, 2, 128, 2), (101, 60, 64, 32, 128, 7),
+             (256, 14200, 32, 32, 128, 1)]
+
+
+@pytest.mark.parametrize("new,old,h,g,d,rows", ALL_FORMS)
+def test_attention_key_scale_byte_zero(dev, new, old, h, g, d, rows):
+    """Blocks whose key scale is 2^-127, seen whole and in part: scores of (nearly) zero, not NaN.  And pages as they are made:
+    zeros."""
+    totals = [old + new - 13 * r for r in range(rows)]
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, g, d, seed=5)
+    for r, t in enumerate(totals):
+        pages.k_exp[torch.from_numpy(table[r, (need(t) - 1) % 2:need(t):2]).long().cuda()] = 0  # the last block among them
+    q = queries(rows * new, h, d, BF, seed=6)
+    bounds = {"max_new": new, "max_kv": max(totals)}
+    check_attention(q, pages, table, [new] * rows, totals, 1, **bounds)
+    check_attention(q, pages, table, [new] * rows, [t - 3 for t in totals], 7, **bounds)
+    pages.k_exp.zero_()
+    check_attention(q, pages, table, [new] * rows, totals, 1, **bounds)
+    out = kv8.attention(q, kv8.KV8Pages.empty(nb, g, d), torch.from_numpy(table).cuda(), ints(starts([new] * rows)), ints(totals), scale=0.1, chunk=1, **bounds)
+    assert (out == 0).all()
+
+
+@pytest.mark.parametrize("new,old,h,g,d,rows", ALL_FORMS[:5])
+@pytest.mark.parametrize("scale,k_exp,size", [(1e-38, 5, 1.0), (2.0 ** -140, 121, 1.0), (2.0 ** -140, 3, 2.0 ** 100), (3e38, 2, 2.0 ** -10), (3e38, 121, 0.0)])
+def test_attention_scale_of_any_size(dev, new, old, h, g, d, rows, scale, k_exp, size):
+    """Scales whose product with a block's leaves fp32's normal range, or whose own with log2 e does: softmax of what the scores are."""
+    totals = [old + new - 13 * r for r in range(rows)]
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, g, d, seed=5)
+    pages.k_exp.fill_(k_exp)
+    q = (queries(rows * new, h, d, BF, seed=6).float() * size).to(BF)
+    check_attention(q, pages, table, [new] * rows, totals, 1, scale=float(np.float32(scale)), max_new=new, max_kv=max(totals))
+
 
 # --- a run of them ----------------------------------------------------------------------------------------------------------
 
