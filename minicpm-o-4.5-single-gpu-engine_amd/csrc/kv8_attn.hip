@@ -202,8 +202,8 @@ struct State {
   Acc o[NT][2];
   float l = 0.f;                // sum of the lane's probabilities; of the query's when the lane groups are added
   float m = -__builtin_inff();  // reference
-  float nb = 7.f;               // 7 - m, 7 where m is -inf
-  bool big = false;             // |m| so large that s - m in one fma would not be exact enough: scale the scores first
+  float nb = 7.f;               // 7 - m, 7 where m is -inf; 0 where `big`
+  bool big = false;             // some query of the wave has a large |m|: `move` computes the exponentials' arguments itself
   int E = 0;                    // biased value exponent that o is in units of; 0: none yet
 
   __device__ __forceinline__ State() {
@@ -249,27 +249,36 @@ struct State {
 #pragma unroll
       for (int r = 0; r < AR; ++r) sc[x][r] = __builtin_amdgcn_ldexpf(sc[x][r] * cm, e);
   }
-  // Moves the reference where a block's scores, in units 1 / c and -inf where invisible, of maximum mx, pass it; scales them
-  // where `big`.
+  // Moves the reference where a block's scores, in units 1 / c and -inf where invisible, of maximum mx, pass it.  Where |m| is
+  // large, s - m + 7 in one fma is not what the scores' own rounding allows: 7 - m rounds too, and a score of m + 8 could reach
+  // 2^16, infinite in fp16.  There s is rounded first, as mx was, and s - m is exact where it counts; nothing may be contracted.
+  // Each query by its own m alone, so that its bits do not depend on the others of the wave.
   __device__ __forceinline__ void move(Acc (&sc)[KG], float& c, float mx) {
+#pragma clang fp contract(off)
     mx *= c;
-    if (__builtin_amdgcn_ballot_w64(mx > m + 8.f)) {
-      const float seen = query_max<MR>(mx), mn = seen > m + 8.f ? seen : m;  // each query by its own scores alone
+    if (__builtin_amdgcn_ballot_w64(mx - m > 8.f)) {
+      const float seen = query_max<MR>(mx), mn = seen - m > 8.f ? seen : m;  // each query by its own scores alone
       const float alpha = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
-      nb = mn == -__builtin_inff() ? 7.f : 7.f - mn;
-      big = big || __builtin_amdgcn_ballot_w64(fabsf(mn) > 4194304.f && mn != -__builtin_inff()) != 0;
+      big = big || __builtin_amdgcn_ballot_w64(large(mn)) != 0;
+      nb = big ? 0.f : mn == -__builtin_inff() ? 7.f : 7.f - mn;
       l *= alpha;
       scale_o(alpha);
     }
     if (big) {
+      const float m0 = m == -__builtin_inff() ? 0.f : m;
+      const bool own = large(m0);
 #pragma unroll
       for (int x = 0; x < KG; ++x)
 #pragma unroll
-        for (int r = 0; r < AR; ++r) sc[x][r] *= c;
+        for (int r = 0; r < AR; ++r) {
+          const float s = sc[x][r] * c;
+          sc[x][r] = own ? (s - m0) + 7.f : fmaf(sc[x][r], c, 7.f - m0);
+        }
       c = 1.f;
     }
   }
+  static __device__ __forceinline__ bool large(float m) { return fabsf(m) > 4194304.f && m != -__builtin_inff(); }
   // a block's probabilities, the operands of P . V
   __device__ __forceinline__ void exps(const Acc (&sc)[KG], float c, f16x8 (&p)[NP]) const {
 #pragma unroll

@@ -639,6 +639,81 @@ def test_attention_scale_of_any_size(dev, new, old, h, g, d, rows, scale, k_exp,
     q = (queries(rows * new, h, d, BF, seed=6).float() * size).to(BF)
     check_attention(q, pages, table, [new] * rows, totals, 1, scale=float(np.float32(scale)), max_new=new, max_kv=max(totals))
 
+@pytest.mark.parametrize("new,old,h,g,d,rows", ALL_FORMS)
+@pytest.mark.parametrize("size,dt", [(22, BF), (24, BF), (25, FP), (26, BF), (27, BF), (28, BF)])
+def test_attention_near_ties_of_large_scores(dev, new, old, h, g, d, rows, size, dt):
+    """Scores of 2^size and a little more, exact in fp32 (scale log2 e = 1): what counts is their difference, 0 to 24 in units of
+    log2, so the bound has no part for the scores' own rounding (`top` = 24 for the exponential's argument)."""
+    totals = [old + new - 13 * r for r in range(rows)]
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, g, d, seed=5)
+    ulp = max(1, 2 ** (size - 23))
+    gen = np.random.default_rng(size)
+    pages.k.zero_()
+    pages.k_exp.fill_(127)
+    c = torch.full((nb, g, 32, 16), 0.0)
+    c[..., :8] = 256
+    diff = [x for x in (0, 8, 16, 24, ulp, 2 * ulp) if x % ulp == 0 and x <= 24 + ulp]
+    c[..., 8] = torch.from_numpy(gen.choice(diff, (nb, g, 32)).astype(np.float32))
+    for r, base in zip(range(rows), (0, ulp, 0, ulp, ulp, 0, 0)):
+        c[int(table[r, 0]), :, :, 8] = base  # the reference is set here, by keys that later ones pass by 8 and more
+    pages.k[:, :, 0] = c.to(torch.float8_e4m3fn).view(torch.uint8).cuda()
+    q = torch.zeros(rows * new, h, d, device="cuda", dtype=dt)
+    q[..., :8], q[..., 8] = 2.0 ** (size - 11), 1
+    scale = float(np.float32(np.log(2)))
+    assert np.float32(scale) * np.float32(1.4426950408889634) == 1
+    k, v = scaled(pages)
+    o, mag, _ = ok.attention(q.double().cpu().numpy(), k, v, table, starts([new] * rows), totals, scale, 1)
+    out = kv8.attention(q, pages, torch.from_numpy(table).cuda(), ints(starts([new] * rows)), ints(totals), scale=scale, chunk=1, max_new=new, max_kv=max(totals))
+    bound = attn_bound(o, mag, np.full(o.shape[:2], 24 + ulp), 1, dt)
+    assert (np.abs(out.double().cpu().numpy() - o) <= bound).all()
+
+
+@pytest.mark.parametrize("new,old,h,g,d,rows", ALL_FORMS[:5])
+def test_attention_largest_score_takes_all(dev, new, old, h, g, d, rows):
+    """Scores of 2^60 and more: the output is the winning key's value, which is exact in 16 bits.  (Scores whose first two lie
+    within the fp32 rounding of D products, 2^-17 of their absolute sums, are left out: under 1% of them.)"""
+    totals = [old + new - 13 * r for r in range(rows)]
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, g, d, seed=5)
+    pages.k_exp.add_(60)
+    q = queries(rows * new, h, d, BF, seed=6)
+    k, v = scaled(pages)
+    out = kv8.attention(q, pages, torch.from_numpy(table).cuda(), ints(starts([new] * rows)), ints(totals), scale=0.125, chunk=1, max_new=new,
+                        max_kv=max(totals)).double().cpu().numpy()
+    qd, left, n = q.double().cpu().numpy(), 0, 0
+    for r, t in enumerate(totals):
+        ids = table[r, :need(t)]
+        for x in range(h):
+            kk, vv = k[ids, x // (h // g)].reshape(-1, d)[:t], v[ids, x // (h // g)].reshape(-1, d)[:t]
+            qq = qd[r * new:(r + 1) * new, x]
+            s, a = qq @ kk.T, np.abs(qq) @ np.abs(kk).T
+            hide = np.arange(t)[None] > t - new + np.arange(new)[:, None]
+            s[hide], a[hide] = -np.inf, 0
+            top = s.max(1, keepdims=True)
+            sure = (s >= top - 2.0 ** -17 * a.max(1, keepdims=True)).sum(1) == 1
+            assert np.array_equal(out[r * new:(r + 1) * new, x][sure], vv[s.argmax(1)][sure])
+            none = hide.all(1)  # the first queries of a row with fewer keys than queries
+            assert (out[r * new:(r + 1) * new, x][none] == 0).all()
+            left, n = left + (~sure & ~none).sum(), n + (~none).sum()
+    assert left <= 0.01 * n + 1
+
+
+@pytest.mark.parametrize("new,old,h,g,d,rows", ALL_FORMS[1:3] + ALL_FORMS[4:])
+def test_attention_queries_do_not_touch_each_other(dev, new, old, h, g, d, rows):
+    """Queries of scores of 2^40 among the others, in the same tile and wave: the others' bits stay."""
+    totals = [old + new] * rows
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, g, d, seed=5)
+    q = queries(rows * new, h, d, BF, seed=6)
+    hit = torch.zeros(rows * new, h, dtype=torch.bool, device="cuda")
+    hit[1::9, 1::2] = True
+    args = (pages, torch.from_numpy(table).cuda(), ints(starts([new] * rows)), ints(totals))
+    kw = dict(scale=d ** -0.5, chunk=1, max_new=new, max_kv=max(totals))
+    want = kv8.attention(q, *args, **kw)
+    got = kv8.attention(torch.where(hit[..., None], q * 2.0 ** 40, q), *args, **kw)
+    assert torch.isfinite(got).all() and torch.equal(got[~hit], want[~hit]) and not torch.equal(got[hit], want[hit])
+
 
 # --- a run of them ----------------------------------------------------------------------------------------------------------
 
