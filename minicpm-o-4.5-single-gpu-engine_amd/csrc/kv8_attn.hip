@@ -204,7 +204,7 @@ struct State {
   float m = -__builtin_inff();  // reference
   float nb = 7.f;               // 7 - m, 7 where m is -inf; 0 where `big`
   bool big = false;             // some query of the wave has a large |m|: `move` computes the exponentials' arguments itself
-  int E = 0;                    // biased value exponent that o is in units of; 0: none yet
+  int E = -1;                   // biased value exponent that o is in units of (0 is 2^-127); -1: none yet
 
   __device__ __forceinline__ State() {
 #pragma unroll
@@ -225,7 +225,7 @@ struct State {
   // o in units of exponent e from here on
   __device__ __forceinline__ void raise(int e) {
     if (e > E) {
-      scale_o(E == 0 ? 0.f : pow2_bits(E - e + 127));
+      scale_o(E < 0 ? 0.f : pow2_bits(E - e + 127));
       E = e;
     }
   }
@@ -320,7 +320,7 @@ struct State {
     const float mn = fmaxf(m, m2);
     const float f1 = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
     const float f2 = m2 == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m2 - mn);
-    const float g1 = E == en ? f1 : f1 * (E == 0 ? 0.f : pow2_bits(E - en + 127)), g2 = e2 == en ? f2 : f2 * (e2 == 0 ? 0.f : pow2_bits(e2 - en + 127));
+    const float g1 = E == en ? f1 : f1 * (E < 0 ? 0.f : pow2_bits(E - en + 127)), g2 = e2 == en ? f2 : f2 * (e2 < 0 ? 0.f : pow2_bits(e2 - en + 127));
     l = l * f1 + l2 * f2;
 #pragma unroll
     for (int x = 0; x < NT; ++x)
@@ -336,7 +336,7 @@ struct State {
   template <bool BF>
   __device__ __forceinline__ void store(const t2w_kv8_attention_args& a, const KV8Split& sp, const Tile& t, int kv_head, int part, int parts,
                                         int mrow, int g) const {
-    const float unit = pow2_bits(E) * 0.0078125f;  // 2^(E - 127 - 7); E = 0: no value block at all, o is zero
+    const int unit = E - 127 - 7;  // o counts 2^unit
     float sum = l + __shfl_xor(l, 32, 64);
     if constexpr (MR == 16) sum += __shfl_xor(sum, 16, 64);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -352,7 +352,7 @@ struct State {
           uint32_t w[4];
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            const float u = o[x][0][r + y] * inv * unit, v = o[x][1][r + y] * inv * unit;
+            const float u = __builtin_amdgcn_ldexpf(o[x][0][r + y] * inv, unit), v = __builtin_amdgcn_ldexpf(o[x][1][r + y] * inv, unit);
             w[y] = BF ? pack2(u, v) : pack2h(u, v);
           }
           *(uint4*)(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -368,8 +368,8 @@ struct State {
           const int d = MR == 16 ? 32 * x + 8 * g : 64 * x + 4 * r + 8 * g;
 #pragma unroll
           for (int y = 0; y < 4; y += 2)
-            *(float4*)(po + d + 2 * y) = make_float4(o[x][0][r + y] * inv * unit, o[x][1][r + y] * inv * unit, o[x][0][r + y + 1] * inv * unit,
-                                                     o[x][1][r + y + 1] * inv * unit);
+            *(float4*)(po + d + 2 * y) = make_float4(__builtin_amdgcn_ldexpf(o[x][0][r + y] * inv, unit), __builtin_amdgcn_ldexpf(o[x][1][r + y] * inv, unit),
+                                                     __builtin_amdgcn_ldexpf(o[x][0][r + y + 1] * inv, unit), __builtin_amdgcn_ldexpf(o[x][1][r + y + 1] * inv, unit));
         }
       if (g == 0) *(float2*)ml = make_float2(m, sum);
     }

@@ -69,10 +69,15 @@ class KV8Pages:
         """What blocks ``ids`` (all by default) hold: keys and values, fp32 [n, kv_heads, 32, head_dim]."""
         pick = (lambda t: t) if ids is None else (lambda t: t[ids])  # noqa: E731
         code = lambda t: pick(t).view(torch.float8_e4m3fn).float()  # noqa: E731
-        scale = lambda e: torch.exp2(pick(e).float() - 127)[:, :, None, None]  # noqa: E731
+
+        def scaled(x, e):  # in two steps, each a normal power of two
+            e = pick(e).float()[:, :, None, None] - 127
+            half = torch.floor(e / 2)
+            return x * torch.exp2(half) * torch.exp2(e - half)
+
         k = code(self.k).transpose(2, 3).flatten(3)
         v = code(self.v).permute(0, 1, 2, 5, 3, 4).flatten(4).flatten(2, 3)
-        return k * scale(self.k_exp), v * scale(self.v_exp)
+        return scaled(k, self.k_exp), scaled(v, self.v_exp)
 
 
 def _ints(what: str, t: torch.Tensor, n: int, dev) -> int:

@@ -714,6 +714,19 @@ def test_attention_queries_do_not_touch_each_other(dev, new, old, h, g, d, rows)
     got = kv8.attention(torch.where(hit[..., None], q * 2.0 ** 40, q), *args, **kw)
     assert torch.isfinite(got).all() and torch.equal(got[~hit], want[~hit]) and not torch.equal(got[hit], want[hit])
 
+@pytest.mark.parametrize("new,old,h,g,d,rows", ALL_FORMS[:5])
+def test_attention_value_scale_byte_zero(dev, new, old, h, g, d, rows):
+    """Values of scale 2^-127 (and a little more) are what they are, not zeros."""
+    totals = [old + new - 13 * r for r in range(rows)]
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, g, d, seed=5)
+    q = queries(rows * new, h, d, BF, seed=6)
+    for low in (0, 2):
+        pages.v_exp.copy_(torch.randint(0, low + 1, pages.v_exp.shape, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda"))
+        out = check_attention(q, pages, table, [new] * rows, totals, 1, max_new=new, max_kv=max(totals))
+        sees = torch.tensor([t - new + i >= 0 for t in totals for i in range(new)], device="cuda")  # rows of fewer keys than queries
+        assert (out[sees].abs() > 0).double().mean() > 0.99 and (out[~sees] == 0).all()
+
 
 # --- a run of them ----------------------------------------------------------------------------------------------------------
 
