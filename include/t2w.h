@@ -367,14 +367,19 @@ typedef struct {
 } t2w_kv8_append_args;
 int t2w_kv8_append(const t2w_kv8_append_args* a, void* stream);
 
-/* out = softmax(scale q K^T) V of every new token over its row's cache (its own and the other new tokens appended before),
- * fp32 softmax and sums.  heads / kv_heads (1 to 16) query heads share a key head, in order.  chunk: 0 a query sees all
- * of its row; c > 0 it sees the row's earlier tokens and those new ones whose chunk of c new tokens is not behind its own
- * (1: causal).  A query that sees nothing gets zeros.  `out` may be `q` itself (same strides) but overlaps no operand
- * otherwise.  Rows of `out` behind the last token are left as they were.  A row
- * longer than its table is wide, or one with block ids outside the pages that a query sees, gets NaN.
+/* out = softmax(scale q K^T) V of every new token over its row's cache (its own and the other new tokens appended before).
+ * heads / kv_heads (1 to 16) query heads share a key head, in order.  chunk: 0 a query sees all of its row; c > 0 it sees the
+ * row's earlier tokens and those new ones whose chunk of c new tokens is not behind its own (1: causal).  A query that sees
+ * nothing gets zeros.  `out` may be `q` itself (same strides) but overlaps no operand otherwise.  Rows of `out` behind the last
+ * token are left as they were (all of them after a plan that could not be served).  A row longer than its table is wide, or
+ * one with block ids outside the pages that a query sees, gets NaN.
+ * Scores, maxima, exponentials and sums are fp32; q times the keys' codes, before their scale, has to stay within fp32's
+ * range.  A term's weight, exp(score) times its value block's scale, is rounded to fp16's 11 bits for the matrix unit; far below
+ * the query's largest weight it is off by 2^-32 of that instead (2^-22 while the value exponents of the row's blocks span 10 or
+ * less), so value scales may lie as far apart as they can.
  * At most 2^24 new tokens.  max_new: 0, or a bound on every row's new tokens; max_kv: 0, or one on kv_total: they choose
- * the kernel and how it splits the keys.  A row of more than max_new new tokens may get NaN; one of more than max_kv keys is still right. */
+ * the kernel and how it splits the keys.  A row of more than max_new new tokens may get NaN; one of more than max_kv keys is
+ * still right. */
 typedef struct {
   t2w_kv8_pages pages;
   const void* q; void* out;       /* [n_tok, heads, head_dim], token rows ldq / ldo elements apart (multiples of 8) */

@@ -189,9 +189,33 @@ __device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float(
 //    probabilities are 2^(s - m + 7) <= 2^15 in fp16, so most blocks need no exchange between lanes and no rescaling of the
 //    outputs, and a probability keeps fp16's 11 bits down to 2^-21 of the largest and 2^-32 of it absolutely.  fp16 and not
 //    bf16: bf16's 8 bits would cost as much again as the output's own rounding.
-//  * value codes enter as fp16, exact, times 2^(their exponent - E + 7), E the largest value exponent so far: 22 powers of two
-//    below the largest block's scale stay exact.
+//  * value codes enter as fp16, exact, times 2^(their exponent - E + 7), E the largest value exponent so far, while the exponents
+//    span at most NEAR; a block that nobody sees yet can change nothing but E, which scales o exactly.
+//  * from the first block on that lies further apart (`wide`) the scale is a part of the weight: the operands of P . V are
+//    2^(s - m + exponent - k + 7) <= 2^15 and the codes times 2^7, with k a reference of each query that moves as m does.  What
+//    counts is then a term's own size, p times its scale, however far scales lie apart: a block of large values and no weight
+//    takes no bits from the others, nor the other way round.  l takes its exponentials in fp32 there.
+//  * a weight is off by 2^-12 of it or by 2^-25, half of fp16's smallest step, where the largest is 2^7 and more (2^(7 - NEAR)
+//    of those before the exponents span more than that): 2^-32 of the largest p times scale, 2^-22 at worst, a key.
 //  * sums of probabilities are of the same rounded fp16 values as the outputs' (fp32 dot products, a lane its own keys').
+constexpr int NEAR = 10;
+
+constexpr int WIDE = 1 << 20;    // in place of a value unit: exponents lie far apart
+
+// Value exponents (biased) of the blocks so far, -1 where one counts for nobody.  The unit that the block's values need:
+// the largest of them, or WIDE from where they span more than NEAR on.
+struct Units {
+  int hi = -1;
+  unsigned lo = 255;
+  __device__ __forceinline__ int add(int e) {
+    hi = max(hi, e);
+    lo = min(lo, (unsigned)e);
+    return hi - (int)lo > NEAR ? WIDE : hi;
+  }
+  // exponent of the factor of the block's codes, 7 above what its values are in units of it
+  static __device__ __forceinline__ int factor(int e, int unit) { return (unit == WIDE ? 0 : e - unit) + 127 + 7; }
+};
+
 template <int MR, int D>
 struct State {
   static constexpr int AR = MR == 16 ? 4 : 16;     // values of an accumulator
@@ -202,9 +226,12 @@ struct State {
   Acc o[NT][2];
   float l = 0.f;                // sum of the lane's probabilities; of the query's when the lane groups are added
   float m = -__builtin_inff();  // reference
-  float nb = 7.f;               // 7 - m, 7 where m is -inf; 0 where `big`
-  bool big = false;             // some query of the wave has a large |m|: `move` computes the exponentials' arguments itself
+  float nb = 7.f;               // 7 - m, 7 where m is -inf; 0 where `big`; -k where `wide`
+  bool big = false;             // some query of the wave has a large |m|
   int E = -1;                   // biased value exponent that o is in units of (0 is 2^-127); -1: none yet
+  bool wide = false;            // value exponents lie far apart: o is in units of 2^k, each query's own
+  uint32_t one = 0x3c003c00;    // a pair of fp16 ones, for the sums of probabilities; zeros where `wide`
+  bool slow = false;            // big or wide: `move` computes the exponentials' arguments itself
 
   __device__ __forceinline__ State() {
 #pragma unroll
@@ -222,13 +249,6 @@ struct State {
 #pragma unroll
         for (int r = 0; r < AR; ++r) o[x][j][r] *= f;
   }
-  // o in units of exponent e from here on
-  __device__ __forceinline__ void raise(int e) {
-    if (e > E) {
-      scale_o(E < 0 ? 0.f : pow2_bits(E - e + 127));
-      E = e;
-    }
-  }
   // key of score r of tile x within its block
   static __device__ __forceinline__ int key_of(int x, int r, int g) { return MR == 16 ? 8 * g + 4 * x + r : 16 * (r >> 3) + 8 * g + (r & 7); }
 
@@ -240,40 +260,61 @@ struct State {
       for (int r = 0; r < AR; ++r) mx = fmaxf(mx, sc[x][r]);
     return mx;
   }
-  // Whether a block's factor c = cm 2^e is a normal number; where it is not, its scores are scaled themselves, in fp32's whole
-  // range (a factor of 0 would make NaN of an invisible score's -inf).
-  static __device__ __forceinline__ bool normal(int e) { return e >= -125 && e <= 126; }
-  static __device__ __forceinline__ void scale_scores(Acc (&sc)[KG], float cm, int e) {
+  // A block's factor c = cm 2^ex is a normal number for |ex| <= NORMAL; where it is not, its scores are scaled themselves, in
+  // fp32's whole range (a factor of 0 would make NaN of an invisible score's -inf).
+  static constexpr int NORMAL = 125;
+  static __device__ __forceinline__ void scale_scores(Acc (&sc)[KG], float cm, int ex) {
 #pragma unroll
     for (int x = 0; x < KG; ++x)
 #pragma unroll
-      for (int r = 0; r < AR; ++r) sc[x][r] = __builtin_amdgcn_ldexpf(sc[x][r] * cm, e);
+      for (int r = 0; r < AR; ++r) sc[x][r] = __builtin_amdgcn_ldexpf(sc[x][r] * cm, ex);
+  }
+  // Scores of keys from `lim` on are -inf, the others NaN where `off`.
+  static __device__ __forceinline__ void mask(Acc (&sc)[KG], bool off, int key0, int lim, int g) {
+#pragma unroll
+    for (int x = 0; x < KG; ++x)
+#pragma unroll
+      for (int r = 0; r < AR; ++r) sc[x][r] = key0 + key_of(x, r, g) < lim ? (off ? __builtin_nanf("") : sc[x][r]) : -__builtin_inff();
   }
   // Moves the reference where a block's scores, in units 1 / c and -inf where invisible, of maximum mx, pass it.  Where |m| is
   // large, s - m + 7 in one fma is not what the scores' own rounding allows: 7 - m rounds too, and a score of m + 8 could reach
   // 2^16, infinite in fp16.  There s is rounded first, as mx was, and s - m is exact where it counts; nothing may be contracted.
   // Each query by its own m alone, so that its bits do not depend on the others of the wave.
-  __device__ __forceinline__ void move(Acc (&sc)[KG], float& c, float mx) {
+  __device__ __forceinline__ void move(Acc (&sc)[KG], float& c, float mx, int vx, int e) {
 #pragma clang fp contract(off)
     mx *= c;
-    if (__builtin_amdgcn_ballot_w64(mx - m > 8.f)) {
-      const float seen = query_max<MR>(mx), mn = seen - m > 8.f ? seen : m;  // each query by its own scores alone
+    // one comparison for both: some maximum passes the reference by 8, or the unit rises (then every lane's does)
+    if (__builtin_amdgcn_ballot_w64(fmaxf(mx - m, -1.f) > (e > E ? -2.f : 8.f))) {
+      nb = e == WIDE && !wide ? -(float)E : nb;
+      wide = wide || e == WIDE;
+      const bool up = !wide && e > E;
+      float seen = mx;
+      if (wide || __builtin_amdgcn_ballot_w64(mx - m > 8.f)) seen = query_max<MR>(mx);
+      const float mn = seen - m > 8.f ? seen : m;  // each query by its own scores alone
       const float alpha = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
       big = big || __builtin_amdgcn_ballot_w64(large(mn)) != 0;
-      nb = big ? 0.f : mn == -__builtin_inff() ? 7.f : 7.f - mn;
+      // wide: scores count from mn now, and k with them; then k moves to the largest weight where that passes it by 8
+      const float n = nb + (mn == m ? 0.f : fminf(mn - m, 1e30f)), need = mn == -__builtin_inff() ? -1e30f : seen - mn + (float)vx;
+      const float nk = need + n > 8.f ? -need : n;
+      const float f = wide ? __builtin_amdgcn_exp2f(nk - n) : up ? (E < 0 ? 0.f : alpha * pow2_bits(E - e + 127)) : alpha;
+      nb = wide ? nk : big ? 0.f : mn == -__builtin_inff() ? 7.f : 7.f - mn;
+      E = up ? e : E;
+      slow = big || wide;
+      one = wide ? 0 : one;  // `move` sums them, below
+      m = mn;
       l *= alpha;
-      scale_o(alpha);
+      scale_o(f);
     }
-    if (big) {
-      const float m0 = m == -__builtin_inff() ? 0.f : m;
+    if (slow) {
+      const float m0 = m == -__builtin_inff() ? 0.f : m, add = wide ? (float)vx : 0.f;
       const bool own = large(m0);
 #pragma unroll
       for (int x = 0; x < KG; ++x)
 #pragma unroll
         for (int r = 0; r < AR; ++r) {
-          const float s = sc[x][r] * c;
-          sc[x][r] = own ? (s - m0) + 7.f : fmaf(sc[x][r], c, 7.f - m0);
+          const float s = sc[x][r] * c, arg = own ? (s - m0) + 7.f : fmaf(sc[x][r], c, 7.f - m0);
+          if (wide) l += __builtin_amdgcn_exp2f(arg);
+          sc[x][r] = arg + add;
         }
       c = 1.f;
     }
@@ -297,13 +338,13 @@ struct State {
       }
   }
   __device__ __forceinline__ void sum(f16x8 p) {
-    const f16x2_t one = {(_Float16)1.0f, (_Float16)1.0f};
 #pragma unroll
-    for (int z = 0; z < 8; z += 2) l = __builtin_amdgcn_fdot2(f16x2_t{p[z], p[z + 1]}, one, l, false);
+    for (int z = 0; z < 8; z += 2) l = __builtin_amdgcn_fdot2(f16x2_t{p[z], p[z + 1]}, __builtin_bit_cast(f16x2_t, one), l, false);
   }
 
   // the other state of the same rows, left in LDS by another wave (`put`), folded into this one
-  static constexpr int WORDS = NT * 2 * AR + 2;
+  static constexpr int WORDS = NT * 2 * AR + 3;
+  __device__ __forceinline__ int unit() const { return wide ? WIDE : E; }
   __device__ __forceinline__ void put(float (*dst)[64], int lane) const {
 #pragma unroll
     for (int x = 0; x < NT; ++x)
@@ -311,16 +352,32 @@ struct State {
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int r = 0; r < AR; ++r) dst[(x * 2 + j) * AR + r][lane] = o[x][j][r];
-    dst[WORDS - 2][lane] = m;
-    dst[WORDS - 1][lane] = l;
+    dst[WORDS - 3][lane] = m;
+    dst[WORDS - 2][lane] = l;
+    dst[WORDS - 1][lane] = nb;
   }
   __device__ __forceinline__ void fold(const float (*src)[64], int e2, int lane) {
-    const float m2 = src[WORDS - 2][lane], l2 = src[WORDS - 1][lane];
-    const int en = max(E, e2);
+    const float m2 = src[WORDS - 3][lane], l2 = src[WORDS - 2][lane];
     const float mn = fmaxf(m, m2);
     const float f1 = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
     const float f2 = m2 == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m2 - mn);
-    const float g1 = E == en ? f1 : f1 * (E < 0 ? 0.f : pow2_bits(E - en + 127)), g2 = e2 == en ? f2 : f2 * (e2 < 0 ? 0.f : pow2_bits(e2 - en + 127));
+    float g1, g2;
+    if (!wide && e2 != WIDE && (E < 0 || e2 < 0 || abs(E - e2) <= 60)) {
+      const int en = max(E, e2);
+      g1 = E == en ? f1 : f1 * (E < 0 ? 0.f : pow2_bits(E - en + 127));
+      g2 = e2 == en ? f2 : f2 * (e2 < 0 ? 0.f : pow2_bits(e2 - en + 127));
+      E = en;
+    } else {  // each query's unit: the larger one, as above, or where they lie far apart that of the larger weight times scale
+      float k1 = wide ? -nb : (float)E, k2 = e2 == WIDE ? -src[WORDS - 1][lane] : (float)e2;
+      k1 = m == -__builtin_inff() ? k2 : k1;
+      k2 = m2 == -__builtin_inff() ? k1 : k2;
+      const bool near = fabsf(k1 - k2) <= 60.f;
+      const float a1 = near ? k1 : (m - mn) + k1, a2 = near ? k2 : (m2 - mn) + k2, kn = fmaxf(a1, a2);
+      g1 = (near ? f1 : 1.f) * __builtin_amdgcn_exp2f(a1 - kn);
+      g2 = (near ? f2 : 1.f) * __builtin_amdgcn_exp2f(a2 - kn);
+      wide = true;
+      nb = -kn;
+    }
     l = l * f1 + l2 * f2;
 #pragma unroll
     for (int x = 0; x < NT; ++x)
@@ -329,17 +386,21 @@ struct State {
 #pragma unroll
         for (int r = 0; r < AR; ++r) o[x][j][r] = o[x][j][r] * g1 + src[(x * 2 + j) * AR + r][lane] * g2;
     m = mn;
-    E = en;
   }
 
   // Row mrow of the tile (lane group g): to the outputs, or to the call's workspace where the tile has several parts
   template <bool BF>
   __device__ __forceinline__ void store(const t2w_kv8_attention_args& a, const KV8Split& sp, const Tile& t, int kv_head, int part, int parts,
                                         int mrow, int g) const {
-    const int unit = E - 127 - 7;  // o counts 2^unit
     float sum = l + __shfl_xor(l, 32, 64);
     if constexpr (MR == 16) sum += __shfl_xor(sum, 16, 64);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    float inv = sum == 0.f ? 0.f : 1.f / sum;
+    int unit = E - 127 - 7;  // o counts 2^unit
+    if (wide) {
+      const float k = fmaxf(-nb, -1000.f), whole = rintf(k);
+      unit = (int)whole - 127 - 7;
+      inv *= __builtin_amdgcn_exp2f(k - whole);
+    }
     // values r .. r + 3 of both tiles of a pair are 8 consecutive channels, from d on
     if (parts == 1) {
       const int tok = mrow / sp.G, hq = mrow - tok * sp.G;
@@ -432,6 +493,7 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
     for (int n = 0; n < NQ; ++n) q[n] = *(const uint4*)(src + (LG * (n >> 1) + g) * 16 + (n & 1) * 8);
   }
   St st;
+  Units units;
 
   // the lane's place in a block's keys and values; its loads lie at constant distances from there (load offsets)
   const uint32_t koff = MR == 16 ? g * 512 + (8 * (i >> 2) + (i & 3)) * 16 : g * 512 + ((i & 0x13) | ((i & 4) << 1) | ((i & 8) >> 1)) * 16;
@@ -458,7 +520,7 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
     // the wave's blocks b0 + kw, + KW, ...: ids and exponents of the next 64 of them one a lane
     for (int base = b0 + kw; base < b1; base += 64 * KW) {
       const int mine = base + lane * KW;
-      int id = mine >= b1 ? 0 : sp.per_row > 0 && base == ahead ? id_ahead : table[mine], ke = 255, ve = 0;
+      int id = mine >= b1 ? 0 : sp.per_row > 0 && base == ahead ? id_ahead : table[mine], ke = 255, ve = -1;
       if ((unsigned)id < (unsigned)a.pages.n_blocks) {
         ke = a.pages.k_exp[(size_t)id * a.pages.kv_heads + kv_head];
         ve = a.pages.v_exp[(size_t)id * a.pages.kv_heads + kv_head];
@@ -484,17 +546,12 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
         }
         if (next >= 0) load_k(next);
         const bool off = kx > 254;  // a block id outside the pages, or an E8M0 NaN
-        const int ex = sp.ce + (off ? 0 : kx - 127);
+        const int ex = sp.ce + kx - 127;
         float c = __builtin_amdgcn_ldexpf(sp.cm, ex);
-        if (off || !St::normal(ex) || key0 + KV8_BLOCK > lim_lo) {  // or some query of the wave does not see all of the block
-          if (!St::normal(ex)) {
-            St::scale_scores(sc, sp.cm, ex);
-            c = 1.f;
-          }
-#pragma unroll
-          for (int z = 0; z < KG; ++z)
-#pragma unroll
-            for (int r = 0; r < AR; ++r) sc[z][r] = key0 + St::key_of(z, r, g) < lim ? (off ? __builtin_nanf("") : sc[z][r]) : -__builtin_inff();
+        if (max(key0 + KV8_BLOCK - lim_lo, kx - 254) > 0) St::mask(sc, off, key0, lim, g);  // or some query of the wave does not see all of the block
+        if (abs(ex) > St::NORMAL) {
+          St::scale_scores(sc, sp.cm, ex);
+          c = 1.f;
         }
         if (off || key0 + KV8_BLOCK > t.total) {  // values behind the last token count as zeros, whatever they are
 #pragma unroll
@@ -505,13 +562,13 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
             vf[w].z &= (uint32_t)keep; vf[w].w &= (uint32_t)(keep >> 32);
           }
         }
-        st.move(sc, c, St::top(sc));
-        st.raise(vx);
+        const int unit = units.add(vx);
+        st.move(sc, c, St::top(sc), vx, unit);
         f16x8 p[NP];
         st.exps(sc, c, p);
 #pragma unroll
         for (int w = 0; w < NP; ++w) st.sum(p[w]);
-        const float vs = pow2_bits(vx - st.E + 127 + 7);
+        const float vs = pow2_bits(Units::factor(vx, unit));
 #pragma unroll
         for (int w = 0; w < NL; ++w) {
           const int z = MR == 16 ? w : w / 2, kk = MR == 16 ? 0 : w % 2;
@@ -527,7 +584,7 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
   for (int w = KW / 2; w >= 1; w /= 2) {
     if (kw >= w && kw < 2 * w) {
       st.put(s_acc[(kw - w) * RW + rw], lane);
-      if (lane == 0) s_e[wave] = st.E;
+      if (lane == 0) s_e[wave] = st.unit();
     }
     __syncthreads();
     if (kw < w) st.fold(s_acc[kw * RW + rw], s_e[wave + w * RW], lane);
@@ -593,7 +650,7 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
   };
   auto exps_of = [&](int chunk, int& id, int& ke, int& ve) {
     ke = 127;
-    ve = 0;
+    ve = -1;
     if (b0 + chunk * 64 + lane >= b1) return;  // a last step's second block beyond the part: nobody sees it
     if ((unsigned)id < (unsigned)a.pages.n_blocks) {
       ke = a.pages.k_exp[(size_t)id * a.pages.kv_heads + kv_head];
@@ -605,11 +662,12 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
   };
   int id = ids_of(0), ke, ve;
   exps_of(0, id, ke, ve);
-  int id2 = ids_of(1), ke2 = 127, ve2 = 0;
+  int id2 = ids_of(1), ke2 = 127, ve2 = -1;
 
   uint4 rk[NC], rv[NC];
   int nke[2], nve[2];  // exponents of the step in registers
-  int nE = 0;          // value unit of the step that was converted last
+  Units units;         // of the blocks that were converted
+  int nE[2], nS[2];    // value units of the step in registers, and the exponents of its codes' factors
   auto load = [&](int s) {
     const int x = 2 * (s & 31);
     if (s > 0 && x == 0) { id = id2; ke = ke2; ve = ve2; id2 = ids_of(s / 32 + 1); }
@@ -626,7 +684,11 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
   };
   // the step in registers to LDS, in four pieces a chunk; `unit` comes first
   auto unit = [&](int s) {
-    nE = max(nE, max(nve[0], nve[1]));
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      nE[y] = units.add(nve[y]);
+      nS[y] = Units::factor(nve[y], nE[y]);
+    }
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int y = __builtin_amdgcn_readfirstlane((tid + T * n) / CB), r = (tid + T * n) % CB, key0 = (b0 + 2 * s + y) * KV8_BLOCK;
@@ -648,7 +710,7 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
       if constexpr (BF) *kd = __builtin_bit_cast(uint4, codes_bf16(lo, hi));
       else *kd = __builtin_bit_cast(uint4, codes_f16(lo, hi, 1.f));
     } else {  // values: group of 8 keys, channel pair -> an operand of 8 keys for each channel
-      const float vs = pow2_bits((y ? nve[1] : nve[0]) - nE + 127 + 7);
+      const float vs = pow2_bits(y ? nS[1] : nS[0]);
       const uint32_t lo = (piece & 1) ? rv[n].z : rv[n].x, hi = (piece & 1) ? rv[n].w : rv[n].y;
       s_v[buf][y][r / (D / 2) * D + (piece & 1) * (D / 2) + r % (D / 2)] = __builtin_bit_cast(uint4, codes_f16(lo, hi, vs));
     }
@@ -671,22 +733,20 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
   // and into mx while P . V runs, where the next step's codes are converted too (cbuf >= 0).  The order within a phase is
   // pinned, a few vector instructions behind each MFMA, so that both units work at once.
   float mx;
-  auto block = [&](int buf, int y, int key0, int kx, int E, typename St::Acc (&sc)[1], int nbuf, int ny, typename St::Acc (&sn)[1], auto conv, int cbuf) {
+  auto block = [&](int buf, int y, int key0, int kx, int vx, int E, typename St::Acc (&sc)[1], int nbuf, int ny, typename St::Acc (&sn)[1], auto conv, int cbuf) {
     read_k(nbuf, ny);
-    const bool off = kx > 254;
-    const int ex = sp.ce + (off ? 0 : kx - 127);
+    const int ex = sp.ce + kx - 127;
     float c = __builtin_amdgcn_ldexpf(sp.cm, ex);
-    if (off || !St::normal(ex) || key0 + KV8_BLOCK > lim_lo) {
-      if (!St::normal(ex)) {
-        St::scale_scores(sc, sp.cm, ex);
-        c = 1.f;
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sc[0][r] = key0 + St::key_of(0, r, g) < lim ? (off ? __builtin_nanf("") : sc[0][r]) : -__builtin_inff();
+    if (max(key0 + KV8_BLOCK - lim_lo, kx - 254) > 0) {
+      St::mask(sc, kx > 254, key0, lim, g);
       mx = St::top(sc);
     }
-    st.move(sc, c, mx);
-    st.raise(E);
+    if (abs(ex) > St::NORMAL) {
+      St::scale_scores(sc, sp.cm, ex);
+      c = 1.f;
+      mx = St::top(sc);
+    }
+    st.move(sc, c, mx, vx, E);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
@@ -732,7 +792,7 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
   unit(0);
 #pragma unroll
   for (int z = 0; z < 4 * NC; ++z) convert(z, 0);
-  int kx0 = nke[0], kx1 = nke[1], E = nE;
+  int kx0 = nke[0], kx1 = nke[1], vx0 = nve[0], vx1 = nve[1], E0 = nE[0], E1 = nE[1];
   if (steps > 1) load(1);
   __syncthreads();
   typename St::Acc s0[1], s1[1];
@@ -743,21 +803,22 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
   for (int s = 0; s < steps; ++s) {
     const int nxt = cur == 2 ? 0 : cur + 1, key0 = (b0 + 2 * s) * KV8_BLOCK;
     const bool on = key0 < lim_hi, more = s + 1 < steps;
-    int nkx0 = 127, nkx1 = 127;
+    int nkx0 = 127, nkx1 = 127, nvx0 = -1, nvx1 = -1;
     if (more) {
       unit(s + 1);
       nkx0 = nke[0]; nkx1 = nke[1];
+      nvx0 = nve[0]; nvx1 = nve[1];
     }
     if (on) {
-      block(cur, 0, key0, kx0, E, s0, cur, 1, s1, std::true_type(), nxt);  // after the last step: into a buffer that nobody reads
+      block(cur, 0, key0, kx0, vx0, E0, s0, cur, 1, s1, std::true_type(), nxt);  // after the last step: into a buffer that nobody reads
     } else {
 #pragma unroll
       for (int z = 0; z < 4 * NC; ++z) convert(z, nxt);
     }
     if (s + 2 < steps) load(s + 2);
     __syncthreads();
-    if (on) block(cur, 1, key0 + KV8_BLOCK, kx1, E, s1, nxt, 0, s0, std::false_type(), 0);
-    kx0 = nkx0; kx1 = nkx1; E = nE;
+    if (on) block(cur, 1, key0 + KV8_BLOCK, kx1, vx1, E1, s1, nxt, 0, s0, std::false_type(), 0);
+    kx0 = nkx0; kx1 = nkx1; vx0 = nvx0; vx1 = nvx1; E0 = nE[0]; E1 = nE[1];
     cur = nxt;
   }
   if (mrow < t.rows) st.template store<BF>(a, sp, t, kv_head, part, parts, mrow, g);

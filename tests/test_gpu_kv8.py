@@ -727,6 +727,79 @@ def test_attention_value_scale_byte_zero(dev, new, old, h, g, d, rows):
         sees = torch.tensor([t - new + i >= 0 for t in totals for i in range(new)], device="cuda")  # rows of fewer keys than queries
         assert (out[sees].abs() > 0).double().mean() > 0.99 and (out[~sees] == 0).all()
 
+def range_floor(q, pages, table, new, totals, scale, chunk):
+    """Beside the relative rounding: a term's weight p_j 2^e_j is an fp16 number that may lie 2^10 below its query's reference
+    before value scales are far apart, off by 2^-25 at most where the largest one is 2^(7 - 10) or more: 2^-22 of that a key."""
+    k, _ = scaled(pages)
+    size = np.broadcast_to(448.0 * np.exp2(pages.v_exp.cpu().numpy().astype(float) - 127)[..., None, None], k.shape)
+    w, _, _ = ok.attention(q.double().cpu().numpy(), k, size, table, starts(new), totals, scale, chunk)
+    return 2.0 ** -22 * max(totals) * w
+
+
+def check_range(q, pages, table, new, totals, chunk, **kw):
+    d = pages.head_dim
+    k, v = scaled(pages)
+    o, mag, top = ok.attention(q.double().cpu().numpy(), k, v, table, starts(new), totals, d ** -0.5, chunk)
+    out = kv8.attention(q, pages, torch.from_numpy(table).cuda(), ints(starts(new)), ints(totals), scale=d ** -0.5, chunk=chunk, **kw)
+    bound = attn_bound(o, mag, top, d, q.dtype) + range_floor(q, pages, table, new, totals, d ** -0.5, chunk)
+    worst = float((np.abs(out.double().cpu().numpy() - o) / bound).max())
+    assert worst <= 1, worst
+
+
+@pytest.mark.parametrize("new,old,h,g,d,rows", ALL_FORMS)
+@pytest.mark.parametrize("diff,below", [(24, 0), (24, 80), (40, 80), (40, 30), (60, 60), (100, 160), (120, 100)])
+def test_attention_value_scales_far_apart(dev, new, old, h, g, d, rows, diff, below):
+    """One block of values 2^diff times the others', its scores about 2^below times less likely: whichever of them counts is right.
+    It stands first in some rows, in the middle or near the end in others."""
+    totals = [old + new - 13 * r for r in range(rows)]
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, g, d, seed=5)
+    pages.k_exp.fill_(121)
+    pages.v_exp.fill_(100)
+    q = queries(rows * new, h, d, BF, seed=6)
+    w = 448 if below >= 80 else 256
+    q[..., 0] = below * d ** 0.5 / (1.4427 * w * 2.0 ** -6)
+    pages.k[:, :, 0, :, 0] = 0
+    code = torch.tensor([-float(w)]).to(torch.float8_e4m3fn).view(torch.uint8).item()
+    for r, t in enumerate(totals):
+        b = int(table[r, (0, need(t) // 2, need(old) - 1)[(r + new) % 3]])
+        pages.v_exp[b] = 100 + diff
+        pages.k[b, :, 0, :, 0] = code if below else 0
+    check_range(q, pages, table, [new] * rows, totals, 1, max_new=new, max_kv=max(totals))
+
+
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("new,old,h,g,d,rows", ALL_FORMS)
+def test_attention_value_scales_of_every_size(dev, new, old, h, g, d, rows, dt):
+    """Value scales drawn from 2^-60 to 2^8 for every block and head, in no order."""
+    totals = [old + new - 13 * r for r in range(rows)]
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, g, d, seed=5)
+    pages.v_exp.copy_(torch.randint(67, 132, pages.v_exp.shape, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda"))
+    q = queries(rows * new, h, d, dt, seed=6)
+    for size in (1, 12):
+        check_range(q * size, pages, table, [new] * rows, totals, 1, max_new=new, max_kv=max(totals))
+
+
+@pytest.mark.parametrize("new,old,h,g,d,rows", [(40, 100, 4, 2, 64, 3), (40, 100, 2, 2, 128, 3)] + ALL_FORMS[4:])
+@pytest.mark.parametrize("last", [1, 2, 3])
+def test_attention_unseen_scales_change_nothing(dev, new, old, h, g, d, rows, last):
+    """The value scales of the row's last blocks 2^130 times the others': queries that see none of them keep their bits."""
+    totals = [old + new] * rows
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, g, d, seed=5)
+    q = queries(rows * new, h, d, BF, seed=6)
+    args = (pages, torch.from_numpy(table).cuda(), ints(starts([new] * rows)), ints(totals))
+    kw = dict(scale=d ** -0.5, chunk=1, max_new=new, max_kv=max(totals))
+    want = kv8.attention(q, *args, **kw)
+    first = (need(old + new) - last) * 32 - old  # the first query that sees one of them
+    for r in range(rows):
+        pages.v_exp[torch.from_numpy(table[r, need(old + new) - last:need(old + new)]).long().cuda()] = 250
+    got = kv8.attention(q, *args, **kw)
+    for r in range(rows):
+        assert torch.equal(got[r * new:r * new + max(first, 0)], want[r * new:r * new + max(first, 0)])
+        assert not torch.equal(got[r * new + max(first, 0):(r + 1) * new], want[r * new + max(first, 0):(r + 1) * new])
+
 
 # --- a run of them ----------------------------------------------------------------------------------------------------------
 
