@@ -325,8 +325,9 @@ int t2w_attention(const void* q, const void* k_pool, const void* v_pool, void* o
 
 enum { T2W_KV8_BLOCK = 32, T2W_KV8_BF16 = 0, T2W_KV8_FP16 = 1 };
 
-/* Value (token t of its block, channel d) is code * 2^(exponent - 127).  Key codes: byte (d / 16) * 512 + t * 16 + d % 16
- * of the (block, head)'s 32 * head_dim; value codes: byte (t / 8) * 8 * head_dim + (d / 2) * 16 + (d % 2) * 8 + t % 8. */
+/* Value (token t of its block, channel d) is code * 2^(exponent - 127), NaN for exponent 255 (E8M0).  Key codes: byte
+ * (d / 16) * 512 + t * 16 + d % 16 of the (block, head)'s 32 * head_dim; value codes: byte
+ * (t / 8) * 8 * head_dim + (d / 2) * 16 + (d % 2) * 8 + t % 8. */
 typedef struct {
   void* k; void* v;               /* [n_blocks, kv_heads, 32 * head_dim] e4m3 codes, 16-byte aligned */
   uint8_t* k_exp; uint8_t* v_exp; /* [n_blocks, kv_heads] */
@@ -371,8 +372,8 @@ int t2w_kv8_append(const t2w_kv8_append_args* a, void* stream);
  * heads / kv_heads (1 to 16) query heads share a key head, in order.  chunk: 0 a query sees all of its row; c > 0 it sees the
  * row's earlier tokens and those new ones whose chunk of c new tokens is not behind its own (1: causal).  A query that sees
  * nothing gets zeros.  `out` may be `q` itself (same strides) but overlaps no operand otherwise.  Rows of `out` behind the last
- * token are left as they were (all of them after a plan that could not be served).  A row longer than its table is wide, or
- * one with block ids outside the pages that a query sees, gets NaN.
+ * token are left as they were (all of them after a plan that could not be served).  A row longer than its table is wide gets
+ * NaN, and so does a query that sees a block id outside the pages or a block with a scale of NaN.
  * Scores, maxima, exponentials and sums are fp32; q times the keys' codes, before their scale, has to stay within fp32's
  * range.  A term's weight, exp(score) times its value block's scale, is rounded to fp16's 11 bits for the matrix unit; far below
  * the query's largest weight it is off by 2^-32 of that instead (2^-22 while the value exponents of the row's blocks span 10 or

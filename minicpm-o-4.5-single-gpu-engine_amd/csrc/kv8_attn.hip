@@ -181,6 +181,13 @@ __device__ __forceinline__ float query_max(float v) {
   return v;
 }
 
+// Exponent bytes of a block, in scalar registers: an E8M0 NaN among the values' is one among the keys', whose NaN scores reach
+// who sees the block and nobody else, and counts for no unit
+__device__ __forceinline__ void nan_scales(int& kx, int& vx) {
+  kx = vx == 255 ? 255 : kx;
+  vx = kx == 255 ? -1 : vx;
+}
+
 __device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float((uint32_t)min(max(biased, 0), 254) << 23); }
 
 // Softmax and output state of a wave's MR packed rows (lane column = query), shared by both kernels.  Scores are in units of
@@ -531,7 +538,8 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
       load_k(__builtin_amdgcn_readlane(id, 0));
       load_v(__builtin_amdgcn_readlane(id, 0));
       for (int x = 0; x < n; ++x) {
-        const int kx = __builtin_amdgcn_readlane(ke, x), vx = __builtin_amdgcn_readlane(ve, x);
+        int kx = __builtin_amdgcn_readlane(ke, x), vx = __builtin_amdgcn_readlane(ve, x);
+        nan_scales(kx, vx);
         const int next = x + 1 < n ? __builtin_amdgcn_readlane(id, x + 1) : -1, key0 = (base + x * KW) * KV8_BLOCK;
         typename St::Acc sc[KG];
 #pragma unroll
@@ -674,6 +682,8 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
     if (x == 32) exps_of(s / 32 + 1, id2, ke2, ve2);
     nke[0] = __builtin_amdgcn_readlane(ke, x); nke[1] = __builtin_amdgcn_readlane(ke, x + 1);
     nve[0] = __builtin_amdgcn_readlane(ve, x); nve[1] = __builtin_amdgcn_readlane(ve, x + 1);
+    nan_scales(nke[0], nve[0]);
+    nan_scales(nke[1], nve[1]);
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int y = __builtin_amdgcn_readfirstlane((tid + T * n) / CB), r = (tid + T * n) % CB;

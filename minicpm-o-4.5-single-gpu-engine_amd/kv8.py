@@ -71,7 +71,8 @@ class KV8Pages:
         code = lambda t: pick(t).view(torch.float8_e4m3fn).float()  # noqa: E731
 
         def scaled(x, e):  # in two steps, each a normal power of two
-            e = pick(e).float()[:, :, None, None] - 127
+            e = pick(e).float()[:, :, None, None]
+            e = torch.where(e == 255, torch.nan, e - 127)  # E8M0's NaN
             half = torch.floor(e / 2)
             return x * torch.exp2(half) * torch.exp2(e - half)
 

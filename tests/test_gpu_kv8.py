@@ -800,6 +800,26 @@ def test_attention_unseen_scales_change_nothing(dev, new, old, h, g, d, rows, la
         assert torch.equal(got[r * new:r * new + max(first, 0)], want[r * new:r * new + max(first, 0)])
         assert not torch.equal(got[r * new + max(first, 0):(r + 1) * new], want[r * new + max(first, 0):(r + 1) * new])
 
+@pytest.mark.parametrize("new,old,h,g,d,rows", ALL_FORMS)
+@pytest.mark.parametrize("keys", [True, False])
+def test_attention_nan_scales(dev, new, old, h, g, d, rows, keys):
+    """An E8M0 NaN among the keys' or the values' scales: NaN for every query that sees some of the block, the others as ever."""
+    totals = [old + new] * rows
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, g, d, seed=5)
+    q = queries(rows * new, h, d, BF, seed=6)
+    args = (pages, torch.from_numpy(table).cuda(), ints(starts([new] * rows)), ints(totals))
+    kw = dict(scale=d ** -0.5, chunk=1, max_new=new, max_kv=max(totals))
+    want = kv8.attention(q, *args, **kw)
+    b = need(old + new) - 1
+    (pages.k_exp if keys else pages.v_exp)[int(table[0, b]), 1] = 255
+    got = kv8.attention(q, *args, **kw)
+    hit = torch.zeros(rows * new, h, dtype=torch.bool, device="cuda")
+    hit[max(0, b * 32 - old):new, h // g:2 * (h // g)] = True
+    assert got[hit].isnan().all() and torch.equal(got[~hit], want[~hit])
+    k, v = pages.values([int(table[0, b])])
+    assert (k if keys else v)[0, 1].isnan().all() and torch.isfinite((v if keys else k)[0]).all() and torch.isfinite(k[0, 0]).all()
+
 
 # --- a run of them ----------------------------------------------------------------------------------------------------------
 
