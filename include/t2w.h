@@ -352,12 +352,12 @@ typedef struct {
 int t2w_kv8_plan(const t2w_kv8_plan_args* a, void* stream);
 
 /* Quantizes the new tokens' keys and values into their rows' blocks.  A block's scale is the smallest power of two that
- * keeps its largest magnitude within 448; a block in use whose scale a new token raises has its old codes requantized.  A
- * token and head with a key or value that is not finite counts for no scale and is stored as NaN keys and zero values:
- * queries that see it get NaN, others do not.  New blocks are zero behind their last token; other places and blocks stay as
- * they are.  A block may belong to one row only (blocks shared by rows may be read, not appended to); block ids outside the
- * pages are skipped.  max_new: 0, or the longest row's new tokens, which sizes the grid (longer rows are stored all the
- * same). */
+ * keeps its largest magnitude within 448; a block in use whose scale a new token raises has its old codes requantized, one
+ * whose scale is NaN (filled elsewhere) keeps it.  A token and head with a key or value that is not finite counts for no
+ * scale and is stored as NaN keys and zero values: queries that see it get NaN, others do not.  New blocks are zero behind
+ * their last token; other places and blocks stay as they are.  A block may belong to one row only (blocks shared by rows
+ * may be read, not appended to); block ids outside the pages are skipped.  max_new: 0, or the longest row's new tokens,
+ * which sizes the grid (longer rows are stored all the same). */
 typedef struct {
   t2w_kv8_pages pages;
   const void* k; const void* v;   /* [n_tok, kv_heads, head_dim], token rows ldk / ldv elements apart (multiples of 8) */

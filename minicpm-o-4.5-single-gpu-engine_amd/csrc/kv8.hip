@@ -187,6 +187,14 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
 
+// four values times inv, clamped to +-448 and rounded to nearest even e4m3, packed low byte first: mx_pack4 with the factor itself,
+// which is subnormal for scales of 2^127
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d, float inv) {
+  auto cl = [](float x) { return fminf(fmaxf(x, -448.0f), 448.0f); };
+  const int w = __builtin_amdgcn_cvt_pk_fp8_f32(cl(a * inv), cl(b * inv), 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(cl(c * inv), cl(d * inv), w, true);
+}
+
 // codes of four bytes times f (a power of two <= 1), rounded to nearest even; NaN stays NaN
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float f) {
   const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
@@ -341,7 +349,8 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(t2w_kv8_append_args a, 
         shift = max(e - was, 0);
         e = max(e, was);
       }
-      e = min(max(e, -126), 126);
+      // a block that was filled elsewhere may have the scale 2^127, or an E8M0 NaN (128 here): it keeps it
+      const float inv = __builtin_amdgcn_ldexpf(1.f, -e);
       const float f = shift < 126 ? __uint_as_float((uint32_t)(127 - shift) << 23) : 0.f;
       if (lane == 0) *exps = (uint8_t)(e + 127);
       if (!is_v) {
@@ -355,8 +364,8 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(t2w_kv8_append_args a, 
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const uint4 u = xk[n][h];
-              r[2 * h] = mx_pack4(lo16<BF>(u.x), hi16<BF>(u.x), lo16<BF>(u.y), hi16<BF>(u.y), e);
-              r[2 * h + 1] = mx_pack4(lo16<BF>(u.z), hi16<BF>(u.z), lo16<BF>(u.w), hi16<BF>(u.w), e);
+              r[2 * h] = pack4(lo16<BF>(u.x), hi16<BF>(u.x), lo16<BF>(u.y), hi16<BF>(u.y), inv);
+              r[2 * h + 1] = pack4(lo16<BF>(u.z), hi16<BF>(u.z), lo16<BF>(u.w), hi16<BF>(u.w), inv);
             }
             o = make_uint4(r[0], r[1], r[2], r[3]);
             if ((bad >> t) & 1u) o = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
@@ -379,8 +388,8 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(t2w_kv8_append_args a, 
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t* x = xv + gg * 8 + 4 * h;
-            r[h] = mx_pack4(lo16<BF>(x[0]), lo16<BF>(x[1]), lo16<BF>(x[2]), lo16<BF>(x[3]), e);
-            r[2 + h] = mx_pack4(hi16<BF>(x[0]), hi16<BF>(x[1]), hi16<BF>(x[2]), hi16<BF>(x[3]), e);
+            r[h] = pack4(lo16<BF>(x[0]), lo16<BF>(x[1]), lo16<BF>(x[2]), lo16<BF>(x[3]), inv);
+            r[2 + h] = pack4(hi16<BF>(x[0]), hi16<BF>(x[1]), hi16<BF>(x[2]), hi16<BF>(x[3]), inv);
           }
           if (!fresh) {  // the group's other places keep what they hold; its old tokens at the new scale
             const uint4 u = dst[g * (D / 2)];

@@ -247,6 +247,32 @@ def test_append_rows_of_a_larger_call(dev, first):
     for name, a, b in zip(("k", "v", "k_exp", "v_exp"), host(pages), want):
         assert np.array_equal(a, b), name
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_append_to_blocks_of_foreign_scales(dev, d, dt):
+    """Blocks filled elsewhere, of the scales 2^127 (byte 254), 2^-127 (0) and 2^-126 (1), go on with them or with what the new tokens
+    need; one of an E8M0 NaN stays NaN."""
+    old, new = [9, 9, 9, 9, 30], [3, 3, 3, 3, 9]
+    totals = [a + b for a, b in zip(old, new)]
+    table, nb = random_table(totals, 0, seed=1)
+    k, v = new_kv(sum(new), 2, d, dt, seed=3)
+    k[0], v[1] = torch.finfo(dt).max, torch.finfo(dt).max
+    k[3:6] *= 0
+    for heads in (slice(0, 2), slice(1, 2)):
+        pages = random_pages(nb, 2, d, seed=2)
+        for r, e in ((0, 254), (1, 0), (2, 1)):
+            pages.k_exp[int(table[r, 0]), heads], pages.v_exp[int(table[r, 0]), heads] = e, e
+        check_append(pages, k, v, table, new, totals)
+    pages = random_pages(nb, 2, d, seed=2)
+    pages.k_exp[int(table[3, 0]), 1] = 255
+    want = host(pages)
+    ok.append(*want, k.double().cpu().numpy(), v.double().cpu().numpy(), table, starts(new), totals)
+    kv8.append(pages, k, v, torch.from_numpy(table).cuda(), ints(starts(new)), ints(totals))
+    for i, (a, b) in enumerate(zip(host(pages), want)):
+        if i == 0:  # codes under a scale of NaN stand for nothing
+            a[int(table[3, 0]), 1] = b[int(table[3, 0]), 1] = 0
+        assert np.array_equal(a, b)
+
 
 # --- attention ------------------------------------------------------------------------------------------------------------
 
