@@ -34,6 +34,11 @@ _I32 = torch.int32
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 
 
+def _small(what: str, n: int) -> None:
+    if n > 0x7FFFFFFF:  # the struct's ints would wrap
+        raise ValueError(f"kv8: {what} beyond 2^31 - 1")
+
+
 class KV8Pages:
     """The cache's memory: ``k`` uint8 [n_blocks, kv_heads, head_dim / 16, 32, 16] (chunk of 16 channels, token, channel),
     ``v`` uint8 [n_blocks, kv_heads, 4, head_dim / 2, 2, 8] (8-token group, channel pair, channel, token), both e4m3 codes, and
@@ -52,6 +57,7 @@ class KV8Pages:
         for t in (k, v, k_exp, v_exp):
             if t.dtype != torch.uint8 or not t.is_contiguous() or t.device != dev:
                 raise ValueError("kv8 pages: contiguous uint8 tensors on one device")
+        _small("n_blocks or kv_heads", max(nb, g))
         self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
         self.n_blocks, self.kv_heads, self.head_dim, self.device = nb, g, d, dev
         self.struct = _lib.KV8Pages(k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), nb, g, d)
@@ -95,7 +101,9 @@ def _table(t: torch.Tensor, rows: int, dev) -> tuple[int, int, int]:
     ld, one = t.stride()
     if n != rows or width < 1 or (one != 1 and width > 1):
         raise ValueError(f"kv8: the table must have {rows} rows, each contiguous")
-    return t.data_ptr(), width, ld if rows > 1 else width
+    ld = ld if rows > 1 else width
+    _small("the table's width or row stride", max(width, ld))
+    return t.data_ptr(), width, ld
 
 
 def _tokens(what: str, t: torch.Tensor, n, d: int, dev) -> int:
@@ -109,11 +117,6 @@ def _tokens(what: str, t: torch.Tensor, n, d: int, dev) -> int:
     if n is not None and rows != n:
         raise ValueError(f"kv8: {what} must have {n} tokens")
     return ld if rows > 1 else heads * d
-
-
-def _small(what: str, n: int) -> None:
-    if n > 0x7FFFFFFF:  # the struct's ints would wrap
-        raise ValueError(f"kv8: {what} beyond 2^31 - 1")
 
 
 def _call(fn, args, dev, what: str) -> None:
@@ -139,6 +142,7 @@ class KV8Plan:
     def __init__(self, n_rows: int, n_tok: int, device="cuda"):
         if not 0 <= n_rows <= MAX_ROWS or n_tok < 0:
             raise ValueError(f"kv8 plan: 0 to {MAX_ROWS} rows, n_tok not negative")
+        _small("n_tok", n_tok)
         self.n_rows, self.n_tok = int(n_rows), int(n_tok)
         sizes = (n_rows, n_rows + 1, n_tok, n_tok, n_tok, 1, 1)
         first = [0]
@@ -160,6 +164,7 @@ class KV8Plan:
         a, dev = self._args, self.device
         a.kv_len, a.new_len = _ints("kv_len", kv_len, self.n_rows, dev), _ints("new_len", new_len, self.n_rows, dev)
         a.table, a.width, a.ld_table = _table(table, self.n_rows, dev)
+        _small("free_ids", free_ids.shape[0])
         a.n_free = free_ids.shape[0]
         a.free_ids = _ints("free_ids", free_ids, a.n_free, dev)
         a.free_head = _ints("free_head", free_head, 1, dev)
@@ -179,7 +184,7 @@ def append(pages: KV8Pages, k: torch.Tensor, v: torch.Tensor, table: torch.Tenso
     a joint projection), into their rows' blocks.  ``max_new``: the longest row's new tokens if known (sizes the grid)."""
     dev, d, rows = pages.device, pages.head_dim, kv_total.shape[0]
     ldk, ldv = _tokens("k", k, None, d, dev), _tokens("v", v, k.shape[0], d, dev)
-    _small("max_new", max_new)
+    _small("n_tok or max_new", max(k.shape[0], max_new))
     if k.dtype != v.dtype or k.shape[1] != pages.kv_heads or v.shape[1] != pages.kv_heads:
         raise ValueError(f"kv8 append: k and v of one type with {pages.kv_heads} heads")
     a = _lib.KV8AppendArgs(pages.struct, k.data_ptr(), v.data_ptr(), ldk, ldv, _DTYPES[k.dtype], k.shape[0], *_table(table, rows, dev),
@@ -196,7 +201,7 @@ def attention(q: torch.Tensor, pages: KV8Pages, table: torch.Tensor, row_start: 
     of more than ``max_new`` may get NaN).  ``out`` may be ``q``; its rows behind the last token are left as they were."""
     dev, d, rows = pages.device, pages.head_dim, kv_total.shape[0]
     ldq = _tokens("q", q, None, d, dev)
-    _small("chunk, max_new or max_kv", max(chunk, max_new, max_kv))
+    _small("n_tok, chunk, max_new or max_kv", max(q.shape[0], chunk, max_new, max_kv))
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         ldo = q.shape[1] * d

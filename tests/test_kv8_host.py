@@ -219,3 +219,25 @@ def test_steps_without_bounds_take_no_prompt_tiles():
 def test_a_chunk_among_resting_rows_is_split(rows):
     """256 tokens of one row over a long cache: the tile form in parts, its 256 parts of 256 packed rows, however many rows rest."""
     assert workspace(256, rows, 600, max_new=256, max_kv=16756) == 65536 * (128 + 2) * 4
+
+def test_counts_beyond_32_bits_are_refused():
+    """Sizes that the C structs' ints cannot hold: refused, not wrapped (tensors without memory stand for the large ones)."""
+    big, dev = (1 << 32) + 4, torch.device("meta")
+    m = lambda *s, dtype=torch.int32: torch.empty(s, dtype=dtype, device="meta")  # noqa: E731
+    with pytest.raises(ValueError, match="2\\^31"):
+        kv8.KV8Plan(4, 1 << 31, device="meta")
+    p = kv8.KV8Pages(m(4, 2, 4, 32, 16, dtype=torch.uint8), m(4, 2, 4, 32, 2, 8, dtype=torch.uint8), m(4, 2, dtype=torch.uint8), m(4, 2, dtype=torch.uint8))
+    plan = kv8.KV8Plan(2, 8, device="meta")
+    with pytest.raises(ValueError, match="2\\^31"):
+        plan.build(m(2), m(2), m(2, 3), m(big), m(1))
+    for table in (m(2, big), m(2, big)[:, :3]):
+        with pytest.raises(ValueError, match="2\\^31"):
+            plan.build(m(2), m(2), table, m(8), m(1))
+    x = m(big, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="2\\^31"):
+        kv8.append(p, x, x, m(2, 3), m(3), m(2))
+    with pytest.raises(ValueError, match="2\\^31"):
+        kv8.attention(x, p, m(2, 3), m(3), m(2), scale=0.1)
+    with pytest.raises(ValueError, match="2\\^31"):
+        kv8.KV8Pages(m(big, 2, 4, 32, 16, dtype=torch.uint8), m(big, 2, 4, 32, 2, 8, dtype=torch.uint8), m(big, 2, dtype=torch.uint8), m(big, 2, dtype=torch.uint8))
+    assert dev == plan.device
