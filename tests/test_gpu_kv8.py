@@ -846,6 +846,65 @@ def test_attention_nan_scales(dev, new, old, h, g, d, rows, keys):
     k, v = pages.values([int(table[0, b])])
     assert (k if keys else v)[0, 1].isnan().all() and torch.isfinite((v if keys else k)[0]).all() and torch.isfinite(k[0, 0]).all()
 
+def tile_parts_workspace():
+    """What a call of the tile form in parts asks for (256 parts of 256 packed rows): no other form asks for as much."""
+    return 256 * 256 * (128 + 2) * 4
+
+
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("G,g,rows,new,old", [(16, 8, 7, 32, 4100), (8, 8, 7, 63, 4100), (4, 8, 7, 127, 4100), (2, 8, 4, 250, 8200), (1, 32, 1, 250, 35000)])
+def test_attention_tile_form_of_every_group(dev, dt, G, g, rows, new, old):
+    """Groups of 16, 8, 4, 2 and 1 query heads in the tile form, its key lists in parts (the last one's of more than 128 blocks); the
+    size of the workspace says that the form was taken."""
+    import ctypes
+    from t2w_amd import _lib
+    totals = [old + new - 40 * r for r in range(rows)]
+    table, nb = random_table(totals, 0, seed=G)
+    pages = random_pages(nb, g, 128, seed=new)
+    q = queries(rows * new, G * g, 128, dt, seed=g)
+    a = _lib.KV8AttentionArgs(pages.struct, 1 << 20, 1 << 20, G * g * 128, G * g * 128, 0, rows * new, G * g, 1 << 20, table.shape[1], table.shape[1], 1 << 20,
+                              1 << 20, rows, 1, 0.1, new, max(totals))
+    assert _lib.lib().t2w_kv8_attention_workspace_bytes(ctypes.byref(a)) == tile_parts_workspace()
+    check_attention(q, pages, table, [new] * rows, totals, 1, max_new=new, max_kv=max(totals))
+
+
+@pytest.mark.parametrize("new,h,g,d", [(2, 4, 2, 64), (20, 4, 2, 128), (40, 2, 2, 128), (300, 2, 2, 128)])
+def test_attention_rows_beyond_the_bound(dev, new, h, g, d):
+    """A row of more new tokens than max_new says: NaN, or right; the others are right."""
+    totals = [new + 100, 90, new + 7]
+    table, nb = random_table(totals, 0, seed=1)
+    pages = random_pages(nb, g, d, seed=5)
+    q = queries(2 * new + 1, h, d, BF, seed=6)
+    k, v = scaled(pages)
+    new_l = [new, 1, new]
+    o, mag, top = ok.attention(q.double().cpu().numpy(), k, v, table, starts(new_l), totals, d ** -0.5, 1)
+    bound = attn_bound(o, mag, top, d, BF)
+    for most in (1, max(1, new // 2), new - 1):
+        out = kv8.attention(q, pages, torch.from_numpy(table).cuda(), ints(starts(new_l)), ints(totals), scale=d ** -0.5, chunk=1, max_new=most, max_kv=50)
+        got = out.double().cpu().numpy()
+        right = np.abs(got - o) <= bound
+        for a, b in zip(starts(new_l), starts(new_l)[1:]):
+            assert right[a:b].all() or (b - a > most and np.isnan(got[a:b]).all())
+
+
+@pytest.mark.parametrize("h,g,d,rows,most,first", [(4, 2, 64, 75, 40, 1), (4, 2, 64, 75, 40, 70), (8, 1, 128, 20, 1, 7), (64, 32, 128, 10, 101, 3), (64, 32, 128, 75, 60, 60)])
+@pytest.mark.parametrize("bounds", [False, True])
+def test_attention_rows_of_a_larger_call(dev, h, g, d, rows, most, first, bounds):
+    """The last rows of a call by slices of its tables; the tokens before them are left alone."""
+    new = [(most, 1, 0, most // 2 + 1, most)[r % 5] for r in range(rows)]
+    totals = [n + (0, 33, 70, 5)[r % 4] for r, n in enumerate(new)]
+    table, nb = random_table(totals, 1, seed=rows)
+    pages = random_pages(nb, g, d, seed=5)
+    q = queries(sum(new), h, d, BF, seed=6)
+    k, v = scaled(pages)
+    o, mag, top = ok.attention(q.double().cpu().numpy(), k, v, table, starts(new), totals, d ** -0.5, 1)
+    out = torch.full_like(q, 5)
+    kw = {"max_new": most, "max_kv": max(totals)} if bounds else {}
+    kv8.attention(q, pages, torch.from_numpy(table).cuda()[first:], ints(starts(new))[first:], ints(totals)[first:], scale=d ** -0.5, chunk=1, out=out, **kw)
+    at = starts(new)[first]
+    assert (out[:at] == 5).all()
+    assert (np.abs(out.double().cpu().numpy() - o) <= attn_bound(o, mag, top, d, BF))[at:].all()
+
 
 # --- a run of them ----------------------------------------------------------------------------------------------------------
 
