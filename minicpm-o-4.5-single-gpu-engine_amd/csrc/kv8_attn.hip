@@ -453,7 +453,7 @@ struct State {
 // where a copy reaches 5.14 and reads alone 5.87).  One register set a block: the next block's keys load as soon as the
 // scores have used these, its values after P . V; two sets spilled and took 221 us.  MR = 16 (16x16x32 MFMA) has half the
 // softmax work of MR = 32 (32x32x16) where rows allow it.  Heads of 64 run four workgroups a CU, so that 1,024 workgroups of
-// windows are all resident (64 rows of 50 tokens over 370 keys: 16.5 us; three a CU 19.7).
+// windows are all resident (64 rows of 50 tokens over 370 keys: 17.2 us; 16.5 against 19.7 with three a CU when both were built).
 //
 // With S^T = K . Q^T the score MFMA leaves a lane scores of its own query only; the rows of K are fed in an order that makes
 // them the 8 (MR = 16) or 2 x 8 keys whose value bytes the same lane loads as the P . V operand:
@@ -608,10 +608,10 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
 //
 // A 32x32x16 MFMA keeps the matrix unit for 32 cycles and the vector issue port for 16: four vector instructions behind each
 // are free.  So a block's exponentials run between the next block's score MFMAs, and the conversion and the next maximum
-// between the value MFMAs.  2,048 tokens over 32,000 (32 heads over 8 of 128, fp16, causal): 1,070 us, 1.03 PFLOP/s against
-// 1.17 of a large library product on the same card; 45% of the cycles on the matrix unit, 43% issuing vector instructions,
-// the LDS reads (16 KB a wave and block) about half.  Without the interleaving 1,190 us; sums on the matrix unit 1,115; four
-// waves and two workgroups a CU 1,174 against 1,096 in the same run.
+// between the value MFMAs.  2,048 tokens over 32,000 (32 heads over 8 of 128, fp16, causal): 1,106 us, 1.00 PFLOP/s against
+// 1.17 of a large library product on the same card; 44% of the cycles on the matrix unit, 42% issuing vector instructions,
+// the LDS reads (16 KB a wave and block) about half.  Without the interleaving 1,190 us against 1,115 then; four waves and two
+// workgroups a CU 1,174 against 1,096 in the same run.
 template <bool BF, int D, int RW>
 __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_attention_args a, KV8Split sp) {
   typedef State<32, D> St;
@@ -834,8 +834,8 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
   if (mrow < t.rows) st.template store<BF>(a, sp, t, kv_head, part, parts, mrow, g);
 }
 
-// Joins the parts of split tiles, WR waves to a packed row (4 where a row has many parts): each wave sums its share of them,
-// a lane D / 64 channels.
+// Joins the parts of split tiles, WR waves to a packed row: each wave sums its share of them, a lane D / 64 channels.  Four
+// waves where a row has more than 8 parts: 47 parts 24.9 us a call, 32.7 with one wave; 4 parts 21.2 and 20.7.
 template <bool BF, int D, int WR>
 __global__ void __launch_bounds__(256) kv8_join_kernel(t2w_kv8_attention_args a, KV8Split sp) {
   constexpr int NV = D / 64;
@@ -909,7 +909,8 @@ Choice choose(const t2w_kv8_attention_args& a) {
   // whose 256-row tiles (and parts) fill the chip, one workgroup a CU, and are mostly full: 32 heads over 8 (us, direct /
   // tile): one row of 8,000 tokens 625 / 550, 2,048 behind 32,000 1,250 / 1,095, four of 500 30.7 / 27.8; a row of 1,000
   // tokens alone (128 workgroups) 24.7 / 37.8, 32 of 70 behind 2,000 (tiles 55% full) 130 / 161.  With heads of 64 the
-  // direct form was the faster one everywhere (128-row tiles: 1,000 tokens 14.8 / 24.6, 8,000 202 / 214).
+  // direct form was the faster one of those tried (tiles of 128 rows, four waves: 1,000 tokens of 16 heads 14.8 / 24.6, 8,000
+  // 202 / 214).
   c.mr = packed <= 16 ? 16 : 32;
   c.rw = packed <= 32 ? 1 : 2;
   c.tile = false;

@@ -8,9 +8,11 @@ host, so that one captured graph serves steps of any lengths::
     pages = KV8Pages.empty(n_blocks, kv_heads, head_dim)
     plan = KV8Plan(rows, n_tok)                                       # buffers, made once
     plan.build(kv_len, new_len, table, free_ids, free_head)           # block tables and slot maps
-    append(pages, k, v, table, plan.row_start, plan.kv_total)
-    out = attention(q, pages, table, plan.row_start, plan.kv_total, scale=head_dim ** -0.5, chunk=1)
+    append(pages, k, v, table, plan.row_start, plan.kv_total, max_new=longest)
+    out = attention(q, pages, table, plan.row_start, plan.kv_total, scale=head_dim ** -0.5, chunk=1, max_new=longest, max_kv=bound)
 
+``longest`` and ``bound`` are what the host knows of the rows' new and total tokens, 0 for nothing: they pick the kernel and its
+split (a step of single tokens whose ``max_new`` is not said runs on tiles made for more).
 The next step's ``kv_len`` and ``free_head`` are ``plan.kv_total`` and ``plan.free_head``; a plan's outputs must not be its own
 inputs, so a loop alternates two plans or copies them.  Lengths, tables and ids are int32 tensors on the GPU.  No gradients
 flow through these calls.
@@ -198,7 +200,8 @@ def attention(q: torch.Tensor, pages: KV8Pages, table: torch.Tensor, row_start: 
     """softmax(scale q K^T) V of every new token ``q`` [n_tok, heads, head_dim] over its row's cache; ``heads`` is 1 to 16 times
     the pages' heads.  ``chunk``: 0 a token sees all of its row, c > 0 the row's earlier tokens and the new ones of its own and
     earlier chunks of c (1: causal).  ``max_new`` / ``max_kv``: bounds on the rows' new and total tokens, 0 unknown (a row
-    of more than ``max_new`` may get NaN).  ``out`` may be ``q``; its rows behind the last token are left as they were."""
+    of more than ``max_new`` may get NaN).  ``out`` may be ``q``; its rows behind the last token are left as they were, all of
+    them after a plan that could not be served (an ``out`` made here is then uninitialised)."""
     dev, d, rows = pages.device, pages.head_dim, kv_total.shape[0]
     ldq = _tokens("q", q, None, d, dev)
     _small("n_tok, chunk, max_new or max_kv", max(q.shape[0], chunk, max_new, max_kv))
