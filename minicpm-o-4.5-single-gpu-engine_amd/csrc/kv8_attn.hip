@@ -283,6 +283,7 @@ struct State {
 #pragma unroll
       for (int r = 0; r < AR; ++r) sc[x][r] = key0 + key_of(x, r, g) < lim ? (off ? __builtin_nanf("") : sc[x][r]) : -__builtin_inff();
   }
+  // (Branches that few blocks take are marked unlikely, out of the loops' way: 1,106 -> 1,095 us on the long chunk.)
   // Moves the reference where a block's scores, in units 1 / c and -inf where invisible, of maximum mx, pass it.  Where |m| is
   // large, s - m + 7 in one fma is not what the scores' own rounding allows: 7 - m rounds too, and a score of m + 8 could reach
   // 2^16, infinite in fp16.  There s is rounded first, as mx was, and s - m is exact where it counts; nothing may be contracted.
@@ -291,7 +292,7 @@ struct State {
 #pragma clang fp contract(off)
     mx *= c;
     // one comparison for both: some maximum passes the reference by 8, or the unit rises (then every lane's does)
-    if (__builtin_amdgcn_ballot_w64(fmaxf(mx - m, -1.f) > (e > E ? -2.f : 8.f))) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(fmaxf(mx - m, -1.f) > (e > E ? -2.f : 8.f)) != 0, 0)) {
       nb = e == WIDE && !wide ? -(float)E : nb;
       wide = wide || e == WIDE;
       const bool up = !wide && e > E;
@@ -312,7 +313,7 @@ struct State {
       l *= alpha;
       scale_o(f);
     }
-    if (slow) {
+    if (__builtin_expect(slow, 0)) {
       const float m0 = m == -__builtin_inff() ? 0.f : m, add = wide ? (float)vx : 0.f;
       const bool own = large(m0);
 #pragma unroll
@@ -453,7 +454,7 @@ struct State {
 // where a copy reaches 5.14 and reads alone 5.87).  One register set a block: the next block's keys load as soon as the
 // scores have used these, its values after P . V; two sets spilled and took 221 us.  MR = 16 (16x16x32 MFMA) has half the
 // softmax work of MR = 32 (32x32x16) where rows allow it.  Heads of 64 run four workgroups a CU, so that 1,024 workgroups of
-// windows are all resident (64 rows of 50 tokens over 370 keys: 17.2 us; 16.5 against 19.7 with three a CU when both were built).
+// windows are all resident (64 rows of 50 tokens over 370 keys: 17.1 us; 16.5 against 19.7 with three a CU when both were built).
 //
 // With S^T = K . Q^T the score MFMA leaves a lane scores of its own query only; the rows of K are fed in an order that makes
 // them the 8 (MR = 16) or 2 x 8 keys whose value bytes the same lane loads as the P . V operand:
@@ -556,8 +557,8 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
         const bool off = kx > 254;  // a block id outside the pages, or an E8M0 NaN
         const int ex = sp.ce + kx - 127;
         float c = __builtin_amdgcn_ldexpf(sp.cm, ex);
-        if (max(key0 + KV8_BLOCK - lim_lo, kx - 254) > 0) St::mask(sc, off, key0, lim, g);  // or some query of the wave does not see all of the block
-        if (abs(ex) > St::NORMAL) {
+        if (__builtin_expect(max(key0 + KV8_BLOCK - lim_lo, kx - 254) > 0, 0)) St::mask(sc, off, key0, lim, g);  // or some query of the wave does not see all of the block
+        if (__builtin_expect(abs(ex) > St::NORMAL, 0)) {
           St::scale_scores(sc, sp.cm, ex);
           c = 1.f;
         }
@@ -608,7 +609,7 @@ __global__ void __launch_bounds__(256, OCC) kv8_attn_direct_kernel(t2w_kv8_atten
 //
 // A 32x32x16 MFMA keeps the matrix unit for 32 cycles and the vector issue port for 16: four vector instructions behind each
 // are free.  So a block's exponentials run between the next block's score MFMAs, and the conversion and the next maximum
-// between the value MFMAs.  2,048 tokens over 32,000 (32 heads over 8 of 128, fp16, causal): 1,106 us, 1.00 PFLOP/s against
+// between the value MFMAs.  2,048 tokens over 32,000 (32 heads over 8 of 128, fp16, causal): 1,094 us, 1.01 PFLOP/s against
 // 1.17 of a large library product on the same card; 44% of the cycles on the matrix unit, 42% issuing vector instructions,
 // the LDS reads (16 KB a wave and block) about half.  Without the interleaving 1,190 us against 1,115 then; four waves and two
 // workgroups a CU 1,174 against 1,096 in the same run.
@@ -747,11 +748,11 @@ __global__ void __launch_bounds__(64 * RW, 2) kv8_attn_tile_kernel(t2w_kv8_atten
     read_k(nbuf, ny);
     const int ex = sp.ce + kx - 127;
     float c = __builtin_amdgcn_ldexpf(sp.cm, ex);
-    if (max(key0 + KV8_BLOCK - lim_lo, kx - 254) > 0) {
+    if (__builtin_expect(max(key0 + KV8_BLOCK - lim_lo, kx - 254) > 0, 0)) {
       St::mask(sc, kx > 254, key0, lim, g);
       mx = St::top(sc);
     }
-    if (abs(ex) > St::NORMAL) {
+    if (__builtin_expect(abs(ex) > St::NORMAL, 0)) {
       St::scale_scores(sc, sp.cm, ex);
       c = 1.f;
       mx = St::top(sc);
