@@ -905,6 +905,34 @@ def test_attention_rows_of_a_larger_call(dev, h, g, d, rows, most, first, bounds
     assert (out[:at] == 5).all()
     assert (np.abs(out.double().cpu().numpy() - o) <= attn_bound(o, mag, top, d, BF))[at:].all()
 
+def test_graph_of_a_chunk_among_rows(dev):
+    """One captured call in the tile form in parts serves other lengths: one row with all the tokens, some rows, every row, none;
+    how many tiles there are, and so how many parts, is found at each replay."""
+    rows, n_tok, h, g, d = 9, 256, 32, 8, 128
+    table, nb = random_table([16900] * 2 + [300] * 7, 0, seed=1)
+    pages = random_pages(nb, g, d, seed=2)
+    q = queries(n_tok, h, d, BF, seed=3)
+    dt, start, total = torch.from_numpy(table).cuda(), ints([0] * (rows + 1)), ints([0] * rows)
+    out = torch.zeros_like(q)
+    call = lambda: kv8.attention(q, pages, dt, start, total, scale=d ** -0.5, chunk=1, max_new=n_tok, max_kv=16900, out=out)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    k, v = scaled(pages)
+    for new, kv in (([256] + [0] * 8, [16900, 5, 0, 0, 9, 0, 0, 0, 0]), ([100, 90, 0, 1, 30, 0, 20, 0, 15], [16900, 16000, 7, 300, 200, 0, 290, 0, 15]),
+                    ([0] * 9, [0] * 9), ([28] * 9, [16900, 16900] + [300 - 30 * r for r in range(7)]), ([0, 200] + [0] * 7, [100, 16500] + [0] * 7)):
+        start.copy_(ints(starts(new)))
+        total.copy_(ints(kv))
+        out.fill_(5)
+        graph.replay()
+        torch.cuda.synchronize()
+        n = sum(new)
+        o, mag, top = ok.attention(q.double().cpu().numpy(), k, v, table, starts(new), kv, d ** -0.5, 1)
+        bound = attn_bound(o, mag, top, d, BF)
+        assert (np.abs(out.double().cpu().numpy() - o) <= bound)[:n].all() and (out[n:] == 5).all()
+
 
 # --- a run of them ----------------------------------------------------------------------------------------------------------
 
