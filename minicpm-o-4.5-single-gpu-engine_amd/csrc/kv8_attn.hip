@@ -79,7 +79,7 @@ __device__ __forceinline__ bool find_tile(const t2w_kv8_attention_args& a, const
     auto tiles_of = [&](int r) {
       if (r >= a.n_rows) return 0;
       const int start = a.row_start[r], stop = a.row_start[r + 1];
-      return stop > start ? min((stop - start - 1) / s.tt + 1, 1 << 18) : 0;  // 2^24 tokens, tiles of 16 or more: 2^20 + 4,096 in all
+      return stop > start ? min((stop - start - 1) / s.tt + 1, 1 << 18) : 0;  // at most 128 where starts are well formed: no sum wraps
     };
     int mine = 0;
     for (int i = 0; i < step; ++i) mine += tiles_of(lane * step + i);
