@@ -397,6 +397,110 @@ typedef struct {
 size_t t2w_kv8_attention_workspace_bytes(const t2w_kv8_attention_args* a);
 int t2w_kv8_attention(const t2w_kv8_attention_args* a, void* stream);
 
+/* ---------------------------------------------------------------- products with 4-bit weights
+ * Linear layers and gated feed-forward blocks on OCP MXFP4 weights: e2m1 codes (a sign and 0, 0.5, 1, 1.5, 2, 3, 4 or 6) with a
+ * power-of-two scale for every 32 consecutive input columns (E8M0: exponent + 127): 4.25 bits a weight.  With the paged 8-bit cache
+ * and t2w_rope they make up a decoder layer.  No counterpart in the reference, whose own reduced weights are e4m3
+ * (engine/runtime/fp8.py:15-37).
+ *
+ * A matrix is laid out once, by t2w_mx4_pack from codes or by t2w_mx4_quantize from 16- or 32-bit weights, into memory of
+ * t2w_mx4_codes_bytes and t2w_mx4_scales_bytes (the kernels' operand order).  Scales are limited to 2^-23 .. 2^13, where every
+ * weight is exact in bf16 and fp16; a group whose codes are all zero may have any. */
+
+enum { T2W_MX4_BF16 = 0, T2W_MX4_FP16 = 1, T2W_MX4_FP32 = 2 };
+enum { T2W_MX4_SILU = 0, T2W_MX4_GELU = 1 }; /* GELU in its tanh form */
+
+typedef struct {
+  const void* codes; const void* scales; /* as laid out, 16- and 4-byte aligned */
+  int n, k;                              /* output channels (1 to 2^24), input columns (a multiple of 8, 8 to 2^20) */
+} t2w_mx4_weight;
+size_t t2w_mx4_codes_bytes(int n, int k); /* 0: no such size */
+size_t t2w_mx4_scales_bytes(int n, int k);
+
+/* codes [n, k / 2], the even column in a byte's lower nibble (4-byte aligned); scales [n, ceil(k / 32)].  *status, which the
+ * caller clears, gets bit 0 where a scale is out of range: the matrix is then not to be used. */
+typedef struct {
+  const void* codes; const void* scales;
+  int n, k;
+  void* w_codes; void* w_scales;
+  int* status;
+} t2w_mx4_pack_args;
+int t2w_mx4_pack(const t2w_mx4_pack_args* a, void* stream);
+
+/* w [n, k], rows ldw elements apart (bf16, fp16 or fp32).  A group's scale is the smallest power of two, 2^-23 or more, that
+ * keeps its largest magnitude within 6; codes are rounded to nearest, ties to even.  *status, which the caller clears, gets bit 1
+ * where a weight is not finite or beyond 49152 (its group is then zero). */
+typedef struct {
+  const void* w; long long ldw;
+  int dtype, n, k;
+  void* w_codes; void* w_scales;
+  int* status;
+} t2w_mx4_quantize_args;
+int t2w_mx4_quantize(const t2w_mx4_quantize_args* a, void* stream);
+
+/* y = x W^T + bias + residual.  x [m, k] and y [m, n] in one type, bf16 or fp16, rows ldx / ldy elements apart; x is 16-byte
+ * aligned and ldx a multiple of 8, y and the residual [m, n] (ldr; optional) need no more than their elements' alignment (8 bytes
+ * and strides of 4 are faster).  bias [n] fp32, optional.  Sums are fp32, the output is rounded once.  y may be the residual
+ * itself (same rows), and overlaps no operand otherwise.  m is at most 2^21. */
+typedef struct {
+  const void* x; long long ldx;
+  int dtype, m;
+  t2w_mx4_weight w;
+  const float* bias;
+  const void* residual; long long ldr;
+  void* y; long long ldy;
+} t2w_mx4_linear_args;
+int t2w_mx4_linear(const t2w_mx4_linear_args* a, void* stream);
+
+/* y = act(x gate^T) * (x up^T), one kernel; gate and up have the same sizes [n, k].  The rest as in t2w_mx4_linear. */
+typedef struct {
+  const void* x; long long ldx;
+  int dtype, m;
+  t2w_mx4_weight gate, up;
+  int act;
+  void* y; long long ldy;
+} t2w_mx4_gated_args;
+int t2w_mx4_gated(const t2w_mx4_gated_args* a, void* stream);
+
+/* y = (act(x gate^T) * (x up^T)) down^T + residual: gate, up [f, k], down [n, f].  The inner values are rounded to x's type (they
+ * are the second product's operand): of fp16, beyond 65504 they are infinite. */
+typedef struct {
+  const void* x; long long ldx;
+  int dtype, m;
+  t2w_mx4_weight gate, up, down;
+  int act;
+  const void* residual; long long ldr;
+  void* y; long long ldy;
+  void* workspace; size_t workspace_bytes; /* t2w_mx4_ffn_workspace_bytes of the same arguments, 16-byte aligned; nothing in it needs
+                                            * clearing or outlives the call, and calls that may overlap need one each */
+} t2w_mx4_ffn_args;
+size_t t2w_mx4_ffn_workspace_bytes(const t2w_mx4_ffn_args* a);
+int t2w_mx4_ffn(const t2w_mx4_ffn_args* a, void* stream);
+
+/* ---------------------------------------------------------------- rotary positions of several axes
+ * Queries and keys [n_tok, heads, head_dim] (token rows ld* elements apart, a token's heads side by side): pair p of a head's
+ * first `rot` channels turns by pos[axis[p] * ld_pos + token] * inv_freq[p]:
+ *   y0 = scale (x0 cos - x1 sin), y1 = scale (x0 sin + x1 cos)
+ * where (x0, x1) are channels (p, p + rot / 2) (T2W_ROPE_HALVES) or (2 p, 2 p + 1) (T2W_ROPE_NEIGHBOURS); channels from `rot` on are
+ * copied.  The axes are whatever the caller counts on them (time, height, width).  freq[p] is inv_freq[p] / (2 pi) turns in units of
+ * 2^-64, wrapped: angles are exact to 2^-32 turns at every int position.  No counterpart in the reference's path (its DiT has no
+ * positional encoding; t2w_dit_globals.rope_freq is this library's one-axis option there). */
+
+enum { T2W_ROPE_BF16 = 0, T2W_ROPE_FP16 = 1 };
+enum { T2W_ROPE_HALVES = 0, T2W_ROPE_NEIGHBOURS = 1 };
+
+typedef struct {
+  const void* q; const void* k;   /* either may have no heads */
+  void* q_out; void* k_out;       /* may be q and k themselves (same strides); overlap nothing otherwise */
+  long long ldq, ldk, ldq_out, ldk_out; /* multiples of 8; all four 16-byte aligned */
+  int dtype, n_tok, q_heads, k_heads, head_dim, rot, pairs; /* head_dim a multiple of 8, rot of 16 */
+  const uint64_t* freq;           /* [rot / 2] */
+  const uint8_t* axis;            /* [rot / 2], each below n_axes */
+  const int* pos; long long ld_pos; int n_axes; /* [n_axes, n_tok], rows ld_pos apart; up to 16 axes */
+  float scale;
+} t2w_rope_args;
+int t2w_rope(const t2w_rope_args* a, void* stream);
+
 /* ---------------------------------------------------------------- HiFT vocoder (fp32) */
 
 typedef struct t2w_hift t2w_hift;

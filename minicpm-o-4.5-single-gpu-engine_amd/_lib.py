@@ -120,6 +120,39 @@ class KV8AttentionArgs(C.Structure):
                 ("scale", F), ("max_new", I), ("max_kv", I), ("workspace", P), ("workspace_bytes", C.c_size_t)]
 
 
+class MX4Weight(C.Structure):
+    _fields_ = [("codes", P), ("scales", P), ("n", I), ("k", I)]
+
+
+class MX4PackArgs(C.Structure):
+    _fields_ = [("codes", P), ("scales", P), ("n", I), ("k", I), ("w_codes", P), ("w_scales", P), ("status", P)]
+
+
+class MX4QuantizeArgs(C.Structure):
+    _fields_ = [("w", P), ("ldw", C.c_longlong), ("dtype", I), ("n", I), ("k", I), ("w_codes", P), ("w_scales", P), ("status", P)]
+
+
+class MX4LinearArgs(C.Structure):
+    _fields_ = [("x", P), ("ldx", C.c_longlong), ("dtype", I), ("m", I), ("w", MX4Weight), ("bias", P), ("residual", P), ("ldr", C.c_longlong),
+                ("y", P), ("ldy", C.c_longlong)]
+
+
+class MX4GatedArgs(C.Structure):
+    _fields_ = [("x", P), ("ldx", C.c_longlong), ("dtype", I), ("m", I), ("gate", MX4Weight), ("up", MX4Weight), ("act", I), ("y", P),
+                ("ldy", C.c_longlong)]
+
+
+class MX4FFNArgs(C.Structure):
+    _fields_ = [("x", P), ("ldx", C.c_longlong), ("dtype", I), ("m", I), ("gate", MX4Weight), ("up", MX4Weight), ("down", MX4Weight), ("act", I),
+                ("residual", P), ("ldr", C.c_longlong), ("y", P), ("ldy", C.c_longlong), ("workspace", P), ("workspace_bytes", C.c_size_t)]
+
+
+class RopeArgs(C.Structure):
+    _fields_ = [(n, P) for n in ("q", "k", "q_out", "k_out")] + [(n, C.c_longlong) for n in ("ldq", "ldk", "ldq_out", "ldk_out")] + \
+               [(n, I) for n in ("dtype", "n_tok", "q_heads", "k_heads", "head_dim", "rot", "pairs")] + \
+               [("freq", P), ("axis", P), ("pos", P), ("ld_pos", C.c_longlong), ("n_axes", I), ("scale", F)]
+
+
 _SIGS = {
     "t2w_abi_version": (I, []),
     "t2w_last_error": (C.c_char_p, []),
@@ -163,6 +196,15 @@ _SIGS = {
     "t2w_kv8_append": (I, [C.POINTER(KV8AppendArgs), P]),
     "t2w_kv8_attention": (I, [C.POINTER(KV8AttentionArgs), P]),
     "t2w_kv8_attention_workspace_bytes": (C.c_size_t, [C.POINTER(KV8AttentionArgs)]),
+    "t2w_mx4_codes_bytes": (C.c_size_t, [I, I]),
+    "t2w_mx4_scales_bytes": (C.c_size_t, [I, I]),
+    "t2w_mx4_pack": (I, [C.POINTER(MX4PackArgs), P]),
+    "t2w_mx4_quantize": (I, [C.POINTER(MX4QuantizeArgs), P]),
+    "t2w_mx4_linear": (I, [C.POINTER(MX4LinearArgs), P]),
+    "t2w_mx4_gated": (I, [C.POINTER(MX4GatedArgs), P]),
+    "t2w_mx4_ffn": (I, [C.POINTER(MX4FFNArgs), P]),
+    "t2w_mx4_ffn_workspace_bytes": (C.c_size_t, [C.POINTER(MX4FFNArgs)]),
+    "t2w_rope": (I, [C.POINTER(RopeArgs), P]),
     "t2w_device_cus": (I, [C.POINTER(I)]),
     "t2w_stream_create_cu_mask": (I, [C.POINTER(C.c_uint32), I, C.POINTER(P)]),
     "t2w_stream_destroy": (I, [P]),
@@ -193,6 +235,28 @@ def lib():
 def check(rc: int, what: str = "") -> None:
     if rc != 0:
         raise RuntimeError(f"t2w {what}: {lib().t2w_last_error().decode()}")
+
+
+_device_fns = None
+
+
+def launch(fn, args, dev, what: str) -> None:
+    """The library call ``fn(&args, stream)`` on torch's current stream of the tensors' device ``dev``.  The stream comes as torch's
+    raw handle: making a Stream object takes 2 us, a quarter of a short call."""
+    global _device_fns
+    if _device_fns is None:
+        import torch
+
+        _device_fns = (getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device,
+                       getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream), torch.cuda.device)
+    current, raw_stream, device = _device_fns
+    if dev.type != "cuda":
+        raise ValueError(f"{what}: the tensors must be on the GPU")
+    if dev.index == current():
+        check(fn(C.byref(args), raw_stream(dev.index)), what)
+    else:
+        with device(dev):
+            check(fn(C.byref(args), raw_stream(dev.index)), what)
 
 
 TIMER_KINDS = {1: "resid_gemm", 2: "hift_phase", 3: "hift_source", 4: "hift_stft", 5: "hift_istft", 6: "hift_reflect",

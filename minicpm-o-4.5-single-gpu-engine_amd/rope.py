@@ -1,0 +1,107 @@
+"""Rotary positions of several axes for queries and keys (host side of ``t2w_rope``, ``include/t2w.h``): text, images and video.  No
+counterpart in the reference's Token2Wav path, whose DiT has no positional encoding; ``DiTConfig.rope_theta`` is the one-axis
+option there.
+
+A pair of channels turns by the token's position on the pair's axis times the pair's frequency.  Angles are integers: exact at
+every int32 position.  Calls go on the caller's current stream, wait for nothing and can be captured; no gradients flow through
+them::
+
+    rope = Rope([theta ** (-2 * p / d) for p in range(d // 2)], axis=sections(16, 24, 24))   # once, with the model
+    rope.apply(q, k, pos, q_out=q, k_out=k)                                                  # pos int32 [axes, n_tok]
+"""
+
+from __future__ import annotations
+
+import math
+from decimal import Decimal
+from fractions import Fraction
+
+import torch
+
+from . import _lib
+
+_I32 = torch.int32
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_PAIRS = {"halves": 0, "neighbours": 1}
+# an angle's unit is 2^-64 turns, so the circle's number is needed beyond a double
+_TWO_PI = 2 * Fraction(Decimal("3.14159265358979323846264338327950288419716939937510582097494"))
+
+
+def sections(*counts: int) -> list[int]:
+    """Axis of every pair where the first ``counts[0]`` pairs count on axis 0, the next ``counts[1]`` on axis 1 and so on."""
+    return [a for a, n in enumerate(counts) for _ in range(n)]
+
+
+class Rope:
+    """``inv_freq``: a frequency for every pair, radians a position (numbers; ``theta ** (-2 p / rot)`` in the plain form).  ``axis``: the
+    axis each pair counts on (all on axis 0 by default).  ``pairs``: "halves" pairs channel p with p + rot / 2, "neighbours"
+    2 p with 2 p + 1, where rot = 2 len(inv_freq) is a multiple of 16; a head's further channels keep their values.  ``scale``
+    multiplies the turned channels."""
+
+    __slots__ = ("rot", "n_axes", "pairs", "scale", "device", "_freq", "_axis")
+
+    def __init__(self, inv_freq, axis=None, pairs: str = "halves", scale: float = 1.0, device="cuda"):
+        inv = [float(f) for f in inv_freq]
+        axis = [0] * len(inv) if axis is None else [int(a) for a in axis]
+        if not inv or len(inv) % 8 or not all(map(math.isfinite, inv)):
+            raise ValueError("rope: a multiple of 8 finite frequencies")
+        if len(axis) != len(inv) or min(axis) < 0 or max(axis) > 15:
+            raise ValueError("rope: an axis (0 to 15) for every frequency")
+        if pairs not in _PAIRS:
+            raise ValueError("rope: pairs must be 'halves' or 'neighbours'")
+        if not math.isfinite(scale):
+            raise ValueError("rope: scale must be finite")
+        self.rot, self.n_axes, self.pairs, self.scale = 2 * len(inv), max(axis) + 1, pairs, float(scale)
+        turns = [round(Fraction(f) / _TWO_PI * 2 ** 64) % 2 ** 64 for f in inv]
+        self._freq = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64, device=device)
+        self._axis = torch.tensor(axis, dtype=torch.uint8, device=device)
+        self.device = self._freq.device
+
+    def apply(self, q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, *, q_out: torch.Tensor | None = None,
+              k_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """Turns ``q`` [n_tok, heads, head_dim] and ``k`` [n_tok, kv_heads, head_dim] (or None), bf16 or fp16, token rows strided by
+        multiples of 8.  ``pos`` int32 [axes, n_tok] ([n_tok] for one axis), with at least the axes that the pairs count on.  The
+        outputs, new tensors by default, may be ``q`` and ``k`` themselves."""
+        dev = self.device
+        if q.dtype not in _DTYPES:
+            raise ValueError("rope: q must be bfloat16 or float16")
+        n, heads, d = q.shape if q.dim() == 3 else (0, 0, 0)
+        ldq = _tokens("q", q, n, d, q.dtype, dev)
+        if pos.dim() == 1:
+            pos = pos[None]
+        if pos.dtype is not _I32 or pos.dim() != 2 or pos.shape[1] != n or pos.device != dev or (pos.stride(1) != 1 and n > 1):
+            raise ValueError(f"rope: pos must be int32 [axes, {n}] on {dev}, each row contiguous")
+        if pos.shape[0] < self.n_axes:
+            raise ValueError(f"rope: pos must have the {self.n_axes} axes that the pairs count on")
+        if q_out is None:
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif q_out.shape != q.shape:
+            raise ValueError("rope: q_out must have q's shape")
+        if max(n, heads, d) > 0x7FFFFFFF:  # the struct's ints would wrap
+            raise ValueError("rope: at most 2^24 tokens")
+        a = _lib.RopeArgs(q=q.data_ptr(), q_out=q_out.data_ptr(), ldq=ldq, ldq_out=_tokens("q_out", q_out, n, d, q.dtype, dev), dtype=_DTYPES[q.dtype],
+                          n_tok=n, q_heads=heads, head_dim=d, rot=self.rot, pairs=_PAIRS[self.pairs], freq=self._freq.data_ptr(),
+                          axis=self._axis.data_ptr(), pos=pos.data_ptr(), ld_pos=pos.stride(0) if self.n_axes > 1 else n, n_axes=self.n_axes, scale=self.scale)
+        if k is not None:
+            a.ldk = _tokens("k", k, n, d, q.dtype, dev)
+            if k_out is None:
+                k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+            elif k_out.shape != k.shape:
+                raise ValueError("rope: k_out must have k's shape")
+            a.ldk_out = _tokens("k_out", k_out, n, d, q.dtype, dev)
+            a.k, a.k_out, a.k_heads = k.data_ptr(), k_out.data_ptr(), k.shape[1]
+        elif k_out is not None:
+            raise ValueError("rope: k_out without k")
+        _lib.launch(_lib.lib().t2w_rope, a, dev, "rope")
+        return q_out, k_out
+
+
+def _tokens(what: str, t: torch.Tensor, n: int, d: int, dtype, dev) -> int:
+    """Elements between the token rows of [n_tok, heads, head_dim] (a token's heads lie side by side)."""
+    if t.dim() != 3 or t.dtype is not dtype or t.device != dev:
+        raise ValueError(f"rope: {what} must be {dtype} [n_tok, heads, head_dim] on {dev}")
+    rows, heads, width = t.shape
+    ld, head, one = t.stride()
+    if rows != n or width != d or one != 1 or (head != d and heads > 1):
+        raise ValueError(f"rope: {what} must be [{n}, heads, {d}], a token's heads side by side")
+    return ld if rows > 1 else heads * d
