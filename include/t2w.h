@@ -449,7 +449,11 @@ typedef struct {
   const float* bias;
   const void* residual; long long ldr;
   void* y; long long ldy;
+  void* workspace; size_t workspace_bytes; /* t2w_mx4_linear_workspace_bytes of the same arguments (0 for few rows, at most 34 MB):
+                                            * 16-byte aligned; nothing in it needs clearing or outlives the call, and calls that
+                                            * may overlap need one each */
 } t2w_mx4_linear_args;
+size_t t2w_mx4_linear_workspace_bytes(const t2w_mx4_linear_args* a);
 int t2w_mx4_linear(const t2w_mx4_linear_args* a, void* stream);
 
 /* y = act(x gate^T) * (x up^T), one kernel; gate and up have the same sizes [n, k].  The rest as in t2w_mx4_linear. */
@@ -459,7 +463,9 @@ typedef struct {
   t2w_mx4_weight gate, up;
   int act;
   void* y; long long ldy;
+  void* workspace; size_t workspace_bytes; /* as t2w_mx4_linear's, of t2w_mx4_gated_workspace_bytes */
 } t2w_mx4_gated_args;
+size_t t2w_mx4_gated_workspace_bytes(const t2w_mx4_gated_args* a);
 int t2w_mx4_gated(const t2w_mx4_gated_args* a, void* stream);
 
 /* y = (act(x gate^T) * (x up^T)) down^T + residual: gate, up [f, k], down [n, f].  The inner values are rounded to x's type (they
@@ -471,8 +477,7 @@ typedef struct {
   int act;
   const void* residual; long long ldr;
   void* y; long long ldy;
-  void* workspace; size_t workspace_bytes; /* t2w_mx4_ffn_workspace_bytes of the same arguments, 16-byte aligned; nothing in it needs
-                                            * clearing or outlives the call, and calls that may overlap need one each */
+  void* workspace; size_t workspace_bytes; /* as t2w_mx4_linear's, of t2w_mx4_ffn_workspace_bytes (the inner rows and up to 34 MB) */
 } t2w_mx4_ffn_args;
 size_t t2w_mx4_ffn_workspace_bytes(const t2w_mx4_ffn_args* a);
 int t2w_mx4_ffn(const t2w_mx4_ffn_args* a, void* stream);

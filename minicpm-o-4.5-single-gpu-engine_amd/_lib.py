@@ -134,12 +134,12 @@ class MX4QuantizeArgs(C.Structure):
 
 class MX4LinearArgs(C.Structure):
     _fields_ = [("x", P), ("ldx", C.c_longlong), ("dtype", I), ("m", I), ("w", MX4Weight), ("bias", P), ("residual", P), ("ldr", C.c_longlong),
-                ("y", P), ("ldy", C.c_longlong)]
+                ("y", P), ("ldy", C.c_longlong), ("workspace", P), ("workspace_bytes", C.c_size_t)]
 
 
 class MX4GatedArgs(C.Structure):
     _fields_ = [("x", P), ("ldx", C.c_longlong), ("dtype", I), ("m", I), ("gate", MX4Weight), ("up", MX4Weight), ("act", I), ("y", P),
-                ("ldy", C.c_longlong)]
+                ("ldy", C.c_longlong), ("workspace", P), ("workspace_bytes", C.c_size_t)]
 
 
 class MX4FFNArgs(C.Structure):
@@ -201,6 +201,8 @@ _SIGS = {
     "t2w_mx4_pack": (I, [C.POINTER(MX4PackArgs), P]),
     "t2w_mx4_quantize": (I, [C.POINTER(MX4QuantizeArgs), P]),
     "t2w_mx4_linear": (I, [C.POINTER(MX4LinearArgs), P]),
+    "t2w_mx4_linear_workspace_bytes": (C.c_size_t, [C.POINTER(MX4LinearArgs)]),
+    "t2w_mx4_gated_workspace_bytes": (C.c_size_t, [C.POINTER(MX4GatedArgs)]),
     "t2w_mx4_gated": (I, [C.POINTER(MX4GatedArgs), P]),
     "t2w_mx4_ffn": (I, [C.POINTER(MX4FFNArgs), P]),
     "t2w_mx4_ffn_workspace_bytes": (C.c_size_t, [C.POINTER(MX4FFNArgs)]),

@@ -7,81 +7,11 @@
 
 #include <type_traits>
 
-#include "mx4_internal.h"
+#include "mx4_device.h"
 
 namespace t2w {
 
 namespace {
-
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-
-// eight codes (columns 0 .. 7, the lowest nibble first) times the scale, as the matrix unit's operand
-template <bool BF>
-__device__ __forceinline__ uint4 widen(uint32_t c, float scale) {
-  if constexpr (BF)
-    return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0)),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1)),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2)),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3)));
-  else
-    return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 0)),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 1)),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 2)),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 3)));
-}
-
-template <bool BF>
-__device__ __forceinline__ f32x4 mma(uint4 a, uint4 b, f32x4 c) {
-  if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
-  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-
-// the float 2^(byte i of w - 127)
-__device__ __forceinline__ float scale_of(uint32_t w, int i) { return __uint_as_float(((w >> (8 * i)) & 0xffu) << 23); }
-
-template <bool BF>
-__device__ __forceinline__ float load1(const void* p, long long i) {
-  const uint16_t h = ((const uint16_t*)p)[i];
-  return BF ? bf2f(h) : h2f(h);
-}
-template <bool BF>
-__device__ __forceinline__ uint16_t round1(float v) {
-  return BF ? f2bf(v) : f2h(v);
-}
-
-__device__ __forceinline__ float gate_act(float g, int act) { return act == T2W_MX4_SILU ? silu(g) : gelu_tanh(g); }
-
-// Outputs n .. n + 3 of row m from their sums
-template <bool BF>
-__device__ __forceinline__ void finish(const Mx4Args& a, int m, int n, const float (&v)[4]) {
-  const long long o = (long long)m * a.ldy + n;
-  uint16_t* y = (uint16_t*)a.y;
-  if (a.quad) {
-    float r[4] = {v[0], v[1], v[2], v[3]};
-    if (a.bias) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] += a.bias[n + e];
-    }
-    if (a.residual) {
-      const uint2 h = *(const uint2*)((const uint16_t*)a.residual + (long long)m * a.ldr + n);
-      r[0] += BF ? lo2f(h.x) : lo2h(h.x);
-      r[1] += BF ? hi2f(h.x) : hi2h(h.x);
-      r[2] += BF ? lo2f(h.y) : lo2h(h.y);
-      r[3] += BF ? hi2f(h.y) : hi2h(h.y);
-    }
-    *(uint2*)(y + o) = BF ? make_uint2(pack2(r[0], r[1]), pack2(r[2], r[3])) : make_uint2(pack2h(r[0], r[1]), pack2h(r[2], r[3]));
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if (n + e >= a.n) break;
-    float r = v[e];
-    if (a.bias) r += a.bias[n + e];
-    if (a.residual) r += load1<BF>(a.residual, (long long)m * a.ldr + n + e);
-    y[o + e] = round1<BF>(r);
-  }
-}
 
 // --- few rows --------------------------------------------------------------------------------------------------------
 // A workgroup owns RB blocks of 16 channels (GATED: the same block of both matrices) and 16 CB rows of x; its waves take the units
@@ -288,7 +218,7 @@ hipError_t mx4_quantize(const t2w_mx4_quantize_args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-hipError_t mx4_product(const Mx4Args& a, bool bf, bool gated, hipStream_t st) {
+hipError_t mx4_rows(const Mx4Args& a, bool bf, bool gated, hipStream_t st) {
   if (gated) {
     if (a.m <= 16) return bf ? launch_rows<true, 1, 2, true>(a, st) : launch_rows<false, 1, 2, true>(a, st);
     return bf ? launch_rows<true, 4, 2, true>(a, st) : launch_rows<false, 4, 2, true>(a, st);

@@ -51,11 +51,25 @@ bool on_weight(const Rows& r, const t2w_mx4_weight& w) {
   return rows_meet(r, Rows{w.codes, c, c, 1}) || rows_meet(r, Rows{w.scales, s, s, 1});
 }
 
-int run(const Mx4Args& g, int dtype, bool gated, void* stream, const char* what) {
+// bytes of the parts that a product splits into
+size_t part_bytes(int m, int n, int k, long long ldx, bool gated) { return mx4_takes_tiles(m, ldx) ? mx4_tiles_workspace(m, n, k, gated) : 0; }
+
+// the workspace against what a call needs and its other operands
+const char* check_workspace(const void* ws, size_t have, size_t need, const Rows& out, const Rows& x, const void* residual, long long ldr) {
+  if (need == 0) return nullptr;
+  if (!ws || have < need) return "mx4: workspace too small";
+  if ((uintptr_t)ws & 15) return "mx4: workspace must be 16-byte aligned";
+  const Rows w{ws, (long long)need, (long long)need, 1};
+  if (rows_meet(w, out) || rows_meet(w, x) || (residual && rows_meet(w, Rows{residual, ldr * 2, out.width, out.n}))) return "mx4: the workspace overlaps an operand";
+  return nullptr;
+}
+
+int run(const Mx4Args& g, int dtype, bool gated, void* workspace, void* stream, const char* what) {
   Mx4Args a = g;
   const auto whole = [](const void* p, long long ld, int m) { return !((uintptr_t)p & 7) && (m == 1 || ld % 4 == 0); };
   a.quad = a.n % 4 == 0 && whole(a.y, a.ldy, a.m) && (!a.residual || whole(a.residual, a.ldr, a.m));
-  const hipError_t e = mx4_product(a, dtype == T2W_MX4_BF16, gated, (hipStream_t)stream);
+  const bool bf = dtype == T2W_MX4_BF16;
+  const hipError_t e = mx4_takes_tiles(a.m, a.ldx) ? mx4_tiles(a, bf, gated, workspace, (hipStream_t)stream) : mx4_rows(a, bf, gated, (hipStream_t)stream);
   return e == hipSuccess ? 0 : xerr(what, e);
 }
 
@@ -86,6 +100,11 @@ int t2w_mx4_quantize(const t2w_mx4_quantize_args* a, void* stream) {
   return e == hipSuccess ? 0 : xerr("mx4 quantize", e);
 }
 
+size_t t2w_mx4_linear_workspace_bytes(const t2w_mx4_linear_args* a) {
+  if (!a || check_weight(a->w) || a->m < 1 || a->m > MAX_ROWS) return 0;
+  return part_bytes(a->m, a->w.n, a->w.k, a->ldx, false);
+}
+
 int t2w_mx4_linear(const t2w_mx4_linear_args* a, void* stream) {
   if (!a) return xerr("mx4 linear: null arguments");
   if (const char* e = check_weight(a->w)) return xerr(e);
@@ -94,11 +113,17 @@ int t2w_mx4_linear(const t2w_mx4_linear_args* a, void* stream) {
   if ((uintptr_t)a->bias & 3) return xerr("mx4: misaligned bias");
   const Rows out{a->y, a->ldy * 2, 2LL * a->w.n, a->m};
   if (on_weight(out, a->w) || (a->bias && rows_meet(out, Rows{a->bias, 4LL * a->w.n, 4LL * a->w.n, 1}))) return xerr("mx4: the outputs overlap the weight or bias");
+  const size_t need = t2w_mx4_linear_workspace_bytes(a);
+  if (const char* e = check_workspace(a->workspace, a->workspace_bytes, need, out, Rows{a->x, a->ldx * 2, 2LL * a->w.k, a->m}, a->residual, a->ldr)) return xerr(e);
+  if (need) {
+    const Rows ws{a->workspace, (long long)need, (long long)need, 1};
+    if (on_weight(ws, a->w) || (a->bias && rows_meet(ws, Rows{a->bias, 4LL * a->w.n, 4LL * a->w.n, 1}))) return xerr("mx4: the workspace overlaps an operand");
+  }
   Mx4Args g{};
   g.w[0] = (const uint8_t*)a->w.codes, g.s[0] = (const uint8_t*)a->w.scales;
   g.x = a->x, g.ldx = a->ldx, g.m = a->m, g.n = a->w.n, g.k = a->w.k;
   g.bias = a->bias, g.residual = a->residual, g.ldr = a->ldr, g.y = a->y, g.ldy = a->ldy;
-  return run(g, a->dtype, false, stream, "mx4 linear");
+  return run(g, a->dtype, false, a->workspace, stream, "mx4 linear");
 }
 
 static const char* check_gated(const t2w_mx4_weight& gate, const t2w_mx4_weight& up, int act) {
@@ -117,6 +142,11 @@ static Mx4Args gated_args(const t2w_mx4_weight& gate, const t2w_mx4_weight& up, 
   return g;
 }
 
+size_t t2w_mx4_gated_workspace_bytes(const t2w_mx4_gated_args* a) {
+  if (!a || check_gated(a->gate, a->up, a->act) || a->m < 1 || a->m > MAX_ROWS) return 0;
+  return part_bytes(a->m, a->gate.n, a->gate.k, a->ldx, true);
+}
+
 int t2w_mx4_gated(const t2w_mx4_gated_args* a, void* stream) {
   if (!a) return xerr("mx4 gated: null arguments");
   if (const char* e = check_gated(a->gate, a->up, a->act)) return xerr(e);
@@ -124,7 +154,11 @@ int t2w_mx4_gated(const t2w_mx4_gated_args* a, void* stream) {
   if (a->m == 0) return 0;
   const Rows out{a->y, a->ldy * 2, 2LL * a->gate.n, a->m};
   if (on_weight(out, a->gate) || on_weight(out, a->up)) return xerr("mx4: the outputs overlap a weight");
-  return run(gated_args(a->gate, a->up, a->x, a->ldx, a->m, a->act, a->y, a->ldy), a->dtype, true, stream, "mx4 gated");
+  const size_t need = t2w_mx4_gated_workspace_bytes(a);
+  if (const char* e = check_workspace(a->workspace, a->workspace_bytes, need, out, Rows{a->x, a->ldx * 2, 2LL * a->gate.k, a->m}, nullptr, 0)) return xerr(e);
+  const Rows ws{a->workspace, (long long)need, (long long)need, 1};
+  if (need && (on_weight(ws, a->gate) || on_weight(ws, a->up))) return xerr("mx4: the workspace overlaps an operand");
+  return run(gated_args(a->gate, a->up, a->x, a->ldx, a->m, a->act, a->y, a->ldy), a->dtype, true, a->workspace, stream, "mx4 gated");
 }
 
 // the inner rows lie in the workspace, each at a 16-byte boundary
@@ -138,29 +172,31 @@ static const char* check_ffn(const t2w_mx4_ffn_args* a) {
   return check_rows(a->x, a->ldx, a->gate.k, a->y, a->ldy, a->down.n, a->residual, a->ldr, a->dtype, a->m);
 }
 
+// the inner rows, then (16-byte aligned: rows are) the parts of whichever product needs more
+static size_t inner_bytes(const t2w_mx4_ffn_args& a) { return (size_t)a.m * inner_ld(a) * 2; }
+
 size_t t2w_mx4_ffn_workspace_bytes(const t2w_mx4_ffn_args* a) {
-  if (!a || check_gated(a->gate, a->up, a->act) || a->m < 0 || a->m > MAX_ROWS) return 0;
-  return (size_t)a->m * inner_ld(*a) * 2;
+  if (!a || check_gated(a->gate, a->up, a->act) || check_weight(a->down) || a->m < 1 || a->m > MAX_ROWS) return 0;
+  const size_t p = part_bytes(a->m, a->gate.n, a->gate.k, a->ldx, true), q = part_bytes(a->m, a->down.n, a->down.k, inner_ld(*a), false);
+  return inner_bytes(*a) + (p > q ? p : q);
 }
 
 int t2w_mx4_ffn(const t2w_mx4_ffn_args* a, void* stream) {
   if (const char* e = check_ffn(a)) return xerr(e);
   if (a->m == 0) return 0;
   const size_t need = t2w_mx4_ffn_workspace_bytes(a);
-  if (!a->workspace || a->workspace_bytes < need) return xerr("mx4 ffn: workspace too small");
-  if ((uintptr_t)a->workspace & 15) return xerr("mx4 ffn: workspace must be 16-byte aligned");
   const Rows out{a->y, a->ldy * 2, 2LL * a->down.n, a->m}, ws{a->workspace, (long long)need, (long long)need, 1};
   if (on_weight(out, a->gate) || on_weight(out, a->up) || on_weight(out, a->down)) return xerr("mx4: the outputs overlap a weight");
-  if (rows_meet(ws, out) || rows_meet(ws, Rows{a->x, a->ldx * 2, 2LL * a->gate.k, a->m}) ||
-      (a->residual && rows_meet(ws, Rows{a->residual, a->ldr * 2, 2LL * a->down.n, a->m})) || on_weight(ws, a->gate) || on_weight(ws, a->up) || on_weight(ws, a->down))
-    return xerr("mx4 ffn: the workspace overlaps an operand");
+  if (const char* e = check_workspace(a->workspace, a->workspace_bytes, need, out, Rows{a->x, a->ldx * 2, 2LL * a->gate.k, a->m}, a->residual, a->ldr)) return xerr(e);
+  if (on_weight(ws, a->gate) || on_weight(ws, a->up) || on_weight(ws, a->down)) return xerr("mx4: the workspace overlaps an operand");
   const long long ldh = inner_ld(*a);
-  if (int rc = run(gated_args(a->gate, a->up, a->x, a->ldx, a->m, a->act, a->workspace, ldh), a->dtype, true, stream, "mx4 ffn")) return rc;
+  void* part = (uint8_t*)a->workspace + inner_bytes(*a);
+  if (int rc = run(gated_args(a->gate, a->up, a->x, a->ldx, a->m, a->act, a->workspace, ldh), a->dtype, true, part, stream, "mx4 ffn")) return rc;
   Mx4Args g{};
   g.w[0] = (const uint8_t*)a->down.codes, g.s[0] = (const uint8_t*)a->down.scales;
   g.x = a->workspace, g.ldx = ldh, g.m = a->m, g.n = a->down.n, g.k = a->down.k;
   g.residual = a->residual, g.ldr = a->ldr, g.y = a->y, g.ldy = a->ldy;
-  return run(g, a->dtype, false, stream, "mx4 ffn");
+  return run(g, a->dtype, false, part, stream, "mx4 ffn");
 }
 
 }  // extern "C"

@@ -29,6 +29,7 @@ _WEIGHTS = _DTYPES | {torch.float32: 2}
 _ACTS = {"silu": 0, "gelu": 1}
 _E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 _F32 = torch.float32
+FEW_ROWS = 16      # up to here a linear or gated call needs no workspace
 
 
 class MX4Weight:
@@ -124,10 +125,25 @@ def _residual(x: torch.Tensor, n: int, residual) -> tuple:
     return (None, 0) if residual is None else (residual.data_ptr(), _rows("residual", residual, x.shape[0], n, x.dtype, x.device))
 
 
+def _run(name: str, a, dev, workspace) -> None:
+    """The call ``t2w_mx4_<name>`` with the caller's workspace or one of its own."""
+    L = _lib.lib()
+    if workspace is None:
+        need = getattr(L, f"t2w_mx4_{name}_workspace_bytes")(C.byref(a)) if a.m > FEW_ROWS or name == "ffn" else 0
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError("mx4: a contiguous workspace on the weights' device")
+    if workspace is not None:
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _lib.launch(getattr(L, f"t2w_mx4_{name}"), a, dev, f"mx4_{name}")
+
+
 def linear(x: torch.Tensor, w: MX4Weight, *, bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
-           out: torch.Tensor | None = None) -> torch.Tensor:
+           out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """x w^T + bias + residual: ``x`` [rows, k] bf16 or fp16 (rows may be strided by multiples of 8), ``bias`` fp32 [n], ``residual``
-    [rows, n] of x's type.  ``out`` may be ``residual``."""
+    [rows, n] of x's type.  ``out`` may be ``residual``.  ``workspace``: memory for calls that make none
+    (``t2w_mx4_linear_workspace_bytes``)."""
     ldx, dev = _input(x, w), w.device
     out, ldy = _output(x, w.n, out)
     b = None
@@ -136,7 +152,7 @@ def linear(x: torch.Tensor, w: MX4Weight, *, bias: torch.Tensor | None = None, r
             raise ValueError(f"mx4: bias must be a contiguous float32 vector of {w.n} on {dev}")
         b = bias.data_ptr()
     a = _lib.MX4LinearArgs(x.data_ptr(), ldx, _DTYPES[x.dtype], x.shape[0], w.struct, b, *_residual(x, w.n, residual), out.data_ptr(), ldy)
-    _lib.launch(_lib.lib().t2w_mx4_linear, a, dev, "mx4_linear")
+    _run("linear", a, dev, workspace)
     return out
 
 
@@ -148,12 +164,13 @@ def _pair(gate: MX4Weight, up: MX4Weight, act: str) -> int:
     return _ACTS[act]
 
 
-def gated(x: torch.Tensor, gate: MX4Weight, up: MX4Weight, *, act: str = "silu", out: torch.Tensor | None = None) -> torch.Tensor:
+def gated(x: torch.Tensor, gate: MX4Weight, up: MX4Weight, *, act: str = "silu", out: torch.Tensor | None = None,
+          workspace: torch.Tensor | None = None) -> torch.Tensor:
     """act(x gate^T) * (x up^T) in one kernel; ``act`` is "silu" or "gelu" (the tanh form)."""
     k, ldx = _pair(gate, up, act), _input(x, gate)
     out, ldy = _output(x, gate.n, out)
     a = _lib.MX4GatedArgs(x.data_ptr(), ldx, _DTYPES[x.dtype], x.shape[0], gate.struct, up.struct, k, out.data_ptr(), ldy)
-    _lib.launch(_lib.lib().t2w_mx4_gated, a, gate.device, "mx4_gated")
+    _run("gated", a, gate.device, workspace)
     return out
 
 
@@ -165,13 +182,7 @@ def ffn(x: torch.Tensor, gate: MX4Weight, up: MX4Weight, down: MX4Weight, *, act
     if down.device != dev:
         raise ValueError("mx4: the weights must be on one device")
     out, ldy = _output(x, down.n, out)
-    L = _lib.lib()
     a = _lib.MX4FFNArgs(x.data_ptr(), ldx, _DTYPES[x.dtype], x.shape[0], gate.struct, up.struct, down.struct, k, *_residual(x, down.n, residual),
                         out.data_ptr(), ldy)
-    if workspace is None:
-        workspace = torch.empty(L.t2w_mx4_ffn_workspace_bytes(C.byref(a)), dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or not workspace.is_contiguous():
-        raise ValueError("mx4 ffn: a contiguous workspace on the weights' device")
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _lib.launch(L.t2w_mx4_ffn, a, dev, "mx4_ffn")
+    _run("ffn", a, dev, workspace)
     return out

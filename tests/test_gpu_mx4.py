@@ -127,9 +127,9 @@ def test_quantize_limits(dev):
     w = torch.zeros(3, 64, device="cuda")
     w[1, 5], w[2, 40] = 49152.0, 2.0 ** -24
     assert torch.equal(mx4.MX4Weight.quantize(w).values(), w)
-    strided = torch.randn(9, 300, device="cuda")[::2, 4:260]
-    assert torch.equal(mx4.MX4Weight.quantize(strided).values(), mx4.MX4Weight.quantize(strided.contiguous()).values())
-    assert torch.equal(mx4.MX4Weight.quantize(strided.T).values(), mx4.MX4Weight.quantize(strided.T.contiguous()).values()) if strided.shape[0] % 8 == 0 else True
+    strided = torch.randn(16, 300, device="cuda")[::2, 4:260]
+    for t in (strided, strided.T):
+        assert torch.equal(mx4.MX4Weight.quantize(t).values(), mx4.MX4Weight.quantize(t.contiguous()).values())
     for bad in (float("nan"), float("inf"), -float("inf"), 49200.0):
         w[0, 3] = bad
         with pytest.raises(ValueError, match="finite"):
@@ -235,6 +235,17 @@ def test_linear_beyond_32_bit_offsets(dev):
         assert ((mx4.linear(x, w)[:, -60:].double() - ref).abs() <= tol + rounding(ref.abs() + tol, BF)).all()
 
 
+def test_rows_far_apart(dev):
+    """Rows of x more than 2^24 elements apart, whose places in a tile would pass a 32-bit offset, and just below."""
+    n, k, m = 40, 256, 70
+    w, v = random_weight(n, k, 3)
+    for ld in ((1 << 24) - 8, 1 << 24):
+        x = torch.zeros(m, ld, dtype=BF, device="cuda")[:, ld - k:]
+        x.copy_(rand((m, k), BF, 4))
+        check_linear(x, w, v)
+        check_linear(x[:9], w, v)
+
+
 def test_no_rows(dev):
     w, _ = random_weight(48, 64, 1)
     x = torch.empty(0, 64, dtype=BF, device="cuda")
@@ -272,7 +283,7 @@ def test_ffn(dev, m, hidden, inner, dt, act):
     got = mx4.ffn(x, g, u, d, act=act, residual=res)
     assert ((got.double() - y).abs() <= tol).all()
     own = res.clone()
-    assert torch.equal(mx4.ffn(x, g, u, d, act=act, residual=own, out=own, workspace=torch.empty(m, inner + 8, dtype=dt, device="cuda")), got)
+    assert torch.equal(mx4.ffn(x, g, u, d, act=act, residual=own, out=own, workspace=torch.empty(2 * m * inner + (36 << 20), dtype=torch.uint8, device="cuda")), got)
 
 
 def test_gate_far_from_zero(dev):

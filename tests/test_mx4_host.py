@@ -72,6 +72,33 @@ def test_ffn_workspace():
     assert fn(C.byref(ffn_args(m=-1))) == 0 and fn(C.byref(ffn_args(m=0))) == 0
 
 
+def test_workspaces():
+    """None for few rows; beyond, bounded whatever the sizes; too small, misaligned or overlapping ones are refused."""
+    L = _lib.lib()
+    need = lambda **kw: L.t2w_mx4_linear_workspace_bytes(C.byref(linear_args(**kw)))  # noqa: E731
+    assert need(m=1) == need(m=16) == need(m=0) == need(m=64, k=12) == 0
+    split = need(m=64, n=512, k=4096, ldx=4096, ldy=512, ldr=512)
+    assert split > 0
+    for m in (17, 64, 65, 200, 1000, 1 << 21):
+        for n in (1, 100, 4096, 100000, 1 << 24):
+            for k in (8, 1024, 14336, 1 << 20):
+                assert need(m=m, n=n, k=k) <= 34 << 20
+                g = _lib.MX4GatedArgs(x=M, ldx=k, dtype=0, m=m, gate=weight(n, k), up=weight(n, k), act=0, y=M, ldy=n)
+                assert L.t2w_mx4_gated_workspace_bytes(C.byref(g)) <= 34 << 20
+    big = {"m": 64, "n": 512, "k": 4096, "ldx": 4096, "ldy": 512, "ldr": 512}
+    for kw, text in (({}, "too small"), ({"workspace": 50 * M, "workspace_bytes": split - 1}, "too small"), ({"workspace": 50 * M + 8, "workspace_bytes": split}, "aligned"),
+                     ({"workspace": 4 * M, "workspace_bytes": split}, "workspace overlaps"), ({"workspace": M, "workspace_bytes": split}, "workspace overlaps"),
+                     ({"workspace": 3 * M, "workspace_bytes": split}, "workspace overlaps"), ({"workspace": 100 * M, "workspace_bytes": split}, "workspace overlaps"),
+                     ({"workspace": 2 * M - 16, "workspace_bytes": split}, "workspace overlaps")):
+        refused(L.t2w_mx4_linear, linear_args(**(big | kw)), text)
+    g = {"x": M, "ldx": 4096, "dtype": 0, "m": 64, "gate": weight(512, 4096), "up": weight(512, 4096, at=140), "act": 0, "y": 4 * M, "ldy": 512}
+    need_g = L.t2w_mx4_gated_workspace_bytes(C.byref(_lib.MX4GatedArgs(**g)))
+    for kw, text in (({}, "too small"), ({"workspace": 4 * M, "workspace_bytes": need_g}, "workspace overlaps"), ({"workspace": 140 * M, "workspace_bytes": need_g}, "workspace overlaps")):
+        refused(L.t2w_mx4_gated, _lib.MX4GatedArgs(**(g | kw)), text)
+    f = ffn_args(m=64, workspace=50 * M, workspace_bytes=64 * 64 * 2)
+    assert L.t2w_mx4_ffn_workspace_bytes(C.byref(f)) >= 64 * 64 * 2
+
+
 def test_weight_sizes():
     L = _lib.lib()
     assert (L.t2w_mx4_codes_bytes(1, 8), L.t2w_mx4_scales_bytes(1, 8)) == (1024, 256)
