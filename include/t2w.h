@@ -441,7 +441,7 @@ int t2w_mx4_quantize(const t2w_mx4_quantize_args* a, void* stream);
 /* y = x W^T + bias + residual.  x [m, k] and y [m, n] in one type, bf16 or fp16, rows ldx / ldy elements apart; x is 16-byte
  * aligned and ldx a multiple of 8, y and the residual [m, n] (ldr; optional) need no more than their elements' alignment (8 bytes
  * and strides of 4 are faster).  bias [n] fp32, optional.  Sums are fp32, the output is rounded once.  y may be the residual
- * itself (same rows), and overlaps no operand otherwise.  m is at most 2^21. */
+ * itself (same rows), and overlaps no operand otherwise.  m is at most 2^20. */
 typedef struct {
   const void* x; long long ldx;
   int dtype, m;
@@ -449,7 +449,7 @@ typedef struct {
   const float* bias;
   const void* residual; long long ldr;
   void* y; long long ldy;
-  void* workspace; size_t workspace_bytes; /* t2w_mx4_linear_workspace_bytes of the same arguments (0 for few rows, at most 34 MB):
+  void* workspace; size_t workspace_bytes; /* t2w_mx4_linear_workspace_bytes of the same arguments (0 for most calls, at most 34 MB):
                                             * 16-byte aligned; nothing in it needs clearing or outlives the call, and calls that
                                             * may overlap need one each */
 } t2w_mx4_linear_args;

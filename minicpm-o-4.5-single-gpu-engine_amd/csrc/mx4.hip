@@ -5,6 +5,8 @@
 // only roundings are the fp32 additions' and the output's.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "mx4_device.h"
@@ -14,106 +16,146 @@ namespace t2w {
 namespace {
 
 // --- few rows --------------------------------------------------------------------------------------------------------
-// A workgroup owns RB blocks of 16 channels (GATED: the same block of both matrices) and 16 CB rows of x; its waves take the units
-// of 512 columns in turn, each converting its codes in registers, and their sums meet in LDS in the order of the waves.
-template <bool BF, int CB, int RB, bool GATED>
+// Up to 16 rows of x (a grid's y: 16 more).  A workgroup takes blocks of 16 channels in turn; each of its waves has units of 512
+// columns (GATED: even waves of the gate's matrix, odd ones of the other), whose codes it converts in registers, and the waves'
+// sums meet in LDS in the order of the waves.  The stream of codes is what bounds it: a step's registers are loaded again, with
+// the wave's next unit, as soon as the step is converted, so that a wave always has about 4 KB in flight, across units and blocks.
+// XL: x lies in LDS, brought there once by each workgroup (16-byte chunk c of a step of row r at c ^ r: 16 rows' reads cover all
+// banks), zero behind k.  A wave reads 4 KB of it a step's 1 KB of codes; from memory (rows too long for LDS) that alone would take the
+// L1 cache's whole bandwidth at 1 row, where 16 lanes read the same bytes.
+template <bool BF, bool GATED, bool XL>
 __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Args a) {
-  extern __shared__ float4 part[];  // [waves][RB][CB][64]
+  extern __shared__ uint4 lds[];  // XL: x [rows][units][4][16]; then sums [2][waves][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const int steps = (a.k + 127) >> 7, units = (a.k + 511) >> 9, q = lane >> 4;
-  const int nb = (a.n + 15) >> 4;
-  f32x4 acc[RB][CB];
+  const int steps = (a.k + 127) >> 7, units = (a.k + 511) >> 9, q = lane >> 4, nb = (a.n + 15) >> 4;
+  const int first = GATED ? wave >> 1 : wave, stride = GATED ? waves >> 1 : waves;  // this wave's units
+  const int m0 = 16 * blockIdx.y, rows = min(16, a.m - m0), row = min(lane & 15, rows - 1);  // lanes behind the last row repeat it: not stored
+  const uint16_t* x = (const uint16_t*)a.x + (long long)m0 * a.ldx;
+  uint4* xs = lds;
+  f32x4* part = (f32x4*)(lds + (XL ? rows * units * 64 : 0));
+  const uint8_t* w = GATED && (wave & 1) ? a.w[1] : a.w[0];
+  const uint8_t* s = GATED && (wave & 1) ? a.s[1] : a.s[0];
+
+  uint4 code[4];
+  uint32_t sc, scn = 0;
+  // step t of unit u of block g; behind the last step the last again, against columns of x that are zero
+  const auto load = [&](int g, int u, int t) {
+    code[t] = *(const uint4*)(w + ((size_t)g * steps + min(4 * u + t, steps - 1)) * 1024 + (uint32_t)(lane * 16));
+  };
+  const auto load_scales = [&](int g, int u) { return *(const uint32_t*)(s + ((size_t)g * units + u) * 256 + (uint32_t)(lane * 4)); };
+
+  int g = blockIdx.x, u = first;
+  sc = load_scales(g, u);
 #pragma unroll
-  for (int r = 0; r < RB; ++r)
-#pragma unroll
-    for (int c = 0; c < CB; ++c) acc[r][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const uint4* w[RB];
-  const uint32_t* s[RB];
-#pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    const int b = GATED ? (int)blockIdx.x : min((int)blockIdx.x * RB + r, nb - 1);
-    w[r] = (const uint4*)a.w[GATED ? r : 0] + (size_t)b * steps * 64 + lane;
-    s[r] = (const uint32_t*)a.s[GATED ? r : 0] + (size_t)b * units * 64 + lane;
-  }
-  const uint16_t* x[CB];
-#pragma unroll
-  for (int c = 0; c < CB; ++c) {
-    const int m = min((int)blockIdx.y * 16 * CB + 16 * c + (lane & 15), a.m - 1);  // rows behind the last repeat it: not stored
-    x[c] = (const uint16_t*)a.x + (long long)m * a.ldx + 32 * q;
-  }
-  for (int u = wave; u < units; u += waves) {
-    const int n_steps = min(4, steps - 4 * u);
-    uint32_t sc[RB];
-    uint4 code[RB][4];
-#pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      sc[r] = s[r][(size_t)u * 64];
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-        if (t < n_steps) code[r][t] = w[r][(size_t)(4 * u + t) * 64];
+  for (int t = 0; t < 4; ++t) load(g, u, t);
+  asm volatile("" ::: "memory");
+  if constexpr (XL) {
+    const int chunks = units * 64;  // of a row
+    for (int i = threadIdx.x; i < rows * chunks; i += blockDim.x) {
+      const int r = i / chunks, c = i - r * chunks;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (8 * c < a.k) v = *(const uint4*)(x + (long long)r * a.ldx + 8 * c);
+      xs[r * chunks + ((c & ~15) | ((c ^ r) & 15))] = v;
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+  const uint16_t* xrow = x + (long long)row * a.ldx + 32 * q;
+
+  f32x4 acc[2];
+  const auto unit = [&](auto more, int gn, int un) {
+    constexpr bool MORE = decltype(more)::value;
+    if (MORE) scn = load_scales(gn, un);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      if (t >= n_steps) break;
-      const int k0 = 512 * u + 128 * t;
-      uint4 xf[CB][4];
-      const bool whole = k0 + 128 <= a.k;
+      uint4 xf[4];
 #pragma unroll
-      for (int c = 0; c < CB; ++c)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          xf[c][j] = make_uint4(0, 0, 0, 0);
-          if (whole || k0 + 32 * q + 8 * j < a.k) xf[c][j] = *(const uint4*)(x[c] + k0 + 8 * j);
-        }
-#pragma unroll
-      for (int r = 0; r < RB; ++r) {
-        const float f = scale_of(sc[r], t);
-        const uint32_t cw[4] = {code[r][t].x, code[r][t].y, code[r][t].z, code[r][t].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 wf = widen<BF>(cw[j], f);
-#pragma unroll
-          for (int c = 0; c < CB; ++c) acc[r][c] = mma<BF>(wf, xf[c][j], acc[r][c]);
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (XL) {
+          xf[j] = xs[(row * units + u) * 64 + 16 * t + ((4 * q + j) ^ row)];
+        } else {
+          xf[j] = make_uint4(0, 0, 0, 0);
+          const int k0 = 512 * u + 128 * t + 8 * j;
+          if (k0 + 32 * q < a.k) xf[j] = *(const uint4*)(xrow + k0);
         }
       }
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < RB; ++r)
-#pragma unroll
-    for (int c = 0; c < CB; ++c) part[((wave * RB + r) * CB + c) * 64 + lane] = __builtin_bit_cast(float4, acc[r][c]);
-  __syncthreads();
-  constexpr int TILES = GATED ? CB : RB * CB;
-  for (int t = wave; t < TILES; t += waves) {
-    float v[GATED ? 2 : 1][4];
-#pragma unroll
-    for (int g = 0; g < (GATED ? 2 : 1); ++g) {
-      const int at = GATED ? g * CB + t : t;
-      float4 p = part[at * 64 + lane];
-      for (int i = 1; i < waves; ++i) {
-        const float4 o = part[(i * RB * CB + at) * 64 + lane];
-        p.x += o.x, p.y += o.y, p.z += o.z, p.w += o.w;
+      const float f = scale_of(sc, t);
+      const uint4 w0 = widen<BF>(code[t].x, f), w1 = widen<BF>(code[t].y, f), w2 = widen<BF>(code[t].z, f), w3 = widen<BF>(code[t].w, f);
+      if (MORE) {
+        load(gn, un, t);
+        asm volatile("" ::: "memory");
       }
-      v[g][0] = p.x, v[g][1] = p.y, v[g][2] = p.z, v[g][3] = p.w;
+      acc[0] = mma<BF>(w0, xf[0], acc[0]);
+      acc[1] = mma<BF>(w1, xf[1], acc[1]);
+      acc[0] = mma<BF>(w2, xf[2], acc[0]);
+      acc[1] = mma<BF>(w3, xf[3], acc[1]);
     }
-    const int c = GATED ? t : t % CB, r = GATED ? 0 : t / CB;
-    const int n = ((int)blockIdx.x * (GATED ? 1 : RB) + r) * 16 + 4 * q, m = (int)blockIdx.y * 16 * CB + 16 * c + (lane & 15);
-    if (m >= a.m || n >= a.n) continue;
-    if constexpr (GATED) {
+    if (MORE) sc = scn;
+  };
+
+  for (int turn = 0; g < nb; turn ^= 1) {
+    acc[0] = acc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (; u + stride < units; u += stride) unit(std::true_type{}, g, u + stride);
+    const int gn = g + gridDim.x;
+    if (gn < nb) unit(std::true_type{}, gn, first);
+    else unit(std::false_type{}, 0, 0);
+    u = first;
+    f32x4* p = part + turn * waves * 64;
+    p[wave * 64 + lane] = acc[0] + acc[1];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the codes in flight are not waited for
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (wave == 0) {  // the others go on; the sums' other half is theirs until the next barrier
+      f32x4 v = p[lane], o = p[GATED ? 64 + lane : lane];
+      for (int i = 1; i < stride; ++i) {
+        v += p[(GATED ? 2 * i : i) * 64 + lane];
+        if constexpr (GATED) o += p[(2 * i + 1) * 64 + lane];
+      }
+      const int n = g * 16 + 4 * q, m = m0 + (lane & 15);
+      if (m < a.m && n < a.n) {
+        float r[4] = {v[0], v[1], v[2], v[3]};
+        if constexpr (GATED) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[0][e] = gate_act(v[0][e], a.act) * v[1][e];
+          for (int e = 0; e < 4; ++e) r[e] = gate_act(r[e], a.act) * o[e];
+        }
+        finish<BF>(a, m, n, r);
+      }
     }
-    finish<BF>(a, m, n, v[0]);
+    g = gn;
   }
 }
 
-template <bool BF, int CB, int RB, bool GATED>
-hipError_t launch_rows(const Mx4Args& a, hipStream_t st) {
-  constexpr int MOST = RB * CB > 4 ? 8 : 16;  // 64 KB of sums
-  const int units = mx4_units(a.k), rounds = (units + MOST - 1) / MOST, waves = (units + rounds - 1) / rounds;
-  const int nb = mx4_blocks(a.n);
-  const dim3 grid(GATED ? nb : (nb + RB - 1) / RB, (a.m + 16 * CB - 1) / (16 * CB));
-  mx4_rows_kernel<BF, CB, RB, GATED><<<grid, waves * 64, (size_t)waves * RB * CB * 1024, st>>>(a);
+struct RowsPlan {
+  int waves;
+  size_t bytes;  // of LDS
+};
+
+RowsPlan rows_plan(int m, int k, bool gated, bool xl) {
+  const int units = mx4_units(k), two = gated ? 2 : 1;
+  const int rounds = (units * two + 15) / 16, waves = (units + rounds - 1) / rounds * two;
+  return {waves, (xl ? (size_t)std::min(m, 16) * units * 1024 : 0) + (size_t)2 * waves * 1024};
+}
+
+constexpr size_t LDS_CU = 160 * 1024;
+
+template <bool BF, bool GATED, bool XL>
+hipError_t launch_rows(const Mx4Args& a, const RowsPlan& p, hipStream_t st) {
+  if (p.bytes > 64 * 1024) {  // beyond the default a function has to be told, on each device
+    static std::atomic<uint64_t> told{0};
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (!(told.load(std::memory_order_acquire) & bit)) {
+      e = hipFuncSetAttribute((const void*)mx4_rows_kernel<BF, GATED, XL>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_CU);
+      if (e != hipSuccess) return e;
+      told.fetch_or(bit, std::memory_order_release);
+    }
+  }
+  const int nb = mx4_blocks(a.n), fit = std::max(1, std::min(16 / p.waves, (int)(LDS_CU / p.bytes)));  // workgroups a CU
+  const int rounds = (nb + 256 * fit - 1) / (256 * fit);
+  mx4_rows_kernel<BF, GATED, XL><<<dim3((nb + rounds - 1) / rounds, (a.m + 15) / 16), p.waves * 64, p.bytes, st>>>(a);
   return hipGetLastError();
 }
 
@@ -218,13 +260,17 @@ hipError_t mx4_quantize(const t2w_mx4_quantize_args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+bool mx4_rows_in_lds(int m, int k, bool gated) { return rows_plan(m, k, gated, true).bytes <= LDS_CU; }
+
 hipError_t mx4_rows(const Mx4Args& a, bool bf, bool gated, hipStream_t st) {
-  if (gated) {
-    if (a.m <= 16) return bf ? launch_rows<true, 1, 2, true>(a, st) : launch_rows<false, 1, 2, true>(a, st);
-    return bf ? launch_rows<true, 4, 2, true>(a, st) : launch_rows<false, 4, 2, true>(a, st);
-  }
-  if (a.m <= 16) return bf ? launch_rows<true, 1, 1, false>(a, st) : launch_rows<false, 1, 1, false>(a, st);
-  return bf ? launch_rows<true, 4, 1, false>(a, st) : launch_rows<false, 4, 1, false>(a, st);
+  const bool xl = mx4_rows_in_lds(a.m, a.k, gated);
+  const RowsPlan p = rows_plan(a.m, a.k, gated, xl);
+  const auto go = [&](auto b, auto g) {
+    constexpr bool BF = decltype(b)::value, GATED = decltype(g)::value;
+    return xl ? launch_rows<BF, GATED, true>(a, p, st) : launch_rows<BF, GATED, false>(a, p, st);
+  };
+  if (gated) return bf ? go(std::true_type{}, std::true_type{}) : go(std::false_type{}, std::true_type{});
+  return bf ? go(std::true_type{}, std::false_type{}) : go(std::false_type{}, std::false_type{});
 }
 
 }  // namespace t2w

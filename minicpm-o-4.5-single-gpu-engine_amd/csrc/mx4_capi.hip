@@ -15,7 +15,7 @@ namespace {
 
 int xerr(const char* what, hipError_t e = hipSuccess) { return set_error(what, e); }
 
-constexpr int MAX_ROWS = 1 << 21, MAX_N = 1 << 24, MAX_K = 1 << 20;
+constexpr int MAX_ROWS = 1 << 20, MAX_N = 1 << 24, MAX_K = 1 << 20;
 
 const char* check_size(int n, int k) {
   if (n < 1 || n > MAX_N) return "mx4: n must be 1 to 2^24";
@@ -33,7 +33,7 @@ const char* check_weight(const t2w_mx4_weight& w) {
 // x [m, k] and y [m, n] in 16 bits
 const char* check_rows(const void* x, long long ldx, int k, void* y, long long ldy, int n, const void* residual, long long ldr, int dtype, int m) {
   if (dtype != T2W_MX4_BF16 && dtype != T2W_MX4_FP16) return "mx4: dtype must be bf16 or fp16";
-  if (m < 0 || m > MAX_ROWS) return "mx4: m must be 0 to 2^21";
+  if (m < 0 || m > MAX_ROWS) return "mx4: m must be 0 to 2^20";
   if (m == 0) return nullptr;
   if (!x || !y) return "mx4: null rows";
   if (((uintptr_t)x & 15) || (m > 1 && ldx % 8)) return "mx4: x must be 16-byte aligned, its row stride a multiple of 8";
@@ -52,7 +52,7 @@ bool on_weight(const Rows& r, const t2w_mx4_weight& w) {
 }
 
 // bytes of the parts that a product splits into
-size_t part_bytes(int m, int n, int k, long long ldx, bool gated) { return mx4_takes_tiles(m, ldx) ? mx4_tiles_workspace(m, n, k, gated) : 0; }
+size_t part_bytes(int m, int n, int k, long long ldx, bool gated) { return mx4_takes_tiles(m, n, k, ldx, gated) ? mx4_tiles_workspace(m, n, k, gated) : 0; }
 
 // the workspace against what a call needs and its other operands
 const char* check_workspace(const void* ws, size_t have, size_t need, const Rows& out, const Rows& x, const void* residual, long long ldr) {
@@ -69,7 +69,7 @@ int run(const Mx4Args& g, int dtype, bool gated, void* workspace, void* stream, 
   const auto whole = [](const void* p, long long ld, int m) { return !((uintptr_t)p & 7) && (m == 1 || ld % 4 == 0); };
   a.quad = a.n % 4 == 0 && whole(a.y, a.ldy, a.m) && (!a.residual || whole(a.residual, a.ldr, a.m));
   const bool bf = dtype == T2W_MX4_BF16;
-  const hipError_t e = mx4_takes_tiles(a.m, a.ldx) ? mx4_tiles(a, bf, gated, workspace, (hipStream_t)stream) : mx4_rows(a, bf, gated, (hipStream_t)stream);
+  const hipError_t e = mx4_takes_tiles(a.m, a.n, a.k, a.ldx, gated) ? mx4_tiles(a, bf, gated, workspace, (hipStream_t)stream) : mx4_rows(a, bf, gated, (hipStream_t)stream);
   return e == hipSuccess ? 0 : xerr(what, e);
 }
 

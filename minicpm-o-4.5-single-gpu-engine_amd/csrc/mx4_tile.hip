@@ -25,19 +25,19 @@ struct MxTile {
   static constexpr int NW = WM * WN, BM = 16 * TM * WM, NB = TN * WN;   // waves; rows; weight blocks
   static constexpr int CB = GATED ? NB / 2 : NB;                         // blocks of output channels
   static constexpr int LD = BM / 4 / NW;                                 // 1 KB copies a stage and wave
+  static constexpr int LOADS = LD + 2 * TN;                              // a stage's, of a wave
   static_assert(BM % (4 * NW) == 0, "copies spread evenly");
   const Mx4Args& a;
   __amdgpu_buffer_rsrc_t xr;
   uint32_t off[LD];
   int lane, wave, wm, wn, steps, units;
-  const uint4* w[TN];      // scalar: this wave's blocks
-  const uint32_t* s[TN];
+  __amdgpu_buffer_rsrc_t wr[GATED ? 2 : 1], sr[GATED ? 2 : 1];  // this wave's blocks of each matrix
   f32x4 acc[TN][TM];
   uint4 xf[TM];
 
   __device__ __forceinline__ MxTile(const Mx4Args& a_, int mt, int nt) : a(a_) {
     lane = threadIdx.x & 63;
-    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % NW;
     wm = wave / WN, wn = wave % WN;
     steps = (a.k + 127) >> 7, units = (a.k + 511) >> 9;
     const int m0 = mt * BM;
@@ -47,13 +47,13 @@ struct MxTile {
       const int r = (wave * LD + i) * 4 + (lane >> 4);
       off[i] = m0 + r < a.m ? (uint32_t)r * (uint32_t)(a.ldx * 2) + (uint32_t)(((lane & 15) ^ (r & 15)) * 16) : OUTSIDE;
     }
-    const int nb = (a.n + 15) >> 4;
+    // blocks behind the last are out of bounds as well
+    constexpr int WB = GATED ? TN / 2 : TN;
+    const int b0 = nt * CB + wn * WB, have = max(0, min(WB, ((a.n + 15) >> 4) - b0));
 #pragma unroll
-    for (int t = 0; t < TN; ++t) {
-      const int g = GATED && t >= TN / 2 ? 1 : 0;
-      const int b = min(nt * CB + wn * (GATED ? TN / 2 : TN) + (GATED ? t % (TN / 2) : t), nb - 1);
-      w[t] = (const uint4*)a.w[g] + (size_t)b * steps * 64;
-      s[t] = (const uint32_t*)a.s[g] + (size_t)b * units * 64;
+    for (int g = 0; g < (GATED ? 2 : 1); ++g) {
+      wr[g] = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w[g] + (size_t)b0 * steps * 1024), 0, have * steps * 1024, 0x00020000);
+      sr[g] = __builtin_amdgcn_make_buffer_rsrc((void*)(a.s[g] + (size_t)b0 * units * 256), 0, have * units * 256, 0x00020000);
     }
 #pragma unroll
     for (int t = 0; t < TN; ++t)
@@ -66,18 +66,22 @@ struct MxTile {
     uint32_t e[TN];
   };
 
-  // the loads of stage st
-  __device__ __forceinline__ void issue(uint4* xs, Codes& cd, int st) const {
+  // the loads of stage st; none of a stage from s1 on (the registers and LDS get zeros, so that no branch parts the loop)
+  __device__ __forceinline__ void issue(uint4* xs, Codes& cd, int st, int s1) const {
+    const int end = st < s1 ? a.k : 0;
 #pragma unroll
     for (int i = 0; i < LD; ++i) {
       const int r = (wave * LD + i) * 4 + (lane >> 4);
-      const uint32_t o = 128 * st + 8 * ((lane & 15) ^ (r & 15)) < a.k ? off[i] : OUTSIDE;
+      const uint32_t o = 128 * st + 8 * ((lane & 15) ^ (r & 15)) < end ? off[i] : OUTSIDE;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_ptr_t)(xs + (wave * LD + i) * 64), 16, o, st * 256, 0, 0);
     }
+    const uint32_t at = st < s1 ? (uint32_t)lane * 16 : OUTSIDE;
 #pragma unroll
     for (int t = 0; t < TN; ++t) {
-      cd.c[t] = *(const uint4*)((const uint8_t*)(w[t] + (size_t)st * 64) + (uint32_t)(lane * 16));
-      cd.e[t] = *(const uint32_t*)((const uint8_t*)(s[t] + (size_t)(st >> 2) * 64) + (uint32_t)(lane * 4));
+      constexpr int WB = GATED ? TN / 2 : TN;
+      const int g = t / WB, b = t % WB;
+      cd.c[t] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(wr[g], at, (b * steps + st) * 1024, 0));
+      cd.e[t] = __builtin_amdgcn_raw_buffer_load_b32(sr[g], at >> 2, (b * units + (st >> 2)) * 256, 0);
     }
     asm volatile("" ::: "memory");  // the loads stay here: left to itself the compiler sinks them to their use, a stage later
   }
@@ -111,36 +115,41 @@ struct MxTile {
     }
   }
 
-  // stage st in (xc, cc), the next one in (xn, cn); s1: behind the last
+  // stage st in (xc, cc), the next one in (xn, cn); D: the buffers; s1: behind the last
+  template <int D>
   __device__ __forceinline__ void stage(uint4* xc, uint4* xn, Codes& cc, Codes& cn, uint4 (&w0)[TN], uint4 (&w1)[TN], int st, int s1) {
     step(w0, w1, xc, cc, st, 1);
     step(w1, w0, xc, cc, st, 2);
     step(w0, w1, xc, cc, st, 3);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __syncthreads();
-    const int nx = min(st + 1, s1 - 1);
-    issue(xc, cc, min(st + 2, s1 - 1));
-    step(w1, w0, xn, cn, nx, 0);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((D - 2) * LOADS) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    issue(xc, cc, st + D, s1);
+    step(w1, w0, xn, cn, st + 1, 0);
   }
 
-  __device__ __forceinline__ void run(uint4* x0, uint4* x1, int s0, int s1) {
-    Codes c0, c1;
+  template <int D>
+  __device__ __forceinline__ void run(uint4* const (&x)[D], int s0, int s1, int n) {
+    Codes c[D];
     uint4 w0[TN], w1[TN];
-    issue(x0, c0, s0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    issue(x1, c1, min(s0 + 1, s1 - 1));
 #pragma unroll
-    for (int i = 0; i < TM; ++i) xf[i] = xread(x0, i, 0);
+    for (int d = 0; d < D; ++d) issue(x[d], c[d], s0 + d, s1);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * LOADS) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 #pragma unroll
-    for (int t = 0; t < TN; ++t) w0[t] = widen<BF>(c0.c[t].x, __uint_as_float(((c0.e[t] >> (8 * (s0 & 3))) & 0xffu) << 23));
-    int st = s0;
-    for (; st + 1 < s1; st += 2) {
-      stage(x0, x1, c0, c1, w0, w1, st, s1);
-      stage(x1, x0, c1, c0, w0, w1, st + 1, s1);
+    for (int i = 0; i < TM; ++i) xf[i] = xread(x[0], i, 0);
+#pragma unroll
+    for (int t = 0; t < TN; ++t) w0[t] = widen<BF>(c[0].c[t].x, __uint_as_float(((c[0].e[t] >> (8 * (s0 & 3))) & 0xffu) << 23));
+    int i = 0;
+    for (; i + D <= n; i += D) {
+#pragma unroll
+      for (int d = 0; d < D; ++d) stage<D>(x[d], x[(d + 1) % D], c[d], c[(d + 1) % D], w0, w1, s0 + i + d, s1);
     }
-    if (st < s1) stage(x0, x1, c0, c1, w0, w1, st, s1);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last stage's repeated loads into LDS
+#pragma unroll
+    for (int d = 0; d < D - 1; ++d)
+      if (i + d < n) stage<D>(x[d], x[d + 1], c[d], c[d + 1], w0, w1, s0 + i + d, s1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was issued into LDS behind the last stage
   }
 };
 
@@ -168,16 +177,44 @@ __device__ __forceinline__ int2 tile_at(int b, int tm, int tn) {
   return make_int2(4 * grp + in % rows, in / rows);
 }
 
-template <bool BF, bool GATED, int TM, int TN, int WM, int WN, bool PART>
-__global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tile_kernel(const Mx4Args a, int tm, int tn, int splits, f32x4* part) {
+// KG groups of waves share a tile, each with its run of the stages and buffers of its own; the first adds up.
+template <bool BF, bool GATED, int TM, int TN, int WM, int WN, int D, int KG, bool PART>
+__global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx4_tile_kernel(const Mx4Args a, int tm, int tn, int splits, f32x4* part) {
   typedef MxTile<BF, GATED, TM, TN, WM, WN> T;
-  __shared__ uint4 x0[T::BM * 16], x1[T::BM * 16];
+  constexpr int XS = T::BM * 16;
+  __shared__ uint4 x0[KG * XS], x1[KG * XS], x2[D > 2 ? KG * XS : 1], x3[D > 3 ? KG * XS : 1];  // objects of their own: see the top
   const int total = tm * tn;
   const int split = PART ? (int)blockIdx.x / total : 0, b = (int)blockIdx.x - split * total;
   const int2 at = tile_at(b, tm, tn);
   T t(a, at.x, at.y);
-  const int s0 = PART ? (int)((long long)t.steps * split / splits) : 0, s1 = PART ? (int)((long long)t.steps * (split + 1) / splits) : t.steps;
-  t.run(x0, x1, s0, s1);
+  int s0 = PART ? (int)((long long)t.steps * split / splits) : 0, s1 = PART ? (int)((long long)t.steps * (split + 1) / splits) : t.steps;
+  int n = s1 - s0;  // stages to go through: the same for all groups, whose barriers are common
+  const int kg = KG > 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / (64 * T::NW)) : 0;
+  if constexpr (KG > 1) {
+    n = (n + KG - 1) / KG;
+    s0 += kg * n, s1 = min(s1, s0 + n);
+  }
+  const int xo = kg * XS;
+  if constexpr (D == 2) t.template run<2>({x0 + xo, x1 + xo}, s0, s1, n);
+  else if constexpr (D == 3) t.template run<3>({x0 + xo, x1 + xo, x2 + xo}, s0, s1, n);
+  else t.template run<4>({x0 + xo, x1 + xo, x2 + xo, x3 + xo}, s0, s1, n);
+  if constexpr (KG > 1) {
+    static_assert(KG == 2 && T::NW * TM * TN * 64 <= KG * XS, "the second group's sums fit a buffer");
+    __syncthreads();  // every wave is through with the buffers
+    f32x4* p = (f32x4*)x0 + (t.wave * TM * TN) * 64 + t.lane;
+    if (kg == 1) {
+#pragma unroll
+      for (int y = 0; y < TN; ++y)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) p[(y * TM + i) * 64] = t.acc[y][i];
+    }
+    __syncthreads();
+    if (kg == 1) return;
+#pragma unroll
+    for (int y = 0; y < TN; ++y)
+#pragma unroll
+      for (int i = 0; i < TM; ++i) t.acc[y][i] += p[(y * TM + i) * 64];
+  }
   if constexpr (PART) {
     f32x4* p = part + (size_t)(blockIdx.x * T::NW + t.wave) * (TM * TN * 64) + t.lane;
 #pragma unroll
@@ -213,50 +250,88 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const Mx4Args a, int tm, 
   block_store<BF, GATED, TM, TN, WM, WN>(a, at.x, at.y, w % NW, blk / TM, blk % TM, v, u);
 }
 
-template <bool BF, bool GATED, int TM, int TN, int WM, int WN>
+template <bool BF, bool GATED, int TM, int TN, int WM, int WN, int D, int KG>
 hipError_t launch(const Mx4Args& a, int splits, float* part, hipStream_t st) {
   typedef MxTile<BF, GATED, TM, TN, WM, WN> T;
   const int tm = (a.m + T::BM - 1) / T::BM, tn = (mx4_blocks(a.n) + T::CB - 1) / T::CB;
   if (splits <= 1) {
-    mx4_tile_kernel<BF, GATED, TM, TN, WM, WN, false><<<tm * tn, 64 * T::NW, 0, st>>>(a, tm, tn, 1, nullptr);
+    mx4_tile_kernel<BF, GATED, TM, TN, WM, WN, D, KG, false><<<tm * tn, 64 * T::NW * KG, 0, st>>>(a, tm, tn, 1, nullptr);
     return hipGetLastError();
   }
-  mx4_tile_kernel<BF, GATED, TM, TN, WM, WN, true><<<tm * tn * splits, 64 * T::NW, 0, st>>>(a, tm, tn, splits, (f32x4*)part);
+  mx4_tile_kernel<BF, GATED, TM, TN, WM, WN, D, KG, true><<<tm * tn * splits, 64 * T::NW * KG, 0, st>>>(a, tm, tn, splits, (f32x4*)part);
   mx4_join_kernel<BF, GATED, TM, TN, WM, WN><<<(tm * tn * T::NW * TM * (GATED ? TN / 2 : TN) + 3) / 4, 256, 0, st>>>(a, tm, tn, splits, (const f32x4*)part);
   return hipGetLastError();
 }
 
-// The one tile: 64 rows by 256 weight channels (gated: 128 of each matrix), four waves of 64 x 64, two workgroups a CU.
-constexpr int TILE_M = 64, TILE_N = 256, SLOTS = 512;
+// The tiles, each with four waves side by side: rows, weight channels (gated: half of each matrix), groups of waves that split k, and
+// what a pass of its stages takes in microseconds with one workgroup on a CU and, of each, with several (measured: 14336 columns
+// by 16 to 300 rows).  The narrow ones finish a stage sooner, the wide one moves least: 64 rows x 14336 x 4096, both matrices,
+// took 25.1 / 25.4 / 28.7 us (the wide one with k in two parts), 2005 rows 60% more / 5% more / 370 us.
+struct Shape {
+  int bm, bn, kg;
+  float one, many;
+};
+constexpr Shape SHAPES[3] = {{32, 128, 2, 0.60f, 0.60f}, {64, 128, 1, 0.59f, 0.48f}, {64, 256, 1, 1.00f, 0.85f}};
 
 struct Plan {
-  int tiles, splits;
+  int shape, tiles, splits;
+  float us;
 };
 
-// k is split where the tiles do not fill the chip's places, into parts of four stages at least
+// The cheapest by that model: 5 us for a launch, its first loads and stores; where k is split over workgroups 3 us and the
+// parts' way to memory and back (8 TB/s) more.  k is split so that the workgroups fill the 256 CUs once or twice, 512 at most.
 Plan plan(int m, int n, int k, bool gated) {
-  const int tn = gated ? (n + TILE_N / 2 - 1) / (TILE_N / 2) : (n + TILE_N - 1) / TILE_N;
-  const long long tiles = (long long)((m + TILE_M - 1) / TILE_M) * tn;
-  if (tiles > SLOTS / 2) return {(int)tiles, 1};
-  const int by_k = mx4_steps(k) / 4, by_n = SLOTS / (int)tiles;
-  return {(int)tiles, std::max(1, std::min(by_k, by_n))};
+  Plan best{0, 0, 1, 3e38f};
+  const int steps = mx4_steps(k), cols = gated ? 2 * n : n;
+  for (int i = 0; i < 3; ++i) {
+    const Shape& s = SHAPES[i];
+    const long long tiles = (long long)((m + s.bm - 1) / s.bm) * ((cols + s.bn - 1) / s.bn);
+    int last = 0;
+    for (const int fill : {0, 128, 256, 512}) {
+      const int splits = fill == 0 ? 1 : (int)std::min<long long>(fill / tiles, steps / (2 * s.kg));
+      if (splits <= last) continue;
+      last = splits;
+      const int passes = (steps + splits * s.kg - 1) / (splits * s.kg);
+      const long long wgs = tiles * splits;
+      // several workgroups a CU share it; the last round counts whole while rounds are few
+      const float turns = wgs <= 256 ? s.one : s.many * (wgs < 2048 ? (float)((wgs + 255) / 256) : (float)wgs / 256);
+      float us = 5.f + passes * turns;
+      if (splits > 1) us += 3.f + (float)wgs * s.bm * s.bn * 8 / 8e6f;
+      if (us < best.us) best = {i, (int)std::min<long long>(tiles, 1 << 30), splits, us};
+    }
+  }
+  return best;
+}
+
+template <bool BF, bool GATED>
+hipError_t launch_plan(const Mx4Args& a, const Plan& p, float* part, hipStream_t st) {
+  switch (p.shape) {
+    case 0: return launch<BF, GATED, 2, 2, 1, 4, 4, 2>(a, p.splits, part, st);
+    case 1: return launch<BF, GATED, 4, 2, 1, 4, 4, 1>(a, p.splits, part, st);
+    default: return launch<BF, GATED, 4, 4, 1, 4, 2, 1>(a, p.splits, part, st);
+  }
 }
 
 }  // namespace
 
-// a row's place in its tile is a 31-bit byte offset
-bool mx4_takes_tiles(int m, long long ldx) { return m > 16 && ldx < (1 << 24); }
+bool mx4_takes_tiles(int m, int n, int k, long long ldx, bool gated) {
+  if (ldx >= (1 << 24)) return false;  // a row's place in its tile is a 31-bit byte offset
+  if (m > 16) return true;
+  if (mx4_rows_in_lds(m, k, gated)) return false;
+  // few rows, too long for the LDS: 17.5 us of 16 rows x 14336 columns x 4096 channels (tiles 14.8), 6.8 of 5464 x 2048 (11.1)
+  return plan(m, n, k, gated).us < 2.f + 1.1e-3f * k * ((mx4_blocks(n) + 255) / 256);
+}
 
 size_t mx4_tiles_workspace(int m, int n, int k, bool gated) {
   const Plan p = plan(m, n, k, gated);
-  return p.splits > 1 ? (size_t)p.tiles * p.splits * TILE_M * TILE_N * 4 : 0;
+  return p.splits > 1 ? (size_t)p.tiles * p.splits * SHAPES[p.shape].bm * SHAPES[p.shape].bn * 4 : 0;
 }
 
 hipError_t mx4_tiles(const Mx4Args& a, bool bf, bool gated, void* workspace, hipStream_t st) {
-  const int splits = plan(a.m, a.n, a.k, gated).splits;
+  const Plan p = plan(a.m, a.n, a.k, gated);
   float* part = (float*)workspace;
-  if (gated) return bf ? launch<true, true, 4, 4, 1, 4>(a, splits, part, st) : launch<false, true, 4, 4, 1, 4>(a, splits, part, st);
-  return bf ? launch<true, false, 4, 4, 1, 4>(a, splits, part, st) : launch<false, false, 4, 4, 1, 4>(a, splits, part, st);
+  if (gated) return bf ? launch_plan<true, true>(a, p, part, st) : launch_plan<false, true>(a, p, part, st);
+  return bf ? launch_plan<true, false>(a, p, part, st) : launch_plan<false, false>(a, p, part, st);
 }
 
 }  // namespace t2w

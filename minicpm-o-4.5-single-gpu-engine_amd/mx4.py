@@ -29,7 +29,6 @@ _WEIGHTS = _DTYPES | {torch.float32: 2}
 _ACTS = {"silu": 0, "gelu": 1}
 _E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 _F32 = torch.float32
-FEW_ROWS = 16      # up to here a linear or gated call needs no workspace
 
 
 class MX4Weight:
@@ -111,7 +110,7 @@ def _input(x: torch.Tensor, w: MX4Weight) -> int:
     if x.dtype not in _DTYPES:
         raise ValueError("mx4: x must be bfloat16 or float16")
     if x.shape[0] > 0x7FFFFFFF:  # the struct's int would wrap
-        raise ValueError("mx4: at most 2^21 rows")
+        raise ValueError("mx4: at most 2^20 rows")
     return _rows("x", x, None, w.k, x.dtype, w.device)
 
 
@@ -129,7 +128,7 @@ def _run(name: str, a, dev, workspace) -> None:
     """The call ``t2w_mx4_<name>`` with the caller's workspace or one of its own."""
     L = _lib.lib()
     if workspace is None:
-        need = getattr(L, f"t2w_mx4_{name}_workspace_bytes")(C.byref(a)) if a.m > FEW_ROWS or name == "ffn" else 0
+        need = getattr(L, f"t2w_mx4_{name}_workspace_bytes")(C.byref(a))
         if need:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     elif workspace.device != dev or not workspace.is_contiguous():

@@ -29,7 +29,7 @@ def linear_args(**kw):
     return _lib.MX4LinearArgs(**({"x": 1 * M, "ldx": 256, "dtype": 0, "m": 4, "w": w, "bias": 2 * M, "residual": 3 * M, "ldr": 64, "y": 4 * M, "ldy": 64} | kw))
 
 
-ROWS_BAD = [({"dtype": 2}, "dtype"), ({"m": -1}, "m must be"), ({"m": (1 << 21) + 1}, "m must be"), ({"x": None}, "null rows"), ({"y": None}, "null rows"),
+ROWS_BAD = [({"dtype": 2}, "dtype"), ({"m": -1}, "m must be"), ({"m": (1 << 20) + 1}, "m must be"), ({"x": None}, "null rows"), ({"y": None}, "null rows"),
             ({"x": M + 8}, "aligned"), ({"ldx": 260}, "aligned"), ({"y": 4 * M + 1}, "misaligned"), ({"ldx": 248}, "rows overlap"), ({"ldy": 63}, "rows overlap"),
             ({"y": M + 64}, "overlap x")]
 LINEAR_BAD = ROWS_BAD + [({"n": 0}, "n must be"), ({"n": (1 << 24) + 1}, "n must be"), ({"k": 4}, "k must be"), ({"k": 252}, "k must be"), ({"k": (1 << 20) + 8}, "k must be"),
@@ -76,22 +76,22 @@ def test_workspaces():
     """None for few rows; beyond, bounded whatever the sizes; too small, misaligned or overlapping ones are refused."""
     L = _lib.lib()
     need = lambda **kw: L.t2w_mx4_linear_workspace_bytes(C.byref(linear_args(**kw)))  # noqa: E731
-    assert need(m=1) == need(m=16) == need(m=0) == need(m=64, k=12) == 0
-    split = need(m=64, n=512, k=4096, ldx=4096, ldy=512, ldr=512)
+    assert need(m=1) == need(m=16) == need(m=0) == need(m=64, k=12) == 0  # (k=256: the rows fit the LDS)
+    split = need(m=64, n=512, k=14336, ldx=14336, ldy=512, ldr=512)
     assert split > 0
-    for m in (17, 64, 65, 200, 1000, 1 << 21):
+    for m in (17, 64, 65, 200, 1000, 1 << 20):
         for n in (1, 100, 4096, 100000, 1 << 24):
             for k in (8, 1024, 14336, 1 << 20):
                 assert need(m=m, n=n, k=k) <= 34 << 20
                 g = _lib.MX4GatedArgs(x=M, ldx=k, dtype=0, m=m, gate=weight(n, k), up=weight(n, k), act=0, y=M, ldy=n)
                 assert L.t2w_mx4_gated_workspace_bytes(C.byref(g)) <= 34 << 20
-    big = {"m": 64, "n": 512, "k": 4096, "ldx": 4096, "ldy": 512, "ldr": 512}
+    big = {"m": 64, "n": 512, "k": 14336, "ldx": 14336, "ldy": 512, "ldr": 512}
     for kw, text in (({}, "too small"), ({"workspace": 50 * M, "workspace_bytes": split - 1}, "too small"), ({"workspace": 50 * M + 8, "workspace_bytes": split}, "aligned"),
                      ({"workspace": 4 * M, "workspace_bytes": split}, "workspace overlaps"), ({"workspace": M, "workspace_bytes": split}, "workspace overlaps"),
                      ({"workspace": 3 * M, "workspace_bytes": split}, "workspace overlaps"), ({"workspace": 100 * M, "workspace_bytes": split}, "workspace overlaps"),
                      ({"workspace": 2 * M - 16, "workspace_bytes": split}, "workspace overlaps")):
         refused(L.t2w_mx4_linear, linear_args(**(big | kw)), text)
-    g = {"x": M, "ldx": 4096, "dtype": 0, "m": 64, "gate": weight(512, 4096), "up": weight(512, 4096, at=140), "act": 0, "y": 4 * M, "ldy": 512}
+    g = {"x": M, "ldx": 14336, "dtype": 0, "m": 64, "gate": weight(512, 14336), "up": weight(512, 14336, at=140), "act": 0, "y": 4 * M, "ldy": 512}
     need_g = L.t2w_mx4_gated_workspace_bytes(C.byref(_lib.MX4GatedArgs(**g)))
     for kw, text in (({}, "too small"), ({"workspace": 4 * M, "workspace_bytes": need_g}, "workspace overlaps"), ({"workspace": 140 * M, "workspace_bytes": need_g}, "workspace overlaps")):
         refused(L.t2w_mx4_gated, _lib.MX4GatedArgs(**(g | kw)), text)
