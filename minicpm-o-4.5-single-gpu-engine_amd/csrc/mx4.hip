@@ -101,6 +101,9 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Args a) {
     if (gn < nb) unit(std::true_type{}, gn, first);
     else unit(std::false_type{}, 0, 0);
     u = first;
+    const int n = g * 16 + 4 * q, m = m0 + (lane & 15);
+    Extra ex{};
+    if (!GATED && wave == 0) ex = fetch<BF>(a, m, n);
     f32x4* p = part + turn * waves * 64;
     p[wave * 64 + lane] = acc[0] + acc[1];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the codes in flight are not waited for
@@ -112,15 +115,12 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Args a) {
         v += p[(GATED ? 2 * i : i) * 64 + lane];
         if constexpr (GATED) o += p[(2 * i + 1) * 64 + lane];
       }
-      const int n = g * 16 + 4 * q, m = m0 + (lane & 15);
-      if (m < a.m && n < a.n) {
-        float r[4] = {v[0], v[1], v[2], v[3]};
-        if constexpr (GATED) {
+      float r[4] = {v[0], v[1], v[2], v[3]};
+      if constexpr (GATED) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) r[e] = gate_act(r[e], a.act) * o[e];
-        }
-        finish<BF>(a, m, n, r);
+        for (int e = 0; e < 4; ++e) r[e] = gate_act(r[e], a.act) * o[e];
       }
+      finish<BF>(a, m, n, r, ex);
     }
     g = gn;
   }

@@ -46,35 +46,58 @@ __device__ __forceinline__ uint16_t round1(float v) {
 
 __device__ __forceinline__ float gate_act(float g, int act) { return act == T2W_MX4_SILU ? silu(g) : gelu_tanh(g); }
 
-// Outputs n .. n + 3 of row m from their sums
+// What outputs n .. n + 3 of row m need besides their sums, as loaded: ahead of the stores (the compiler may not move a load
+// across them, as the residual may be y itself), so that an epilogue waits for memory once and not for every block.  Places
+// behind the last read the last.
+struct Extra {
+  float bias[4];
+  uint32_t res[4];  // quad: two words, else four values
+};
+
 template <bool BF>
-__device__ __forceinline__ void finish(const Mx4Args& a, int m, int n, const float (&v)[4]) {
-  const long long o = (long long)m * a.ldy + n;
-  uint16_t* y = (uint16_t*)a.y;
+__device__ __forceinline__ Extra fetch(const Mx4Args& a, int m, int n) {
+  Extra x = {{0.f, 0.f, 0.f, 0.f}, {0, 0, 0, 0}};
+  const uint16_t* res = (const uint16_t*)a.residual + (long long)min(m, a.m - 1) * a.ldr;
   if (a.quad) {
-    float r[4] = {v[0], v[1], v[2], v[3]};
+    const int c = min(n, a.n - 4);
     if (a.bias) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] += a.bias[n + e];
+      for (int e = 0; e < 4; ++e) x.bias[e] = a.bias[c + e];
     }
     if (a.residual) {
-      const uint2 h = *(const uint2*)((const uint16_t*)a.residual + (long long)m * a.ldr + n);
-      r[0] += BF ? lo2f(h.x) : lo2h(h.x);
-      r[1] += BF ? hi2f(h.x) : hi2h(h.x);
-      r[2] += BF ? lo2f(h.y) : lo2h(h.y);
-      r[3] += BF ? hi2f(h.y) : hi2h(h.y);
+      const uint2 h = *(const uint2*)(res + c);
+      x.res[0] = h.x, x.res[1] = h.y;
     }
-    *(uint2*)(y + o) = BF ? make_uint2(pack2(r[0], r[1]), pack2(r[2], r[3])) : make_uint2(pack2h(r[0], r[1]), pack2h(r[2], r[3]));
-    return;
+    return x;
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    if (n + e >= a.n) break;
-    float r = v[e];
-    if (a.bias) r += a.bias[n + e];
-    if (a.residual) r += load1<BF>(a.residual, (long long)m * a.ldr + n + e);
-    y[o + e] = round1<BF>(r);
+    const int c = min(n + e, a.n - 1);
+    if (a.bias) x.bias[e] = a.bias[c];
+    if (a.residual) x.res[e] = res[c];
   }
+  return x;
+}
+
+// Outputs n .. n + 3 of row m from their sums
+template <bool BF>
+__device__ __forceinline__ void finish(const Mx4Args& a, int m, int n, const float (&v)[4], const Extra& x) {
+  if (m >= a.m || n >= a.n) return;
+  uint16_t* y = (uint16_t*)a.y + (long long)m * a.ldy + n;
+  float r[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r[e] = v[e] + x.bias[e];
+  if (a.quad) {
+    r[0] += BF ? lo2f(x.res[0]) : lo2h(x.res[0]);
+    r[1] += BF ? hi2f(x.res[0]) : hi2h(x.res[0]);
+    r[2] += BF ? lo2f(x.res[1]) : lo2h(x.res[1]);
+    r[3] += BF ? hi2f(x.res[1]) : hi2h(x.res[1]);
+    *(uint2*)y = BF ? make_uint2(pack2(r[0], r[1]), pack2(r[2], r[3])) : make_uint2(pack2h(r[0], r[1]), pack2h(r[2], r[3]));
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n + e < a.n) y[e] = round1<BF>(r[e] + (BF ? lo2f(x.res[e]) : lo2h(x.res[e])));
 }
 
 }  // namespace

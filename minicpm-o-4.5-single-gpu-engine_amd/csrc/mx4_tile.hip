@@ -49,7 +49,7 @@ struct MxTile {
     }
     // blocks behind the last are out of bounds as well
     constexpr int WB = GATED ? TN / 2 : TN;
-    const int b0 = nt * CB + wn * WB, have = max(0, min(WB, ((a.n + 15) >> 4) - b0));
+    const int b0 = __builtin_amdgcn_readfirstlane(nt * CB + wn * WB), have = __builtin_amdgcn_readfirstlane(max(0, min(WB, ((a.n + 15) >> 4) - b0)));
 #pragma unroll
     for (int g = 0; g < (GATED ? 2 : 1); ++g) {
       wr[g] = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w[g] + (size_t)b0 * steps * 1024), 0, have * steps * 1024, 0x00020000);
@@ -153,19 +153,23 @@ struct MxTile {
   }
 };
 
-// outputs of block (t, i) of a wave from its sums p (and u of the second matrix)
-template <bool BF, bool GATED, int TM, int TN, int WM, int WN>
-__device__ __forceinline__ void block_store(const Mx4Args& a, int mt, int nt, int wave, int t, int i, f32x4 p, f32x4 u) {
+// first output (row, channel) of this lane in block (t, i) of a wave
+template <bool GATED, int TM, int TN, int WM, int WN>
+__device__ __forceinline__ int2 place(int mt, int nt, int wave, int t, int i) {
   const int lane = threadIdx.x & 63, wm = wave / WN, wn = wave % WN;
   constexpr int OT = GATED ? TN / 2 : TN;
-  const int m = (mt * WM + wm) * 16 * TM + 16 * i + (lane & 15), n = ((nt * WN + wn) * OT + t) * 16 + 4 * (lane >> 4);
-  if (m >= a.m || n >= a.n) return;
+  return make_int2((mt * WM + wm) * 16 * TM + 16 * i + (lane & 15), ((nt * WN + wn) * OT + t) * 16 + 4 * (lane >> 4));
+}
+
+// the outputs at a place from their sums p (and u of the second matrix)
+template <bool BF, bool GATED>
+__device__ __forceinline__ void block_store(const Mx4Args& a, int2 at, f32x4 p, f32x4 u, const Extra& ex) {
   float o[4] = {p[0], p[1], p[2], p[3]};
   if constexpr (GATED) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = gate_act(o[e], a.act) * u[e];
   }
-  finish<BF>(a, m, n, o);
+  finish<BF>(a, at.x, at.y, o, ex);
 }
 
 // tile number b of tm x tn tiles -> (row, column): an XCD gets a run of tiles (workgroups go round the 8 XCDs), which walks
@@ -223,10 +227,19 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx4_tile_kernel(const Mx
       for (int i = 0; i < TM; ++i) p[(y * TM + i) * 64] = t.acc[y][i];
   } else {
     constexpr int OT = GATED ? TN / 2 : TN;
+    Extra ex[OT][TM];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int y = 0; y < OT; ++y) block_store<BF, GATED, TM, TN, WM, WN>(a, at.x, at.y, t.wave, y, i, t.acc[y][i], t.acc[GATED ? y + OT : y][i]);
+      for (int y = 0; y < OT; ++y) {
+        const int2 o = place<GATED, TM, TN, WM, WN>(at.x, at.y, t.wave, y, i);
+        ex[y][i] = GATED ? Extra{} : fetch<BF>(a, o.x, o.y);
+      }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int y = 0; y < OT; ++y)
+        block_store<BF, GATED>(a, place<GATED, TM, TN, WM, WN>(at.x, at.y, t.wave, y, i), t.acc[y][i], t.acc[GATED ? y + OT : y][i], ex[y][i]);
   }
 }
 
@@ -240,6 +253,8 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const Mx4Args a, int tm, 
   const int2 at = tile_at(w / NW, tm, tn);
   const size_t stride = (size_t)tm * tn * NW * (TM * TN * 64);
   const f32x4* p = part + ((size_t)w * (TM * TN) + blk) * 64 + lane;
+  const int2 o = place<GATED, TM, TN, WM, WN>(at.x, at.y, w % NW, blk / TM, blk % TM);
+  const Extra ex = GATED ? Extra{} : fetch<BF>(a, o.x, o.y);
   f32x4 v = p[0], u = f32x4{0.f, 0.f, 0.f, 0.f};
   if constexpr (GATED) u = p[OT * TM * 64];
 #pragma unroll 4
@@ -247,7 +262,7 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const Mx4Args a, int tm, 
     v += p[s * stride];
     if constexpr (GATED) u += p[s * stride + OT * TM * 64];
   }
-  block_store<BF, GATED, TM, TN, WM, WN>(a, at.x, at.y, w % NW, blk / TM, blk % TM, v, u);
+  block_store<BF, GATED>(a, o, v, u, ex);
 }
 
 template <bool BF, bool GATED, int TM, int TN, int WM, int WN, int D, int KG>
@@ -264,21 +279,21 @@ hipError_t launch(const Mx4Args& a, int splits, float* part, hipStream_t st) {
 }
 
 // The tiles, each with four waves side by side: rows, weight channels (gated: half of each matrix), groups of waves that split k, and
-// what a pass of its stages takes in microseconds with one workgroup on a CU and, of each, with several (measured: 14336 columns
-// by 16 to 300 rows).  The narrow ones finish a stage sooner, the wide one moves least: 64 rows x 14336 x 4096, both matrices,
-// took 25.1 / 25.4 / 28.7 us (the wide one with k in two parts), 2005 rows 60% more / 5% more / 370 us.
+// the microseconds of a pass (a stage of each group) with one workgroup on a CU and, of each, with several.  Measured: 4096
+// channels x 14336 columns x 32 rows take 38 / 84 / 106 us (k in parts: 16 / 19 / 20), 14336 x 4096 x 2, gated, of 200 rows 70 / 54 / 56
+// and of 2005 rows 620 / 374 / 360.
 struct Shape {
   int bm, bn, kg;
   float one, many;
 };
-constexpr Shape SHAPES[3] = {{32, 128, 2, 0.60f, 0.60f}, {64, 128, 1, 0.59f, 0.48f}, {64, 256, 1, 1.00f, 0.85f}};
+constexpr Shape SHAPES[3] = {{32, 128, 2, 0.55f, 0.62f}, {64, 128, 1, 0.70f, 0.44f}, {64, 256, 1, 0.90f, 0.79f}};
 
 struct Plan {
   int shape, tiles, splits;
   float us;
 };
 
-// The cheapest by that model: 5 us for a launch, its first loads and stores; where k is split over workgroups 3 us and the
+// The cheapest by that model: 5 us for a launch, its first loads and stores; where k is split over workgroups 4.5 us and the
 // parts' way to memory and back (8 TB/s) more.  k is split so that the workgroups fill the 256 CUs once or twice, 512 at most.
 Plan plan(int m, int n, int k, bool gated) {
   Plan best{0, 0, 1, 3e38f};
@@ -296,7 +311,7 @@ Plan plan(int m, int n, int k, bool gated) {
       // several workgroups a CU share it; the last round counts whole while rounds are few
       const float turns = wgs <= 256 ? s.one : s.many * (wgs < 2048 ? (float)((wgs + 255) / 256) : (float)wgs / 256);
       float us = 5.f + passes * turns;
-      if (splits > 1) us += 3.f + (float)wgs * s.bm * s.bn * 8 / 8e6f;
+      if (splits > 1) us += 4.5f + (float)wgs * s.bm * s.bn * 8 / 8e6f;
       if (us < best.us) best = {i, (int)std::min<long long>(tiles, 1 << 30), splits, us};
     }
   }
@@ -307,7 +322,7 @@ template <bool BF, bool GATED>
 hipError_t launch_plan(const Mx4Args& a, const Plan& p, float* part, hipStream_t st) {
   switch (p.shape) {
     case 0: return launch<BF, GATED, 2, 2, 1, 4, 4, 2>(a, p.splits, part, st);
-    case 1: return launch<BF, GATED, 4, 2, 1, 4, 4, 1>(a, p.splits, part, st);
+    case 1: return launch<BF, GATED, 4, 2, 1, 4, 2, 1>(a, p.splits, part, st);
     default: return launch<BF, GATED, 4, 4, 1, 4, 2, 1>(a, p.splits, part, st);
   }
 }

@@ -24,13 +24,22 @@ __global__ __launch_bounds__(256) void rope_kernel(const t2w_rope_args a, int he
   const int wid = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
   const int total = (int)gridDim.x * 4;
   if (sub >= hpw) return;
-  const int heads = a.q_heads + a.k_heads;
+  const int heads = a.q_heads + a.k_heads, at0 = HALVES ? 8 * i : 16 * i, at1 = HALVES ? 8 * i + (a.rot >> 1) : 16 * i + 8;
   uint64_t freq[8];
   int axis[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) freq[e] = a.freq[8 * i + e], axis[e] = a.axis[8 * i + e];
   for (int item = wid; item < a.n_tok * head_splits; item += total) {
     const int tok = item / head_splits, split = item - tok * head_splits;
+    const auto source = [&](int h) {
+      return h < a.q_heads ? (const uint16_t*)a.q + (long long)tok * a.ldq + h * a.head_dim
+                           : (const uint16_t*)a.k + (long long)tok * a.ldk + (h - a.q_heads) * a.head_dim;
+    };
+    int h = split * hpw + sub;
+    if (h >= heads) continue;
+    // a head's channels are on their way while the angles, then while the head before are worked on
+    const uint16_t* src = source(h);
+    uint4 u0 = *(const uint4*)(src + at0), u1 = *(const uint4*)(src + at1);
     float cs[8], sn[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -39,14 +48,16 @@ __global__ __launch_bounds__(256) void rope_kernel(const t2w_rope_args a, int he
       sincospif((float)turn * 0x1p-31f, &sn[e], &cs[e]);
       sn[e] *= a.scale, cs[e] *= a.scale;
     }
-    for (int h = split * hpw + sub; h < heads; h += head_splits * hpw) {
-      const bool isq = h < a.q_heads;
-      const int hh = isq ? h : h - a.q_heads;
-      const uint16_t* src = (const uint16_t*)(isq ? a.q : a.k) + (long long)tok * (isq ? a.ldq : a.ldk) + hh * a.head_dim;
-      uint16_t* dst = (uint16_t*)(isq ? a.q_out : a.k_out) + (long long)tok * (isq ? a.ldq_out : a.ldk_out) + hh * a.head_dim;
-      const int at0 = HALVES ? 8 * i : 16 * i, at1 = HALVES ? 8 * i + (a.rot >> 1) : 16 * i + 8;
-      const uint4 u0 = *(const uint4*)(src + at0), u1 = *(const uint4*)(src + at1);
+    while (true) {
+      const int next = h + head_splits * hpw;
       const uint32_t w[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+      const uint16_t* here = src;
+      if (next < heads) {
+        src = source(next);
+        u0 = *(const uint4*)(src + at0), u1 = *(const uint4*)(src + at1);
+      }
+      uint16_t* dst = h < a.q_heads ? (uint16_t*)a.q_out + (long long)tok * a.ldq_out + h * a.head_dim
+                                    : (uint16_t*)a.k_out + (long long)tok * a.ldk_out + (h - a.q_heads) * a.head_dim;
       float v[16];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[2 * e] = BF ? lo2f(w[e]) : lo2h(w[e]), v[2 * e + 1] = BF ? hi2f(w[e]) : hi2h(w[e]);
@@ -62,8 +73,10 @@ __global__ __launch_bounds__(256) void rope_kernel(const t2w_rope_args a, int he
       for (int e = 0; e < 8; ++e) r[e] = BF ? pack2(o[2 * e], o[2 * e + 1]) : pack2h(o[2 * e], o[2 * e + 1]);
       *(uint4*)(dst + at0) = make_uint4(r[0], r[1], r[2], r[3]);
       *(uint4*)(dst + at1) = make_uint4(r[4], r[5], r[6], r[7]);
-      if (src != dst)
-        for (int c = a.rot + 8 * i; c < a.head_dim; c += 8 * lph) *(uint4*)(dst + c) = *(const uint4*)(src + c);
+      if (here != dst)
+        for (int c = a.rot + 8 * i; c < a.head_dim; c += 8 * lph) *(uint4*)(dst + c) = *(const uint4*)(here + c);
+      if (next >= heads) break;
+      h = next;
     }
   }
 }

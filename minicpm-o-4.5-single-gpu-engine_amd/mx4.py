@@ -29,6 +29,7 @@ _WEIGHTS = _DTYPES | {torch.float32: 2}
 _ACTS = {"silu": 0, "gelu": 1}
 _E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 _F32 = torch.float32
+IN_LDS = 4096      # columns of 16 rows that fit the LDS: such calls need no workspace
 
 
 class MX4Weight:
@@ -95,47 +96,53 @@ class MX4Weight:
         return v.permute(0, 3, 1, 2, 4).reshape(16 * blocks, 128 * steps)[:self.n, :self.k].contiguous()
 
 
+# A step's calls take 4 to 8 us on the GPU, about what the host needs for a call: the checks below look at each property once.
+
 def _rows(what: str, t: torch.Tensor, m, width: int, dtype, dev) -> int:
     """Elements between the rows of [m, width]."""
-    if t.dim() != 2 or t.dtype is not dtype or t.device != dev:
+    shape = t.shape
+    if t.dtype is not dtype or len(shape) != 2 or t.device != dev:
         raise ValueError(f"mx4: {what} must be {dtype} [rows, {width}] on {dev}")
-    n, k = t.shape
     ld, one = t.stride()
-    if k != width or (m is not None and n != m) or (one != 1 and k > 1):
+    if shape[1] != width or (m is not None and shape[0] != m) or (one != 1 and width > 1):
         raise ValueError(f"mx4: {what} must be [{'rows' if m is None else m}, {width}], each row contiguous")
-    return ld if n > 1 else width
+    return ld if shape[0] > 1 else width
 
 
-def _input(x: torch.Tensor, w: MX4Weight) -> int:
-    if x.dtype not in _DTYPES:
+def _input(x: torch.Tensor, w: MX4Weight) -> tuple[int, int, int]:
+    """x's pointer, row stride, type and rows: the first fields of a call's arguments."""
+    dtype = x.dtype
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise ValueError("mx4: x must be bfloat16 or float16")
-    if x.shape[0] > 0x7FFFFFFF:  # the struct's int would wrap
+    ld, m = _rows("x", x, None, w.k, dtype, w.device), x.shape[0]
+    if m > 0x7FFFFFFF:  # the struct's int would wrap
         raise ValueError("mx4: at most 2^20 rows")
-    return _rows("x", x, None, w.k, x.dtype, w.device)
+    return x.data_ptr(), ld, code, m
 
 
-def _output(x: torch.Tensor, n: int, out) -> tuple[torch.Tensor, int]:
+def _output(x: torch.Tensor, m: int, n: int, out, dev) -> tuple[torch.Tensor, int]:
     if out is None:
-        return torch.empty((x.shape[0], n), dtype=x.dtype, device=x.device), n
-    return out, _rows("out", out, x.shape[0], n, x.dtype, x.device)
+        return torch.empty((m, n), dtype=x.dtype, device=dev), n
+    return out, _rows("out", out, m, n, x.dtype, dev)
 
 
-def _residual(x: torch.Tensor, n: int, residual) -> tuple:
-    return (None, 0) if residual is None else (residual.data_ptr(), _rows("residual", residual, x.shape[0], n, x.dtype, x.device))
+def _residual(x: torch.Tensor, m: int, n: int, residual, dev) -> tuple:
+    return (None, 0) if residual is None else (residual.data_ptr(), _rows("residual", residual, m, n, x.dtype, dev))
 
 
-def _run(name: str, a, dev, workspace) -> None:
-    """The call ``t2w_mx4_<name>`` with the caller's workspace or one of its own."""
-    L = _lib.lib()
-    if workspace is None:
-        need = getattr(L, f"t2w_mx4_{name}_workspace_bytes")(C.byref(a))
+def _run(fn, workspace_bytes, a, dev, workspace, what: str) -> None:
+    """A call with the caller's workspace or one of its own (``workspace_bytes`` None: the call needs none)."""
+    if workspace is not None:
+        if workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError("mx4: a contiguous workspace on the weights' device")
+    elif workspace_bytes is not None:
+        need = workspace_bytes(C.byref(a))
         if need:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or not workspace.is_contiguous():
-        raise ValueError("mx4: a contiguous workspace on the weights' device")
     if workspace is not None:
         a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _lib.launch(getattr(L, f"t2w_mx4_{name}"), a, dev, f"mx4_{name}")
+    _lib.launch(fn, a, dev, what)
 
 
 def linear(x: torch.Tensor, w: MX4Weight, *, bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
@@ -143,15 +150,18 @@ def linear(x: torch.Tensor, w: MX4Weight, *, bias: torch.Tensor | None = None, r
     """x w^T + bias + residual: ``x`` [rows, k] bf16 or fp16 (rows may be strided by multiples of 8), ``bias`` fp32 [n], ``residual``
     [rows, n] of x's type.  ``out`` may be ``residual``.  ``workspace``: memory for calls that make none
     (``t2w_mx4_linear_workspace_bytes``)."""
-    ldx, dev = _input(x, w), w.device
-    out, ldy = _output(x, w.n, out)
+    dev, n = w.device, w.n
+    rows = _input(x, w)
+    m = rows[3]
+    out, ldy = _output(x, m, n, out, dev)
     b = None
     if bias is not None:
-        if bias.dtype is not _F32 or bias.shape != (w.n,) or bias.device != dev or not bias.is_contiguous():
-            raise ValueError(f"mx4: bias must be a contiguous float32 vector of {w.n} on {dev}")
+        if bias.dtype is not _F32 or bias.shape != (n,) or bias.device != dev or not bias.is_contiguous():
+            raise ValueError(f"mx4: bias must be a contiguous float32 vector of {n} on {dev}")
         b = bias.data_ptr()
-    a = _lib.MX4LinearArgs(x.data_ptr(), ldx, _DTYPES[x.dtype], x.shape[0], w.struct, b, *_residual(x, w.n, residual), out.data_ptr(), ldy)
-    _run("linear", a, dev, workspace)
+    L = _lib.lib()
+    a = _lib.MX4LinearArgs(*rows, w.struct, b, *_residual(x, m, n, residual, dev), out.data_ptr(), ldy)
+    _run(L.t2w_mx4_linear, L.t2w_mx4_linear_workspace_bytes if m > 16 or w.k > IN_LDS else None, a, dev, workspace, "mx4_linear")
     return out
 
 
@@ -166,10 +176,11 @@ def _pair(gate: MX4Weight, up: MX4Weight, act: str) -> int:
 def gated(x: torch.Tensor, gate: MX4Weight, up: MX4Weight, *, act: str = "silu", out: torch.Tensor | None = None,
           workspace: torch.Tensor | None = None) -> torch.Tensor:
     """act(x gate^T) * (x up^T) in one kernel; ``act`` is "silu" or "gelu" (the tanh form)."""
-    k, ldx = _pair(gate, up, act), _input(x, gate)
-    out, ldy = _output(x, gate.n, out)
-    a = _lib.MX4GatedArgs(x.data_ptr(), ldx, _DTYPES[x.dtype], x.shape[0], gate.struct, up.struct, k, out.data_ptr(), ldy)
-    _run("gated", a, gate.device, workspace)
+    k, rows, dev = _pair(gate, up, act), _input(x, gate), gate.device
+    out, ldy = _output(x, rows[3], gate.n, out, dev)
+    L = _lib.lib()
+    a = _lib.MX4GatedArgs(*rows, gate.struct, up.struct, k, out.data_ptr(), ldy)
+    _run(L.t2w_mx4_gated, L.t2w_mx4_gated_workspace_bytes if rows[3] > 16 or gate.k > IN_LDS else None, a, dev, workspace, "mx4_gated")
     return out
 
 
@@ -177,11 +188,12 @@ def ffn(x: torch.Tensor, gate: MX4Weight, up: MX4Weight, down: MX4Weight, *, act
         out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """(act(x gate^T) * (x up^T)) down^T + residual.  The inner values are rounded to x's type (of fp16, beyond 65504 they are
     infinite).  ``out`` may be ``residual``."""
-    k, ldx, dev = _pair(gate, up, act), _input(x, gate), gate.device
+    k, rows, dev = _pair(gate, up, act), _input(x, gate), gate.device
     if down.device != dev:
         raise ValueError("mx4: the weights must be on one device")
-    out, ldy = _output(x, down.n, out)
-    a = _lib.MX4FFNArgs(x.data_ptr(), ldx, _DTYPES[x.dtype], x.shape[0], gate.struct, up.struct, down.struct, k, *_residual(x, down.n, residual),
-                        out.data_ptr(), ldy)
-    _run("ffn", a, dev, workspace)
+    m, n = rows[3], down.n
+    out, ldy = _output(x, m, n, out, dev)
+    L = _lib.lib()
+    a = _lib.MX4FFNArgs(*rows, gate.struct, up.struct, down.struct, k, *_residual(x, m, n, residual, dev), out.data_ptr(), ldy)
+    _run(L.t2w_mx4_ffn, L.t2w_mx4_ffn_workspace_bytes, a, dev, workspace, "mx4_ffn")
     return out

@@ -62,46 +62,49 @@ class Rope:
         """Turns ``q`` [n_tok, heads, head_dim] and ``k`` [n_tok, kv_heads, head_dim] (or None), bf16 or fp16, token rows strided by
         multiples of 8.  ``pos`` int32 [axes, n_tok] ([n_tok] for one axis), with at least the axes that the pairs count on.  The
         outputs, new tensors by default, may be ``q`` and ``k`` themselves."""
-        dev = self.device
-        if q.dtype not in _DTYPES:
+        dev, dtype = self.device, q.dtype
+        code = _DTYPES.get(dtype)
+        if code is None:
             raise ValueError("rope: q must be bfloat16 or float16")
         n, heads, d = q.shape if q.dim() == 3 else (0, 0, 0)
-        ldq = _tokens("q", q, n, d, q.dtype, dev)
+        ldq = _tokens("q", q, n, heads, d, dtype, dev)
         if pos.dim() == 1:
             pos = pos[None]
-        if pos.dtype is not _I32 or pos.dim() != 2 or pos.shape[1] != n or pos.device != dev or (pos.stride(1) != 1 and n > 1):
+        shape = pos.shape
+        if pos.dtype is not _I32 or len(shape) != 2 or shape[1] != n or pos.device != dev or (pos.stride(1) != 1 and n > 1):
             raise ValueError(f"rope: pos must be int32 [axes, {n}] on {dev}, each row contiguous")
-        if pos.shape[0] < self.n_axes:
-            raise ValueError(f"rope: pos must have the {self.n_axes} axes that the pairs count on")
+        axes = self.n_axes
+        if shape[0] < axes:
+            raise ValueError(f"rope: pos must have the {axes} axes that the pairs count on")
         if q_out is None:
-            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        elif q_out.shape != q.shape:
-            raise ValueError("rope: q_out must have q's shape")
+            q_out, ldo = torch.empty_like(q, memory_format=torch.contiguous_format), heads * d
+        else:
+            ldo = ldq if q_out is q else _tokens("q_out", q_out, n, heads, d, dtype, dev)
         if max(n, heads, d) > 0x7FFFFFFF:  # the struct's ints would wrap
             raise ValueError("rope: at most 2^24 tokens")
-        a = _lib.RopeArgs(q=q.data_ptr(), q_out=q_out.data_ptr(), ldq=ldq, ldq_out=_tokens("q_out", q_out, n, d, q.dtype, dev), dtype=_DTYPES[q.dtype],
-                          n_tok=n, q_heads=heads, head_dim=d, rot=self.rot, pairs=_PAIRS[self.pairs], freq=self._freq.data_ptr(),
-                          axis=self._axis.data_ptr(), pos=pos.data_ptr(), ld_pos=pos.stride(0) if self.n_axes > 1 else n, n_axes=self.n_axes, scale=self.scale)
+        kp = ko = None
+        g = ldk = ldko = 0
         if k is not None:
-            a.ldk = _tokens("k", k, n, d, q.dtype, dev)
+            g = k.shape[1] if k.dim() == 3 else 0
+            ldk = _tokens("k", k, n, g, d, dtype, dev)
             if k_out is None:
-                k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
-            elif k_out.shape != k.shape:
-                raise ValueError("rope: k_out must have k's shape")
-            a.ldk_out = _tokens("k_out", k_out, n, d, q.dtype, dev)
-            a.k, a.k_out, a.k_heads = k.data_ptr(), k_out.data_ptr(), k.shape[1]
+                k_out, ldko = torch.empty_like(k, memory_format=torch.contiguous_format), g * d
+            else:
+                ldko = ldk if k_out is k else _tokens("k_out", k_out, n, g, d, dtype, dev)
+            kp, ko = k.data_ptr(), k_out.data_ptr()
         elif k_out is not None:
             raise ValueError("rope: k_out without k")
+        a = _lib.RopeArgs(q.data_ptr(), kp, q_out.data_ptr(), ko, ldq, ldk, ldo, ldko, code, n, heads, g, d, self.rot, _PAIRS[self.pairs], self._freq.data_ptr(),
+                          self._axis.data_ptr(), pos.data_ptr(), pos.stride(0) if axes > 1 else n, axes, self.scale)
         _lib.launch(_lib.lib().t2w_rope, a, dev, "rope")
         return q_out, k_out
 
 
-def _tokens(what: str, t: torch.Tensor, n: int, d: int, dtype, dev) -> int:
+def _tokens(what: str, t: torch.Tensor, n: int, heads: int, d: int, dtype, dev) -> int:
     """Elements between the token rows of [n_tok, heads, head_dim] (a token's heads lie side by side)."""
-    if t.dim() != 3 or t.dtype is not dtype or t.device != dev:
+    if t.dtype is not dtype or t.dim() != 3 or t.device != dev:
         raise ValueError(f"rope: {what} must be {dtype} [n_tok, heads, head_dim] on {dev}")
-    rows, heads, width = t.shape
     ld, head, one = t.stride()
-    if rows != n or width != d or one != 1 or (head != d and heads > 1):
-        raise ValueError(f"rope: {what} must be [{n}, heads, {d}], a token's heads side by side")
-    return ld if rows > 1 else heads * d
+    if t.shape != (n, heads, d) or one != 1 or (head != d and heads > 1):
+        raise ValueError(f"rope: {what} must be [{n}, {heads}, {d}], a token's heads side by side")
+    return ld if n > 1 else heads * d
