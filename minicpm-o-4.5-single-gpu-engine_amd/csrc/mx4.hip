@@ -45,22 +45,24 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Args a) {
   const auto load_scales = [&](int g, int u) { return *(const uint32_t*)(s + ((size_t)g * units + u) * 256 + (uint32_t)(lane * 4)); };
 
   int g = blockIdx.x, u = first;
+  if constexpr (XL) {
+    // a unit's 1 KB of a row at a time, straight to LDS, all in flight together; columns behind k are out of the row's bounds: zeros
+    for (int r = GATED ? wave & 1 : 0; r < rows; r += GATED ? 2 : 1) {
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(x + (long long)r * a.ldx), 0, a.k * 2, 0x00020000);
+      const int c = (lane & ~15) | ((lane ^ r) & 15);
+      for (int b = first; b < units; b += stride)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)(xs + (r * units + b) * 64), 16, c * 16, b * 1024, 0, 0);
+    }
+    asm volatile("" ::: "memory");
+  }
   sc = load_scales(g, u);
 #pragma unroll
   for (int t = 0; t < 4; ++t) load(g, u, t);
-  asm volatile("" ::: "memory");
   if constexpr (XL) {
-    const int chunks = units * 64;  // of a row
-    for (int i = threadIdx.x; i < rows * chunks; i += blockDim.x) {
-      const int r = i / chunks, c = i - r * chunks;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (8 * c < a.k) v = *(const uint4*)(x + (long long)r * a.ldx + 8 * c);
-      xs[r * chunks + ((c & ~15) | ((c ^ r) & 15))] = v;
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(5)" ::: "memory");  // x is there, the codes may still be on their way
     __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
   }
+  asm volatile("" ::: "memory");
   const uint16_t* xrow = x + (long long)row * a.ldx + 32 * q;
 
   f32x4 acc[2];

@@ -7,8 +7,8 @@ namespace t2w {
 
 namespace {
 
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 // eight codes (columns 0 .. 7, the lowest nibble first) times the scale, as the matrix unit's operand
 template <bool BF>

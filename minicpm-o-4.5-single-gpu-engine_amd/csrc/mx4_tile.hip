@@ -17,7 +17,6 @@ namespace t2w {
 
 namespace {
 
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
 constexpr uint32_t OUTSIDE = 0x80000000u, BOUND = 0x7fffff00u;  // byte offsets in the tile's rows of x
 
 template <bool BF, bool GATED, int TM, int TN, int WM, int WN>
@@ -33,7 +32,6 @@ struct MxTile {
   int lane, wave, wm, wn, steps, units;
   __amdgpu_buffer_rsrc_t wr[GATED ? 2 : 1], sr[GATED ? 2 : 1];  // this wave's blocks of each matrix
   f32x4 acc[TN][TM];
-  uint4 xf[TM];
 
   __device__ __forceinline__ MxTile(const Mx4Args& a_, int mt, int nt) : a(a_) {
     lane = threadIdx.x & 63;
@@ -92,13 +90,14 @@ struct MxTile {
   }
   static __device__ __forceinline__ uint32_t word(const uint4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
 
-  // the MFMAs of one step on wf and xf; next to them the fragments (xf in place, wn_) of step jn of the stage in xs / cd
-  __device__ __forceinline__ void step(const uint4 (&wf)[TN], uint4 (&wnx)[TN], const uint4* xs, const Codes& cd, int st, int jn) {
+  // The MFMAs of one step on wf and xf; next to them xf's place is filled with the fragments of step jx in xs and wnx with the
+  // codes of step jn of stage st in cd.
+  __device__ __forceinline__ void step(const uint4 (&wf)[TN], uint4 (&wnx)[TN], uint4 (&xf)[TM], const uint4* xs, int jx, const Codes& cd, int st, int jn) {
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
       for (int t = 0; t < TN; ++t) acc[t][i] = mma<BF>(wf[t], xf[i], acc[t][i]);
-      xf[i] = xread(xs, i, jn);
+      xf[i] = xread(xs, i, jx);
 #pragma unroll
       for (int t = i * TN / TM; t < (i + 1) * TN / TM; ++t)
         wnx[t] = widen<BF>(word(cd.c[t], jn), __uint_as_float(((cd.e[t] >> (8 * (st & 3))) & 0xffu) << 23));
@@ -115,40 +114,62 @@ struct MxTile {
     }
   }
 
-  // stage st in (xc, cc), the next one in (xn, cn); D: the buffers; s1: behind the last
-  template <int D>
-  __device__ __forceinline__ void stage(uint4* xc, uint4* xn, Codes& cc, Codes& cn, uint4 (&w0)[TN], uint4 (&w1)[TN], int st, int s1) {
-    step(w0, w1, xc, cc, st, 1);
-    step(w1, w0, xc, cc, st, 2);
-    step(w0, w1, xc, cc, st, 3);
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((D - 2) * LOADS) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    issue(xc, cc, st + D, s1);
-    step(w1, w0, xn, cn, st + 1, 0);
+  // Stage st in (xc, cc), the next one in (xn, cn); the loads of stage st + D go to (xl, cl).
+  // AHEAD 1: fragments are read a step ahead, which 16 MFMAs a step cover; the barrier stands in front of the last step, when every
+  // wave holds its fragments of the stage, and the freed buffer is the one to load (xl is xc).
+  // AHEAD 2: with 4 MFMAs a step a fragment's way from LDS takes longer than a step, so they are read two ahead into two sets in
+  // turn; the barrier stands in the stage's middle, and a buffer more than D lets xl be one that was read a stage ago.
+  template <int D, int AHEAD>
+  __device__ __forceinline__ void stage(uint4* xc, uint4* xn, uint4* xl, Codes& cc, Codes& cn, Codes& cl, uint4 (&w0)[TN], uint4 (&w1)[TN], uint4 (&xa)[TM],
+                                        uint4 (&xb)[TM], int st, int s1) {
+    if constexpr (AHEAD == 1) {
+      step(w0, w1, xa, xc, 1, cc, st, 1);
+      step(w1, w0, xa, xc, 2, cc, st, 2);
+      step(w0, w1, xa, xc, 3, cc, st, 3);
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((D - 2) * LOADS) : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      issue(xl, cl, st + D, s1);
+      step(w1, w0, xa, xn, 0, cn, st + 1, 0);
+    } else {
+      step(w0, w1, xa, xc, 2, cc, st, 1);
+      step(w1, w0, xb, xc, 3, cc, st, 2);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 2) * LOADS) : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      issue(xl, cl, st + D, s1);
+      step(w0, w1, xa, xn, 0, cc, st, 3);
+      step(w1, w0, xb, xn, 1, cn, st + 1, 0);
+    }
   }
 
-  template <int D>
-  __device__ __forceinline__ void run(uint4* const (&x)[D], int s0, int s1, int n) {
-    Codes c[D];
-    uint4 w0[TN], w1[TN];
+  // D stages in flight over XB buffers
+  template <int D, int XB>
+  __device__ __forceinline__ void run(uint4* const (&x)[XB], int s0, int s1, int n) {
+    constexpr int AHEAD = XB > D ? 2 : 1;
+    Codes c[XB];
+    uint4 w0[TN], w1[TN], xa[TM], xb[TM];
 #pragma unroll
     for (int d = 0; d < D; ++d) issue(x[d], c[d], s0 + d, s1);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * LOADS) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < TM; ++i) xf[i] = xread(x[0], i, 0);
+    for (int i = 0; i < TM; ++i) {
+      xa[i] = xread(x[0], i, 0);
+      if (AHEAD == 2) xb[i] = xread(x[0], i, 1);
+    }
 #pragma unroll
     for (int t = 0; t < TN; ++t) w0[t] = widen<BF>(c[0].c[t].x, __uint_as_float(((c[0].e[t] >> (8 * (s0 & 3))) & 0xffu) << 23));
     int i = 0;
-    for (; i + D <= n; i += D) {
+    for (; i + XB <= n; i += XB) {
 #pragma unroll
-      for (int d = 0; d < D; ++d) stage<D>(x[d], x[(d + 1) % D], c[d], c[(d + 1) % D], w0, w1, s0 + i + d, s1);
+      for (int d = 0; d < XB; ++d)
+        stage<D, AHEAD>(x[d], x[(d + 1) % XB], x[(d + D) % XB], c[d], c[(d + 1) % XB], c[(d + D) % XB], w0, w1, xa, xb, s0 + i + d, s1);
     }
 #pragma unroll
-    for (int d = 0; d < D - 1; ++d)
-      if (i + d < n) stage<D>(x[d], x[d + 1], c[d], c[d + 1], w0, w1, s0 + i + d, s1);
+    for (int d = 0; d < XB - 1; ++d)
+      if (i + d < n) stage<D, AHEAD>(x[d], x[(d + 1) % XB], x[(d + D) % XB], c[d], c[(d + 1) % XB], c[(d + D) % XB], w0, w1, xa, xb, s0 + i + d, s1);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was issued into LDS behind the last stage
   }
 };
@@ -182,11 +203,11 @@ __device__ __forceinline__ int2 tile_at(int b, int tm, int tn) {
 }
 
 // KG groups of waves share a tile, each with its run of the stages and buffers of its own; the first adds up.
-template <bool BF, bool GATED, int TM, int TN, int WM, int WN, int D, int KG, bool PART>
+template <bool BF, bool GATED, int TM, int TN, int WM, int WN, int D, int XB, int KG, bool PART>
 __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx4_tile_kernel(const Mx4Args a, int tm, int tn, int splits, f32x4* part) {
   typedef MxTile<BF, GATED, TM, TN, WM, WN> T;
   constexpr int XS = T::BM * 16;
-  __shared__ uint4 x0[KG * XS], x1[KG * XS], x2[D > 2 ? KG * XS : 1], x3[D > 3 ? KG * XS : 1];  // objects of their own: see the top
+  __shared__ uint4 x0[KG * XS], x1[KG * XS], x2[XB > 2 ? KG * XS : 1], x3[XB > 3 ? KG * XS : 1];  // objects of their own: see the top
   const int total = tm * tn;
   const int split = PART ? (int)blockIdx.x / total : 0, b = (int)blockIdx.x - split * total;
   const int2 at = tile_at(b, tm, tn);
@@ -199,9 +220,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx4_tile_kernel(const Mx
     s0 += kg * n, s1 = min(s1, s0 + n);
   }
   const int xo = kg * XS;
-  if constexpr (D == 2) t.template run<2>({x0 + xo, x1 + xo}, s0, s1, n);
-  else if constexpr (D == 3) t.template run<3>({x0 + xo, x1 + xo, x2 + xo}, s0, s1, n);
-  else t.template run<4>({x0 + xo, x1 + xo, x2 + xo, x3 + xo}, s0, s1, n);
+  if constexpr (XB == 2) t.template run<D, 2>({x0 + xo, x1 + xo}, s0, s1, n);
+  else if constexpr (XB == 3) t.template run<D, 3>({x0 + xo, x1 + xo, x2 + xo}, s0, s1, n);
+  else t.template run<D, 4>({x0 + xo, x1 + xo, x2 + xo, x3 + xo}, s0, s1, n);
   if constexpr (KG > 1) {
     static_assert(KG == 2 && T::NW * TM * TN * 64 <= KG * XS, "the second group's sums fit a buffer");
     __syncthreads();  // every wave is through with the buffers
@@ -265,15 +286,15 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const Mx4Args a, int tm, 
   block_store<BF, GATED>(a, o, v, u, ex);
 }
 
-template <bool BF, bool GATED, int TM, int TN, int WM, int WN, int D, int KG>
+template <bool BF, bool GATED, int TM, int TN, int WM, int WN, int D, int XB, int KG>
 hipError_t launch(const Mx4Args& a, int splits, float* part, hipStream_t st) {
   typedef MxTile<BF, GATED, TM, TN, WM, WN> T;
   const int tm = (a.m + T::BM - 1) / T::BM, tn = (mx4_blocks(a.n) + T::CB - 1) / T::CB;
   if (splits <= 1) {
-    mx4_tile_kernel<BF, GATED, TM, TN, WM, WN, D, KG, false><<<tm * tn, 64 * T::NW * KG, 0, st>>>(a, tm, tn, 1, nullptr);
+    mx4_tile_kernel<BF, GATED, TM, TN, WM, WN, D, XB, KG, false><<<tm * tn, 64 * T::NW * KG, 0, st>>>(a, tm, tn, 1, nullptr);
     return hipGetLastError();
   }
-  mx4_tile_kernel<BF, GATED, TM, TN, WM, WN, D, KG, true><<<tm * tn * splits, 64 * T::NW * KG, 0, st>>>(a, tm, tn, splits, (f32x4*)part);
+  mx4_tile_kernel<BF, GATED, TM, TN, WM, WN, D, XB, KG, true><<<tm * tn * splits, 64 * T::NW * KG, 0, st>>>(a, tm, tn, splits, (f32x4*)part);
   mx4_join_kernel<BF, GATED, TM, TN, WM, WN><<<(tm * tn * T::NW * TM * (GATED ? TN / 2 : TN) + 3) / 4, 256, 0, st>>>(a, tm, tn, splits, (const f32x4*)part);
   return hipGetLastError();
 }
@@ -286,7 +307,7 @@ struct Shape {
   int bm, bn, kg;
   float one, many;
 };
-constexpr Shape SHAPES[3] = {{32, 128, 2, 0.55f, 0.62f}, {64, 128, 1, 0.70f, 0.44f}, {64, 256, 1, 0.90f, 0.79f}};
+constexpr Shape SHAPES[3] = {{32, 128, 2, 0.52f, 0.60f}, {64, 128, 1, 0.70f, 0.44f}, {64, 256, 1, 0.90f, 0.79f}};
 
 struct Plan {
   int shape, tiles, splits;
@@ -321,9 +342,9 @@ Plan plan(int m, int n, int k, bool gated) {
 template <bool BF, bool GATED>
 hipError_t launch_plan(const Mx4Args& a, const Plan& p, float* part, hipStream_t st) {
   switch (p.shape) {
-    case 0: return launch<BF, GATED, 2, 2, 1, 4, 4, 2>(a, p.splits, part, st);
-    case 1: return launch<BF, GATED, 4, 2, 1, 4, 2, 1>(a, p.splits, part, st);
-    default: return launch<BF, GATED, 4, 4, 1, 4, 2, 1>(a, p.splits, part, st);
+    case 0: return launch<BF, GATED, 2, 2, 1, 4, 3, 4, 2>(a, p.splits, part, st);
+    case 1: return launch<BF, GATED, 4, 2, 1, 4, 2, 2, 1>(a, p.splits, part, st);
+    default: return launch<BF, GATED, 4, 4, 1, 4, 2, 2, 1>(a, p.splits, part, st);
   }
 }
 

@@ -28,7 +28,7 @@ __global__ __launch_bounds__(256) void rope_kernel(const t2w_rope_args a, int he
   uint64_t freq[8];
   int axis[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) freq[e] = a.freq[8 * i + e], axis[e] = a.axis[8 * i + e];
+  for (int e = 0; e < 8; ++e) freq[e] = a.freq[8 * i + e], axis[e] = min((int)a.axis[8 * i + e], a.n_axes - 1);
   for (int item = wid; item < a.n_tok * head_splits; item += total) {
     const int tok = item / head_splits, split = item - tok * head_splits;
     const auto source = [&](int h) {

@@ -13,8 +13,6 @@ them::
 from __future__ import annotations
 
 import math
-from decimal import Decimal
-from fractions import Fraction
 
 import torch
 
@@ -23,8 +21,18 @@ from . import _lib
 _I32 = torch.int32
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _PAIRS = {"halves": 0, "neighbours": 1}
-# an angle's unit is 2^-64 turns, so the circle's number is needed beyond a double
-_TWO_PI = 2 * Fraction(Decimal("3.14159265358979323846264338327950288419716939937510582097494"))
+# An angle's unit is 2^-64 turns, so one over the circle's number is needed far beyond a double: as an integer in units of 2^-_BITS
+_BITS = 256
+_PI_DIGITS = 314159265358979323846264338327950288419716939937510582097494459230781640628620899862  # pi 10^83
+_PER_RADIAN = 10 ** 83 * 2 ** _BITS // (2 * _PI_DIGITS)
+
+
+def _turns(f: float) -> int:
+    """``f`` radians in turns of 2^-64, wrapped, as a signed 64-bit integer."""
+    num, den = f.as_integer_ratio()  # den is a power of two
+    shift = _BITS - 64 + den.bit_length() - 1
+    t = (num * _PER_RADIAN + (1 << (shift - 1)) >> shift) & 0xFFFFFFFFFFFFFFFF
+    return t - (1 << 64) if t >> 63 else t
 
 
 def sections(*counts: int) -> list[int]:
@@ -43,8 +51,8 @@ class Rope:
     def __init__(self, inv_freq, axis=None, pairs: str = "halves", scale: float = 1.0, device="cuda"):
         inv = [float(f) for f in inv_freq]
         axis = [0] * len(inv) if axis is None else [int(a) for a in axis]
-        if not inv or len(inv) % 8 or not all(map(math.isfinite, inv)):
-            raise ValueError("rope: a multiple of 8 finite frequencies")
+        if not inv or len(inv) % 8 or not all(abs(f) <= 2.0 ** 64 for f in inv):
+            raise ValueError("rope: a multiple of 8 finite frequencies, at most 2^64")
         if len(axis) != len(inv) or min(axis) < 0 or max(axis) > 15:
             raise ValueError("rope: an axis (0 to 15) for every frequency")
         if pairs not in _PAIRS:
@@ -52,9 +60,9 @@ class Rope:
         if not math.isfinite(scale):
             raise ValueError("rope: scale must be finite")
         self.rot, self.n_axes, self.pairs, self.scale = 2 * len(inv), max(axis) + 1, pairs, float(scale)
-        turns = [round(Fraction(f) / _TWO_PI * 2 ** 64) % 2 ** 64 for f in inv]
-        self._freq = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64, device=device)
-        self._axis = torch.tensor(axis, dtype=torch.uint8, device=device)
+        n = len(inv)
+        table = torch.tensor([_turns(f) for f in inv] + [int.from_bytes(bytes(axis[i:i + 8]), "little") for i in range(0, n, 8)], dtype=torch.int64).to(device)
+        self._freq, self._axis = table[:n], table[n:].view(torch.uint8)  # the axes as bytes behind the frequencies
         self.device = self._freq.device
 
     def apply(self, q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, *, q_out: torch.Tensor | None = None,

@@ -158,6 +158,15 @@ def test_linear_sizes(dev, n, k, m, dt):
 
 
 @pytest.mark.parametrize("dt", [BF, FP], ids=str)
+@pytest.mark.parametrize("m,n,k", [(16, 40, 5464), (16, 1027, 14336), (9, 100, 9224), (40, 130, 14336), (3000, 31, 14336), (100, 4100, 9000), (2000, 515, 264), (2000, 1027, 5000),
+                                   (600, 4100, 5000), (4100, 6000, 1032)])
+def test_linear_forms(dev, m, n, k, dt):
+    """Sizes at which each form is chosen: rows too long for the LDS, the three tiles, with k whole and in parts."""
+    w, v = random_weight(n, k, n + k + m)
+    check_linear(rand((m, k), dt, m), w, v, bias=torch.randn(n, device="cuda"), residual=rand((m, n), dt, m + 1))
+
+
+@pytest.mark.parametrize("dt", [BF, FP], ids=str)
 @pytest.mark.parametrize("m", [1, 16, 40, 150, 400])
 def test_linear_strides(dev, m, dt):
     """Rows of wider buffers, outputs at odd strides and offsets, the residual in the outputs' place."""
@@ -254,17 +263,27 @@ def test_no_rows(dev):
 
 # --- gated blocks ----------------------------------------------------------------------------------------------------------------
 
+def check_gated(m, n, k, dt, act):
+    (g, vg), (u, vu) = random_weight(n, k, m), random_weight(n, k, m + 1)
+    x = rand((m, k), dt, m, 8 * k ** -0.5)  # gates and products within fp16's range at every k
+    h, tol = gated_reference(x, vg, vu, act)
+    got = mx4.gated(x, g, u, act=act)
+    tol = tol + rounding(h.abs() + tol, dt)
+    assert ((got.double() - h).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 @pytest.mark.parametrize("dt", [BF, FP], ids=str)
 @pytest.mark.parametrize("m", ROWS)
 def test_gated(dev, m, dt, act):
     for n, k in ((264, 520), (77, 1032)):
-        (g, vg), (u, vu) = random_weight(n, k, m), random_weight(n, k, m + 1)
-        x = rand((m, k), dt, m)
-        h, tol = gated_reference(x, vg, vu, act)
-        got = mx4.gated(x, g, u, act=act)
-        tol = tol + rounding(h.abs() + tol, dt)
-        assert ((got.double() - h).abs() <= tol).all()
+        check_gated(m, n, k, dt, act)
+
+
+@pytest.mark.parametrize("dt", [BF, FP], ids=str)
+@pytest.mark.parametrize("m,n,k", [(16, 40, 5464), (16, 700, 14336), (40, 130, 14336), (3000, 31, 14336), (3000, 130, 264), (3000, 1027, 264), (257, 4100, 5000)])
+def test_gated_forms(dev, m, n, k, dt):
+    check_gated(m, n, k, dt, "silu")
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu"])

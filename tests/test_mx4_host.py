@@ -2,6 +2,7 @@
 
 import ctypes as C
 import math
+from fractions import Fraction
 
 import numpy as np
 import pytest
@@ -228,13 +229,28 @@ def test_rope_slices_of_one_projection():
     refused(_lib.lib().t2w_rope, rope_args(**(both | {"k_out": M + 1040})), "overlaps an input")
 
 
+def _arctan_inverse(x):
+    """arctan(1 / x) in units of 10^-100, from its series."""
+    total = term = 10 ** 100 // x
+    n, sign = 3, -1
+    while term:
+        term //= x * x
+        total += sign * (term // n)
+        n, sign = n + 2, -sign
+    return total
+
+
 def test_rope_object():
     inv = [10000.0 ** (-2 * p / 64) for p in range(32)]
     r = rope.Rope(inv, device="cpu")
     for p in (0, 7, 31):  # the table's turns against the angle itself
         assert abs(int(r._freq[p]) / 2.0 ** 64 % 1 - inv[p] / (2 * math.pi) % 1) < 2 ** -52
+    pi = 4 * (4 * _arctan_inverse(5) - _arctan_inverse(239))  # Machin's formula in units of 10^-100
+    for f in (1.0, -0.5, 0.0, 1e-300, 5e-324, 1e-9, 12345.678, 2.0 ** 64):
+        want = round(Fraction(f) * 10 ** 100 / (2 * pi) * 2 ** 64) % 2 ** 64
+        assert rope._turns(f) % 2 ** 64 == want
     assert rope.sections(2, 0, 3) == [0, 0, 2, 2, 2]
-    for kw, text in (({"inv_freq": inv[:7]}, "multiple of 8"), ({"inv_freq": []}, "multiple of 8"), ({"inv_freq": inv[:7] + [math.inf]}, "finite"), ({"inv_freq": inv, "axis": [0] * 31}, "axis"),
+    for kw, text in (({"inv_freq": inv[:7]}, "multiple of 8"), ({"inv_freq": []}, "multiple of 8"), ({"inv_freq": inv[:7] + [math.inf]}, "finite"), ({"inv_freq": inv[:7] + [math.nan]}, "finite"), ({"inv_freq": inv[:7] + [1e20]}, "2.64"), ({"inv_freq": inv, "axis": [0] * 31}, "axis"),
                      ({"inv_freq": inv, "axis": [0] * 31 + [16]}, "axis"), ({"inv_freq": inv, "axis": [-1] * 32}, "axis"), ({"inv_freq": inv, "pairs": "odd"}, "pairs"), ({"inv_freq": inv, "scale": math.nan}, "scale")):
         with pytest.raises(ValueError, match=text):
             rope.Rope(**({"device": "cpu"} | kw))
