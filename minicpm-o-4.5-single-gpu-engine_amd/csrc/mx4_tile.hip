@@ -202,7 +202,8 @@ __device__ __forceinline__ int2 tile_at(int b, int tm, int tn) {
   return make_int2(4 * grp + in % rows, in / rows);
 }
 
-// KG groups of waves share a tile, each with its run of the stages and buffers of its own; the first adds up.
+// KG groups of waves share a tile, each with its run of the stages and buffers of its own; their sums meet in LDS, and each group
+// finishes its share of the blocks.
 template <bool BF, bool GATED, int TM, int TN, int WM, int WN, int D, int XB, int KG, bool PART>
 __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx4_tile_kernel(const Mx4Args a, int tm, int tn, int splits, f32x4* part) {
   typedef MxTile<BF, GATED, TM, TN, WM, WN> T;
@@ -223,44 +224,51 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx4_tile_kernel(const Mx
   if constexpr (XB == 2) t.template run<D, 2>({x0 + xo, x1 + xo}, s0, s1, n);
   else if constexpr (XB == 3) t.template run<D, 3>({x0 + xo, x1 + xo, x2 + xo}, s0, s1, n);
   else t.template run<D, 4>({x0 + xo, x1 + xo, x2 + xo, x3 + xo}, s0, s1, n);
+  constexpr int OT = GATED ? TN / 2 : TN, BLOCKS = TM * TN, OUT = OT * TM;  // blocks of sums and of outputs of a wave
+  constexpr int MINE = (OUT + KG - 1) / KG;                                  // this group's: kg, kg + KG, ..
+  f32x4 sum[GATED ? 2 : 1][MINE];
   if constexpr (KG > 1) {
-    static_assert(KG == 2 && T::NW * TM * TN * 64 <= KG * XS, "the second group's sums fit a buffer");
+    static_assert(OUT % KG == 0 && KG % 2 == 0 && KG / 2 * T::NW * BLOCKS * 64 <= KG * XS, "whole shares; half of the groups' sums fit a buffer");
     __syncthreads();  // every wave is through with the buffers
-    f32x4* p = (f32x4*)x0 + (t.wave * TM * TN) * 64 + t.lane;
-    if (kg == 1) {
-#pragma unroll
-      for (int y = 0; y < TN; ++y)
-#pragma unroll
-        for (int i = 0; i < TM; ++i) p[(y * TM + i) * 64] = t.acc[y][i];
-    }
-    __syncthreads();
-    if (kg == 1) return;
+    const auto red = [&](int g) { return (f32x4*)(g < KG / 2 ? x0 : x1) + ((g % (KG / 2)) * T::NW + t.wave) * BLOCKS * 64 + t.lane; };
+    f32x4* own = red(kg);
 #pragma unroll
     for (int y = 0; y < TN; ++y)
 #pragma unroll
-      for (int i = 0; i < TM; ++i) t.acc[y][i] += p[(y * TM + i) * 64];
+      for (int i = 0; i < TM; ++i) own[(y * TM + i) * 64] = t.acc[y][i];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < MINE; ++j)
+#pragma unroll
+      for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+        const int at_ = (kg + j * KG + h * OUT) * 64;
+        sum[h][j] = red(0)[at_];
+#pragma unroll
+        for (int g = 1; g < KG; ++g) sum[h][j] += red(g)[at_];
+      }
+  } else {
+#pragma unroll
+    for (int j = 0; j < MINE; ++j)
+#pragma unroll
+      for (int h = 0; h < (GATED ? 2 : 1); ++h) sum[h][j] = t.acc[j / TM + h * OT][j % TM];
   }
   if constexpr (PART) {
-    f32x4* p = part + (size_t)(blockIdx.x * T::NW + t.wave) * (TM * TN * 64) + t.lane;
+    f32x4* p = part + (size_t)(blockIdx.x * T::NW + t.wave) * (BLOCKS * 64) + t.lane;
 #pragma unroll
-    for (int y = 0; y < TN; ++y)
+    for (int j = 0; j < MINE; ++j)
 #pragma unroll
-      for (int i = 0; i < TM; ++i) p[(y * TM + i) * 64] = t.acc[y][i];
+      for (int h = 0; h < (GATED ? 2 : 1); ++h) p[(kg + j * KG + h * OUT) * 64] = sum[h][j];
   } else {
-    constexpr int OT = GATED ? TN / 2 : TN;
-    Extra ex[OT][TM];
+    Extra ex[MINE];
+    int2 o[MINE];
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int j = 0; j < MINE; ++j) {
+      const int b_ = kg + j * KG;
+      o[j] = place<GATED, TM, TN, WM, WN>(at.x, at.y, t.wave, b_ / TM, b_ % TM);
+      ex[j] = GATED ? Extra{} : fetch<BF>(a, o[j].x, o[j].y);
+    }
 #pragma unroll
-      for (int y = 0; y < OT; ++y) {
-        const int2 o = place<GATED, TM, TN, WM, WN>(at.x, at.y, t.wave, y, i);
-        ex[y][i] = GATED ? Extra{} : fetch<BF>(a, o.x, o.y);
-      }
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int y = 0; y < OT; ++y)
-        block_store<BF, GATED>(a, place<GATED, TM, TN, WM, WN>(at.x, at.y, t.wave, y, i), t.acc[y][i], t.acc[GATED ? y + OT : y][i], ex[y][i]);
+    for (int j = 0; j < MINE; ++j) block_store<BF, GATED>(a, o[j], sum[0][j], sum[GATED ? 1 : 0][j], ex[j]);
   }
 }
 
