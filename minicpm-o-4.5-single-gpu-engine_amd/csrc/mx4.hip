@@ -21,8 +21,12 @@ namespace {
 // sums meet in LDS in the order of the waves.  The stream of codes is what bounds it: a step's registers are loaded again, with
 // the wave's next unit, as soon as the step is converted, so that a wave always has about 4 KB in flight, across units and blocks.
 // XL: x lies in LDS, brought there once by each workgroup (16-byte chunk c of a step of row r at c ^ r: 16 rows' reads cover all
-// banks), zero behind k.  A wave reads 4 KB of it a step's 1 KB of codes; from memory (rows too long for LDS) that alone would take the
-// L1 cache's whole bandwidth at 1 row, where 16 lanes read the same bytes.
+// banks), zero behind k.  A wave reads 4 KB of it a step's 1 KB of codes; from memory (rows too long for LDS) that alone takes the
+// L1 cache's whole bandwidth: one row x 14336 x 2 gates of 4096 columns 18.3 us, from LDS 12.4.
+// Measured (kernel times, codes from HBM): 1 row x 6144 x 4096 4.7 us, 3 rows x 128001 x 4096 49 us (5.6 TB/s), one row's gated
+// 14336 x 4096 x 2 12.6 us (5.0 TB/s) and 4096 x 14336 6.7 us (one block a CU: 4.7 TB/s).  Two blocks a wave at a time (half the
+// reads of x) took 10% longer; 4 or 8 waves a workgroup instead of 16 gain nothing at one row and take 26.7 and 18.3 us instead of
+// 16.5 at 16 rows' gated 14336 x 4096 x 2.
 template <bool BF, bool GATED, bool XL>
 __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Args a) {
   extern __shared__ uint4 lds[];  // XL: x [rows][units][4][16]; then sums [2][waves][64]

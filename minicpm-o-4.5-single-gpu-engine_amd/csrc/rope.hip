@@ -3,6 +3,9 @@
 // The angle is computed in turns as 64-bit fixed point: freq[p] is inv_freq[p] / 2 pi in units of 2^-64 turns (wrapped), an integer
 // product wraps whole turns away by itself, and its upper 32 bits are the angle to 2^-32 turns at every int32 position; fp32
 // products lose the angle of far positions (position 10^6 at frequency 1: 0.06 radians).
+//
+// Bound by memory: 37,433 tokens of 40 heads x 128 take 140 us (5.4 TB/s read and written; a copy of that size 5.2).  A lane keeps its
+// eight pairs' sines and cosines for all heads of its token: computed for each head they would be most of the work.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -17,7 +20,7 @@ int set_error(const char* what, hipError_t e);
 
 namespace {
 
-// Lanes: LPH = rot / 16 lanes a head, each 8 pairs (16 channels); a wave turns 64 / LPH heads of one token at a time.
+// Lanes: rot / 16 lanes a head, each 8 pairs (16 channels); a wave turns 64 / LPH heads of one token at a time.
 template <bool BF, bool HALVES>
 __global__ __launch_bounds__(256) void rope_kernel(const t2w_rope_args a, int head_splits) {
   const int lane = threadIdx.x & 63, lph = a.rot >> 4, sub = lane / lph, i = lane - sub * lph, hpw = 64 / lph;
@@ -83,7 +86,9 @@ __global__ __launch_bounds__(256) void rope_kernel(const t2w_rope_args a, int he
 
 hipError_t rope_launch(const t2w_rope_args& a, hipStream_t st) {
   const int hpw = 64 / (a.rot >> 4), turns = (a.q_heads + a.k_heads + hpw - 1) / hpw;
-  const int splits = a.n_tok < 2048 ? turns : 1;
+  // A token's heads go to waves of their own while there are few tokens, though each wave then computes the angles: 64 tokens of 40
+  // heads x 128 take 3.9 us (one wave a token: 5.0), 500 5.3 (5.4), 1000 8.0 (6.1); of 32 heads x 64 3.6 (3.9), 3.8 (4.1), 4.5 (4.4).
+  const int splits = a.n_tok <= 512 ? turns : 1;
   const long long waves = (long long)a.n_tok * splits;
   const unsigned grid = (unsigned)((waves + 3) / 4 < 8192 ? (waves + 3) / 4 : 8192);
   const bool halves = a.pairs == T2W_ROPE_HALVES;

@@ -67,7 +67,7 @@ def test_layouts(dev, n, heads, kv, d, rot, pairs, dt):
     assert torch.equal(qkv, keep)
 
 
-@pytest.mark.parametrize("n", [2047, 2048, 2049, 40000])
+@pytest.mark.parametrize("n", [511, 512, 513, 2049, 40000])
 def test_many_tokens(dev, n):
     """Around the change from a token's heads in several waves to all in one, and more tokens than waves."""
     inv, axis = freqs(64), rope.sections(8, 12, 12)
