@@ -127,25 +127,28 @@ struct MxTile {
   // wave holds its fragments of the stage, and the freed buffer is the one to load (xl is xc).
   // AHEAD 2: with 4 MFMAs a step a fragment's way from LDS takes longer than a step, so they are read two ahead into two sets in
   // turn; the barrier stands in the stage's middle, and a buffer more than D lets xl be one that was read a stage ago.
-  template <int D, int AHEAD>
+  // TAIL: the (TAIL + 1)th stage behind the loop.  Nothing is left to load there, so it loads nothing and knows how many loads are
+  // behind the next stage's (loads that the compiler may drop, as nobody reads what they bring, could not be counted on).
+  template <int D, int AHEAD, int TAIL>
   __device__ __forceinline__ void stage(uint4* xc, uint4* xn, uint4* xl, Codes& cc, Codes& cn, Codes& cl, uint4 (&w0)[TN], uint4 (&w1)[TN], uint4 (&xa)[TM],
                                         uint4 (&xb)[TM], int st, int s1) {
+    constexpr int LATER = (TAIL < 0 ? D - 2 : TAIL < D - 2 ? D - 2 - TAIL : 0) * LOADS;  // in flight behind the next stage's
     if constexpr (AHEAD == 1) {
       step(w0, w1, xa, xc, 1, cc, st, 1);
       step(w1, w0, xa, xc, 2, cc, st, 2);
       step(w0, w1, xa, xc, 3, cc, st, 3);
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((D - 2) * LOADS) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LATER) : "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      issue(xl, cl, st + D, s1);
+      if (TAIL < 0) issue(xl, cl, st + D, s1);
       step(w1, w0, xa, xn, 0, cn, st + 1, 0);
     } else {
       step(w0, w1, xa, xc, 2, cc, st, 1);
       step(w1, w0, xb, xc, 3, cc, st, 2);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 2) * LOADS) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LATER) : "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      issue(xl, cl, st + D, s1);
+      if (TAIL < 0) issue(xl, cl, st + D, s1);
       step(w0, w1, xa, xn, 0, cc, st, 3);
       step(w1, w0, xb, xn, 1, cn, st + 1, 0);
     }
@@ -173,11 +176,16 @@ struct MxTile {
     for (; i + XB <= n; i += XB) {
 #pragma unroll
       for (int d = 0; d < XB; ++d)
-        stage<D, AHEAD>(x[d], x[(d + 1) % XB], x[(d + D) % XB], c[d], c[(d + 1) % XB], c[(d + D) % XB], w0, w1, xa, xb, s0 + i + d, s1);
+        stage<D, AHEAD, -1>(x[d], x[(d + 1) % XB], x[(d + D) % XB], c[d], c[(d + 1) % XB], c[(d + D) % XB], w0, w1, xa, xb, s0 + i + d, s1);
     }
-#pragma unroll
-    for (int d = 0; d < XB - 1; ++d)
-      if (i + d < n) stage<D, AHEAD>(x[d], x[(d + 1) % XB], x[(d + D) % XB], c[d], c[(d + 1) % XB], c[(d + D) % XB], w0, w1, xa, xb, s0 + i + d, s1);
+    static_assert(XB <= 4 && XB - 1 <= D, "the stages behind the loop are all on their way when it ends");
+    if (i < n) stage<D, AHEAD, 0>(x[0], x[1 % XB], x[0], c[0], c[1 % XB], c[0], w0, w1, xa, xb, s0 + i, s1);
+    if constexpr (XB > 2) {
+      if (i + 1 < n) stage<D, AHEAD, 1>(x[1], x[2 % XB], x[0], c[1], c[2 % XB], c[0], w0, w1, xa, xb, s0 + i + 1, s1);
+    }
+    if constexpr (XB > 3) {
+      if (i + 2 < n) stage<D, AHEAD, 2>(x[2], x[3 % XB], x[0], c[2], c[3 % XB], c[0], w0, w1, xa, xb, s0 + i + 2, s1);
+    }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was issued into LDS behind the last stage
   }
 };
