@@ -108,8 +108,8 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Args a) {
     else unit(std::false_type{}, 0, 0);
     u = first;
     const int n = g * 16 + 4 * q, m = m0 + (lane & 15);
-    Extra ex{};
-    if (!GATED && wave == 0) ex = fetch<BF>(a, m, n);
+    Extra ex[1] = {};
+    if (!GATED && wave == 0) fetch(a, {make_int2(m, n)}, ex);
     f32x4* p = part + turn * waves * 64;
     p[wave * 64 + lane] = acc[0] + acc[1];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the codes in flight are not waited for
@@ -126,7 +126,7 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Args a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) r[e] = gate_act(r[e], a.act) * o[e];
       }
-      finish<BF>(a, m, n, r, ex);
+      finish<BF>(a, m, n, r, ex[0]);
     }
     g = gn;
   }

@@ -51,32 +51,44 @@ __device__ __forceinline__ float gate_act(float g, int act) { return act == T2W_
 // behind the last read the last.
 struct Extra {
   float bias[4];
-  uint32_t res[4];  // quad: two words, else four values
+  uint2 res;  // the residual's four values
 };
 
-template <bool BF>
-__device__ __forceinline__ Extra fetch(const Mx4Args& a, int m, int n) {
-  Extra x = {{0.f, 0.f, 0.f, 0.f}, {0, 0, 0, 0}};
-  const uint16_t* res = (const uint16_t*)a.residual + (long long)min(m, a.m - 1) * a.ldr;
+// of N places (row, first channel); the branches, the same for all, stand outside
+template <int N>
+__device__ __forceinline__ void fetch(const Mx4Args& a, const int2 (&at)[N], Extra (&x)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) x[j] = Extra{};
+  const uint16_t* res = (const uint16_t*)a.residual;
   if (a.quad) {
-    const int c = min(n, a.n - 4);
     if (a.bias) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x.bias[e] = a.bias[c + e];
+      for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[j].bias[e] = a.bias[min(at[j].y, a.n - 4) + e];
     }
     if (a.residual) {
-      const uint2 h = *(const uint2*)(res + c);
-      x.res[0] = h.x, x.res[1] = h.y;
-    }
-    return x;
-  }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int c = min(n + e, a.n - 1);
-    if (a.bias) x.bias[e] = a.bias[c];
-    if (a.residual) x.res[e] = res[c];
+      for (int j = 0; j < N; ++j)
+        x[j].res = *(const uint2*)(res + (long long)min(at[j].x, a.m - 1) * a.ldr + min(at[j].y, a.n - 4));
+    }
+    return;
   }
-  return x;
+  if (a.bias) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[j].bias[e] = a.bias[min(at[j].y + e, a.n - 1)];
+  }
+  if (a.residual) {
+    uint32_t r[N][4];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[j][e] = res[(long long)min(at[j].x, a.m - 1) * a.ldr + min(at[j].y + e, a.n - 1)];
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j].res = make_uint2(r[j][0] | r[j][1] << 16, r[j][2] | r[j][3] << 16);
+  }
 }
 
 // Outputs n .. n + 3 of row m from their sums
@@ -84,20 +96,17 @@ template <bool BF>
 __device__ __forceinline__ void finish(const Mx4Args& a, int m, int n, const float (&v)[4], const Extra& x) {
   if (m >= a.m || n >= a.n) return;
   uint16_t* y = (uint16_t*)a.y + (long long)m * a.ldy + n;
+  const float h[4] = {BF ? lo2f(x.res.x) : lo2h(x.res.x), BF ? hi2f(x.res.x) : hi2h(x.res.x), BF ? lo2f(x.res.y) : lo2h(x.res.y), BF ? hi2f(x.res.y) : hi2h(x.res.y)};
   float r[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) r[e] = v[e] + x.bias[e];
+  for (int e = 0; e < 4; ++e) r[e] = v[e] + x.bias[e] + h[e];
   if (a.quad) {
-    r[0] += BF ? lo2f(x.res[0]) : lo2h(x.res[0]);
-    r[1] += BF ? hi2f(x.res[0]) : hi2h(x.res[0]);
-    r[2] += BF ? lo2f(x.res[1]) : lo2h(x.res[1]);
-    r[3] += BF ? hi2f(x.res[1]) : hi2h(x.res[1]);
     *(uint2*)y = BF ? make_uint2(pack2(r[0], r[1]), pack2(r[2], r[3])) : make_uint2(pack2h(r[0], r[1]), pack2h(r[2], r[3]));
     return;
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (n + e < a.n) y[e] = round1<BF>(r[e] + (BF ? lo2f(x.res[e]) : lo2h(x.res[e])));
+    if (n + e < a.n) y[e] = round1<BF>(r[e]);
 }
 
 }  // namespace

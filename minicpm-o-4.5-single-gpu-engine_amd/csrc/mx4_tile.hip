@@ -275,14 +275,14 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx4_tile_kernel(const Mx
 #pragma unroll
       for (int h = 0; h < (GATED ? 2 : 1); ++h) p[(kg + j * KG + h * OUT) * 64] = sum[h][j];
   } else {
-    Extra ex[MINE];
+    Extra ex[MINE] = {};
     int2 o[MINE];
 #pragma unroll
     for (int j = 0; j < MINE; ++j) {
       const int b_ = kg + j * KG;
       o[j] = place<GATED, TM, TN, WM, WN>(at.x, at.y, t.wave, b_ / TM, b_ % TM);
-      ex[j] = GATED ? Extra{} : fetch<BF>(a, o[j].x, o[j].y);
     }
+    if (!GATED) fetch(a, o, ex);
 #pragma unroll
     for (int j = 0; j < MINE; ++j) block_store<BF, GATED>(a, o[j], sum[0][j], sum[GATED ? 1 : 0][j], ex[j]);
   }
@@ -299,7 +299,8 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const Mx4Args a, int tm, 
   const size_t stride = (size_t)tm * tn * NW * (TM * TN * 64);
   const f32x4* p = part + ((size_t)w * (TM * TN) + blk) * 64 + lane;
   const int2 o = place<GATED, TM, TN, WM, WN>(at.x, at.y, w % NW, blk / TM, blk % TM);
-  const Extra ex = GATED ? Extra{} : fetch<BF>(a, o.x, o.y);
+  Extra ex[1] = {};
+  if (!GATED) fetch(a, {o}, ex);
   f32x4 v = p[0], u = f32x4{0.f, 0.f, 0.f, 0.f};
   if constexpr (GATED) u = p[OT * TM * 64];
 #pragma unroll 4
@@ -307,7 +308,7 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const Mx4Args a, int tm, 
     v += p[s * stride];
     if constexpr (GATED) u += p[s * stride + OT * TM * 64];
   }
-  block_store<BF, GATED>(a, o, v, u, ex);
+  block_store<BF, GATED>(a, o, v, u, ex[0]);
 }
 
 template <bool BF, bool GATED, int TM, int TN, int WM, int WN, int D, int XB, int KG>
