@@ -20,23 +20,24 @@ namespace {
 // columns (GATED: even waves of the gate's matrix, odd ones of the other), whose codes it converts in registers, and the waves'
 // sums meet in LDS in the order of the waves.  The stream of codes is what bounds it: a step's registers are loaded again, with
 // the wave's next unit, as soon as the step is converted, so that a wave always has about 4 KB in flight, across units and blocks.
-// XL: x lies in LDS, brought there once by each workgroup (16-byte chunk c of a step of row r at c ^ r: 16 rows' reads cover all
-// banks), zero behind k.  A wave reads 4 KB of it a step's 1 KB of codes; from memory (rows too long for LDS) that alone takes the
-// L1 cache's whole bandwidth: one row x 14336 x 2 gates of 4096 columns 18.3 us, from LDS 12.4.
+// x lies in LDS, brought there once by each workgroup (16-byte chunk c of a step of row r at c ^ r: 16 rows' reads cover all
+// banks), zero behind k.  A wave reads 4 KB of it a step's 1 KB of codes; from memory that alone takes the L1 cache's whole
+// bandwidth: one row x 14336 x 2 gates of 4096 columns 18.3 us, from LDS 12.4.  Of rows too long for LDS (ALL false) the first `held`
+// units are there and the others are read from memory.
 // Measured (kernel times, codes from HBM): 1 row x 6144 x 4096 4.7 us, 3 rows x 128001 x 4096 49 us (5.6 TB/s), one row's gated
 // 14336 x 4096 x 2 12.6 us (5.0 TB/s) and 4096 x 14336 6.7 us (one block a CU: 4.7 TB/s).  Two blocks a wave at a time (half the
 // reads of x) took 10% longer; 4 or 8 waves a workgroup instead of 16 gain nothing at one row and take 26.7 and 18.3 us instead of
 // 16.5 at 16 rows' gated 14336 x 4096 x 2.
-template <bool BF, bool GATED, bool XL>
-__global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Args a) {
-  extern __shared__ uint4 lds[];  // XL: x [rows][units][4][16]; then sums [2][waves][64]
+template <bool BF, bool GATED, bool ALL>
+__global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Args a, int held) {
+  extern __shared__ uint4 lds[];  // x [rows][held][4][16], then sums [2][waves][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int steps = (a.k + 127) >> 7, units = (a.k + 511) >> 9, q = lane >> 4, nb = (a.n + 15) >> 4;
   const int first = GATED ? wave >> 1 : wave, stride = GATED ? waves >> 1 : waves;  // this wave's units
   const int m0 = 16 * blockIdx.y, rows = min(16, a.m - m0), row = min(lane & 15, rows - 1);  // lanes behind the last row repeat it: not stored
   const uint16_t* x = (const uint16_t*)a.x + (long long)m0 * a.ldx;
   uint4* xs = lds;
-  f32x4* part = (f32x4*)(lds + (XL ? rows * units * 64 : 0));
+  f32x4* part = (f32x4*)(lds + rows * held * 64);
   const uint8_t* w = GATED && (wave & 1) ? a.w[1] : a.w[0];
   const uint8_t* s = GATED && (wave & 1) ? a.s[1] : a.s[0];
 
@@ -49,37 +50,33 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Args a) {
   const auto load_scales = [&](int g, int u) { return *(const uint32_t*)(s + ((size_t)g * units + u) * 256 + (uint32_t)(lane * 4)); };
 
   int g = blockIdx.x, u = first;
-  if constexpr (XL) {
-    // a unit's 1 KB of a row at a time, straight to LDS, all in flight together; columns behind k are out of the row's bounds: zeros
-    for (int r = GATED ? wave & 1 : 0; r < rows; r += GATED ? 2 : 1) {
-      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(x + (long long)r * a.ldx), 0, a.k * 2, 0x00020000);
-      const int c = (lane & ~15) | ((lane ^ r) & 15);
-      for (int b = first; b < units; b += stride)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)(xs + (r * units + b) * 64), 16, c * 16, b * 1024, 0, 0);
-    }
-    asm volatile("" ::: "memory");
+  // a unit's 1 KB of a row at a time, straight to LDS, all in flight together; columns behind k are out of the row's bounds: zeros
+  for (int r = GATED ? wave & 1 : 0; r < rows; r += GATED ? 2 : 1) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(x + (long long)r * a.ldx), 0, a.k * 2, 0x00020000);
+    const int c = (lane & ~15) | ((lane ^ r) & 15);
+    for (int b = first; b < held; b += stride)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)(xs + (r * held + b) * 64), 16, c * 16, b * 1024, 0, 0);
   }
+  asm volatile("" ::: "memory");
   sc = load_scales(g, u);
 #pragma unroll
   for (int t = 0; t < 4; ++t) load(g, u, t);
-  if constexpr (XL) {
-    asm volatile("s_waitcnt vmcnt(5)" ::: "memory");  // x is there, the codes may still be on their way
-    __builtin_amdgcn_s_barrier();
-  }
+  asm volatile("s_waitcnt vmcnt(5)" ::: "memory");  // x is there, the codes may still be on their way
+  __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   const uint16_t* xrow = x + (long long)row * a.ldx + 32 * q;
 
   f32x4 acc[2];
-  const auto unit = [&](auto more, int gn, int un) {
-    constexpr bool MORE = decltype(more)::value;
+  const auto unit_of = [&](auto more, auto in, int gn, int un) {
+    constexpr bool MORE = decltype(more)::value, IN = decltype(in)::value;
     if (MORE) scn = load_scales(gn, un);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       uint4 xf[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if constexpr (XL) {
-          xf[j] = xs[(row * units + u) * 64 + 16 * t + ((4 * q + j) ^ row)];
+        if constexpr (IN) {
+          xf[j] = xs[(row * held + u) * 64 + 16 * t + ((4 * q + j) ^ row)];
         } else {
           xf[j] = make_uint4(0, 0, 0, 0);
           const int k0 = 512 * u + 128 * t + 8 * j;
@@ -98,6 +95,10 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Args a) {
       acc[1] = mma<BF>(w3, xf[3], acc[1]);
     }
     if (MORE) sc = scn;
+  };
+  const auto unit = [&](auto more, int gn, int un) {
+    if (ALL || u < held) unit_of(more, std::true_type{}, gn, un);
+    else unit_of(more, std::false_type{}, gn, un);
   };
 
   for (int turn = 0; g < nb; turn ^= 1) {
@@ -132,20 +133,22 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Args a) {
   }
 }
 
-struct RowsPlan {
-  int waves;
-  size_t bytes;  // of LDS
-};
-
-RowsPlan rows_plan(int m, int k, bool gated, bool xl) {
-  const int units = mx4_units(k), two = gated ? 2 : 1;
-  const int rounds = (units * two + 15) / 16, waves = (units + rounds - 1) / rounds * two;
-  return {waves, (xl ? (size_t)std::min(m, 16) * units * 1024 : 0) + (size_t)2 * waves * 1024};
-}
-
 constexpr size_t LDS_CU = 160 * 1024;
 
-template <bool BF, bool GATED, bool XL>
+struct RowsPlan {
+  int waves, held;  // units of x in LDS
+  size_t bytes;     // of LDS
+};
+
+RowsPlan rows_plan(int m, int k, bool gated) {
+  const int units = mx4_units(k), two = gated ? 2 : 1, rows = std::min(m, 16);
+  const int rounds = (units * two + 15) / 16, waves = (units + rounds - 1) / rounds * two;
+  const size_t sums = (size_t)2 * waves * 1024;
+  const int held = (int)std::min<size_t>(units, (LDS_CU - sums) / ((size_t)rows * 1024));
+  return {waves, held, (size_t)rows * held * 1024 + sums};
+}
+
+template <bool BF, bool GATED, bool ALL>
 hipError_t launch_rows(const Mx4Args& a, const RowsPlan& p, hipStream_t st) {
   if (p.bytes > 64 * 1024) {  // beyond the default a function has to be told, on each device
     static std::atomic<uint64_t> told{0};
@@ -154,14 +157,14 @@ hipError_t launch_rows(const Mx4Args& a, const RowsPlan& p, hipStream_t st) {
     if (e != hipSuccess) return e;
     const uint64_t bit = dev < 64 ? 1ull << dev : 0;
     if (!(told.load(std::memory_order_acquire) & bit)) {
-      e = hipFuncSetAttribute((const void*)mx4_rows_kernel<BF, GATED, XL>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_CU);
+      e = hipFuncSetAttribute((const void*)mx4_rows_kernel<BF, GATED, ALL>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_CU);
       if (e != hipSuccess) return e;
       told.fetch_or(bit, std::memory_order_release);
     }
   }
   const int nb = mx4_blocks(a.n), fit = std::max(1, std::min(16 / p.waves, (int)(LDS_CU / p.bytes)));  // workgroups a CU
   const int rounds = (nb + 256 * fit - 1) / (256 * fit);
-  mx4_rows_kernel<BF, GATED, XL><<<dim3((nb + rounds - 1) / rounds, (a.m + 15) / 16), p.waves * 64, p.bytes, st>>>(a);
+  mx4_rows_kernel<BF, GATED, ALL><<<dim3((nb + rounds - 1) / rounds, (a.m + 15) / 16), p.waves * 64, p.bytes, st>>>(a, p.held);
   return hipGetLastError();
 }
 
@@ -266,14 +269,13 @@ hipError_t mx4_quantize(const t2w_mx4_quantize_args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-bool mx4_rows_in_lds(int m, int k, bool gated) { return rows_plan(m, k, gated, true).bytes <= LDS_CU; }
+int mx4_rows_outside(int m, int k, bool gated) { return mx4_units(k) - rows_plan(m, k, gated).held; }
 
 hipError_t mx4_rows(const Mx4Args& a, bool bf, bool gated, hipStream_t st) {
-  const bool xl = mx4_rows_in_lds(a.m, a.k, gated);
-  const RowsPlan p = rows_plan(a.m, a.k, gated, xl);
+  const RowsPlan p = rows_plan(a.m, a.k, gated);
   const auto go = [&](auto b, auto g) {
     constexpr bool BF = decltype(b)::value, GATED = decltype(g)::value;
-    return xl ? launch_rows<BF, GATED, true>(a, p, st) : launch_rows<BF, GATED, false>(a, p, st);
+    return p.held == mx4_units(a.k) ? launch_rows<BF, GATED, true>(a, p, st) : launch_rows<BF, GATED, false>(a, p, st);
   };
   if (gated) return bf ? go(std::true_type{}, std::true_type{}) : go(std::false_type{}, std::true_type{});
   return bf ? go(std::true_type{}, std::false_type{}) : go(std::false_type{}, std::false_type{});

@@ -43,7 +43,7 @@ hipError_t mx4_quantize(const t2w_mx4_quantize_args& a, hipStream_t st);
 // The products: few rows (mx4.hip) and tiles (mx4_tile.hip), which may split k over workgroups (fp32 parts in the workspace,
 // joined by a second kernel).
 hipError_t mx4_rows(const Mx4Args& a, bool bf, bool gated, hipStream_t st);
-bool mx4_rows_in_lds(int m, int k, bool gated);
+int mx4_rows_outside(int m, int k, bool gated);  // units of 512 columns of x that do not fit the LDS
 bool mx4_takes_tiles(int m, int n, int k, long long ldx, bool gated);
 size_t mx4_tiles_workspace(int m, int n, int k, bool gated);
 hipError_t mx4_tiles(const Mx4Args& a, bool bf, bool gated, void* workspace, hipStream_t st);

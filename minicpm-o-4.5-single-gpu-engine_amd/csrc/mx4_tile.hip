@@ -378,9 +378,12 @@ hipError_t launch_plan(const Mx4Args& a, const Plan& p, float* part, hipStream_t
 bool mx4_takes_tiles(int m, int n, int k, long long ldx, bool gated) {
   if (ldx >= (1 << 24)) return false;  // a row's place in its tile is a 31-bit byte offset
   if (m > 16) return true;
-  if (mx4_rows_in_lds(m, k, gated)) return false;
-  // few rows, too long for the LDS: 17.5 us of 16 rows x 14336 columns x 4096 channels (tiles 14.8), 6.8 of 5464 x 2048 (11.1)
-  return plan(m, n, k, gated).us < 2.f + 1.1e-3f * k * ((mx4_blocks(n) + 255) / 256);
+  const int outside = mx4_rows_outside(m, k, gated);
+  if (outside == 0) return false;
+  // few rows, too long for the LDS: by the stream (5.5 TB/s) and what comes from memory for every block of a CU.  4096 channels x 14336
+  // columns x 6, 10 and 16 rows take 10.6, 13.9 and 17.9 us (tiles 13.4 to 13.6), 2048 x 5464 x 16 6.5 (9.5), 20000 x 8192 x 16 34.9 (24.1).
+  const float mb = (gated ? 2 : 1) * 0.53f * n * (k * 1e-6f);
+  return plan(m, n, k, gated).us < 2.5f + mb / 5.5f + 0.45f * outside * ((mx4_blocks(n) + 255) / 256);
 }
 
 size_t mx4_tiles_workspace(int m, int n, int k, bool gated) {
