@@ -1,12 +1,13 @@
 // Products with 4-bit weights over many rows: tiles of x in LDS, codes from memory to registers, conversion beside the MFMAs.
 //
-// A workgroup of WM x WN waves owns 16 TM WM rows of x and TN WN blocks of 16 weight channels (gated: half of them of each
+// A workgroup of WN waves side by side owns 16 TM rows of x and TN WN blocks of 16 weight channels (gated: half of them of each
 // matrix), a wave TM x TN blocks of 16 x 16.  K advances in stages of 128 columns: x is copied into LDS by buffer loads (two
 // buffers, 16-byte chunk c of row r at c ^ (r % 16): the 16 rows of a fragment read cover all 64 banks), a lane's 16 bytes of
 // codes of each block go straight into registers, already in operand order.  A stage is four steps of 32 columns; next to a
 // step's MFMAs the next step's fragments are read and its codes converted.  The barrier stands in front of a stage's last step,
 // whose fragments every wave holds by then: the loads of the stage after next are issued right behind it and have a stage's time.
-// Rows behind the last and columns behind k are out of the buffer's bounds and read as zeros.
+// Rows behind the last and columns behind k are out of the buffer's bounds and read as zeros.  The buffers are objects of their own,
+// named at compile time: behind one indexed array the compiler would wait for all copies before every read.
 //
 // The conversion is one instruction for two weights and shares the wave's time with the MFMAs; the codes come to a CU at a quarter
 // of bf16's bytes, which is why a tile of only 64 rows reaches the rate of a large bf16 product: 64 x 256 tiles run 4001 rows x
@@ -27,9 +28,9 @@ namespace {
 
 constexpr uint32_t OUTSIDE = 0x80000000u, BOUND = 0x7fffff00u;  // byte offsets in the tile's rows of x
 
-template <bool BF, bool GATED, int TM, int TN, int WM, int WN>
+template <bool BF, bool GATED, int TM, int TN, int WN>
 struct MxTile {
-  static constexpr int NW = WM * WN, BM = 16 * TM * WM, NB = TN * WN;   // waves; rows; weight blocks
+  static constexpr int NW = WN, BM = 16 * TM, NB = TN * WN;   // waves; rows; weight blocks
   static constexpr int CB = GATED ? NB / 2 : NB;                         // blocks of output channels
   static constexpr int LD = BM / 4 / NW;                                 // 1 KB copies a stage and wave
   static constexpr int LOADS = LD + 2 * TN;                              // a stage's, of a wave
@@ -37,14 +38,13 @@ struct MxTile {
   const Mx4Args& a;
   __amdgpu_buffer_rsrc_t xr;
   uint32_t off[LD];
-  int lane, wave, wm, wn, steps, units;
+  int lane, wave, steps, units;
   __amdgpu_buffer_rsrc_t wr[GATED ? 2 : 1], sr[GATED ? 2 : 1];  // this wave's blocks of each matrix
   f32x4 acc[TN][TM];
 
   __device__ __forceinline__ MxTile(const Mx4Args& a_, int mt, int nt) : a(a_) {
     lane = threadIdx.x & 63;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % NW;
-    wm = wave / WN, wn = wave % WN;
     steps = (a.k + 127) >> 7, units = (a.k + 511) >> 9;
     const int m0 = mt * BM;
     xr = __builtin_amdgcn_make_buffer_rsrc((void*)((const uint16_t*)a.x + (long long)m0 * a.ldx), 0, (int)BOUND, 0x00020000);
@@ -55,7 +55,7 @@ struct MxTile {
     }
     // blocks behind the last are out of bounds as well
     constexpr int WB = GATED ? TN / 2 : TN;
-    const int b0 = __builtin_amdgcn_readfirstlane(nt * CB + wn * WB), have = __builtin_amdgcn_readfirstlane(max(0, min(WB, ((a.n + 15) >> 4) - b0)));
+    const int b0 = __builtin_amdgcn_readfirstlane(nt * CB + wave * WB), have = __builtin_amdgcn_readfirstlane(max(0, min(WB, ((a.n + 15) >> 4) - b0)));
 #pragma unroll
     for (int g = 0; g < (GATED ? 2 : 1); ++g) {
       wr[g] = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w[g] + (size_t)b0 * steps * 1024), 0, have * steps * 1024, 0x00020000);
@@ -94,7 +94,7 @@ struct MxTile {
 
   __device__ __forceinline__ uint4 xread(const uint4* xs, int i, int j) const {
     const int c = lane & 15, q = lane >> 4;
-    return xs[((wm * TM + i) * 16 + c) * 16 + ((4 * q + j) ^ c)];
+    return xs[(i * 16 + c) * 16 + ((4 * q + j) ^ c)];
   }
   static __device__ __forceinline__ uint32_t word(const uint4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
 
@@ -178,24 +178,22 @@ struct MxTile {
       for (int d = 0; d < XB; ++d)
         stage<D, AHEAD, -1>(x[d], x[(d + 1) % XB], x[(d + D) % XB], c[d], c[(d + 1) % XB], c[(d + D) % XB], w0, w1, xa, xb, s0 + i + d, s1);
     }
-    static_assert(XB <= 4 && XB - 1 <= D, "the stages behind the loop are all on their way when it ends");
-    if (i < n) stage<D, AHEAD, 0>(x[0], x[1 % XB], x[0], c[0], c[1 % XB], c[0], w0, w1, xa, xb, s0 + i, s1);
-    if constexpr (XB > 2) {
-      if (i + 1 < n) stage<D, AHEAD, 1>(x[1], x[2 % XB], x[0], c[1], c[2 % XB], c[0], w0, w1, xa, xb, s0 + i + 1, s1);
-    }
-    if constexpr (XB > 3) {
-      if (i + 2 < n) stage<D, AHEAD, 2>(x[2], x[3 % XB], x[0], c[2], c[3 % XB], c[0], w0, w1, xa, xb, s0 + i + 2, s1);
+    static_assert((XB == 2 || XB == 4) && XB - 1 <= D, "the stages behind the loop are all on their way when it ends");
+    if (i < n) stage<D, AHEAD, 0>(x[0], x[1], x[0], c[0], c[1], c[0], w0, w1, xa, xb, s0 + i, s1);
+    if constexpr (XB == 4) {
+      if (i + 1 < n) stage<D, AHEAD, 1>(x[1], x[2], x[0], c[1], c[2], c[0], w0, w1, xa, xb, s0 + i + 1, s1);
+      if (i + 2 < n) stage<D, AHEAD, 2>(x[2], x[3], x[0], c[2], c[3], c[0], w0, w1, xa, xb, s0 + i + 2, s1);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was issued into LDS behind the last stage
   }
 };
 
 // first output (row, channel) of this lane in block (t, i) of a wave
-template <bool GATED, int TM, int TN, int WM, int WN>
+template <bool GATED, int TM, int TN, int WN>
 __device__ __forceinline__ int2 place(int mt, int nt, int wave, int t, int i) {
-  const int lane = threadIdx.x & 63, wm = wave / WN, wn = wave % WN;
+  const int lane = threadIdx.x & 63;
   constexpr int OT = GATED ? TN / 2 : TN;
-  return make_int2((mt * WM + wm) * 16 * TM + 16 * i + (lane & 15), ((nt * WN + wn) * OT + t) * 16 + 4 * (lane >> 4));
+  return make_int2((mt * TM + i) * 16 + (lane & 15), ((nt * WN + wave) * OT + t) * 16 + 4 * (lane >> 4));
 }
 
 // the outputs at a place from their sums p (and u of the second matrix)
@@ -220,11 +218,11 @@ __device__ __forceinline__ int2 tile_at(int b, int tm, int tn) {
 
 // KG groups of waves share a tile, each with its run of the stages and buffers of its own; their sums meet in LDS, and each group
 // finishes its share of the blocks.
-template <bool BF, bool GATED, int TM, int TN, int WM, int WN, int D, int XB, int KG, bool PART>
-__global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx4_tile_kernel(const Mx4Args a, int tm, int tn, int splits, f32x4* part) {
-  typedef MxTile<BF, GATED, TM, TN, WM, WN> T;
+template <bool BF, bool GATED, int TM, int TN, int WN, int D, int XB, int KG, bool PART>
+__global__ __launch_bounds__(64 * WN * KG, 2) void mx4_tile_kernel(const Mx4Args a, int tm, int tn, int splits, f32x4* part) {
+  typedef MxTile<BF, GATED, TM, TN, WN> T;
   constexpr int XS = T::BM * 16;
-  __shared__ uint4 x0[KG * XS], x1[KG * XS], x2[XB > 2 ? KG * XS : 1], x3[XB > 3 ? KG * XS : 1];  // objects of their own: see the top
+  __shared__ uint4 x0[KG * XS], x1[KG * XS], x2[XB == 4 ? KG * XS : 1], x3[XB == 4 ? KG * XS : 1];  // objects of their own: see the top
   const int total = tm * tn;
   const int split = PART ? (int)blockIdx.x / total : 0, b = (int)blockIdx.x - split * total;
   const int2 at = tile_at(b, tm, tn);
@@ -238,7 +236,6 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx4_tile_kernel(const Mx
   }
   const int xo = kg * XS;
   if constexpr (XB == 2) t.template run<D, 2>({x0 + xo, x1 + xo}, s0, s1, n);
-  else if constexpr (XB == 3) t.template run<D, 3>({x0 + xo, x1 + xo, x2 + xo}, s0, s1, n);
   else t.template run<D, 4>({x0 + xo, x1 + xo, x2 + xo, x3 + xo}, s0, s1, n);
   constexpr int OT = GATED ? TN / 2 : TN, BLOCKS = TM * TN, OUT = OT * TM;  // blocks of sums and of outputs of a wave
   constexpr int MINE = (OUT + KG - 1) / KG;                                  // this group's: kg, kg + KG, ..
@@ -280,7 +277,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx4_tile_kernel(const Mx
 #pragma unroll
     for (int j = 0; j < MINE; ++j) {
       const int b_ = kg + j * KG;
-      o[j] = place<GATED, TM, TN, WM, WN>(at.x, at.y, t.wave, b_ / TM, b_ % TM);
+      o[j] = place<GATED, TM, TN, WN>(at.x, at.y, t.wave, b_ / TM, b_ % TM);
     }
     if (!GATED) fetch(a, o, ex);
 #pragma unroll
@@ -289,16 +286,16 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void mx4_tile_kernel(const Mx
 }
 
 // sums of the parts in the order of the splits; a wave has one block of one wave of one tile (gated: of both matrices)
-template <bool BF, bool GATED, int TM, int TN, int WM, int WN>
+template <bool BF, bool GATED, int TM, int TN, int WN>
 __global__ __launch_bounds__(256) void mx4_join_kernel(const Mx4Args a, int tm, int tn, int splits, const f32x4* part) {
-  constexpr int NW = WM * WN, OT = GATED ? TN / 2 : TN;
+  constexpr int NW = WN, OT = GATED ? TN / 2 : TN;
   const int id = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
   const int blk = id % (OT * TM), w = id / (OT * TM);  // w: tile and wave
   if (w >= tm * tn * NW) return;
   const int2 at = tile_at(w / NW, tm, tn);
   const size_t stride = (size_t)tm * tn * NW * (TM * TN * 64);
   const f32x4* p = part + ((size_t)w * (TM * TN) + blk) * 64 + lane;
-  const int2 o = place<GATED, TM, TN, WM, WN>(at.x, at.y, w % NW, blk / TM, blk % TM);
+  const int2 o = place<GATED, TM, TN, WN>(at.x, at.y, w % NW, blk / TM, blk % TM);
   Extra ex[1] = {};
   if (!GATED) fetch(a, {o}, ex);
   f32x4 v = p[0], u = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -311,16 +308,16 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const Mx4Args a, int tm, 
   block_store<BF, GATED>(a, o, v, u, ex[0]);
 }
 
-template <bool BF, bool GATED, int TM, int TN, int WM, int WN, int D, int XB, int KG>
+template <bool BF, bool GATED, int TM, int TN, int WN, int D, int XB, int KG>
 hipError_t launch(const Mx4Args& a, int splits, float* part, hipStream_t st) {
-  typedef MxTile<BF, GATED, TM, TN, WM, WN> T;
+  typedef MxTile<BF, GATED, TM, TN, WN> T;
   const int tm = (a.m + T::BM - 1) / T::BM, tn = (mx4_blocks(a.n) + T::CB - 1) / T::CB;
   if (splits <= 1) {
-    mx4_tile_kernel<BF, GATED, TM, TN, WM, WN, D, XB, KG, false><<<tm * tn, 64 * T::NW * KG, 0, st>>>(a, tm, tn, 1, nullptr);
+    mx4_tile_kernel<BF, GATED, TM, TN, WN, D, XB, KG, false><<<tm * tn, 64 * T::NW * KG, 0, st>>>(a, tm, tn, 1, nullptr);
     return hipGetLastError();
   }
-  mx4_tile_kernel<BF, GATED, TM, TN, WM, WN, D, XB, KG, true><<<tm * tn * splits, 64 * T::NW * KG, 0, st>>>(a, tm, tn, splits, (f32x4*)part);
-  mx4_join_kernel<BF, GATED, TM, TN, WM, WN><<<(tm * tn * T::NW * TM * (GATED ? TN / 2 : TN) + 3) / 4, 256, 0, st>>>(a, tm, tn, splits, (const f32x4*)part);
+  mx4_tile_kernel<BF, GATED, TM, TN, WN, D, XB, KG, true><<<tm * tn * splits, 64 * T::NW * KG, 0, st>>>(a, tm, tn, splits, (f32x4*)part);
+  mx4_join_kernel<BF, GATED, TM, TN, WN><<<(tm * tn * T::NW * TM * (GATED ? TN / 2 : TN) + 3) / 4, 256, 0, st>>>(a, tm, tn, splits, (const f32x4*)part);
   return hipGetLastError();
 }
 
@@ -367,9 +364,9 @@ Plan plan(int m, int n, int k, bool gated) {
 template <bool BF, bool GATED>
 hipError_t launch_plan(const Mx4Args& a, const Plan& p, float* part, hipStream_t st) {
   switch (p.shape) {
-    case 0: return launch<BF, GATED, 2, 2, 1, 4, 3, 4, 2>(a, p.splits, part, st);
-    case 1: return launch<BF, GATED, 4, 2, 1, 4, 2, 2, 1>(a, p.splits, part, st);
-    default: return launch<BF, GATED, 4, 4, 1, 4, 2, 2, 1>(a, p.splits, part, st);
+    case 0: return launch<BF, GATED, 2, 2, 4, 3, 4, 2>(a, p.splits, part, st);
+    case 1: return launch<BF, GATED, 4, 2, 4, 2, 2, 1>(a, p.splits, part, st);
+    default: return launch<BF, GATED, 4, 4, 4, 2, 2, 1>(a, p.splits, part, st);
   }
 }
 

@@ -374,3 +374,35 @@ def test_other_stream_and_graph(dev, m):
         eager = mx4.linear(mx4.ffn(x, g, u, d, residual=x), g)
         torch.cuda.synchronize()
         assert torch.equal(outs[seed % 2], eager)
+
+
+def test_two_streams_at_once(dev):
+    """Calls of several forms in flight on two streams, each with workspaces of its own."""
+    (g, _), (u, _), (d, _) = random_weight(1400, 520, 1), random_weight(1400, 520, 2), random_weight(520, 1400, 3)
+    xs = [rand((m, 520), BF, m) for m in (1, 16, 70, 700)]
+    want = [mx4.ffn(x, g, u, d, residual=x) for x in xs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = {}
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for turn in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                for j in (range(4) if i == 0 else reversed(range(4))):
+                    got[i, j, turn] = mx4.ffn(xs[j], g, u, d, residual=xs[j])
+    for s in streams:
+        s.synchronize()
+    assert all(torch.equal(y, want[j]) for (_, j, _), y in got.items())
+
+
+def test_inputs_are_read_only(dev):
+    """Weights, rows, bias and residual keep their bytes, and so does what lies around a workspace."""
+    (g, _), (u, _), (d, _) = random_weight(1000, 520, 1), random_weight(1000, 520, 2), random_weight(520, 1000, 3)
+    for m in (3, 50, 600):
+        x, r = rand((m, 520), FP, m), rand((m, 520), FP, 1)
+        ws = torch.full((2 * m * 1000 + (40 << 20),), 0x5A, dtype=torch.uint8, device="cuda")
+        keep = [t.clone() for t in (x, r, g.codes, g.scales, u.codes, d.codes, d.scales)]
+        need = 2 * m * 1000 + (34 << 20)
+        mx4.ffn(x, g, u, d, residual=r, workspace=ws[:need])
+        assert all(torch.equal(a, b) for a, b in zip((x, r, g.codes, g.scales, u.codes, d.codes, d.scales), keep))
+        assert ws[need:].eq(0x5A).all()
