@@ -254,11 +254,14 @@ def launch(fn, args, dev, what: str) -> None:
     current, raw_stream, device = _device_fns
     if dev.type != "cuda":
         raise ValueError(f"{what}: the tensors must be on the GPU")
-    if dev.index == current():
-        check(fn(C.byref(args), raw_stream(dev.index)), what)
+    i = dev.index
+    if i == current():
+        rc = fn(C.byref(args), raw_stream(i))
     else:
         with device(dev):
-            check(fn(C.byref(args), raw_stream(dev.index)), what)
+            rc = fn(C.byref(args), raw_stream(i))
+    if rc:
+        check(rc, what)
 
 
 TIMER_KINDS = {1: "resid_gemm", 2: "hift_phase", 3: "hift_source", 4: "hift_stft", 5: "hift_istft", 6: "hift_reflect",

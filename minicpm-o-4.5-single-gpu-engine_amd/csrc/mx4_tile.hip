@@ -110,13 +110,12 @@ struct MxTile {
       for (int t = i * TN / TM; t < (i + 1) * TN / TM; ++t)
         wnx[t] = widen<BF>(word(cd.c[t], jn), __uint_as_float(((cd.e[t] >> (8 * (st & 3))) & 0xffu) << 23));
     }
-    constexpr int EVERY = TM > 4 ? TM / 4 : 1;  // 4 TN conversions to TM TN MFMAs
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
-      for (int t = 0; t < TN; ++t) {
+      for (int t = 0; t < TN; ++t) {  // an MFMA, a conversion; then a read
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        if ((i * TN + t) % EVERY == 0) __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
       }
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
@@ -154,7 +153,7 @@ struct MxTile {
     }
   }
 
-  // D stages in flight over XB buffers
+  // n stages from s0 on, those from s1 on of zeros; D in flight over XB buffers
   template <int D, int XB>
   __device__ __forceinline__ void run(uint4* const (&x)[XB], int s0, int s1, int n) {
     constexpr int AHEAD = XB > D ? 2 : 1;

@@ -123,7 +123,7 @@ def _input(x: torch.Tensor, w: MX4Weight) -> tuple[int, int, int]:
 
 def _output(x: torch.Tensor, m: int, n: int, out, dev) -> tuple[torch.Tensor, int]:
     if out is None:
-        return torch.empty((m, n), dtype=x.dtype, device=dev), n
+        return x.new_empty((m, n)), n
     return out, _rows("out", out, m, n, x.dtype, dev)
 
 

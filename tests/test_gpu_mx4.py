@@ -406,3 +406,17 @@ def test_inputs_are_read_only(dev):
         mx4.ffn(x, g, u, d, residual=r, workspace=ws[:need])
         assert all(torch.equal(a, b) for a, b in zip((x, r, g.codes, g.scales, u.codes, d.codes, d.scales), keep))
         assert ws[need:].eq(0x5A).all()
+
+
+@pytest.mark.parametrize("m,k", [(1, 392), (7, 8), (16, 136), (20, 8), (40, 392), (333, 1032), (3000, 200), (200, 5000)])
+def test_nothing_of_an_earlier_call_is_left_behind(dev, m, k):
+    """Rows and columns beyond a call's end read as zeros although the LDS of every CU holds NaN of the call before."""
+    w, _ = random_weight(300, k, 1)
+    big, _ = random_weight(4096, 4096, 2)
+    x = rand((m, k), BF, 3)
+    want = mx4.linear(x, w)
+    assert want.isfinite().all()
+    for rows in (1, 16, 32, 4096):
+        nan = torch.full((rows, 4096), float("nan"), dtype=BF, device="cuda")
+        assert mx4.linear(nan, big).isnan().all()
+        assert torch.equal(mx4.linear(x, w), want)
