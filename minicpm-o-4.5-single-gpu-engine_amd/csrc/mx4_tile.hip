@@ -11,7 +11,7 @@
 //
 // The conversion is one instruction for two weights and shares the wave's time with the MFMAs; the codes come to a CU at a quarter
 // of bf16's bytes, which is why a tile of only 64 rows reaches the rate of a large bf16 product: 64 x 256 tiles run 4001 rows x
-// 6144 x 4096 in 156 to 171 us (1.18 to 1.29 PFLOP/s, by machine) and 2005 rows' gated 14336 x 4096 x 2 in 359 to 396 (1.19 to 1.31).
+// 6144 x 4096 in 156 to 176 us (1.15 to 1.29 PFLOP/s, by machine) and 2005 rows' gated 14336 x 4096 x 2 in 359 to 385 (1.22 to 1.31).
 // There the matrix units are busy for 53 to 62% of the cycles at a clock of 2.0 GHz, vector instructions issue in 40% and the waves
 // wait for a quarter of theirs.  With two workgroups a CU the barriers of one fall into the other's MFMAs: 128 x 256 tiles of eight waves, one
 // workgroup a CU, took 9% longer, 256 x 256 (spilling) 21%, waves of 128 x 64 (half the conversions a product) alone on a SIMD 18%.
@@ -124,7 +124,7 @@ struct MxTile {
   // Stage st in (xc, cc), the next one in (xn, cn); the loads of stage st + D go to (xl, cl).
   // AHEAD 1: fragments are read a step ahead, which 16 MFMAs a step cover; the barrier stands in front of the last step, when every
   // wave holds its fragments of the stage, and the freed buffer is the one to load (xl is xc).
-  // AHEAD 2: with 4 MFMAs a step a fragment's way from LDS takes longer than a step, so they are read two ahead into two sets in
+  // AHEAD 2: with 2 or 4 MFMAs a step a fragment's way from LDS takes longer than a step, so they are read two ahead into two sets in
   // turn; the barrier stands in the stage's middle, and a buffer more than D lets xl be one that was read a stage ago.
   // TAIL: the (TAIL + 1)th stage behind the loop.  Nothing is left to load there, so it loads nothing and knows how many loads are
   // behind the next stage's (loads that the compiler may drop, as nobody reads what they bring, could not be counted on).
@@ -240,7 +240,7 @@ __global__ __launch_bounds__(64 * WN * KG, 2) void mx4_tile_kernel(const Mx4Args
   constexpr int MINE = (OUT + KG - 1) / KG;                                  // this group's: kg, kg + KG, ..
   f32x4 sum[GATED ? 2 : 1][MINE];
   if constexpr (KG > 1) {
-    static_assert(OUT % KG == 0 && KG % 2 == 0 && KG / 2 * T::NW * BLOCKS * 64 <= KG * XS, "whole shares; half of the groups' sums fit a buffer");
+    static_assert((OUT % KG == 0 || OUT == 1) && KG % 2 == 0 && KG / 2 * T::NW * BLOCKS * 64 <= KG * XS, "whole shares; half of the groups' sums fit a buffer");
     __syncthreads();  // every wave is through with the buffers
     const auto red = [&](int g) { return (f32x4*)(g < KG / 2 ? x0 : x1) + ((g % (KG / 2)) * T::NW + t.wave) * BLOCKS * 64 + t.lane; };
     f32x4* own = red(kg);
@@ -249,6 +249,7 @@ __global__ __launch_bounds__(64 * WN * KG, 2) void mx4_tile_kernel(const Mx4Args
 #pragma unroll
       for (int i = 0; i < TM; ++i) own[(y * TM + i) * 64] = t.acc[y][i];
     __syncthreads();
+    if (OUT == 1 && kg > 0) return;
 #pragma unroll
     for (int j = 0; j < MINE; ++j)
 #pragma unroll
@@ -321,14 +322,14 @@ hipError_t launch(const Mx4Args& a, int splits, float* part, hipStream_t st) {
 }
 
 // The tiles, each with four waves side by side: rows, weight channels (gated: half of each matrix), groups of waves that split k, and
-// the microseconds of a pass (a stage of each group) with one workgroup on a CU and, of each, with several.  Measured: 4096
-// channels x 14336 columns x 32 rows take 38 / 84 / 106 us (k in parts: 16 / 19 / 20), 14336 x 4096 x 2, gated, of 200 rows 70 / 54 / 56
-// and of 2005 rows 620 / 374 / 360.
+// the microseconds of a pass (a stage of each group) with one workgroup on a CU and, of each, with several.  Measured: 6144
+// channels x 4096 columns x 64 rows take 11.3 / 13.5 / 25 / 35 us, 28000 x 4096 x 32 20 / 16 / 27 / 34, x 100 46 / 40 / 35 / 38,
+// 14336 x 4096 x 2, gated, of 2005 rows in the wide two 374 / 360.
 struct Shape {
   int bm, bn, kg;
   float one, many;
 };
-constexpr Shape SHAPES[3] = {{32, 128, 2, 0.52f, 0.60f}, {64, 128, 1, 0.70f, 0.44f}, {64, 256, 1, 0.90f, 0.79f}};
+constexpr Shape SHAPES[4] = {{16, 128, 2, 0.42f, 0.42f}, {32, 128, 2, 0.52f, 0.60f}, {64, 128, 1, 0.70f, 0.44f}, {64, 256, 1, 0.90f, 0.79f}};
 
 struct Plan {
   int shape, tiles, splits;
@@ -340,7 +341,7 @@ struct Plan {
 Plan plan(int m, int n, int k, bool gated) {
   Plan best{0, 0, 1, 3e38f};
   const int steps = mx4_steps(k), cols = gated ? 2 * n : n;
-  for (int i = 0; i < 3; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const Shape& s = SHAPES[i];
     const long long tiles = (long long)((m + s.bm - 1) / s.bm) * ((cols + s.bn - 1) / s.bn);
     int last = 0;
@@ -363,8 +364,9 @@ Plan plan(int m, int n, int k, bool gated) {
 template <bool BF, bool GATED>
 hipError_t launch_plan(const Mx4Args& a, const Plan& p, float* part, hipStream_t st) {
   switch (p.shape) {
-    case 0: return launch<BF, GATED, 2, 2, 4, 3, 4, 2>(a, p.splits, part, st);
-    case 1: return launch<BF, GATED, 4, 2, 4, 2, 2, 1>(a, p.splits, part, st);
+    case 0: return launch<BF, GATED, 1, 2, 4, 3, 4, 2>(a, p.splits, part, st);
+    case 1: return launch<BF, GATED, 2, 2, 4, 3, 4, 2>(a, p.splits, part, st);
+    case 2: return launch<BF, GATED, 4, 2, 4, 2, 2, 1>(a, p.splits, part, st);
     default: return launch<BF, GATED, 4, 4, 4, 2, 2, 1>(a, p.splits, part, st);
   }
 }
@@ -377,7 +379,7 @@ bool mx4_takes_tiles(int m, int n, int k, long long ldx, bool gated) {
   const int outside = mx4_rows_outside(m, k, gated);
   if (outside == 0) return false;
   // few rows, too long for the LDS: by the stream (5.5 TB/s) and what comes from memory for every block of a CU.  4096 channels x 14336
-  // columns x 6, 10 and 16 rows take 10.6, 13.9 and 17.9 us (tiles 13.4 to 13.6), 2048 x 5464 x 16 6.5 (9.5), 20000 x 8192 x 16 34.9 (24.1).
+  // columns x 6, 10 and 16 rows take 10.6, 13.9 and 17.9 us (tiles 12.4 to 12.6), 2048 x 5464 x 16 6.5 (8.5), 20000 x 8192 x 16 34.9 (24.1).
   const float mb = (gated ? 2 : 1) * 0.53f * n * (k * 1e-6f);
   return plan(m, n, k, gated).us < 2.5f + mb / 5.5f + 0.45f * outside * ((mx4_blocks(n) + 255) / 256);
 }

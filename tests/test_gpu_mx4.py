@@ -158,19 +158,19 @@ def test_linear_sizes(dev, n, k, m, dt):
 
 
 @pytest.mark.parametrize("dt", [BF, FP], ids=str)
-@pytest.mark.parametrize("m,n,k", [(16, 40, 5464), (16, 300, 4096), (16, 1027, 14336), (9, 100, 9224), (40, 130, 14336), (3000, 31, 14336), (100, 4100, 9000), (2000, 515, 264), (2000, 1027, 5000),
+@pytest.mark.parametrize("m,n,k", [(16, 40, 5464), (16, 300, 4096), (16, 1027, 14336), (9, 100, 9224), (40, 130, 14336), (3000, 31, 14336), (100, 4100, 9000), (257, 2001, 1032), (257, 31, 14336), (2000, 515, 264), (2000, 1027, 5000),
                                    (600, 4100, 5000), (4100, 6000, 1032)])
 def test_linear_forms(dev, m, n, k, dt):
-    """Sizes at which each form is chosen: rows too long for the LDS, the three tiles, with k whole and in parts."""
+    """Sizes at which each form is chosen: rows too long for the LDS, the four tiles, with k whole and in parts."""
     w, v = random_weight(n, k, n + k + m)
     check_linear(rand((m, k), dt, m), w, v, bias=torch.randn(n, device="cuda"), residual=rand((m, n), dt, m + 1))
 
 
-@pytest.mark.parametrize("m", [1, 20, 3000])
+@pytest.mark.parametrize("m,n", [(1, 96), (20, 96), (257, 2001), (3000, 96), (3000, 515)])
 @pytest.mark.parametrize("steps", list(range(1, 19)) + [27, 30])
-def test_every_number_of_steps(dev, m, steps):
-    """Columns of 1 to 30 steps of 128: every remainder of the loops, in calls of one row, of a few (two groups of waves) and of many."""
-    n, k = 96, 128 * steps - 8 * (steps % 3)
+def test_every_number_of_steps(dev, m, n, steps):
+    """Columns of 1 to 30 steps of 128: every remainder of the loops, in calls of one row and in those that each of the tiles takes."""
+    k = 128 * steps - 8 * (steps % 3)
     w, v = random_weight(n, k, steps)
     x = rand((m, k), FP, m)
     y = check_linear(x, w, v)
@@ -298,7 +298,7 @@ def test_gated(dev, m, dt, act):
 
 
 @pytest.mark.parametrize("dt", [BF, FP], ids=str)
-@pytest.mark.parametrize("m,n,k", [(16, 40, 5464), (16, 5000, 4096), (16, 700, 14336), (40, 130, 14336), (3000, 31, 14336), (3000, 130, 264), (3000, 1027, 264), (257, 4100, 5000)])
+@pytest.mark.parametrize("m,n,k", [(16, 40, 5464), (16, 5000, 4096), (16, 700, 14336), (40, 130, 14336), (50, 4100, 264), (257, 130, 14336), (3000, 31, 14336), (3000, 130, 264), (3000, 1027, 264), (257, 4100, 5000)])
 def test_gated_forms(dev, m, n, k, dt):
     check_gated(m, n, k, dt, "silu")
 
