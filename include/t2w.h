@@ -409,6 +409,7 @@ int t2w_kv8_attention(const t2w_kv8_attention_args* a, void* stream);
 
 enum { T2W_MX4_BF16 = 0, T2W_MX4_FP16 = 1, T2W_MX4_FP32 = 2 };
 enum { T2W_MX4_SILU = 0, T2W_MX4_GELU = 1 }; /* GELU in its tanh form */
+enum { T2W_MX4_INNER_ROUNDED = 0, T2W_MX4_INNER_WIDE = 1 };
 
 typedef struct {
   const void* codes; const void* scales; /* as laid out, 16- and 4-byte aligned */
@@ -468,13 +469,14 @@ typedef struct {
 size_t t2w_mx4_gated_workspace_bytes(const t2w_mx4_gated_args* a);
 int t2w_mx4_gated(const t2w_mx4_gated_args* a, void* stream);
 
-/* y = (act(x gate^T) * (x up^T)) down^T + residual: gate, up [f, k], down [n, f].  The inner values are rounded to x's type (they
- * are the second product's operand): of fp16, beyond 65504 they are infinite. */
+/* y = (act(x gate^T) * (x up^T)) down^T + residual: gate, up [f, k], down [n, f].  The inner values are the second product's operand.
+ * T2W_MX4_INNER_WIDE: held to 2^-16 of their value over fp32's range (as two bf16 numbers each, which doubles that product's
+ * operations).  T2W_MX4_INNER_ROUNDED: rounded to x's type; of fp16, beyond 65504 they are infinite. */
 typedef struct {
   const void* x; long long ldx;
   int dtype, m;
   t2w_mx4_weight gate, up, down;
-  int act;
+  int act, inner;
   const void* residual; long long ldr;
   void* y; long long ldy;
   void* workspace; size_t workspace_bytes; /* as t2w_mx4_linear's, of t2w_mx4_ffn_workspace_bytes (the inner rows and up to 34 MB) */

@@ -143,7 +143,7 @@ class MX4GatedArgs(C.Structure):
 
 
 class MX4FFNArgs(C.Structure):
-    _fields_ = [("x", P), ("ldx", C.c_longlong), ("dtype", I), ("m", I), ("gate", MX4Weight), ("up", MX4Weight), ("down", MX4Weight), ("act", I),
+    _fields_ = [("x", P), ("ldx", C.c_longlong), ("dtype", I), ("m", I), ("gate", MX4Weight), ("up", MX4Weight), ("down", MX4Weight), ("act", I), ("inner", I),
                 ("residual", P), ("ldr", C.c_longlong), ("y", P), ("ldy", C.c_longlong), ("workspace", P), ("workspace_bytes", C.c_size_t)]
 
 

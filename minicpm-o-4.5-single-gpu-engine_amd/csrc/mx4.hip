@@ -28,7 +28,7 @@ namespace {
 // 14336 x 4096 x 2 12.6 us (5.0 TB/s) and 4096 x 14336 6.7 us (one block a CU: 4.7 TB/s).  Two blocks a wave at a time (half the
 // reads of x) took 10% longer; 4 or 8 waves a workgroup instead of 16 gain nothing at one row and take 26.7 and 18.3 us instead of
 // 16.5 at 16 rows' gated 14336 x 4096 x 2.
-template <bool BF, bool GATED, bool ALL>
+template <bool BF, bool GATED, Form F, bool ALL>
 __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Args a, int held) {
   extern __shared__ uint4 lds[];  // x [rows][held][4][16], then sums [2][waves][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Args a, int hel
     u = first;
     const int n = g * 16 + 4 * q, m = m0 + (lane & 15);
     Extra ex[1] = {};
-    if (!GATED && wave == 0) fetch(a, {make_int2(m, n)}, ex);
+    if (!GATED && wave == 0) fetch<F>(a, {make_int2(m, n)}, ex);
     f32x4* p = part + turn * waves * 64;
     p[wave * 64 + lane] = acc[0] + acc[1];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the codes in flight are not waited for
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(const Mx4Args a, int hel
 #pragma unroll
         for (int e = 0; e < 4; ++e) r[e] = gate_act(r[e], a.act) * o[e];
       }
-      finish<BF>(a, m, n, r, ex[0]);
+      finish<BF, GATED, F>(a, m, n, r, ex[0]);
     }
     g = gn;
   }
@@ -148,7 +148,7 @@ RowsPlan rows_plan(int m, int k, bool gated) {
   return {waves, held, (size_t)rows * held * 1024 + sums};
 }
 
-template <bool BF, bool GATED, bool ALL>
+template <bool BF, bool GATED, Form F, bool ALL>
 hipError_t launch_rows(const Mx4Args& a, const RowsPlan& p, hipStream_t st) {
   if (p.bytes > 64 * 1024) {  // beyond the default a function has to be told, on each device
     static std::atomic<uint64_t> told{0};
@@ -157,14 +157,14 @@ hipError_t launch_rows(const Mx4Args& a, const RowsPlan& p, hipStream_t st) {
     if (e != hipSuccess) return e;
     const uint64_t bit = dev < 64 ? 1ull << dev : 0;
     if (!(told.load(std::memory_order_acquire) & bit)) {
-      e = hipFuncSetAttribute((const void*)mx4_rows_kernel<BF, GATED, ALL>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_CU);
+      e = hipFuncSetAttribute((const void*)mx4_rows_kernel<BF, GATED, F, ALL>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_CU);
       if (e != hipSuccess) return e;
       told.fetch_or(bit, std::memory_order_release);
     }
   }
   const int nb = mx4_blocks(a.n), fit = std::max(1, std::min(16 / p.waves, (int)(LDS_CU / p.bytes)));  // workgroups a CU
   const int rounds = (nb + 256 * fit - 1) / (256 * fit);
-  mx4_rows_kernel<BF, GATED, ALL><<<dim3((nb + rounds - 1) / rounds, (a.m + 15) / 16), p.waves * 64, p.bytes, st>>>(a, p.held);
+  mx4_rows_kernel<BF, GATED, F, ALL><<<dim3((nb + rounds - 1) / rounds, (a.m + 15) / 16), p.waves * 64, p.bytes, st>>>(a, p.held);
   return hipGetLastError();
 }
 
@@ -271,14 +271,13 @@ hipError_t mx4_quantize(const t2w_mx4_quantize_args& a, hipStream_t st) {
 
 int mx4_rows_outside(int m, int k, bool gated) { return mx4_units(k) - rows_plan(m, k, gated).held; }
 
-hipError_t mx4_rows(const Mx4Args& a, bool bf, bool gated, hipStream_t st) {
+hipError_t mx4_rows(const Mx4Args& a, bool bf, bool gated, Form form, hipStream_t st) {
   const RowsPlan p = rows_plan(a.m, a.k, gated);
-  const auto go = [&](auto b, auto g) {
+  return mx4_dispatch(bf, gated, form, [&](auto b, auto g, auto f) {
     constexpr bool BF = decltype(b)::value, GATED = decltype(g)::value;
-    return p.held == mx4_units(a.k) ? launch_rows<BF, GATED, true>(a, p, st) : launch_rows<BF, GATED, false>(a, p, st);
-  };
-  if (gated) return bf ? go(std::true_type{}, std::true_type{}) : go(std::false_type{}, std::true_type{});
-  return bf ? go(std::true_type{}, std::false_type{}) : go(std::false_type{}, std::false_type{});
+    constexpr Form F = decltype(f)::value;
+    return p.held == mx4_units(a.k) ? launch_rows<BF, GATED, F, true>(a, p, st) : launch_rows<BF, GATED, F, false>(a, p, st);
+  });
 }
 
 }  // namespace t2w

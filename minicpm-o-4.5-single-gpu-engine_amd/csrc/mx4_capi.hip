@@ -64,12 +64,15 @@ const char* check_workspace(const void* ws, size_t have, size_t need, const Rows
   return nullptr;
 }
 
-int run(const Mx4Args& g, int dtype, bool gated, void* workspace, void* stream, const char* what) {
+int run(const Mx4Args& g, int dtype, bool gated, Form form, void* workspace, void* stream, const char* what) {
   Mx4Args a = g;
-  const auto whole = [](const void* p, long long ld, int m) { return !((uintptr_t)p & 7) && (m == 1 || ld % 4 == 0); };
-  a.quad = a.n % 4 == 0 && whole(a.y, a.ldy, a.m) && (!a.residual || whole(a.residual, a.ldr, a.m));
+  const int rows = form == Form::PLAIN ? a.m : gated ? 2 * a.m : a.m / 2;  // of y
+  const auto whole = [&](const void* p, long long ld) { return !((uintptr_t)p & 7) && (rows == 1 || ld % 4 == 0); };
+  a.quad = a.n % 4 == 0 && whole(a.y, a.ldy) && (!a.residual || whole(a.residual, a.ldr));
+  a.half = dtype == T2W_MX4_FP16;
   const bool bf = dtype == T2W_MX4_BF16;
-  const hipError_t e = mx4_takes_tiles(a.m, a.n, a.k, a.ldx, gated) ? mx4_tiles(a, bf, gated, workspace, (hipStream_t)stream) : mx4_rows(a, bf, gated, (hipStream_t)stream);
+  const hipError_t e = mx4_takes_tiles(a.m, a.n, a.k, a.ldx, gated) ? mx4_tiles(a, bf, gated, form, workspace, (hipStream_t)stream)
+                                                                    : mx4_rows(a, bf, gated, form, (hipStream_t)stream);
   return e == hipSuccess ? 0 : xerr(what, e);
 }
 
@@ -123,7 +126,7 @@ int t2w_mx4_linear(const t2w_mx4_linear_args* a, void* stream) {
   g.w[0] = (const uint8_t*)a->w.codes, g.s[0] = (const uint8_t*)a->w.scales;
   g.x = a->x, g.ldx = a->ldx, g.m = a->m, g.n = a->w.n, g.k = a->w.k;
   g.bias = a->bias, g.residual = a->residual, g.ldr = a->ldr, g.y = a->y, g.ldy = a->ldy;
-  return run(g, a->dtype, false, a->workspace, stream, "mx4 linear");
+  return run(g, a->dtype, false, Form::PLAIN, a->workspace, stream, "mx4 linear");
 }
 
 static const char* check_gated(const t2w_mx4_weight& gate, const t2w_mx4_weight& up, int act) {
@@ -158,28 +161,31 @@ int t2w_mx4_gated(const t2w_mx4_gated_args* a, void* stream) {
   if (const char* e = check_workspace(a->workspace, a->workspace_bytes, need, out, Rows{a->x, a->ldx * 2, 2LL * a->gate.k, a->m}, nullptr, 0)) return xerr(e);
   const Rows ws{a->workspace, (long long)need, (long long)need, 1};
   if (need && (on_weight(ws, a->gate) || on_weight(ws, a->up))) return xerr("mx4: the workspace overlaps an operand");
-  return run(gated_args(a->gate, a->up, a->x, a->ldx, a->m, a->act, a->y, a->ldy), a->dtype, true, a->workspace, stream, "mx4 gated");
+  return run(gated_args(a->gate, a->up, a->x, a->ldx, a->m, a->act, a->y, a->ldy), a->dtype, true, Form::PLAIN, a->workspace, stream, "mx4 gated");
 }
 
-// The inner rows lie in the workspace, each at a 16-byte boundary, rounded once to x's type: they are the second product's matrix
-// operand, and carrying their fp32 values (as two operands each) would double that product, a third of the block's work.  Output errors
-// grow from the output's own rounding alone to up to sqrt(2) of it (bf16 1.7e-3 to 2.0-2.3e-3, fp16 2.1e-4 to 2.5-3.1e-4, relative).
+// The inner rows lie in the workspace, each at a 16-byte boundary: the second product's matrix operand, of 16 bits.  Wide, a value is two
+// rows' sum, which doubles that product (a third of the block's work) and leaves the outputs' errors at their own rounding's.  Rounded
+// to x's type once, errors grow to up to sqrt(2) of that (bf16 1.7e-3 to 2.0-2.3e-3, fp16 2.1e-4 to 2.5-3.1e-4, relative) and fp16 loses
+// what is beyond 65504.
 static long long inner_ld(const t2w_mx4_ffn_args& a) { return (a.gate.n + 7) / 8 * 8; }
+static int inner_rows(const t2w_mx4_ffn_args& a) { return a.inner == T2W_MX4_INNER_WIDE ? 2 * a.m : a.m; }
 
 static const char* check_ffn(const t2w_mx4_ffn_args* a) {
   if (!a) return "mx4 ffn: null arguments";
   if (const char* e = check_gated(a->gate, a->up, a->act)) return e;
   if (const char* e = check_weight(a->down)) return e;
+  if (a->inner != T2W_MX4_INNER_ROUNDED && a->inner != T2W_MX4_INNER_WIDE) return "mx4 ffn: inner must be rounded or wide";
   if (a->down.k != a->gate.n) return "mx4 ffn: the down projection's columns are not the gate's channels";
   return check_rows(a->x, a->ldx, a->gate.k, a->y, a->ldy, a->down.n, a->residual, a->ldr, a->dtype, a->m);
 }
 
 // the inner rows, then (16-byte aligned: rows are) the parts of whichever product needs more
-static size_t inner_bytes(const t2w_mx4_ffn_args& a) { return (size_t)a.m * inner_ld(a) * 2; }
+static size_t inner_bytes(const t2w_mx4_ffn_args& a) { return (size_t)inner_rows(a) * inner_ld(a) * 2; }
 
 size_t t2w_mx4_ffn_workspace_bytes(const t2w_mx4_ffn_args* a) {
   if (!a || check_gated(a->gate, a->up, a->act) || check_weight(a->down) || a->m < 1 || a->m > MAX_ROWS) return 0;
-  const size_t p = part_bytes(a->m, a->gate.n, a->gate.k, a->ldx, true), q = part_bytes(a->m, a->down.n, a->down.k, inner_ld(*a), false);
+  const size_t p = part_bytes(a->m, a->gate.n, a->gate.k, a->ldx, true), q = part_bytes(inner_rows(*a), a->down.n, a->down.k, inner_ld(*a), false);
   return inner_bytes(*a) + (p > q ? p : q);
 }
 
@@ -192,13 +198,14 @@ int t2w_mx4_ffn(const t2w_mx4_ffn_args* a, void* stream) {
   if (const char* e = check_workspace(a->workspace, a->workspace_bytes, need, out, Rows{a->x, a->ldx * 2, 2LL * a->gate.k, a->m}, a->residual, a->ldr)) return xerr(e);
   if (on_weight(ws, a->gate) || on_weight(ws, a->up) || on_weight(ws, a->down)) return xerr("mx4: the workspace overlaps an operand");
   const long long ldh = inner_ld(*a);
+  const Form form = a->inner == T2W_MX4_INNER_WIDE ? Form::WIDE : Form::PLAIN;
   void* part = (uint8_t*)a->workspace + inner_bytes(*a);
-  if (int rc = run(gated_args(a->gate, a->up, a->x, a->ldx, a->m, a->act, a->workspace, ldh), a->dtype, true, part, stream, "mx4 ffn")) return rc;
+  if (int rc = run(gated_args(a->gate, a->up, a->x, a->ldx, a->m, a->act, a->workspace, ldh), a->dtype, true, form, part, stream, "mx4 ffn")) return rc;
   Mx4Args g{};
   g.w[0] = (const uint8_t*)a->down.codes, g.s[0] = (const uint8_t*)a->down.scales;
-  g.x = a->workspace, g.ldx = ldh, g.m = a->m, g.n = a->down.n, g.k = a->down.k;
+  g.x = a->workspace, g.ldx = ldh, g.m = inner_rows(*a), g.n = a->down.n, g.k = a->down.k;
   g.residual = a->residual, g.ldr = a->ldr, g.y = a->y, g.ldy = a->ldy;
-  return run(g, a->dtype, false, part, stream, "mx4 ffn");
+  return run(g, a->dtype, false, form, part, stream, "mx4 ffn");
 }
 
 }  // extern "C"

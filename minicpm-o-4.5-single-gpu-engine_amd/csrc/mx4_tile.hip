@@ -196,14 +196,14 @@ __device__ __forceinline__ int2 place(int mt, int nt, int wave, int t, int i) {
 }
 
 // the outputs at a place from their sums p (and u of the second matrix)
-template <bool BF, bool GATED>
+template <bool BF, bool GATED, Form F>
 __device__ __forceinline__ void block_store(const Mx4Args& a, int2 at, f32x4 p, f32x4 u, const Extra& ex) {
   float o[4] = {p[0], p[1], p[2], p[3]};
   if constexpr (GATED) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = gate_act(o[e], a.act) * u[e];
   }
-  finish<BF>(a, at.x, at.y, o, ex);
+  finish<BF, GATED, F>(a, at.x, at.y, o, ex);
 }
 
 // tile number b of tm x tn tiles -> (row, column): an XCD gets a run of tiles (workgroups go round the 8 XCDs), which walks
@@ -217,7 +217,7 @@ __device__ __forceinline__ int2 tile_at(int b, int tm, int tn) {
 
 // KG groups of waves share a tile, each with its run of the stages and buffers of its own; their sums meet in LDS, and each group
 // finishes its share of the blocks.
-template <bool BF, bool GATED, int TM, int TN, int WN, int D, int XB, int KG, bool PART>
+template <bool BF, bool GATED, Form F, int TM, int TN, int WN, int D, int XB, int KG, bool PART>
 __global__ __launch_bounds__(64 * WN * KG, 2) void mx4_tile_kernel(const Mx4Args a, int tm, int tn, int splits, f32x4* part) {
   typedef MxTile<BF, GATED, TM, TN, WN> T;
   constexpr int XS = T::BM * 16;
@@ -279,14 +279,14 @@ __global__ __launch_bounds__(64 * WN * KG, 2) void mx4_tile_kernel(const Mx4Args
       const int b_ = kg + j * KG;
       o[j] = place<GATED, TM, TN, WN>(at.x, at.y, t.wave, b_ / TM, b_ % TM);
     }
-    if (!GATED) fetch(a, o, ex);
+    if (!GATED) fetch<F>(a, o, ex);
 #pragma unroll
-    for (int j = 0; j < MINE; ++j) block_store<BF, GATED>(a, o[j], sum[0][j], sum[GATED ? 1 : 0][j], ex[j]);
+    for (int j = 0; j < MINE; ++j) block_store<BF, GATED, F>(a, o[j], sum[0][j], sum[GATED ? 1 : 0][j], ex[j]);
   }
 }
 
 // sums of the parts in the order of the splits; a wave has one block of one wave of one tile (gated: of both matrices)
-template <bool BF, bool GATED, int TM, int TN, int WN>
+template <bool BF, bool GATED, Form F, int TM, int TN, int WN>
 __global__ __launch_bounds__(256) void mx4_join_kernel(const Mx4Args a, int tm, int tn, int splits, const f32x4* part) {
   constexpr int NW = WN, OT = GATED ? TN / 2 : TN;
   const int id = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const Mx4Args a, int tm, 
   const f32x4* p = part + ((size_t)w * (TM * TN) + blk) * 64 + lane;
   const int2 o = place<GATED, TM, TN, WN>(at.x, at.y, w % NW, blk / TM, blk % TM);
   Extra ex[1] = {};
-  if (!GATED) fetch(a, {o}, ex);
+  if (!GATED) fetch<F>(a, {o}, ex);
   f32x4 v = p[0], u = f32x4{0.f, 0.f, 0.f, 0.f};
   if constexpr (GATED) u = p[OT * TM * 64];
 #pragma unroll 4
@@ -305,19 +305,19 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const Mx4Args a, int tm, 
     v += p[s * stride];
     if constexpr (GATED) u += p[s * stride + OT * TM * 64];
   }
-  block_store<BF, GATED>(a, o, v, u, ex[0]);
+  block_store<BF, GATED, F>(a, o, v, u, ex[0]);
 }
 
-template <bool BF, bool GATED, int TM, int TN, int WN, int D, int XB, int KG>
+template <bool BF, bool GATED, Form F, int TM, int TN, int WN, int D, int XB, int KG>
 hipError_t launch(const Mx4Args& a, int splits, float* part, hipStream_t st) {
   typedef MxTile<BF, GATED, TM, TN, WN> T;
   const int tm = (a.m + T::BM - 1) / T::BM, tn = (mx4_blocks(a.n) + T::CB - 1) / T::CB;
   if (splits <= 1) {
-    mx4_tile_kernel<BF, GATED, TM, TN, WN, D, XB, KG, false><<<tm * tn, 64 * T::NW * KG, 0, st>>>(a, tm, tn, 1, nullptr);
+    mx4_tile_kernel<BF, GATED, F, TM, TN, WN, D, XB, KG, false><<<tm * tn, 64 * T::NW * KG, 0, st>>>(a, tm, tn, 1, nullptr);
     return hipGetLastError();
   }
-  mx4_tile_kernel<BF, GATED, TM, TN, WN, D, XB, KG, true><<<tm * tn * splits, 64 * T::NW * KG, 0, st>>>(a, tm, tn, splits, (f32x4*)part);
-  mx4_join_kernel<BF, GATED, TM, TN, WN><<<(tm * tn * T::NW * TM * (GATED ? TN / 2 : TN) + 3) / 4, 256, 0, st>>>(a, tm, tn, splits, (const f32x4*)part);
+  mx4_tile_kernel<BF, GATED, F, TM, TN, WN, D, XB, KG, true><<<tm * tn * splits, 64 * T::NW * KG, 0, st>>>(a, tm, tn, splits, (f32x4*)part);
+  mx4_join_kernel<BF, GATED, F, TM, TN, WN><<<(tm * tn * T::NW * TM * (GATED ? TN / 2 : TN) + 3) / 4, 256, 0, st>>>(a, tm, tn, splits, (const f32x4*)part);
   return hipGetLastError();
 }
 
@@ -361,13 +361,13 @@ Plan plan(int m, int n, int k, bool gated) {
   return best;
 }
 
-template <bool BF, bool GATED>
+template <bool BF, bool GATED, Form F>
 hipError_t launch_plan(const Mx4Args& a, const Plan& p, float* part, hipStream_t st) {
   switch (p.shape) {
-    case 0: return launch<BF, GATED, 1, 2, 4, 3, 4, 2>(a, p.splits, part, st);
-    case 1: return launch<BF, GATED, 2, 2, 4, 3, 4, 2>(a, p.splits, part, st);
-    case 2: return launch<BF, GATED, 4, 2, 4, 2, 2, 1>(a, p.splits, part, st);
-    default: return launch<BF, GATED, 4, 4, 4, 2, 2, 1>(a, p.splits, part, st);
+    case 0: return launch<BF, GATED, F, 1, 2, 4, 3, 4, 2>(a, p.splits, part, st);
+    case 1: return launch<BF, GATED, F, 2, 2, 4, 3, 4, 2>(a, p.splits, part, st);
+    case 2: return launch<BF, GATED, F, 4, 2, 4, 2, 2, 1>(a, p.splits, part, st);
+    default: return launch<BF, GATED, F, 4, 4, 4, 2, 2, 1>(a, p.splits, part, st);
   }
 }
 
@@ -389,11 +389,11 @@ size_t mx4_tiles_workspace(int m, int n, int k, bool gated) {
   return p.splits > 1 ? (size_t)p.tiles * p.splits * SHAPES[p.shape].bm * SHAPES[p.shape].bn * 4 : 0;
 }
 
-hipError_t mx4_tiles(const Mx4Args& a, bool bf, bool gated, void* workspace, hipStream_t st) {
+hipError_t mx4_tiles(const Mx4Args& a, bool bf, bool gated, Form form, void* workspace, hipStream_t st) {
   const Plan p = plan(a.m, a.n, a.k, gated);
-  float* part = (float*)workspace;
-  if (gated) return bf ? launch_plan<true, true>(a, p, part, st) : launch_plan<false, true>(a, p, part, st);
-  return bf ? launch_plan<true, false>(a, p, part, st) : launch_plan<false, false>(a, p, part, st);
+  return mx4_dispatch(bf, gated, form, [&](auto b, auto g, auto f) {
+    return launch_plan<decltype(b)::value, decltype(g)::value, decltype(f)::value>(a, p, (float*)workspace, st);
+  });
 }
 
 }  // namespace t2w

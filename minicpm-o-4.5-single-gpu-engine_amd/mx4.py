@@ -27,6 +27,7 @@ EXPONENTS = -23, 13  # of the scales: every weight is exact in bf16 and fp16
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _WEIGHTS = _DTYPES | {torch.float32: 2}
 _ACTS = {"silu": 0, "gelu": 1}
+_INNER = {"rounded": 0, "wide": 1}
 _E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 _F32 = torch.float32
 IN_LDS = 4096      # columns of 16 rows that fit the LDS: such calls need no workspace
@@ -185,15 +186,18 @@ def gated(x: torch.Tensor, gate: MX4Weight, up: MX4Weight, *, act: str = "silu",
 
 
 def ffn(x: torch.Tensor, gate: MX4Weight, up: MX4Weight, down: MX4Weight, *, act: str = "silu", residual: torch.Tensor | None = None,
-        out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
-    """(act(x gate^T) * (x up^T)) down^T + residual.  The inner values are rounded to x's type (of fp16, beyond 65504 they are
-    infinite).  ``out`` may be ``residual``."""
+        inner: str = "wide", out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """(act(x gate^T) * (x up^T)) down^T + residual.  ``inner`` "wide": the inner values are held to 2^-16 of their value over fp32's
+    range; "rounded": to x's type (of fp16, beyond 65504 they are infinite), which halves the last product's operations.  ``out`` may be
+    ``residual``."""
+    if inner not in _INNER:
+        raise ValueError("mx4: inner must be 'wide' or 'rounded'")
     k, rows, dev = _pair(gate, up, act), _input(x, gate), gate.device
     if down.device != dev:
         raise ValueError("mx4: the weights must be on one device")
     m, n = rows[3], down.n
     out, ldy = _output(x, m, n, out, dev)
     L = _lib.lib()
-    a = _lib.MX4FFNArgs(*rows, gate.struct, up.struct, down.struct, k, *_residual(x, m, n, residual, dev), out.data_ptr(), ldy)
+    a = _lib.MX4FFNArgs(*rows, gate.struct, up.struct, down.struct, k, _INNER[inner], *_residual(x, m, n, residual, dev), out.data_ptr(), ldy)
     _run(L.t2w_mx4_ffn, L.t2w_mx4_ffn_workspace_bytes, a, dev, workspace, "mx4_ffn")
     return out

@@ -73,6 +73,21 @@ def test_ffn_workspace():
     assert fn(C.byref(ffn_args(m=-1))) == 0 and fn(C.byref(ffn_args(m=0))) == 0
 
 
+def test_ffn_inner_values():
+    """Rounded or wide; wide ones take two rows each, and the parts of a product of twice the rows."""
+    L = _lib.lib()
+    for kw, text in (({"inner": 2}, "inner must be"), ({"inner": -1}, "inner must be"), ({"inner": 1}, "workspace too small"), ({"inner": 1, "workspace_bytes": 1023}, "workspace too small"),
+                     ({"inner": 1, "workspace_bytes": 1024, "workspace": 2 * M - 1008}, "workspace overlaps")):
+        refused(L.t2w_mx4_ffn, ffn_args(**kw), text)
+    assert L.t2w_mx4_ffn_workspace_bytes(C.byref(ffn_args(inner=1))) == 2 * 4 * 64 * 2
+    down = weight(n=512, k=5000, at=300)
+    f = ffn_args(m=40, gate=weight(5000, 256), up=weight(5000, 256, at=200), down=down, inner=1, ldy=512, ldr=512)
+    parts = L.t2w_mx4_linear_workspace_bytes(C.byref(linear_args(m=80, n=512, k=5000, ldx=5000)))
+    assert parts > 0 and L.t2w_mx4_ffn_workspace_bytes(C.byref(f)) == 2 * 40 * 5000 * 2 + parts
+    with pytest.raises(ValueError, match="'wide' or 'rounded'"):
+        mx4.ffn(torch.zeros(4, 256, dtype=torch.float16), fake(64, 256), fake(64, 256), fake(256, 64), inner="exact")
+
+
 def test_workspaces():
     """None for few rows; beyond, bounded whatever the sizes; too small, misaligned or overlapping ones are refused."""
     L = _lib.lib()
