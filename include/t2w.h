@@ -503,7 +503,7 @@ typedef struct {
   int dtype, n_tok, q_heads, k_heads, head_dim, rot, pairs; /* head_dim a multiple of 8, rot of 16 */
   const uint64_t* freq;           /* [rot / 2] */
   const uint8_t* axis;            /* [rot / 2], each below n_axes (one that is not counts as the last) */
-  const int* pos; long long ld_pos; int n_axes; /* [n_axes, n_tok], rows ld_pos apart; up to 16 axes */
+  const int* pos; long long ld_pos; int n_axes; /* [n_axes, n_tok], rows ld_pos apart (0: one row for all); up to 16 axes */
   float scale;
 } t2w_rope_args;
 int t2w_rope(const t2w_rope_args* a, void* stream);

@@ -110,7 +110,8 @@ const char* rope_check(const t2w_rope_args& a) {
   if (a.rot < 16 || a.rot > a.head_dim || a.rot % 16) return "rope: rotated channels must be 16 to head_dim, a multiple of 16";
   if (a.n_tok < 0 || a.n_tok > (1 << 24)) return "rope: at most 2^24 tokens";
   if (a.q_heads < 0 || a.k_heads < 0 || a.q_heads > 4096 || a.k_heads > 4096) return "rope: at most 4096 heads";
-  if (a.n_axes < 1 || a.n_axes > 16 || (a.ld_pos < a.n_tok && a.n_axes > 1)) return "rope: 1 to 16 axes, their positions in rows of n_tok";
+  // one row for all axes (text) has stride 0; rows that overlap in part are taken for a mistake
+  if (a.n_axes < 1 || a.n_axes > 16 || (a.n_axes > 1 && a.ld_pos != 0 && a.ld_pos < a.n_tok)) return "rope: 1 to 16 axes, their positions in rows of n_tok";
   if (!std::isfinite(a.scale)) return "rope: scale must be finite";
   if (a.n_tok == 0 || a.q_heads + a.k_heads == 0) return nullptr;
   if (!a.freq || !a.axis || !a.pos) return "rope: null table or positions";

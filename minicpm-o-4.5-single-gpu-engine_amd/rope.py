@@ -68,7 +68,8 @@ class Rope:
     def apply(self, q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, *, q_out: torch.Tensor | None = None,
               k_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
         """Turns ``q`` [n_tok, heads, head_dim] and ``k`` [n_tok, kv_heads, head_dim] (or None), bf16 or fp16, token rows strided by
-        multiples of 8.  ``pos`` int32 [axes, n_tok] ([n_tok] for one axis), with at least the axes that the pairs count on.  The
+        multiples of 8.  ``pos`` int32 [axes, n_tok] ([n_tok] for one axis; text, where all axes count alike,
+        may be ``pos.expand(axes, n_tok)``), with at least the axes that the pairs count on.  The
         outputs, new tensors by default, may be ``q`` and ``k`` themselves."""
         dev, dtype = self.device, q.dtype
         code = _DTYPES.get(dtype)

@@ -104,6 +104,17 @@ def test_scale_and_axes(dev, scale):
         check(got, q, buf[:, 7:28], r, inv, axis, "halves", scale)
 
 
+@pytest.mark.parametrize("n", [1, 6, 700])
+def test_one_row_of_positions_for_all_axes(dev, n):
+    inv, axis = freqs(64), rope.sections(8, 12, 12)
+    r = rope.Rope(inv, axis=axis)
+    q, k = rand((n, 5, 64), BF, 1), rand((n, 2, 64), BF, 2)
+    pos = torch.randint(0, 100000, (1, n), dtype=torch.int32, device="cuda")
+    got = r.apply(q, k, pos.expand(3, n))
+    assert all(torch.equal(a, b) for a, b in zip(got, r.apply(q, k, pos.repeat(3, 1))))
+    check(got[0], q, pos.expand(3, n), r, inv, axis, "halves")
+
+
 def test_strides_and_empty_calls(dev):
     r = rope.Rope(freqs(64))
     pos = torch.arange(6, dtype=torch.int32, device="cuda")

@@ -236,6 +236,14 @@ def test_rope_without_work():
     assert _lib.lib().t2w_rope(C.byref(rope_args(q_heads=0, k_heads=0, q=None, k=None)), None) == 0
 
 
+def test_rope_rows_of_positions():
+    """One row for all axes is taken (refused here for what is behind it), rows that overlap in part or run backwards are not."""
+    refused(_lib.lib().t2w_rope, rope_args(ld_pos=0, freq=None), "null table")
+    refused(_lib.lib().t2w_rope, rope_args(ld_pos=0, k_out=7 * M), "positions")
+    for ld in (1, 3, -4):
+        refused(_lib.lib().t2w_rope, rope_args(ld_pos=ld), "axes")
+
+
 def test_rope_slices_of_one_projection():
     """In place on the query and key columns of one buffer: not refused for overlapping (but for the missing positions here)."""
     both = {"q": M, "k": M + 1024, "q_out": M, "k_out": M + 1024, "ldq": 1024, "ldk": 1024, "ldq_out": 1024, "ldk_out": 1024}
