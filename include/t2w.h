@@ -404,7 +404,7 @@ int t2w_kv8_attention(const t2w_kv8_attention_args* a, void* stream);
  * (engine/runtime/fp8.py:15-37).
  *
  * A matrix is laid out once, by t2w_mx4_pack from codes or by t2w_mx4_quantize from 16- or 32-bit weights, into memory of
- * t2w_mx4_codes_bytes and t2w_mx4_scales_bytes (the kernels' operand order).  Scales are limited to 2^-23 .. 2^13, where every
+ * t2w_mx4_codes_bytes and t2w_mx4_scales_bytes (the kernels' operand order; it overlaps no input).  Scales are limited to 2^-23 .. 2^13, where every
  * weight is exact in bf16 and fp16; a group whose codes are all zero may have any. */
 
 enum { T2W_MX4_BF16 = 0, T2W_MX4_FP16 = 1, T2W_MX4_FP32 = 2 };

@@ -78,6 +78,23 @@ int run(const Mx4Args& g, int dtype, bool gated, Form form, void* workspace, voi
 
 }  // namespace
 
+namespace {
+
+// what laying a matrix out may not be given: outputs that share bytes with each other or with the `n_in` inputs
+const char* check_layout(int n, int k, void* w_codes, void* w_scales, int* status, const Rows* in, int n_in) {
+  const long long c = (long long)t2w_mx4_codes_bytes(n, k), s = (long long)t2w_mx4_scales_bytes(n, k);
+  const Rows out[3] = {{w_codes, c, c, 1}, {w_scales, s, s, 1}, {status, 4, 4, 1}};
+  for (int i = 0; i < 3; ++i) {
+    for (int j = 0; j < i; ++j)
+      if (rows_meet(out[i], out[j])) return "mx4: the laid out codes, scales and status overlap";
+    for (int j = 0; j < n_in; ++j)
+      if (rows_meet(out[i], in[j])) return "mx4: an output overlaps an input";
+  }
+  return nullptr;
+}
+
+}  // namespace
+
 extern "C" {
 
 size_t t2w_mx4_codes_bytes(int n, int k) { return check_size(n, k) ? 0 : (size_t)mx4_blocks(n) * mx4_steps(k) * 1024; }
@@ -88,6 +105,9 @@ int t2w_mx4_pack(const t2w_mx4_pack_args* a, void* stream) {
   if (const char* e = check_size(a->n, a->k)) return xerr(e);
   if (!a->codes || !a->scales || !a->w_codes || !a->w_scales || !a->status) return xerr("mx4 pack: null operand");
   if (((uintptr_t)a->codes & 3) || ((uintptr_t)a->w_codes & 15) || ((uintptr_t)a->w_scales & 3) || ((uintptr_t)a->status & 3)) return xerr("mx4 pack: misaligned operand");
+  const long long c = (long long)a->n * (a->k / 2), s = (long long)a->n * ((a->k + 31) / 32);
+  const Rows in[2] = {{a->codes, c, c, 1}, {a->scales, s, s, 1}};
+  if (const char* e = check_layout(a->n, a->k, a->w_codes, a->w_scales, a->status, in, 2)) return xerr(e);
   const hipError_t e = mx4_pack(*a, (hipStream_t)stream);
   return e == hipSuccess ? 0 : xerr("mx4 pack", e);
 }
@@ -99,6 +119,9 @@ int t2w_mx4_quantize(const t2w_mx4_quantize_args* a, void* stream) {
   if (!a->w || !a->w_codes || !a->w_scales || !a->status) return xerr("mx4 quantize: null operand");
   if (((uintptr_t)a->w & (a->dtype == T2W_MX4_FP32 ? 3 : 1)) || ((uintptr_t)a->w_codes & 15) || ((uintptr_t)a->w_scales & 3) || ((uintptr_t)a->status & 3)) return xerr("mx4 quantize: misaligned operand");
   if (a->n > 1 && a->ldw < a->k) return xerr("mx4 quantize: rows overlap");
+  const long long size = a->dtype == T2W_MX4_FP32 ? 4 : 2;
+  const Rows in{a->w, a->ldw * size, a->k * size, a->n};
+  if (const char* e = check_layout(a->n, a->k, a->w_codes, a->w_scales, a->status, &in, 1)) return xerr(e);
   const hipError_t e = mx4_quantize(*a, (hipStream_t)stream);
   return e == hipSuccess ? 0 : xerr("mx4 quantize", e);
 }

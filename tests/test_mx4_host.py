@@ -135,6 +135,19 @@ def test_quantize_refuses(kw, text):
     refused(_lib.lib().t2w_mx4_quantize, a, text)
 
 
+@pytest.mark.parametrize("kw", [{"w_codes": M}, {"w_codes": M + 112}, {"w_codes": M - 1008}, {"w_codes": 2 * M}, {"w_scales": M + 124}, {"w_scales": 2 * M + 4}, {"w_scales": 3 * M + 1020}, {"status": M + 4},
+                                {"status": 2 * M + 4}, {"status": 3 * M + 512}, {"status": 4 * M + 252}], ids=str)
+def test_layout_in_its_own_inputs_is_refused(kw):
+    """Threads read codes and scales in another order than they write: laid out over its inputs a matrix would be any mixture."""
+    base = {"codes": M, "scales": 2 * M, "n": 4, "k": 64, "w_codes": 3 * M, "w_scales": 4 * M, "status": 5 * M}
+    refused(_lib.lib().t2w_mx4_pack, _lib.MX4PackArgs(**(base | kw)), "overlap")
+    quant = {"w": M, "ldw": 96, "dtype": 2, "n": 4, "k": 64, "w_codes": 3 * M, "w_scales": 4 * M, "status": 5 * M}
+    if not any(2 * M <= v < 2 * M + 64 for v in kw.values()):
+        refused(_lib.lib().t2w_mx4_quantize, _lib.MX4QuantizeArgs(**(quant | kw)), "overlap")
+    if "w_codes" in kw:
+        refused(_lib.lib().t2w_mx4_quantize, _lib.MX4QuantizeArgs(**(quant | {"w": kw["w_codes"] + 512, "w_codes": kw["w_codes"]})), "overlap")
+
+
 def test_calls_without_rows_do_nothing():
     assert _lib.lib().t2w_mx4_linear(C.byref(linear_args(m=0, x=None, y=None, residual=None, bias=None)), None) == 0
     assert _lib.lib().t2w_mx4_ffn(C.byref(ffn_args(m=0, workspace=None, workspace_bytes=0)), None) == 0
