@@ -484,6 +484,12 @@ typedef struct {
 size_t t2w_mx4_ffn_workspace_bytes(const t2w_mx4_ffn_args* a);
 int t2w_mx4_ffn(const t2w_mx4_ffn_args* a, void* stream);
 
+/* The kernel that a product takes: m rows of x, ldx elements apart, by n channels (gated: of each matrix) of k columns; a block's last
+ * product has 2 m rows where the inner values are wide.  tile_rows 0: the kernel of few rows; else tiles of tile_rows by
+ * tile_channels outputs, k in `parts` parts (more than one needs a workspace).  For tests and for choosing batch sizes. */
+typedef struct { int tile_rows, tile_channels, parts; } t2w_mx4_form;
+int t2w_mx4_product_form(int m, int n, int k, long long ldx, int gated, t2w_mx4_form* form);
+
 /* ---------------------------------------------------------------- rotary positions of several axes
  * Queries and keys [n_tok, heads, head_dim] (token rows ld* elements apart, a token's heads side by side): pair p of a head's
  * first `rot` channels turns by pos[axis[p] * ld_pos + token] * inv_freq[p]:

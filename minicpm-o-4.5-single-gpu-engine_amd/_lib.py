@@ -147,6 +147,10 @@ class MX4FFNArgs(C.Structure):
                 ("residual", P), ("ldr", C.c_longlong), ("y", P), ("ldy", C.c_longlong), ("workspace", P), ("workspace_bytes", C.c_size_t)]
 
 
+class MX4Form(C.Structure):
+    _fields_ = [("tile_rows", I), ("tile_channels", I), ("parts", I)]
+
+
 class RopeArgs(C.Structure):
     _fields_ = [(n, P) for n in ("q", "k", "q_out", "k_out")] + [(n, C.c_longlong) for n in ("ldq", "ldk", "ldq_out", "ldk_out")] + \
                [(n, I) for n in ("dtype", "n_tok", "q_heads", "k_heads", "head_dim", "rot", "pairs")] + \
@@ -206,6 +210,7 @@ _SIGS = {
     "t2w_mx4_gated": (I, [C.POINTER(MX4GatedArgs), P]),
     "t2w_mx4_ffn": (I, [C.POINTER(MX4FFNArgs), P]),
     "t2w_mx4_ffn_workspace_bytes": (C.c_size_t, [C.POINTER(MX4FFNArgs)]),
+    "t2w_mx4_product_form": (I, [I, I, I, C.c_longlong, I, C.POINTER(MX4Form)]),
     "t2w_rope": (I, [C.POINTER(RopeArgs), P]),
     "t2w_device_cus": (I, [C.POINTER(I)]),
     "t2w_stream_create_cu_mask": (I, [C.POINTER(C.c_uint32), I, C.POINTER(P)]),

@@ -100,6 +100,13 @@ extern "C" {
 size_t t2w_mx4_codes_bytes(int n, int k) { return check_size(n, k) ? 0 : (size_t)mx4_blocks(n) * mx4_steps(k) * 1024; }
 size_t t2w_mx4_scales_bytes(int n, int k) { return check_size(n, k) ? 0 : (size_t)mx4_blocks(n) * mx4_units(k) * 256; }
 
+int t2w_mx4_product_form(int m, int n, int k, long long ldx, int gated, t2w_mx4_form* form) {
+  if (const char* e = check_size(n, k)) return xerr(e);
+  if (m < 1 || m > 2 * MAX_ROWS || !form) return xerr("mx4 form: 1 to 2^21 rows and a place for the form");
+  *form = mx4_takes_tiles(m, n, k, ldx, gated != 0) ? mx4_tiles_form(m, n, k, gated != 0) : t2w_mx4_form{0, 0, 1};
+  return 0;
+}
+
 int t2w_mx4_pack(const t2w_mx4_pack_args* a, void* stream) {
   if (!a) return xerr("mx4 pack: null arguments");
   if (const char* e = check_size(a->n, a->k)) return xerr(e);

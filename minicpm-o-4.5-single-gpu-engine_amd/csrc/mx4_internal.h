@@ -55,6 +55,7 @@ hipError_t mx4_rows(const Mx4Args& a, bool bf, bool gated, Form form, hipStream_
 int mx4_rows_outside(int m, int k, bool gated);  // units of 512 columns of x that do not fit the LDS
 bool mx4_takes_tiles(int m, int n, int k, long long ldx, bool gated);
 size_t mx4_tiles_workspace(int m, int n, int k, bool gated);
+t2w_mx4_form mx4_tiles_form(int m, int n, int k, bool gated);
 hipError_t mx4_tiles(const Mx4Args& a, bool bf, bool gated, Form form, void* workspace, hipStream_t st);
 
 // f(bf16 operands?, gated?, form) with compile-time arguments

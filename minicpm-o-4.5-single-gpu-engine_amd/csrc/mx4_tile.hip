@@ -389,6 +389,11 @@ size_t mx4_tiles_workspace(int m, int n, int k, bool gated) {
   return p.splits > 1 ? (size_t)p.tiles * p.splits * SHAPES[p.shape].bm * SHAPES[p.shape].bn * 4 : 0;
 }
 
+t2w_mx4_form mx4_tiles_form(int m, int n, int k, bool gated) {
+  const Plan p = plan(m, n, k, gated);
+  return {SHAPES[p.shape].bm, SHAPES[p.shape].bn / (gated ? 2 : 1), p.splits};
+}
+
 hipError_t mx4_tiles(const Mx4Args& a, bool bf, bool gated, Form form, void* workspace, hipStream_t st) {
   const Plan p = plan(a.m, a.n, a.k, gated);
   return mx4_dispatch(bf, gated, form, [&](auto b, auto g, auto f) {

@@ -166,6 +166,14 @@ def linear(x: torch.Tensor, w: MX4Weight, *, bias: torch.Tensor | None = None, r
     return out
 
 
+def form(rows: int, n: int, k: int, *, gated: bool = False, ldx: int | None = None) -> tuple[int, int, int]:
+    """The kernel that a product of these sizes takes: (0, 0, 1) the one for few rows, else tiles of that many rows and output channels
+    and the parts that k is split into.  A block's last product has 2 rows for each of x where its inner values are wide."""
+    f = _lib.MX4Form()
+    _lib.check(_lib.lib().t2w_mx4_product_form(rows, n, k, k if ldx is None else ldx, gated, C.byref(f)), "mx4_product_form")
+    return f.tile_rows, f.tile_channels, f.parts
+
+
 def _pair(gate: MX4Weight, up: MX4Weight, act: str) -> int:
     if act not in _ACTS:
         raise ValueError("mx4: act must be 'silu' or 'gelu'")

@@ -115,6 +115,24 @@ def test_workspaces():
     assert L.t2w_mx4_ffn_workspace_bytes(C.byref(f)) >= 64 * 64 * 2
 
 
+def test_forms():
+    """What a product takes, and that only those in parts ask for memory."""
+    L = _lib.lib()
+    assert mx4.form(1, 6144, 4096) == mx4.form(16, 6144, 4096) == (0, 0, 1)
+    assert mx4.form(4001, 6144, 4096) == (64, 256, 1) and mx4.form(2005, 14336, 4096, gated=True) == (64, 128, 1)
+    assert mx4.form(70, 40, 256, ldx=1 << 24) == (0, 0, 1)  # rows too far apart for a tile
+    for m in (1, 16, 17, 64, 200, 1000):
+        for n in (31, 512, 6144):
+            for k in (264, 4096, 14336):
+                need = L.t2w_mx4_linear_workspace_bytes(C.byref(linear_args(m=m, n=n, k=k, ldx=k)))
+                rows, channels, parts = mx4.form(m, n, k)
+                assert need == (parts * (-(-m // rows) * rows) * (-(-n // channels) * channels) * 4 if parts > 1 else 0)
+    for bad in ((0, 64, 64), ((1 << 21) + 1, 64, 64), (4, 0, 64), (4, 64, 60)):
+        with pytest.raises(RuntimeError, match="mx4"):
+            mx4.form(*bad)
+    assert L.t2w_mx4_product_form(4, 64, 64, 64, 0, None) == 1
+
+
 def test_weight_sizes():
     L = _lib.lib()
     assert (L.t2w_mx4_codes_bytes(1, 8), L.t2w_mx4_scales_bytes(1, 8)) == (1024, 256)
