@@ -496,7 +496,8 @@ int t2w_mx4_product_form(int m, int n, int k, long long ldx, int gated, t2w_mx4_
  *   y0 = scale (x0 cos - x1 sin), y1 = scale (x0 sin + x1 cos)
  * where (x0, x1) are channels (p, p + rot / 2) (T2W_ROPE_HALVES) or (2 p, 2 p + 1) (T2W_ROPE_NEIGHBOURS); channels from `rot` on are
  * copied.  The axes are whatever the caller counts on them (time, height, width).  freq[p] is inv_freq[p] / (2 pi) turns in units of
- * 2^-64, wrapped: angles are exact to 2^-32 turns at every int position.  No counterpart in the reference's path (its DiT has no
+ * 2^-64, wrapped: a position's product with it is exact to 2^-32 turns at every int position, and rounded to fp32 (at most 2^-26 turns)
+ * for its sine and cosine.  No counterpart in the reference's path (its DiT has no
  * positional encoding; t2w_dit_globals.rope_freq is this library's one-axis option there). */
 
 enum { T2W_ROPE_BF16 = 0, T2W_ROPE_FP16 = 1 };

@@ -197,7 +197,8 @@ int t2w_mx4_gated(const t2w_mx4_gated_args* a, void* stream) {
 // The inner rows lie in the workspace, each at a 16-byte boundary: the second product's matrix operand, of 16 bits.  Wide, a value is two
 // rows' sum, which doubles that product (a third of the block's work) and leaves the outputs' errors at their own rounding's.  Rounded
 // to x's type once, errors grow to up to sqrt(2) of that (bf16 1.7e-3 to 2.0-2.3e-3, fp16 2.1e-4 to 2.5-3.1e-4, relative) and fp16 loses
-// what is beyond 65504.
+// what is beyond 65504.  Wide and rounded, a call: 1 x 4096 x 14336 20.4 and 19.7 us, 16 x 2048 x 5464 16.4 and 13.6, 200 x 4096 x
+// 14336 106 and 86, 2005 rows 729 and 543.
 static long long inner_ld(const t2w_mx4_ffn_args& a) { return (a.gate.n + 7) / 8 * 8; }
 static int inner_rows(const t2w_mx4_ffn_args& a) { return a.inner == T2W_MX4_INNER_WIDE ? 2 * a.m : a.m; }
 

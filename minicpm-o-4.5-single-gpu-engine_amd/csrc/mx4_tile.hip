@@ -11,7 +11,7 @@
 //
 // The conversion is one instruction for two weights and shares the wave's time with the MFMAs; the codes come to a CU at a quarter
 // of bf16's bytes, which is why a tile of only 64 rows reaches the rate of a large bf16 product: 64 x 256 tiles run 4001 rows x
-// 6144 x 4096 in 156 to 176 us (1.15 to 1.29 PFLOP/s, by machine) and 2005 rows' gated 14336 x 4096 x 2 in 359 to 385 (1.22 to 1.31).
+// 6144 x 4096 in 156 to 176 us (1.15 to 1.29 PFLOP/s, by machine) and 2005 rows' gated 14336 x 4096 x 2 in 359 to 396 (1.19 to 1.31).
 // There the matrix units are busy for 53 to 62% of the cycles at a clock of 2.0 GHz, vector instructions issue in 40% and the waves
 // wait for a quarter of theirs.  With two workgroups a CU the barriers of one fall into the other's MFMAs: 128 x 256 tiles of eight waves, one
 // workgroup a CU, took 9% longer, 256 x 256 (spilling) 21%, waves of 128 x 64 (half the conversions a product) alone on a SIMD 18%.
@@ -322,9 +322,10 @@ hipError_t launch(const Mx4Args& a, int splits, float* part, hipStream_t st) {
 }
 
 // The tiles, each with four waves side by side: rows, weight channels (gated: half of each matrix), groups of waves that split k, and
-// the microseconds of a pass (a stage of each group) with one workgroup on a CU and, of each, with several.  Measured: 6144
-// channels x 4096 columns x 64 rows take 11.3 / 13.5 / 25 / 35 us, 28000 x 4096 x 32 20 / 16 / 27 / 34, x 100 46 / 40 / 35 / 38,
-// 14336 x 4096 x 2, gated, of 2005 rows in the wide two 374 / 360.
+// the microseconds of a pass (a stage of each group) with one workgroup on a CU and, of each, with several.  Measured with codes from
+// HBM (more matrices in turn than a cache holds): 6144 channels x 4096 columns x 64 rows take 11.4 / 13.9 / 25 / 37 us (the first 9.6
+// with a matrix in the last-level cache), 28000 x 4096 x 32 20 / 16 / 27 / 36, x 100 45 / 38 / 33 / 39; the wide two take 396 / 368 for
+// 2005 rows of 14336 x 4096 x 2, gated, and 395 / 364 for 4010 rows of 4096 x 14336.
 struct Shape {
   int bm, bn, kg;
   float one, many;

@@ -1,8 +1,9 @@
 // Rotary positions of several axes (time, height, width): pair p of a head turns by pos[axis[p]][token] * inv_freq[p].
 //
 // The angle is computed in turns as 64-bit fixed point: freq[p] is inv_freq[p] / 2 pi in units of 2^-64 turns (wrapped), an integer
-// product wraps whole turns away by itself, and its upper 32 bits are the angle to 2^-32 turns at every int32 position; fp32
-// products lose the angle of far positions (position 10^6 at frequency 1: 0.06 radians).
+// product wraps whole turns away by itself, and its upper 32 bits are the angle to 2^-32 turns at every int32 position.  Sine and
+// cosine take it in fp32, which rounds it by at most 2^-26 turns (10^-7 radians, less than their own error), at any position alike;
+// fp32 products lose the angle of far positions (position 10^6 at frequency 1: 0.06 radians).
 //
 // Bound by memory: 37,433 tokens of 40 heads x 128 take 140 us (5.4 TB/s read and written; a copy of that size 5.2).  A lane keeps its
 // eight pairs' sines and cosines for all heads of its token: computed for each head they would be most of the work.

@@ -10,7 +10,8 @@ For callers that run the layers around the paged 8-bit cache (``t2w_amd.kv8``) o
     y = linear(o.flatten(1), o_w, residual=x)
     z = ffn(y, gate_w, up_w, down_w, residual=y)
 
-Activations are bf16 or fp16; weights take their type without a rounding, sums are fp32.  Calls go on the caller's current
+Activations are bf16 or fp16; weights take their type without a rounding, sums are fp32, a block's inner values keep 16 bits of
+precision over fp32's range (or x's type, where asked for).  Calls go on the caller's current
 stream, wait for nothing and can be captured.  No gradients flow through them.
 """
 
@@ -148,8 +149,8 @@ def _run(fn, workspace_bytes, a, dev, workspace, what: str) -> None:
 
 def linear(x: torch.Tensor, w: MX4Weight, *, bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
            out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
-    """x w^T + bias + residual: ``x`` [rows, k] bf16 or fp16 (rows may be strided by multiples of 8), ``bias`` fp32 [n], ``residual``
-    [rows, n] of x's type.  ``out`` may be ``residual``.  ``workspace``: memory for calls that make none
+    """x w^T + bias + residual: ``x`` [rows, k] bf16 or fp16 (rows may be strided by multiples of 8, without overlap), ``bias`` fp32 [n],
+    ``residual`` [rows, n] of x's type.  ``out`` may be ``residual``.  ``workspace``: memory for calls that make none
     (``t2w_mx4_linear_workspace_bytes``)."""
     dev, n = w.device, w.n
     rows = _input(x, w)

@@ -2,8 +2,9 @@
 counterpart in the reference's Token2Wav path, whose DiT has no positional encoding; ``DiTConfig.rope_theta`` is the one-axis
 option there.
 
-A pair of channels turns by the token's position on the pair's axis times the pair's frequency.  Angles are integers: exact at
-every int32 position.  Calls go on the caller's current stream, wait for nothing and can be captured; no gradients flow through
+A pair of channels turns by the token's position on the pair's axis times the pair's frequency.  Angles are integers, products of
+the position with 64 bits of the frequency, and rounded to fp32 only for the sine and cosine: within 2^-26 turns at every int32
+position.  Calls go on the caller's current stream, wait for nothing and can be captured; no gradients flow through
 them::
 
     rope = Rope([theta ** (-2 * p / d) for p in range(d // 2)], axis=sections(16, 24, 24))   # once, with the model

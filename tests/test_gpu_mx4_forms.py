@@ -233,6 +233,15 @@ def test_blocks_columns_in_parts(dev, tile, sizes, dt):
         check_block(m, inner, out, dt)
 
 
+@pytest.mark.parametrize("dt", [BF, FP], ids=str)
+def test_inner_rows_beyond_32_bit_offsets(dev, dt):
+    """Inner rows of 4.6 GB: every 100 rows of x repeat the first, and so do the outputs."""
+    x, g, u, d, res, _, want = whole_numbers(100, 14344, 64, dt)
+    assert 2 * 80000 * 14344 * 2 > 2 ** 32
+    got = mx4.ffn(x.repeat(800, 1), g, u, d, residual=res.repeat(800, 1))
+    assert torch.equal(got, want.repeat(800, 1))
+
+
 # --- products in parts as programs call them ------------------------------------------------------------------------------------------
 
 SPLIT = [(40, 512, 5000), (40, 14336, 264), (200, 264, 9224)]  # rows, hidden, inner: parts in the last product, in the gated one, in the last
